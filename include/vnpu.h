@@ -186,8 +186,21 @@ typedef enum vnpu_opcode_t {
     VNPU_OP_COPY            = 14,
     VNPU_OP_MEMSET          = 15,
     VNPU_OP_BARRIER         = 16,
-    VNPU_OP_COUNT           = 17
+    VNPU_OP_COUNT           = 17,
+    /* MI355X extension (additive; no reference counterpart): the paged int8
+     * KV cache, see vnpu_kv_cache_t.  Opcodes from VNPU_OP_COUNT to 63 stay
+     * invalid commands. */
+    VNPU_OP_KV_APPEND_I8    = 64,
+    VNPU_OP_KV_ATTENTION_I8 = 65,
+    VNPU_OP_KV_READ_F32     = 66
 } vnpu_opcode_t;
+
+/* MI355X extension: position rotation of VNPU_OP_KV_APPEND_I8. */
+typedef enum vnpu_rotation_t {
+    VNPU_ROTATE_NONE        = 0,
+    VNPU_ROTATE_HALF        = 1,   /* pairs (j, j + rope_dim / 2), as ROPE_F32 */
+    VNPU_ROTATE_INTERLEAVED = 2    /* pairs (2j, 2j + 1) */
+} vnpu_rotation_t;
 
 /* reference include/vnpu.h:186-197 */
 typedef struct vnpu_config_t {
@@ -457,6 +470,129 @@ typedef struct vnpu_memset_args_t {
     uint32_t reserved0;
 } vnpu_memset_args_t;
 
+/* ----------------------------------------------------------------------- */
+/* MI355X extension (additive; no reference counterpart): a paged cache of   */
+/* keys and values in int8, the commands that append to it, attend over it   */
+/* and read it back.                                                         */
+/*                                                                           */
+/* A page holds page_size consecutive tokens of one sequence; row b of the   */
+/* table names the pages of sequence b in order, so token i of it is slot    */
+/* i % page_size of page table[b][i / page_size].  A cached value is its     */
+/* int8 code times the scale of its (page, kv head); keys and values have    */
+/* scales of their own.  V is stored with the tokens of a page side by side, */
+/* which is the operand order of the product with the softmax weights.       */
+/*                                                                           */
+/* The new (or read) tokens of a call are `tokens` rows.  With seq_start     */
+/* ([batch + 1], not decreasing) rows seq_start[b] .. seq_start[b + 1] - 1   */
+/* are sequence b's, and rows behind seq_start[batch] are left as they are;  */
+/* without it every sequence has tokens / batch of them.  Element d of head  */
+/* h of row r = b's token i is at r * token_stride + h * head_stride + d     */
+/* with seq_start, at b * batch_stride + i * token_stride + h * head_stride  */
+/* + d without.  A stride of 0 is the packed row's: head_stride head_dim,    */
+/* token_stride heads * head_dim, batch_stride tokens / batch *              */
+/* token_stride; [batch][heads][tokens][head_dim] is {heads * n * head_dim,  */
+/* head_dim, n * head_dim}.  Strides count floats; outputs' rows may not     */
+/* overlap.                                                                  */
+/*                                                                           */
+/* k, v and the scales must be device memory; table, the length arrays and   */
+/* the f32 tensors may be host memory, staged as everywhere.  Lengths and    */
+/* pages are read on the GPU: a negative or too long length, a seq_start     */
+/* that decreases or passes `tokens`, or a page outside [0, pages) of a      */
+/* token that the call touches fails the stream at its next sync             */
+/* (VNPU_ERR_DEVICE_ERROR); nothing outside the given buffers is touched,    */
+/* and what such a call wrote is unspecified.                                */
+/* ----------------------------------------------------------------------- */
+typedef struct vnpu_kv_cache_t {
+    int8_t *k;                  /* [pages][kv_heads][page_size][head_dim], 16-byte aligned */
+    int8_t *v;                  /* [pages][kv_heads][head_dim][page_size], 16-byte aligned */
+    float *k_scales;            /* [pages][kv_heads] */
+    float *v_scales;            /* [pages][kv_heads] */
+    const int32_t *table;       /* [batch][table_ld] */
+    uint32_t pages;
+    uint32_t page_size;         /* 16, 32, 64, 128 or 256 */
+    uint32_t kv_heads;
+    uint32_t head_dim;          /* a multiple of 16, up to 256 */
+    uint32_t table_ld;          /* pages that a sequence can have */
+    uint32_t reserved0;
+} vnpu_kv_cache_t;
+
+/* Token i of sequence b is written to position past[b] + i.  K and, where Q
+ * is given, Q (to Q_out, which may be Q with Q's strides) are turned by
+ * position * scaling * theta_base^(-2j / rope_dim), angles in 64 bits, each
+ * result rounded once to f32; elements from rope_dim on are left.  V goes in
+ * as it is.  Per (page, kv head), a = the largest magnitude of the page's new
+ * tokens: the scale becomes max(s0, a / 127), s0 being its scale if it keeps
+ * older tokens (slots below past[b] % page_size) and 0 if not; where that
+ * raises s0 the older codes are rounded anew to code * (s0 / scale); new
+ * codes are round-half-away(x * (1 / scale)) in +-127.  A scale below 2^-126
+ * is 0 (codes 0); an infinity or NaN among a page's new values makes its
+ * scale NaN and leaves its codes.  A page that two sequences of one call write to has unspecified
+ * contents afterwards. */
+typedef struct vnpu_kv_append_i8_args_t {
+    vnpu_kv_cache_t cache;
+    const float *Q;             /* optional: queries to turn */
+    float *Q_out;
+    const float *K;
+    const float *V;
+    const int32_t *past;        /* [batch]: tokens cached before */
+    const int32_t *seq_start;   /* optional [batch + 1] */
+    uint32_t batch;
+    uint32_t tokens;
+    uint32_t heads;             /* of Q; ignored without Q */
+    uint32_t q_batch_stride, q_token_stride, q_head_stride;
+    uint32_t o_batch_stride, o_token_stride, o_head_stride;   /* of Q_out */
+    uint32_t k_batch_stride, k_token_stride, k_head_stride;
+    uint32_t v_batch_stride, v_token_stride, v_head_stride;
+    uint32_t rotation;          /* vnpu_rotation_t */
+    uint32_t rope_dim;          /* even, at most head_dim; 0 = head_dim */
+    float theta_base;           /* <= 0 means 10000 */
+    float scaling;              /* <= 0 means 1 */
+} vnpu_kv_append_i8_args_t;
+
+/* O = softmax(scale * Q . K) . V over the cached tokens, query head h with kv
+ * head h / (heads / kv_heads).  Query i of the n of sequence b sees keys
+ * j < kv_len[b] (kv_len counts the new tokens once they are appended) and,
+ * causal, j <= kv_len[b] - n + i; one that sees none gives zeros.  Q may be
+ * O, with the same strides.  Sums and softmax statistics are f32; queries
+ * and weights enter the products with 22 bits or more (about 1e-7 of
+ * the result).  A query row with an infinity or NaN, or one that sees a page
+ * with such a scale, gives NaN.  Calls that split the keys of a sequence
+ * over workgroups keep partial results in `workspace` (device memory of
+ * vnpu_kv_attention_workspace bytes or more, 16-byte aligned, of no other
+ * call that may run at the same time), or with NULL in the stream's own. */
+typedef struct vnpu_kv_attention_i8_args_t {
+    vnpu_kv_cache_t cache;
+    const float *Q;
+    float *O;
+    const int32_t *kv_len;      /* [batch] */
+    const int32_t *seq_start;   /* optional [batch + 1] */
+    void *workspace;            /* optional */
+    uint64_t workspace_bytes;
+    uint32_t batch;
+    uint32_t tokens;
+    uint32_t heads;             /* a multiple of kv_heads */
+    uint32_t q_batch_stride, q_token_stride, q_head_stride;
+    uint32_t o_batch_stride, o_token_stride, o_head_stride;
+    uint32_t max_tokens;        /* no sequence has more new tokens; 0 = tokens */
+    uint32_t max_kv;            /* no kv_len is larger; 0 = table_ld * page_size */
+    uint32_t causal;
+    float scale;                /* <= 0 means 1/sqrt(head_dim) */
+    uint32_t reserved0;
+} vnpu_kv_attention_i8_args_t;
+
+/* K, V (either may be NULL) = the values of the cached tokens first[b] + i. */
+typedef struct vnpu_kv_read_f32_args_t {
+    vnpu_kv_cache_t cache;
+    float *K;
+    float *V;
+    const int32_t *first;       /* optional [batch]; NULL = 0 */
+    const int32_t *seq_start;   /* optional [batch + 1] */
+    uint32_t batch;
+    uint32_t tokens;
+    uint32_t k_batch_stride, k_token_stride, k_head_stride;
+    uint32_t v_batch_stride, v_token_stride, v_head_stride;
+} vnpu_kv_read_f32_args_t;
+
 /* The fixed 208-byte command packet: reference include/vnpu.h:447-468. */
 typedef struct vnpu_command_t {
     uint32_t opcode;
@@ -477,6 +613,9 @@ typedef struct vnpu_command_t {
         vnpu_mtp_head_f32_args_t mtp_head;
         vnpu_copy_args_t copy;
         vnpu_memset_args_t memset;
+        vnpu_kv_append_i8_args_t kv_append;
+        vnpu_kv_attention_i8_args_t kv_attention;
+        vnpu_kv_read_f32_args_t kv_read;
         uint8_t raw[192];
     } args;
 } vnpu_command_t;
@@ -791,6 +930,32 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_pack_weights_i8_masked(vnpu_device_t *devi
 VNPU_API vnpu_status_t VNPU_CALL vnpu_attention_f32_noalloc(vnpu_stream_t *stream,
                                                             const vnpu_attention_f32_args_t *args);
 
+/* MI355X extension (additive): submit one KV command + sync, as the wrappers
+ * above do for theirs. */
+VNPU_API vnpu_status_t VNPU_CALL vnpu_kv_append_i8(vnpu_stream_t *stream,
+                                                   const vnpu_kv_append_i8_args_t *args);
+VNPU_API vnpu_status_t VNPU_CALL vnpu_kv_attention_i8(vnpu_stream_t *stream,
+                                                      const vnpu_kv_attention_i8_args_t *args);
+VNPU_API vnpu_status_t VNPU_CALL vnpu_kv_read_f32(vnpu_stream_t *stream,
+                                                  const vnpu_kv_read_f32_args_t *args);
+
+/* MI355X extension (additive): bytes of workspace that this call of
+ * KV_ATTENTION_I8 needs on this device (0: none).  Only its sizes, strides
+ * and whether seq_start is given count, not what its arrays hold, so one answer
+ * holds for every step of a decode loop.  0 for a call that is refused. */
+VNPU_API uint64_t VNPU_CALL vnpu_kv_attention_workspace(const vnpu_device_t *device,
+                                                        const vnpu_kv_attention_i8_args_t *args);
+
+/* MI355X extension (additive): enqueues KV_* commands (no others) and does
+ * nothing else: no allocation, no event, no synchronization, so a caller may
+ * capture it into a HIP graph of the stream.  Every pointer must be device
+ * memory, and a KV_ATTENTION_I8 that needs a workspace must be given one; each
+ * captured graph that may run beside another needs one of its own.  Returns
+ * VNPU_ERR_INVALID_ARGUMENT with nothing enqueued where a command is refused. */
+VNPU_API vnpu_status_t VNPU_CALL vnpu_kv_enqueue_noalloc(vnpu_stream_t *stream,
+                                                         const vnpu_command_t *commands,
+                                                         uint64_t count);
+
 /* Helpers (reference include/vnpu.h:745-750). */
 VNPU_API uint16_t VNPU_CALL vnpu_float_to_bf16(float value);
 VNPU_API uint16_t VNPU_CALL vnpu_float_to_f16(float value);
@@ -826,6 +991,10 @@ VNPU_STATIC_ASSERT(sizeof(vnpu_device_info_t) == 304, "device info");
 VNPU_STATIC_ASSERT(sizeof(vnpu_device_status_t) == 152, "device status");
 VNPU_STATIC_ASSERT(sizeof(vnpu_trace_summary_t) == 112, "trace summary");
 VNPU_STATIC_ASSERT(sizeof(vnpu_tune_result_t) == 72, "tune result");
+VNPU_STATIC_ASSERT(sizeof(vnpu_kv_cache_t) == 64, "kv cache");
+VNPU_STATIC_ASSERT(sizeof(vnpu_kv_append_i8_args_t) == 192, "kv append args");
+VNPU_STATIC_ASSERT(sizeof(vnpu_kv_attention_i8_args_t) == 168, "kv attention args");
+VNPU_STATIC_ASSERT(sizeof(vnpu_kv_read_f32_args_t) == 128, "kv read args");
 #endif
 
 #endif /* VNPU_H */

@@ -1015,6 +1015,234 @@ void exec_attention(vnpu_stream_t *s, const vnpu_attention_f32_args_t &a, ExecSt
     account_attention(a, st);
 }
 
+// ---------------------------------------------------------------------------
+// The paged int8 KV cache (no reference counterpart).  A command's arguments
+// are checked and its kernel parameters built by kv_*_params; with a Stager
+// host pointers are staged as everywhere, without one they are refused.
+// ---------------------------------------------------------------------------
+
+struct KvTensor {
+    k::KvRows rows;
+    uint64_t span = 0;   // floats from the first element to behind the last
+};
+
+// Strides with their defaults.  An output's rows may not overlap: its
+// dimensions, from the smallest stride up, each step over the one below.
+KvTensor kv_rows(uint32_t bs, uint32_t ts, uint32_t hs, uint64_t heads, uint64_t dim, uint64_t batch,
+                 uint64_t tokens, bool ragged, bool output)
+{
+    KvTensor t;
+    const uint64_t n = ragged ? tokens : tokens / batch;
+    t.rows.head = hs ? hs : dim;
+    t.rows.token = ts ? ts : heads * dim;
+    t.rows.batch = ragged ? 0 : bs ? bs : n * t.rows.token;
+    std::pair<uint64_t, uint64_t> dims[3] = {
+        {t.rows.head, heads}, {t.rows.token, n}, {t.rows.batch, ragged ? 1 : batch}};
+    std::sort(dims, dims + 3);
+    t.span = dim;
+    for (const auto &d : dims) {
+        if (d.second <= 1) continue;
+        require(!output || d.first >= t.span, "kv output rows overlap");
+        t.span += (d.second - 1) * d.first;
+    }
+    return t;
+}
+
+// Where a KV command's pointers may lead: host memory that is staged, device
+// memory only, or anywhere (its sizes alone are asked for).
+struct KvSource {
+    Stager *stager = nullptr;
+    bool sizes_only = false;
+    template <typename T>
+    T *device(T *p, const char *what) const
+    {
+        require(sizes_only || is_device_pointer(p), what);
+        return p;
+    }
+    template <typename T>
+    const T *in(const T *p, uint64_t count) const
+    {
+        if (!p) return nullptr;
+        return stager ? stager->in(p, count * sizeof(T)) : device(p, "kv tensor in host memory");
+    }
+    // Rows behind the last sequence and between strides stay as they are, so
+    // a staged output takes the caller's contents with it.
+    float *out(float *p, uint64_t count) const
+    {
+        return stager ? stager->inout(p, count * sizeof(float)) : device(p, "kv tensor in host memory");
+    }
+};
+
+k::KvCall kv_call_params(vnpu_stream_t *s, const vnpu_kv_cache_t &c, const int32_t *lengths, const int32_t *seq_start,
+                         uint32_t batch, uint32_t tokens, const KvSource &src)
+{
+    require(c.k && c.v && c.k_scales && c.v_scales && c.table && c.pages && c.kv_heads && c.table_ld,
+            "invalid kv cache");
+    require(c.page_size >= 16 && c.page_size <= 256 && !(c.page_size & (c.page_size - 1)),
+            "kv page_size is 16, 32, 64, 128 or 256");
+    require(c.head_dim && c.head_dim <= 256 && c.head_dim % 16 == 0, "kv head_dim is a multiple of 16 up to 256");
+    require(!((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15), "kv codes are 16-byte aligned");
+    // Pages and positions are int32 on the device, grids 16 bits in y.
+    require(c.pages <= 0x7fffffffu && c.table_ld <= 0x7fffffffu / c.page_size && c.kv_heads <= 65535, "kv cache too large");
+    require(batch && tokens && batch <= (1u << 24) && tokens <= (1u << 28), "invalid kv batch or tokens");
+    require(seq_start || tokens % batch == 0, "kv tokens is a multiple of batch without seq_start");
+    k::KvCall p;
+    p.c.k = src.device(c.k, "the kv cache is device memory");
+    p.c.v = src.device(c.v, "the kv cache is device memory");
+    p.c.ks = src.device(c.k_scales, "the kv cache is device memory");
+    p.c.vs = src.device(c.v_scales, "the kv cache is device memory");
+    p.c.pages = c.pages;
+    p.c.page_size = c.page_size;
+    p.c.log_page = static_cast<uint32_t>(__builtin_ctz(c.page_size));
+    p.c.kv_heads = c.kv_heads;
+    p.c.head_dim = c.head_dim;
+    p.c.table_ld = c.table_ld;
+    p.batch = batch;
+    p.tokens = tokens;
+    p.err = s->err_dev;
+    p.c.table = src.in(c.table, static_cast<uint64_t>(batch) * c.table_ld);
+    p.lengths = src.in(lengths, batch);
+    p.seq_start = src.in(seq_start, batch + 1ull);
+    return p;
+}
+
+k::KvAppend kv_append_params(vnpu_stream_t *s, const vnpu_kv_append_i8_args_t &a, const KvSource &src)
+{
+    require(a.K && a.V && a.past, "invalid kv_append arguments");
+    require(a.rotation <= VNPU_ROTATE_INTERLEAVED, "invalid kv_append rotation");
+    require(!a.Q == !a.Q_out, "kv_append takes Q with Q_out");
+    k::KvAppend p;
+    p.call = kv_call_params(s, a.cache, a.past, a.seq_start, a.batch, a.tokens, src);
+    const uint32_t D = a.cache.head_dim, G = a.cache.kv_heads;
+    p.rotation = a.rotation;
+    p.rope_dim = a.rope_dim ? a.rope_dim : D;
+    require(p.rope_dim <= D && !(p.rope_dim & 1u), "kv rope_dim is even, up to head_dim");
+    p.theta = a.theta_base > 0.0f ? a.theta_base : 10000.0f;
+    p.scaling = a.scaling > 0.0f ? a.scaling : 1.0f;
+    const bool ragged = a.seq_start != nullptr;
+    const KvTensor kt = kv_rows(a.k_batch_stride, a.k_token_stride, a.k_head_stride, G, D, a.batch, a.tokens, ragged, false);
+    const KvTensor vt = kv_rows(a.v_batch_stride, a.v_token_stride, a.v_head_stride, G, D, a.batch, a.tokens, ragged, false);
+    p.k = kt.rows;
+    p.v = vt.rows;
+    if (a.Q) {
+        require(a.heads && a.heads % G == 0 && a.heads <= 65535, "kv heads is a multiple of kv_heads");
+        const KvTensor qt = kv_rows(a.q_batch_stride, a.q_token_stride, a.q_head_stride, a.heads, D, a.batch, a.tokens, ragged, false);
+        const KvTensor ot = kv_rows(a.o_batch_stride, a.o_token_stride, a.o_head_stride, a.heads, D, a.batch, a.tokens, ragged, true);
+        const bool same = a.Q_out == a.Q;
+        require(!same || (qt.rows.batch == ot.rows.batch && qt.rows.token == ot.rows.token && qt.rows.head == ot.rows.head),
+                "kv_append turns Q in place with Q's strides only");
+        p.q = qt.rows;
+        p.o = ot.rows;
+        if (!same || a.rotation != VNPU_ROTATE_NONE) p.heads = a.heads;
+        p.Q_out = src.out(a.Q_out, ot.span);
+        p.Q = same ? p.Q_out : src.in(a.Q, qt.span);
+    }
+    p.K = src.in(a.K, kt.span);
+    p.V = src.in(a.V, vt.span);
+    return p;
+}
+
+k::KvAttn kv_attention_params(vnpu_stream_t *s, const vnpu_kv_attention_i8_args_t &a, const KvSource &src)
+{
+    require(a.Q && a.O && a.kv_len, "invalid kv_attention arguments");
+    k::KvAttn p;
+    p.call = kv_call_params(s, a.cache, a.kv_len, a.seq_start, a.batch, a.tokens, src);
+    const uint32_t D = a.cache.head_dim;
+    require(a.heads && a.heads % a.cache.kv_heads == 0 && a.heads <= 65535, "kv heads is a multiple of kv_heads");
+    const bool ragged = a.seq_start != nullptr;
+    const KvTensor qt = kv_rows(a.q_batch_stride, a.q_token_stride, a.q_head_stride, a.heads, D, a.batch, a.tokens, ragged, false);
+    const KvTensor ot = kv_rows(a.o_batch_stride, a.o_token_stride, a.o_head_stride, a.heads, D, a.batch, a.tokens, ragged, true);
+    const bool same = a.O == a.Q;
+    require(!same || (qt.rows.batch == ot.rows.batch && qt.rows.token == ot.rows.token && qt.rows.head == ot.rows.head),
+            "kv_attention takes O as Q with Q's strides only");
+    p.q = qt.rows;
+    p.o = ot.rows;
+    p.heads = a.heads;
+    const uint32_t capacity = a.cache.table_ld * a.cache.page_size;
+    p.max_tokens = !ragged ? a.tokens / a.batch : a.max_tokens ? std::min(a.max_tokens, a.tokens) : a.tokens;
+    p.max_kv = a.max_kv ? std::min(a.max_kv, capacity) : capacity;
+    p.causal = a.causal != 0;
+    p.scale = a.scale > 0.0f ? a.scale : 1.0f / std::sqrt(static_cast<float>(D));
+    p.cus = s->device ? std::max(1u, s->device->cu_count) : 256;
+    p.O = src.out(a.O, ot.span);
+    p.Q = same ? p.O : src.in(a.Q, qt.span);
+    return p;
+}
+
+// The workspace that the caller gave; null: none given.
+void *kv_given_workspace(const vnpu_kv_attention_i8_args_t &a, size_t need)
+{
+    if (!a.workspace || !need) return nullptr;
+    require(a.workspace_bytes >= need && !(reinterpret_cast<uintptr_t>(a.workspace) & 15) && is_device_pointer(a.workspace),
+            "kv workspace too small, unaligned or in host memory");
+    return a.workspace;
+}
+
+k::KvRead kv_read_params(vnpu_stream_t *s, const vnpu_kv_read_f32_args_t &a, const KvSource &src)
+{
+    require(a.K || a.V, "invalid kv_read arguments");
+    k::KvRead p;
+    p.call = kv_call_params(s, a.cache, a.first, a.seq_start, a.batch, a.tokens, src);
+    const uint32_t D = a.cache.head_dim, G = a.cache.kv_heads;
+    const bool ragged = a.seq_start != nullptr;
+    const KvTensor kt = kv_rows(a.k_batch_stride, a.k_token_stride, a.k_head_stride, G, D, a.batch, a.tokens, ragged, a.K != nullptr);
+    const KvTensor vt = kv_rows(a.v_batch_stride, a.v_token_stride, a.v_head_stride, G, D, a.batch, a.tokens, ragged, a.V != nullptr);
+    p.k = kt.rows;
+    p.v = vt.rows;
+    p.K = a.K ? src.out(a.K, kt.span) : nullptr;
+    p.V = a.V ? src.out(a.V, vt.span) : nullptr;
+    return p;
+}
+
+// What the host knows: lengths are on the GPU, so attention counts max_kv
+// keys for every sequence and token.
+void account_kv(const vnpu_command_t &cmd, uint64_t max_kv, ExecStats &st)
+{
+    if (cmd.opcode == VNPU_OP_KV_APPEND_I8) {
+        const auto &a = cmd.args.kv_append;
+        const uint64_t qn = a.Q ? static_cast<uint64_t>(a.tokens) * a.heads * a.cache.head_dim : 0;
+        const uint64_t kn = static_cast<uint64_t>(a.tokens) * a.cache.kv_heads * a.cache.head_dim;
+        st.bytes_read += (qn + 2 * kn) * 4;
+        st.bytes_written += qn * 4 + 2 * kn;
+        st.flops += (a.rotation ? 3 * (qn + kn) : 0) + 4 * kn;
+    } else if (cmd.opcode == VNPU_OP_KV_ATTENTION_I8) {
+        const auto &a = cmd.args.kv_attention;
+        const uint64_t qn = static_cast<uint64_t>(a.tokens) * a.heads * a.cache.head_dim;
+        st.bytes_read += qn * 4 + 2ull * a.batch * max_kv * a.cache.kv_heads * a.cache.head_dim;
+        st.bytes_written += qn * 4;
+        st.flops += 4 * qn * max_kv;
+    } else {
+        const auto &a = cmd.args.kv_read;
+        const uint64_t kn = static_cast<uint64_t>(a.tokens) * a.cache.kv_heads * a.cache.head_dim;
+        const uint64_t sides = (a.K ? 1 : 0) + (a.V ? 1 : 0);
+        st.bytes_read += sides * kn;
+        st.bytes_written += sides * kn * 4;
+        st.flops += sides * kn;
+    }
+}
+
+void exec_kv(vnpu_stream_t *s, const vnpu_command_t &cmd, ExecStats &st)
+{
+    Stager sg(s->hip, s);
+    uint64_t max_kv = 0;
+    if (cmd.opcode == VNPU_OP_KV_APPEND_I8) {
+        k::kv_append(s->hip, kv_append_params(s, cmd.args.kv_append, {&sg}));
+    } else if (cmd.opcode == VNPU_OP_KV_ATTENTION_I8) {
+        const auto &a = cmd.args.kv_attention;
+        const k::KvAttn p = kv_attention_params(s, a, {&sg});
+        const size_t need = k::kv_attention_ws_bytes(p);
+        void *ws = kv_given_workspace(a, need);
+        if (!ws) ws = s->ensure_workspace(need);
+        k::kv_attention(s->hip, p, ws);
+        max_kv = p.max_kv;
+    } else {
+        k::kv_read(s->hip, kv_read_params(s, cmd.args.kv_read, {&sg}));
+    }
+    VNPU_HIP(hipGetLastError());
+    sg.finish();
+    account_kv(cmd, max_kv, st);
+}
+
 void exec_copy(vnpu_stream_t *s, const vnpu_copy_args_t &a, ExecStats &st)
 {
     // execute_copy (scheduler.cpp:643-651): memmove semantics for host copies
@@ -1073,6 +1301,40 @@ void enqueue_attention_noalloc(vnpu_stream_t *s, const vnpu_attention_f32_args_t
     k::attention(s->hip, p, ws);
     VNPU_HIP(hipGetLastError());
     account_attention(a, st);
+}
+
+uint64_t kv_attention_workspace(const vnpu_device_t *dev, const vnpu_kv_attention_i8_args_t &a)
+{
+    vnpu_stream_t on;   // carries the device only
+    on.device = const_cast<vnpu_device_t *>(dev);
+    return k::kv_attention_ws_bytes(kv_attention_params(&on, a, {nullptr, true}));
+}
+
+void enqueue_kv_noalloc(vnpu_stream_t *s, const vnpu_command_t *commands, uint64_t count, ExecStats &st)
+{
+    for (int pass = 0; pass < 2; ++pass)   // all are checked before one is enqueued
+        for (uint64_t i = 0; i < count; ++i) {
+            const vnpu_command_t &cmd = commands[i];
+            require(is_kv_opcode(cmd.opcode), "only KV commands run without allocation");
+            uint64_t max_kv = 0;
+            if (cmd.opcode == VNPU_OP_KV_APPEND_I8) {
+                const k::KvAppend p = kv_append_params(s, cmd.args.kv_append, {});
+                if (pass) k::kv_append(s->hip, p);
+            } else if (cmd.opcode == VNPU_OP_KV_ATTENTION_I8) {
+                const k::KvAttn p = kv_attention_params(s, cmd.args.kv_attention, {});
+                const size_t need = k::kv_attention_ws_bytes(p);
+                void *ws = kv_given_workspace(cmd.args.kv_attention, need);
+                require(ws || !need, "this kv_attention needs a workspace");
+                if (pass) k::kv_attention(s->hip, p, ws);
+                max_kv = p.max_kv;
+            } else {
+                const k::KvRead p = kv_read_params(s, cmd.args.kv_read, {});
+                if (pass) k::kv_read(s->hip, p);
+            }
+            if (!pass) continue;
+            VNPU_HIP(hipGetLastError());
+            account_kv(cmd, max_kv, st);
+        }
 }
 
 void execute_command(vnpu_device_t *dev, vnpu_stream_t *s, const vnpu_command_t &cmd,
@@ -1146,6 +1408,11 @@ void execute_command(vnpu_device_t *dev, vnpu_stream_t *s, const vnpu_command_t 
         return;
     case VNPU_OP_MEMSET:
         exec_memset(s, cmd.args.memset, st);
+        return;
+    case VNPU_OP_KV_APPEND_I8:
+    case VNPU_OP_KV_ATTENTION_I8:
+    case VNPU_OP_KV_READ_F32:
+        exec_kv(s, cmd, st);
         return;
     default:
         throw ArgError("invalid opcode");
@@ -1286,6 +1553,22 @@ extern "C" VNPU_API int32_t VNPU_CALL vnpu_debug_route(const vnpu_command_t *cmd
             p.own_ws = !(mode & 2u);
             p.Q = a.Q; p.K = a.K; p.V = a.V; p.mask = a.mask; p.O = a.O;
             std::snprintf(out, size, "%s ws=%zu", vnpu::k::attention_route(p), vnpu::k::attention_ws_bytes(p));
+            return VNPU_OK;
+        }
+        if (vnpu::is_kv_opcode(cmd->opcode)) {
+            vnpu_stream_t on;   // of no device
+            const vnpu::KvSource sizes{nullptr, true};
+            if (cmd->opcode == VNPU_OP_KV_ATTENTION_I8) {
+                const vnpu::k::KvAttn p = vnpu::kv_attention_params(&on, cmd->args.kv_attention, sizes);
+                std::snprintf(out, size, "%s ws=%zu", vnpu::k::kv_attention_route(p).c_str(),
+                              vnpu::k::kv_attention_ws_bytes(p));
+            } else if (cmd->opcode == VNPU_OP_KV_APPEND_I8) {
+                (void)vnpu::kv_append_params(&on, cmd->args.kv_append, sizes);
+                std::snprintf(out, size, "append");
+            } else {
+                (void)vnpu::kv_read_params(&on, cmd->args.kv_read, sizes);
+                std::snprintf(out, size, "read");
+            }
             return VNPU_OK;
         }
         if (cmd->opcode == VNPU_OP_MATMUL_F32) {   // no tile mask, no requested K depth

@@ -7,6 +7,7 @@
 
 #include <hip/hip_runtime.h>
 #include <cstdint>
+#include <string>
 
 namespace vnpu {
 namespace k {
@@ -242,6 +243,59 @@ void attention_exact_decode(hipStream_t s, const Attn &a, float *ws);
 constexpr size_t kAttnScratchBytes = 64ull << 20;
 void attention_scratch_setup(int hip_device);
 float *attention_scratch(int hip_device);
+
+// ---- paged int8 KV cache (kv_cache.hip, kv_attention.hip) ----
+// Rows of a call's tokens: element d of head h of sequence b's token i is at
+// base(b) + i * token + h * head + d, base(b) = b * batch, or seq_start[b] *
+// token where seq_start is given.
+struct KvRows {
+    uint64_t batch = 0, token = 0, head = 0;
+};
+struct KvCache {
+    int8_t *k = nullptr, *v = nullptr;
+    float *ks = nullptr, *vs = nullptr;
+    const int32_t *table = nullptr;
+    uint32_t pages = 0, page_size = 0, log_page = 0, kv_heads = 0, head_dim = 0, table_ld = 0;
+};
+// What every KV command has: lengths[b] is past, kv_len or first (null: 0).
+// A kernel that meets a length or page out of range leaves it and stores 2
+// into *err (host-coherent, read at the stream's sync).
+struct KvCall {
+    KvCache c;
+    const int32_t *lengths = nullptr, *seq_start = nullptr;
+    uint32_t batch = 0, tokens = 0;
+    uint32_t *err = nullptr;
+};
+struct KvAppend {
+    KvCall call;
+    const float *Q = nullptr, *K = nullptr, *V = nullptr;
+    float *Q_out = nullptr;
+    uint32_t heads = 0;            // 0: no Q
+    KvRows q, o, k, v;
+    uint32_t rotation = 0, rope_dim = 0;
+    float theta = 10000.0f, scaling = 1.0f;
+};
+struct KvAttn {
+    KvCall call;
+    const float *Q = nullptr;
+    float *O = nullptr;
+    uint32_t heads = 0, max_tokens = 0, max_kv = 0, causal = 0;
+    KvRows q, o;
+    float scale = 1.0f;
+    uint32_t cus = 256;
+};
+struct KvRead {
+    KvCall call;
+    float *K = nullptr, *V = nullptr;
+    KvRows k, v;
+};
+void kv_append(hipStream_t s, const KvAppend &p);
+void kv_read(hipStream_t s, const KvRead &p);
+// ws holds kv_attention_ws_bytes(p) bytes (0: none is used).
+size_t kv_attention_ws_bytes(const KvAttn &p);
+void kv_attention(hipStream_t s, const KvAttn &p, void *ws);
+// Its kernels and how the work is split, by name.
+std::string kv_attention_route(const KvAttn &p);
 
 // ---- fills (ops.hip) ----
 void fill_u8(hipStream_t s, void *dst, uint8_t value, uint64_t bytes);

@@ -1,0 +1,342 @@
+// kv_cache.hip - KV_APPEND_I8 and KV_READ_F32: what writes the paged int8 KV
+// cache and what reads it back, on gfx950.
+//
+// Append, for new token i of sequence b at position p = past[b] + i:
+//   angle_j = p * scaling * theta^(-2j / R), j < R / 2 (R = rope_dim)
+//   (x, y) -> (f32(x cos - y sin), f32(x sin + y cos)), cos and sin in f32,
+//   the products exact in f64, so each result is rounded once;
+//   per (page, kv head): a = max |x| of the page's new tokens,
+//   s = max(n0 ? s0 : 0, f32(a / 127)) for n0 tokens kept from before,
+//   kept codes -> round(code * f32(s0 / s)) where s > s0,
+//   new codes = round(x * f32(1 / s)), half away from zero, in +-127.
+// One page and kv head is one workgroup: it alone reads and writes that
+// page's codes and scale, so nothing is atomic and results do not depend on
+// order.  The new tokens' f32 values are read once and stay in registers
+// between the largest magnitude and the codes.
+#include "device_math.hpp"
+#include "kv_common.hpp"
+
+#include <cmath>
+#include <map>
+#include <mutex>
+#include <tuple>
+
+namespace vnpu {
+namespace k {
+namespace {
+
+// Turns (angle / 2 pi) per position of each pair, computed on the host.
+struct Rates {
+    double turns[128];
+};
+
+// cos and sin of 2 pi t.  t less its nearest quarter leaves |x| <= pi / 4, where
+// the Taylor series to x^14 and x^13 are within 2e-14: the f32 results are the
+// correctly rounded ones but for about one in 10^6.  f64 because t is
+// exact to 2^-53 of itself only there: position 100000 in f32 would be off by
+// 0.006 rad.
+__device__ __forceinline__ void cos_sin_turns(double t, float &c, float &s)
+{
+    const double quarter = rint(4.0 * t);
+    const double x = 6.283185307179586476925 * fma(-0.25, quarter, t);
+    const double z = x * x;
+    double pc = -1.0 / 87178291200.0, ps = 1.0 / 6227020800.0;
+    pc = fma(pc, z, 1.0 / 479001600.0);
+    ps = fma(ps, z, -1.0 / 39916800.0);
+    pc = fma(pc, z, -1.0 / 3628800.0);
+    ps = fma(ps, z, 1.0 / 362880.0);
+    pc = fma(pc, z, 1.0 / 40320.0);
+    ps = fma(ps, z, -1.0 / 5040.0);
+    pc = fma(pc, z, -1.0 / 720.0);
+    ps = fma(ps, z, 1.0 / 120.0);
+    pc = fma(pc, z, 1.0 / 24.0);
+    ps = fma(ps, z, -1.0 / 6.0);
+    pc = fma(pc, z, -0.5);
+    const double cx = fma(pc, z, 1.0), sx = fma(ps * z, x, x);
+    const int q = static_cast<int>(static_cast<long long>(quarter) & 3);
+    const double a = q & 1 ? sx : cx, b = q & 1 ? cx : sx;
+    c = static_cast<float>(q == 1 || q == 2 ? -a : a);
+    s = static_cast<float>(q >= 2 ? -b : b);
+}
+
+__device__ __forceinline__ float2 turned(float2 x, float c, float s)
+{
+    const double a = x.x, b = x.y, cd = c, sd = s;
+    return make_float2(static_cast<float>(fma(a, cd, -(b * sd))), static_cast<float>(fma(a, sd, b * cd)));
+}
+
+// Round half away from zero into +-127.
+__device__ __forceinline__ int code_of(float x, float by)
+{
+    return static_cast<int>(fminf(fmaxf(roundf(__fmul_rn(x, by)), -127.0f), 127.0f));
+}
+__device__ __forceinline__ uint32_t rescaled4(uint32_t codes, float ratio)
+{
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r |= (static_cast<uint32_t>(code_of(static_cast<float>(static_cast<int8_t>(codes >> (8 * i))), ratio)) & 255u) << (8 * i);
+    return r;
+}
+
+// Largest bits of |x| over the workgroup: orders magnitudes, infinity and NaN.
+template <int T>
+__device__ __forceinline__ uint32_t block_largest(uint32_t v, uint32_t *red)
+{
+    for (int o = 32; o; o >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o)));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    uint32_t r = red[0];
+    for (int w = 1; w < T / 64; ++w) r = max(r, red[w]);
+    return r;
+}
+
+struct PageScale {
+    float scale, ratio, inv;
+};
+__device__ __forceinline__ PageScale page_scale(uint32_t largest, bool kept, float before)
+{
+    float s = __fdiv_rn(__uint_as_float(largest), 127.0f);
+    if (s < 1.17549435e-38f) s = 0.0f;   // no reciprocal in f32
+    if (largest >= 0x7f800000u) s = __uint_as_float(0x7fc00000u);
+    PageScale r;
+    r.scale = !kept ? s : before != before || s != s ? __uint_as_float(0x7fc00000u) : fmaxf(before, s);
+    r.ratio = kept && r.scale > before ? __fdiv_rn(before, r.scale) : 1.0f;
+    r.inv = r.scale > 0.0f ? __fdiv_rn(1.0f, r.scale) : 0.0f;
+    return r;
+}
+
+// Thread e of m * D / 2 pairs has pair e % (D / 2) of token e / (D / 2); pairs
+// per thread: PAIRS.  Codes go through LDS (dynamic, page_size * D bytes) so
+// that the cache is written 16 bytes at a time.
+template <int T, int PAIRS>
+__global__ __launch_bounds__(T) void kv_append_kernel(KvAppend p, Rates rates, uint32_t half_magic)
+{
+    extern __shared__ __align__(16) int8_t tile[];
+    __shared__ uint32_t red[2][T / 64];
+    const KvCall &c = p.call;
+    const uint32_t h = blockIdx.y, tid = threadIdx.x;
+    if (blockIdx.x == 0 && h == 0) kv::check_all(c, true, kv::capacity(c));
+    uint32_t b;
+    kv::Piece pc;
+    if (!kv::find_piece(c, blockIdx.x, b, pc)) return;
+    const uint32_t D = c.c.head_dim, half = D / 2, ps = c.c.page_size, turns = p.rotation ? p.rope_dim / 2 : 0;
+    const uint32_t pairs = pc.m * half;
+    const uint64_t position = static_cast<uint64_t>(c.lengths[b]) + pc.first;
+    const uint64_t unit = static_cast<uint64_t>(pc.page) * c.c.kv_heads + h;
+    const float *K = p.K + kv::rows_base(c, p.k, b, pc.seq) + pc.first * p.k.token + h * p.k.head;
+    const float *V = p.V + kv::rows_base(c, p.v, b, pc.seq) + pc.first * p.v.token + h * p.v.head;
+    const float k_before = c.c.ks[unit], v_before = c.c.vs[unit];
+    const uint32_t group = p.heads / c.c.kv_heads;
+
+    float2 kx[PAIRS], vx[PAIRS];
+    uint32_t k_most = 0, v_most = 0;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+        const uint32_t e = tid + i * T;
+        kx[i] = vx[i] = make_float2(0.0f, 0.0f);
+        if (e >= pairs) continue;
+        const uint32_t t = __umulhi(e, half_magic), j = e - t * half;
+        const bool turn = j < turns;
+        const uint32_t d0 = turn && p.rotation == 1 ? j : 2 * j, d1 = turn && p.rotation == 1 ? j + turns : 2 * j + 1;
+        const float *kr = K + t * p.k.token, *vr = V + t * p.v.token;
+        kx[i] = make_float2(kr[d0], kr[d1]);
+        vx[i] = make_float2(vr[2 * j], vr[2 * j + 1]);
+        float cs = 1.0f, sn = 0.0f;
+        if (turn) {
+            cos_sin_turns(static_cast<double>(position + t) * rates.turns[j], cs, sn);
+            kx[i] = turned(kx[i], cs, sn);
+        }
+        k_most = max(k_most, max(__float_as_uint(kx[i].x) & 0x7fffffffu, __float_as_uint(kx[i].y) & 0x7fffffffu));
+        v_most = max(v_most, max(__float_as_uint(vx[i].x) & 0x7fffffffu, __float_as_uint(vx[i].y) & 0x7fffffffu));
+        for (uint32_t g = 0; g < group; ++g) {
+            const uint32_t qh = h * group + g;
+            const float *qr = p.Q + kv::rows_base(c, p.q, b, pc.seq) + (pc.first + t) * p.q.token + qh * p.q.head;
+            float *qo = p.Q_out + kv::rows_base(c, p.o, b, pc.seq) + (pc.first + t) * p.o.token + qh * p.o.head;
+            float2 x = make_float2(qr[d0], qr[d1]);
+            if (turn) x = turned(x, cs, sn);
+            qo[d0] = x.x;
+            qo[d1] = x.y;
+        }
+    }
+    k_most = block_largest<T>(k_most, red[0]);
+    v_most = block_largest<T>(v_most, red[1]);
+    const bool kept = pc.slot > 0;
+    const PageScale ks = page_scale(k_most, kept, k_before), vs = page_scale(v_most, kept, v_before);
+
+    // K: [slot][D], the new tokens' bytes are one run.
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+        const uint32_t e = tid + i * T;
+        if (e >= pairs) continue;
+        const uint32_t t = __umulhi(e, half_magic), j = e - t * half;
+        const bool first_half = j < turns && p.rotation == 1;
+        tile[t * D + (first_half ? j : 2 * j)] = static_cast<int8_t>(code_of(kx[i].x, ks.inv));
+        tile[t * D + (first_half ? j + turns : 2 * j + 1)] = static_cast<int8_t>(code_of(kx[i].y, ks.inv));
+    }
+    __syncthreads();
+    uint4 *kp = reinterpret_cast<uint4 *>(c.c.k + unit * ps * D);
+    const uint4 *tp = reinterpret_cast<const uint4 *>(tile);
+    const uint32_t row16 = D / 16;
+    const uint32_t k_bytes16 = ks.scale == ks.scale ? pc.m * row16 : 0;   // under a NaN scale the codes stay
+    for (uint32_t e = tid; e < k_bytes16; e += T) kp[pc.slot * row16 + e] = tp[e];
+    if (ks.ratio != 1.0f)
+        for (uint32_t e = tid; e < pc.slot * row16; e += T) {
+            const uint4 o = kp[e];
+            kp[e] = make_uint4(rescaled4(o.x, ks.ratio), rescaled4(o.y, ks.ratio), rescaled4(o.z, ks.ratio), rescaled4(o.w, ks.ratio));
+        }
+    __syncthreads();
+
+    // V: [D][slot], rows of page_size bytes of which the new tokens are a part.
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+        const uint32_t e = tid + i * T;
+        if (e >= pairs) continue;
+        const uint32_t t = __umulhi(e, half_magic), j = e - t * half;
+        tile[2 * j * ps + pc.slot + t] = static_cast<int8_t>(code_of(vx[i].x, vs.inv));
+        tile[(2 * j + 1) * ps + pc.slot + t] = static_cast<int8_t>(code_of(vx[i].y, vs.inv));
+    }
+    __syncthreads();
+    uint4 *vp = reinterpret_cast<uint4 *>(c.c.v + unit * ps * D);
+    const uint32_t log16 = c.c.log_page - 4, end = pc.slot + pc.m;
+    const uint32_t from16 = vs.ratio != 1.0f ? 0 : pc.slot / 16, to16 = (end + 15) / 16, n16 = to16 - from16;
+    const uint32_t v_bytes16 = vs.scale == vs.scale ? D * n16 : 0;
+    for (uint32_t e = tid; e < v_bytes16; e += T) {
+        const uint32_t d = e / n16, s16 = from16 + e % n16, s0 = 16 * s16;
+        const uint32_t at = (d << log16) + s16;
+        const uint4 fresh = tp[at];
+        if (s0 >= pc.slot && s0 + 16 <= end) {
+            vp[at] = fresh;
+            continue;
+        }
+        const uint4 old = vp[at];
+        const uint32_t o4[4] = {old.x, old.y, old.z, old.w}, f4[4] = {fresh.x, fresh.y, fresh.z, fresh.w};
+        uint32_t r4[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t moved = vs.ratio != 1.0f ? rescaled4(o4[w], vs.ratio) : o4[w];
+            r4[w] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t slot = s0 + 4 * w + i, m = 255u << (8 * i);
+                r4[w] |= (slot < pc.slot ? moved : slot < end ? f4[w] : o4[w]) & m;
+            }
+        }
+        vp[at] = make_uint4(r4[0], r4[1], r4[2], r4[3]);
+    }
+    if (tid == 0) {
+        c.c.ks[unit] = ks.scale;
+        c.c.vs[unit] = vs.scale;
+    }
+}
+
+constexpr int kReadThreads = 256;
+
+// One page and kv head to f32 rows.  V's codes pass through LDS (dynamic,
+// page_size rows of D + 4 bytes) to turn [D][slot] into rows.
+__global__ __launch_bounds__(kReadThreads) void kv_read_kernel(KvRead p)
+{
+    extern __shared__ __align__(16) int8_t tile[];
+    const KvCall &c = p.call;
+    const uint32_t h = blockIdx.y, tid = threadIdx.x;
+    if (blockIdx.x == 0 && h == 0) kv::check_all(c, true, kv::capacity(c));
+    uint32_t b;
+    kv::Piece pc;
+    if (!kv::find_piece(c, blockIdx.x, b, pc)) return;
+    const uint32_t D = c.c.head_dim, ps = c.c.page_size, quads = D / 4;
+    const uint64_t unit = static_cast<uint64_t>(pc.page) * c.c.kv_heads + h;
+    if (p.K) {
+        const float scale = c.c.ks[unit];
+        const uint32_t *codes = reinterpret_cast<const uint32_t *>(c.c.k + (unit * ps + pc.slot) * D);
+        float *out = p.K + kv::rows_base(c, p.k, b, pc.seq) + pc.first * p.k.token + h * p.k.head;
+        for (uint32_t e = tid; e < pc.m * quads; e += kReadThreads) {
+            const uint32_t t = e / quads, d = 4 * (e % quads), w = codes[e];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                out[t * p.k.token + d + i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i))) * scale;
+        }
+    }
+    if (p.V) {
+        const float scale = c.c.vs[unit];
+        const uint32_t *codes = reinterpret_cast<const uint32_t *>(c.c.v + unit * ps * D);
+        const uint32_t from4 = pc.slot / 4, n4 = (pc.slot + pc.m + 3) / 4 - from4, row = D + 4;
+        for (uint32_t e = tid; e < D * n4; e += kReadThreads) {
+            const uint32_t d = e / n4, s4 = from4 + e % n4, w = codes[d * (ps / 4) + s4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tile[(4 * s4 + i) * row + d] = static_cast<int8_t>(w >> (8 * i));
+        }
+        __syncthreads();
+        float *out = p.V + kv::rows_base(c, p.v, b, pc.seq) + pc.first * p.v.token + h * p.v.head;
+        for (uint32_t e = tid; e < pc.m * quads; e += kReadThreads) {
+            const uint32_t t = e / quads, d = 4 * (e % quads);
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + (pc.slot + t) * row + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                out[t * p.v.token + d + i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i))) * scale;
+        }
+    }
+}
+
+// Kept by value for a (theta, rope_dim, scaling): 128 powers are microseconds on the host.
+Rates rates_of(float theta, uint32_t dim, float scaling)
+{
+    static std::mutex mutex;
+    static auto *known = new std::map<std::tuple<float, uint32_t, float>, Rates>();
+    std::lock_guard<std::mutex> lock(mutex);
+    const auto key = std::make_tuple(theta, dim, scaling);
+    auto it = known->find(key);
+    if (it != known->end()) return it->second;
+    Rates r{};
+    for (uint32_t j = 0; j < dim / 2; ++j)
+        r.turns[j] = static_cast<double>(scaling) * std::pow(static_cast<double>(theta), -2.0 * j / dim) / (2.0 * M_PI);
+    if (known->size() >= 64) known->clear();
+    known->emplace(key, r);
+    return r;
+}
+
+}  // namespace
+
+namespace {
+// Pages of 256 tokens and heads of 256 take more LDS than a kernel has unasked.
+template <typename Kernel>
+void allow_lds(Kernel kernel, size_t bytes)
+{
+    if (bytes > 60 * 1024)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                  static_cast<int>(bytes));
+}
+
+template <int T, int PAIRS>
+void launch_append(hipStream_t s, const KvAppend &p, const Rates &rates, uint32_t magic)
+{
+    const size_t lds = static_cast<size_t>(p.call.c.page_size) * p.call.c.head_dim;
+    allow_lds(kv_append_kernel<T, PAIRS>, lds);
+    kv_append_kernel<T, PAIRS><<<dim3(kv::unit_count(p.call), p.call.c.kv_heads), T, lds, s>>>(p, rates, magic);
+}
+}  // namespace
+
+void kv_append(hipStream_t s, const KvAppend &p)
+{
+    const KvCall &c = p.call;
+    const Rates rates = p.rotation ? rates_of(p.theta, p.rope_dim, p.scaling) : Rates{};
+    const uint32_t half = c.c.head_dim / 2;
+    const uint32_t magic = static_cast<uint32_t>((0x100000000ull + half - 1) / half);   // exact below 2^16
+    // Pairs of a page's new tokens: at most page_size * D / 2 = 32768.
+    const uint32_t most = std::min(c.seq_start ? c.tokens : c.tokens / c.batch, c.c.page_size) * half;
+    if (most <= 256) launch_append<256, 1>(s, p, rates, magic);
+    else if (most <= 1024) launch_append<256, 4>(s, p, rates, magic);
+    else if (most <= 4096) launch_append<256, 16>(s, p, rates, magic);
+    else if (most <= 16384) launch_append<1024, 16>(s, p, rates, magic);
+    else launch_append<1024, 32>(s, p, rates, magic);
+}
+
+void kv_read(hipStream_t s, const KvRead &p)
+{
+    const KvCall &c = p.call;
+    const size_t lds = p.V ? static_cast<size_t>(c.c.page_size) * (c.c.head_dim + 4) : 0;
+    allow_lds(kv_read_kernel, lds);
+    kv_read_kernel<<<dim3(kv::unit_count(c), c.c.kv_heads), kReadThreads, lds, s>>>(p);
+}
+
+}  // namespace k
+}  // namespace vnpu

@@ -263,6 +263,8 @@ VNPU_API const char *VNPU_CALL vnpu_opcode_name(uint32_t opcode)
                                   "ROPE_F32", "SWIGLU_F32", "GELU_F32", "ADD_F32", "MUL_F32",
                                   "ATTENTION_F32", "QUANTIZE_I8", "PACK_WEIGHTS_I8",
                                   "MTP_HEAD_F32", "COPY", "MEMSET", "BARRIER"};
+    static const char *kv[] = {"KV_APPEND_I8", "KV_ATTENTION_I8", "KV_READ_F32"};
+    if (is_kv_opcode(opcode)) return kv[opcode - VNPU_OP_KV_APPEND_I8];
     return opcode < sizeof(names) / sizeof(names[0]) ? names[opcode] : "UNKNOWN";
 }
 
@@ -812,6 +814,52 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_attention_f32_noalloc(vnpu_stream_t *strea
     }
 }
 
+VNPU_API uint64_t VNPU_CALL vnpu_kv_attention_workspace(const vnpu_device_t *device,
+                                                        const vnpu_kv_attention_i8_args_t *args)
+{
+    if (!device || !args) return 0;
+    try {
+        return kv_attention_workspace(device, *args);
+    } catch (const std::exception &e) {
+        debug_log("vnpu_kv_attention_workspace: %s", e.what());
+    } catch (...) {
+    }
+    return 0;
+}
+
+// KV_* commands for callers that cannot allocate (graph capture, serving
+// loops): checked first, then enqueued; nothing else touches the stream.
+VNPU_API vnpu_status_t VNPU_CALL vnpu_kv_enqueue_noalloc(vnpu_stream_t *stream, const vnpu_command_t *commands,
+                                                         uint64_t count)
+{
+    if (!stream || (!commands && count)) return VNPU_ERR_INVALID_ARGUMENT;
+    vnpu_device_t *d = stream->device;
+    try {
+        ExecStats st;
+        std::lock_guard<std::mutex> lock(stream->mutex);
+        VNPU_HIP(hipSetDevice(d->hip_device));
+        enqueue_kv_noalloc(stream, commands, count, st);
+        d->bytes_read.fetch_add(st.bytes_read);
+        d->bytes_written.fetch_add(st.bytes_written);
+        d->flops.fetch_add(st.flops);
+        if (count) d->last_opcode.store(commands[count - 1].opcode);
+        return VNPU_OK;
+    } catch (const ArgError &e) {
+        debug_log("vnpu_kv_enqueue_noalloc: %s", e.what());
+        return VNPU_ERR_INVALID_ARGUMENT;
+    } catch (const std::exception &e) {
+        debug_log("vnpu_kv_enqueue_noalloc: %s", e.what());
+        (void)hipGetLastError();
+        const uint32_t code = static_cast<uint32_t>(-VNPU_ERR_INTERNAL);
+        d->error.store(code);
+        d->regs[VNPU_REG_ERROR / 4].store(code);
+        stream->last_error.store(code);
+        return VNPU_ERR_INTERNAL;
+    } catch (...) {
+        return VNPU_ERR_INTERNAL;
+    }
+}
+
 VNPU_API vnpu_status_t VNPU_CALL vnpu_stream_sync(vnpu_stream_t *stream)
 {
     if (!stream) return VNPU_ERR_INVALID_ARGUMENT;
@@ -833,10 +881,11 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_stream_sync(vnpu_stream_t *stream)
         d->error.store(code);
         d->regs[VNPU_REG_ERROR / 4].store(code);
     } else if (stream->err_host && __atomic_exchange_n(stream->err_host, 0u, __ATOMIC_ACQ_REL) != 0) {
-        // A kernel's bounded wait gave up (its output is not valid): a
-        // failed command, sticky on this stream as in the reference
-        // (runtime.cpp:1248-1254, 1281-1289).
-        debug_log("vnpu_stream_sync: a kernel's bounded wait gave up; its output is invalid");
+        // A kernel's bounded wait gave up, or a KV command met a length or page
+        // out of range (its output is not valid): a failed command, sticky on
+        // this stream as in the reference (runtime.cpp:1248-1254, 1281-1289).
+        debug_log("vnpu_stream_sync: a kernel's bounded wait gave up, or a KV length or page was out of range; "
+                  "its output is invalid");
         const uint32_t code = static_cast<uint32_t>(-VNPU_ERR_INTERNAL);
         stream->last_error.store(code);
         d->error.store(code);
@@ -981,7 +1030,7 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_stream_submit(vnpu_stream_t *stream,
             }
             ExecStats st;
             vnpu_status_t rc = VNPU_OK;
-            if (cmd.opcode >= VNPU_OP_COUNT) {
+            if (cmd.opcode >= VNPU_OP_COUNT && !is_kv_opcode(cmd.opcode)) {
                 rc = VNPU_ERR_INVALID_COMMAND;
             } else {
                 try {
@@ -1210,6 +1259,9 @@ VNPU_SYNC_WRAPPER(vnpu_add_f32, VNPU_OP_ADD_F32, binary, vnpu_binary_f32_args_t)
 VNPU_SYNC_WRAPPER(vnpu_mul_f32, VNPU_OP_MUL_F32, binary, vnpu_binary_f32_args_t)
 VNPU_SYNC_WRAPPER(vnpu_attention_f32, VNPU_OP_ATTENTION_F32, attention, vnpu_attention_f32_args_t)
 VNPU_SYNC_WRAPPER(vnpu_mtp_head_f32, VNPU_OP_MTP_HEAD_F32, mtp_head, vnpu_mtp_head_f32_args_t)
+VNPU_SYNC_WRAPPER(vnpu_kv_append_i8, VNPU_OP_KV_APPEND_I8, kv_append, vnpu_kv_append_i8_args_t)
+VNPU_SYNC_WRAPPER(vnpu_kv_attention_i8, VNPU_OP_KV_ATTENTION_I8, kv_attention, vnpu_kv_attention_i8_args_t)
+VNPU_SYNC_WRAPPER(vnpu_kv_read_f32, VNPU_OP_KV_READ_F32, kv_read, vnpu_kv_read_f32_args_t)
 
 #undef VNPU_SYNC_WRAPPER
 
@@ -1238,7 +1290,8 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_trace_get_summary(const vnpu_device_t *dev
     tr.resolve();
     std::memset(summary, 0, sizeof(*summary));
     std::lock_guard<std::mutex> lock(tr.mutex);
-    uint64_t per_op[VNPU_OP_COUNT] = {};
+    constexpr uint32_t kOps = VNPU_OP_KV_READ_F32 + 1;
+    uint64_t per_op[kOps] = {};
     for (const auto &r : tr.records) {
         summary->events++;
         summary->total_time_ns += r.gpu_ns;
@@ -1250,7 +1303,7 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_trace_get_summary(const vnpu_device_t *dev
         summary->bytes_read += r.bytes_read;
         summary->bytes_written += r.bytes_written;
         summary->flops += r.flops;
-        if (r.opcode < VNPU_OP_COUNT) per_op[r.opcode] += r.gpu_ns;
+        if (r.opcode < kOps) per_op[r.opcode] += r.gpu_ns;
     }
     if (summary->total_time_ns) {
         const double s = static_cast<double>(summary->total_time_ns) * 1e-9;
@@ -1258,7 +1311,7 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_trace_get_summary(const vnpu_device_t *dev
         summary->achieved_gbytes_s =
             static_cast<double>(summary->bytes_read + summary->bytes_written) / s * 1e-9;
     }
-    for (uint32_t op = 0; op < VNPU_OP_COUNT; ++op)
+    for (uint32_t op = 0; op < kOps; ++op)
         if (per_op[op] > summary->hot_time_ns) {
             summary->hot_time_ns = per_op[op];
             summary->hot_opcode = op;

@@ -248,6 +248,12 @@ void execute_command(vnpu_device_t *dev, vnpu_stream_t *s, const vnpu_command_t 
 // nothing.  Throws ArgError for invalid arguments, host pointers or a
 // scratch need above k::kAttnScratchBytes.
 void enqueue_attention_noalloc(vnpu_stream_t *s, const vnpu_attention_f32_args_t &a, ExecStats &st);
+// KV_* commands without allocation (vnpu_kv_enqueue_noalloc): check every
+// command, then enqueue all.  Throws ArgError with nothing enqueued.
+void enqueue_kv_noalloc(vnpu_stream_t *s, const vnpu_command_t *commands, uint64_t count, ExecStats &st);
+// Bytes of workspace of a KV_ATTENTION_I8 call; throws ArgError where it is refused.
+uint64_t kv_attention_workspace(const vnpu_device_t *dev, const vnpu_kv_attention_i8_args_t &a);
+inline bool is_kv_opcode(uint32_t op) { return op >= VNPU_OP_KV_APPEND_I8 && op <= VNPU_OP_KV_READ_F32; }
 // Pack int8 weights (synchronous); B and tile_mask may be host or device
 // pointers.  A non-null tile_mask ([ceil(K/64)][mask_ld] bytes; mask_ld 0 =
 // ceil(N/64)) packs the 64 x 64 tiles whose byte is zero as zeros.

@@ -39,9 +39,11 @@ OP_NOP, OP_MATMUL_F32, OP_MATMUL_I8, OP_RMSNORM_F32, OP_SOFTMAX_F32 = 0, 1, 2, 3
 OP_ROPE_F32, OP_SWIGLU_F32, OP_GELU_F32, OP_ADD_F32, OP_MUL_F32 = 5, 6, 7, 8, 9
 OP_ATTENTION_F32, OP_QUANTIZE_I8, OP_PACK_WEIGHTS_I8, OP_MTP_HEAD_F32 = 10, 11, 12, 13
 OP_COPY, OP_MEMSET, OP_BARRIER, OP_COUNT = 14, 15, 16, 17
+OP_KV_APPEND_I8, OP_KV_ATTENTION_I8, OP_KV_READ_F32 = 64, 65, 66   # MI355X additive extension
 
 UNIT_AUTO, UNIT_VOODOO, UNIT_WILDCAT, UNIT_CELL, UNIT_GPU = 0, 1, 2, 3, 16
 EPI_NONE, EPI_RELU, EPI_SILU, EPI_GELU_TANH, EPI_GELU_ERF = 0, 1, 2, 3, 4
+ROTATE_NONE, ROTATE_HALF, ROTATE_INTERLEAVED = 0, 1, 2
 QUANT_PER_ROW, QUANT_PER_COLUMN, QUANT_PER_TENSOR = 0, 1, 2
 COPY_H2H, COPY_H2D, COPY_D2H, COPY_D2D = 0, 1, 2, 3
 
@@ -236,13 +238,46 @@ class MemsetArgs(C.Structure):
                 ("reserved0", C.c_uint32)]
 
 
+def _strides(*prefixes):
+    return [(f"{p}_{n}_stride", C.c_uint32) for p in prefixes for n in ("batch", "token", "head")]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("table", C.c_void_p), ("pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("table_ld", C.c_uint32),
+                ("reserved0", C.c_uint32)]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [("cache", KvCache), ("Q", C.c_void_p), ("Q_out", C.c_void_p), ("K", C.c_void_p),
+                ("V", C.c_void_p), ("past", C.c_void_p), ("seq_start", C.c_void_p), ("batch", C.c_uint32),
+                ("tokens", C.c_uint32), ("heads", C.c_uint32), *_strides("q", "o", "k", "v"),
+                ("rotation", C.c_uint32), ("rope_dim", C.c_uint32), ("theta_base", C.c_float),
+                ("scaling", C.c_float)]
+
+
+class KvAttentionArgs(C.Structure):
+    _fields_ = [("cache", KvCache), ("Q", C.c_void_p), ("O", C.c_void_p), ("kv_len", C.c_void_p),
+                ("seq_start", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+                ("batch", C.c_uint32), ("tokens", C.c_uint32), ("heads", C.c_uint32), *_strides("q", "o"),
+                ("max_tokens", C.c_uint32), ("max_kv", C.c_uint32), ("causal", C.c_uint32),
+                ("scale", C.c_float), ("reserved0", C.c_uint32)]
+
+
+class KvReadArgs(C.Structure):
+    _fields_ = [("cache", KvCache), ("K", C.c_void_p), ("V", C.c_void_p), ("first", C.c_void_p),
+                ("seq_start", C.c_void_p), ("batch", C.c_uint32), ("tokens", C.c_uint32), *_strides("k", "v")]
+
+
 class _CmdArgs(C.Union):
     _fields_ = [("matmul_f32", MatmulF32Args), ("matmul_i8", MatmulI8Args),
                 ("rmsnorm", RmsnormArgs), ("softmax", SoftmaxArgs), ("rope", RopeArgs),
                 ("binary", BinaryArgs), ("unary", UnaryArgs), ("swiglu", SwigluArgs),
                 ("attention", AttentionArgs), ("quantize_i8", QuantizeArgs),
                 ("pack_weights_i8", PackArgs), ("mtp_head", MtpHeadArgs),
-                ("copy", CopyArgs), ("memset", MemsetArgs), ("raw", C.c_uint8 * 192)]
+                ("copy", CopyArgs), ("memset", MemsetArgs), ("kv_append", KvAppendArgs),
+                ("kv_attention", KvAttentionArgs), ("kv_read", KvReadArgs), ("raw", C.c_uint8 * 192)]
 
 
 class Command(C.Structure):
@@ -259,7 +294,8 @@ OP_FIELD = {
     OP_MUL_F32: ("binary", BinaryArgs), OP_ATTENTION_F32: ("attention", AttentionArgs),
     OP_QUANTIZE_I8: ("quantize_i8", QuantizeArgs), OP_PACK_WEIGHTS_I8: ("pack_weights_i8", PackArgs),
     OP_MTP_HEAD_F32: ("mtp_head", MtpHeadArgs), OP_COPY: ("copy", CopyArgs),
-    OP_MEMSET: ("memset", MemsetArgs),
+    OP_MEMSET: ("memset", MemsetArgs), OP_KV_APPEND_I8: ("kv_append", KvAppendArgs),
+    OP_KV_ATTENTION_I8: ("kv_attention", KvAttentionArgs), OP_KV_READ_F32: ("kv_read", KvReadArgs),
 }
 
 # Every function the C ABI exports (vnpu.h:474-751, vnpu_backend.h:150):
@@ -339,6 +375,11 @@ SIGNATURES = {
     "vnpu_get_backend_v1": (vp, []),
     "vnpu_stream_hip_handle": (vp, [vp]),  # MI355X additive extension
     "vnpu_attention_f32_noalloc": (st, [vp, vp]),  # MI355X additive extension
+    "vnpu_kv_append_i8": (st, [vp, vp]),           # the paged int8 KV cache: MI355X additive extension
+    "vnpu_kv_attention_i8": (st, [vp, vp]),
+    "vnpu_kv_read_f32": (st, [vp, vp]),
+    "vnpu_kv_attention_workspace": (u64, [vp, vp]),
+    "vnpu_kv_enqueue_noalloc": (st, [vp, vp, u64]),
 }
 
 LAYOUT = {  # LP64 sizes measured on the reference header
@@ -346,6 +387,7 @@ LAYOUT = {  # LP64 sizes measured on the reference header
     QuantizeArgs: 48, Config: 48, DeviceInfo: 304, DeviceStatus: 152, TraceSummary: 112,
     TuneResult: 72, SpeculativeConfig: 32, SpeculativeResult: 312, ClusterConfig: 32,
     RemoteNodeConfig: 32, ClusterStats: 80, NodeConfig: 40,
+    KvCache: 64, KvAppendArgs: 192, KvAttentionArgs: 168, KvReadArgs: 128,
 }
 
 
