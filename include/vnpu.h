@@ -521,13 +521,13 @@ typedef struct vnpu_kv_cache_t {
  * position * scaling * theta_base^(-2j / rope_dim), angles in 64 bits, each
  * result rounded once to f32; elements from rope_dim on are left.  V goes in
  * as it is.  Per (page, kv head), a = the largest magnitude of the page's new
- * tokens: the scale becomes max(s0, a / 127), s0 being its scale if it keeps
- * older tokens (slots below past[b] % page_size) and 0 if not; where that
+ * tokens: the scale becomes max(s0, a * f32(1 / 127)), s0 being its scale if it
+ * keeps older tokens (slots below past[b] % page_size) and 0 if not; where that
  * raises s0 the older codes are rounded anew to code * (s0 / scale); new
  * codes are round-half-away(x * (1 / scale)) in +-127.  A scale below 2^-126
  * is 0 (codes 0); an infinity or NaN among a page's new values makes its
- * scale NaN and leaves its codes.  A page that two sequences of one call write to has unspecified
- * contents afterwards. */
+ * scale NaN and leaves its codes.  A page that two sequences of one call
+ * write to has unspecified contents afterwards. */
 typedef struct vnpu_kv_append_i8_args_t {
     vnpu_kv_cache_t cache;
     const float *Q;             /* optional: queries to turn */

@@ -6,7 +6,7 @@
 //   (x, y) -> (f32(x cos - y sin), f32(x sin + y cos)), cos and sin in f32,
 //   the products exact in f64, so each result is rounded once;
 //   per (page, kv head): a = max |x| of the page's new tokens,
-//   s = max(n0 ? s0 : 0, f32(a / 127)) for n0 tokens kept from before,
+//   s = max(n0 ? s0 : 0, f32(a * f32(1 / 127))) for n0 tokens kept from before,
 //   kept codes -> round(code * f32(s0 / s)) where s > s0,
 //   new codes = round(x * f32(1 / s)), half away from zero, in +-127.
 // One page and kv head is one workgroup: it alone reads and writes that
@@ -65,10 +65,11 @@ __device__ __forceinline__ float2 turned(float2 x, float c, float s)
     return make_float2(static_cast<float>(fma(a, cd, -(b * sd))), static_cast<float>(fma(a, sd, b * cd)));
 }
 
-// Round half away from zero into +-127.
+// Round half away from zero into +-127.  The product is rounded by itself:
+// fused into the rounding's subtraction it would decide ties from more bits.
 __device__ __forceinline__ int code_of(float x, float by)
 {
-    return static_cast<int>(fminf(fmaxf(roundf(__fmul_rn(x, by)), -127.0f), 127.0f));
+    return static_cast<int>(fminf(fmaxf(roundf(dev::mul_rn(x, by)), -127.0f), 127.0f));
 }
 __device__ __forceinline__ uint32_t rescaled4(uint32_t codes, float ratio)
 {
@@ -96,7 +97,7 @@ struct PageScale {
 };
 __device__ __forceinline__ PageScale page_scale(uint32_t largest, bool kept, float before)
 {
-    float s = __fdiv_rn(__uint_as_float(largest), 127.0f);
+    float s = dev::mul_rn(__uint_as_float(largest), 1.0f / 127.0f);
     if (s < 1.17549435e-38f) s = 0.0f;   // no reciprocal in f32
     if (largest >= 0x7f800000u) s = __uint_as_float(0x7fc00000u);
     PageScale r;

@@ -85,7 +85,7 @@ def append_side(codes, scales, x, ids, past):
         for h in range(x.shape[1]):
             new = x[lo - past:hi - past, h]
             before = scales[page, h] if lo > first else None
-            s = np.float32(np.abs(new).max()) / np.float32(127)
+            s = np.float32(np.abs(new).max()) * (np.float32(1) / np.float32(127))
             s = np.float32(0) if s < np.float32(2.0**-126) else s
             if not np.all(np.isfinite(new)) or (before is not None and np.isnan(before)):
                 s = np.float32(np.nan)

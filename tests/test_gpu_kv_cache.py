@@ -150,6 +150,23 @@ def test_append_scales_at_the_borders(gpu, what):
     append_case(gpu, 4, 2, 64, 16, [5, 2], [12, 12], rotation, change=change)
 
 
+def test_append_products_that_round_to_a_half(gpu):
+    """x / scale in f32 is a whole number and a half where the exact product is not: the code goes by the f32 product."""
+    largest = np.float32(3.3)
+    inv = np.float32(1) / (largest * (np.float32(1) / np.float32(127)))
+    x = ((np.arange(126)[:, None] + 0.5) / inv).astype(np.float32)
+    x = (x.view(np.int32) + np.arange(-2, 3)).view(np.float32).reshape(-1)
+    exact = x.astype(np.float64) * np.float64(inv)
+    x = x[((x * inv) % 1 == 0.5) & (exact % 1 != 0.5)]
+    assert x.size > 30 and (exact % 1 < 0.5).any()
+
+    def change(c, k, v):
+        v[:] = np.resize(np.concatenate([x, -x]), v.shape)
+        v[:, :, 0] = largest
+        k[:] = v[:, :, ::-1]
+    append_case(gpu, 1, 1, 256, 16, [0, 16], [16, 3], rotation=0, change=change)
+
+
 def test_append_again_and_further_back(gpu):
     """The same tokens twice give the same; a sequence taken back to an earlier length goes on from there."""
     rng = np.random.default_rng(8)
