@@ -1149,6 +1149,11 @@ k::KvAttn kv_attention_params(vnpu_stream_t *s, const vnpu_kv_attention_i8_args_
     p.call = kv_call_params(s, a.cache, a.kv_len, a.seq_start, a.batch, a.tokens, src);
     const uint32_t D = a.cache.head_dim;
     require(a.heads && a.heads % a.cache.kv_heads == 0 && a.heads <= 65535, "kv heads is a multiple of kv_heads");
+    // Rows of a kv head and workgroups count in 32 bits.
+    require(static_cast<uint64_t>(a.tokens) * (a.heads / a.cache.kv_heads) < (1u << 31) &&
+                static_cast<uint64_t>(a.tokens) * a.heads < (1ull << 36) &&
+                static_cast<uint64_t>(a.batch) * a.cache.kv_heads < (1u << 30),
+            "kv_attention too large");
     const bool ragged = a.seq_start != nullptr;
     const KvTensor qt = kv_rows(a.q_batch_stride, a.q_token_stride, a.q_head_stride, a.heads, D, a.batch, a.tokens, ragged, false);
     const KvTensor ot = kv_rows(a.o_batch_stride, a.o_token_stride, a.o_head_stride, a.heads, D, a.batch, a.tokens, ragged, true);

@@ -21,6 +21,7 @@
 // loop but the row's maximum.
 #include "device_math.hpp"
 #include "kv_common.hpp"
+#include "lds_dma.hpp"
 
 #include <algorithm>
 #include <cstdio>
@@ -471,6 +472,26 @@ __global__ __launch_bounds__(256, DP * RT <= 128 ? 2 : 1) void kv_attention_stre
     }
 }
 
+// Parts of a row, `step` floats apart, each o / l with its m and l behind it:
+// weighed by l 2^(m - max m).  One wave.
+__device__ __forceinline__ void join_parts(const float *at, uint64_t step, uint32_t parts, uint32_t D, uint32_t lane, float *out)
+{
+    float M = kNegInf, L = 0.0f, o[4] = {};
+    for (uint32_t i = lane; i < parts; i += 64) M = fmaxf(M, at[i * step + D]);
+    for (int x = 32; x; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
+    const float base = M == kNegInf ? 0.0f : M;
+    for (uint32_t i = 0; i < parts; ++i) {
+        const float x = at[i * step + D + 1] * __builtin_amdgcn_exp2f(at[i * step + D] - base);
+        L += x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (lane + 64 * r < D) o[r] = fmaf(x, at[i * step + lane + 64 * r], o[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (lane + 64 * r < D) out[lane + 64 * r] = L != 0.0f ? o[r] / L : 0.0f;
+}
+
 // A sequence's parts together, one wave for a row.
 __global__ __launch_bounds__(64) void kv_attention_merge(KvAttn p, Split sp, const float *ws, uint32_t ws_rows)
 {
@@ -484,137 +505,344 @@ __global__ __launch_bounds__(64) void kv_attention_merge(KvAttn p, Split sp, con
     if (row >= seq.n * group) return;
     const uint64_t step = static_cast<uint64_t>(c.c.kv_heads) * ws_rows * (D + 2);
     const float *at = ws + ((static_cast<uint64_t>(slot) * c.c.kv_heads + h) * ws_rows + row) * (D + 2);
-    float M = kNegInf, L = 0.0f, o[4] = {};
-    for (uint32_t i = lane; i < sl.parts; i += 64) M = fmaxf(M, at[i * step + D]);
-    for (int x = 32; x; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
-    const float base = M == kNegInf ? 0.0f : M;
-    for (uint32_t i = 0; i < sl.parts; ++i) {
-        const float x = at[i * step + D + 1] * __builtin_amdgcn_exp2f(at[i * step + D] - base);
-        L += x;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (lane + 64 * r < D) o[r] = fmaf(x, at[i * step + lane + 64 * r], o[r]);
+    join_parts(at, step, sl.parts, D, lane,
+               p.O + kv::rows_base(c, p.o, sl.b, seq) + row / group * p.o.token + (h * group + row % group) * p.o.head);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: a workgroup of four waves takes 64 RT rows, each wave 16 RT of
+// them, and its part of the keys 64 at a time.  The chunk's K codes are copied
+// into LDS in operand order, its V codes pass through registers to be turned into
+// f16 once for the four waves; both of the next chunk are on their way while
+// this one is computed, and one barrier a chunk hands the buffers over.
+// ---------------------------------------------------------------------------
+
+struct Tiles {
+    uint32_t per_seq;      // tiles a sequence (without seq_start)
+    uint32_t count;        // room for tiles a kv head
+    uint32_t parts;        // key ranges of a tile
+    uint32_t low_rows;     // sequences with more rows are this kernel's
+};
+
+// Tile -> sequence and its tile, as find_unit does: ceil(rows / M) tiles of a
+// sequence fit between floor(first row / M) + b and the next sequence's.
+template <uint32_t M>
+__device__ __forceinline__ bool find_tile(const KvAttn &p, const Tiles &tl, uint32_t group, uint32_t unit, uint32_t &b, uint32_t &tile)
+{
+    const KvCall &c = p.call;
+    if (!c.seq_start) {
+        b = unit / tl.per_seq;
+        tile = unit % tl.per_seq;
+        return b < c.batch;
     }
-    float *out = p.O + kv::rows_base(c, p.o, sl.b, seq) + row / group * p.o.token + (h * group + row % group) * p.o.head;
+    uint32_t before = 0;
+    for (uint32_t i = 0; i < c.batch; i += 64) {
+        const uint32_t at = i + (threadIdx.x & 63);
+        const bool here = at < c.batch &&
+                          static_cast<uint64_t>(static_cast<uint32_t>(c.seq_start[at])) * group / M + at <= unit;
+        before += __popcll(__ballot(here));
+    }
+    if (!before) return false;
+    b = before - 1;
+    tile = unit - (static_cast<uint32_t>(static_cast<uint64_t>(static_cast<uint32_t>(c.seq_start[b])) * group / M) + b);
+    return true;
+}
+// The sequence of a tile and whether it is this kernel's.
+__device__ __forceinline__ bool tile_sequence(const KvAttn &p, const Tiles &tl, uint32_t group, uint32_t b, kv::Seq &seq, uint32_t &len)
+{
+    seq = kv::sequence(p.call, b);
+    const int32_t n = p.call.lengths[b];
+    len = static_cast<uint32_t>(n);
+    return seq.ok && n >= 0 && len <= p.max_kv && seq.n <= p.max_tokens && static_cast<uint64_t>(seq.n) * group > tl.low_rows;
+}
+
+template <int DP, int RT>
+__global__ __launch_bounds__(256, 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
+{
+    constexpr int DS = DP / 64, DT = DP / 16;
+    constexpr uint32_t M = 64 * RT;
+    constexpr uint32_t kK = 4 * DS * 1024, kV = DT * 2048, kBuf = kK + kV;   // bytes of a chunk's operands
+    extern __shared__ __align__(1024) int8_t lds[];
+    const KvCall &c = p.call;
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t G = c.c.kv_heads, h = blockIdx.x % G, D = c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
+    if (blockIdx.x == 0 && blockIdx.y == 0) kv::check_all(c, false, p.max_kv);
+    // The last tiles of a causal sequence have the most keys: they come first.
+    uint32_t b, tile, len;
+    kv::Seq seq;
+    const uint32_t unit = tl.count - 1 - blockIdx.x / G;
+    if (!find_tile<M>(p, tl, group, unit, b, tile) || !tile_sequence(p, tl, group, b, seq, len)) return;
+    b = __builtin_amdgcn_readfirstlane(b);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    len = __builtin_amdgcn_readfirstlane(len);
+    const uint32_t rows = __builtin_amdgcn_readfirstlane(seq.n) * group, n = __builtin_amdgcn_readfirstlane(seq.n);
+    if (static_cast<uint64_t>(tile) * M >= rows) return;
+    const uint32_t row0 = tile * M + wave * 16 * RT;   // the wave's first
+    auto sees = [&](uint32_t row) -> int {
+        return p.causal ? max(0, static_cast<int>(len) - static_cast<int>(n) + static_cast<int>(row / group) + 1) : static_cast<int>(len);
+    };
+    // Keys of the tile, of the wave; below `least` every row of the wave sees all.
+    const int tile_keys = sees(min(rows, tile * M + M) - 1);
+    const int wave_keys = row0 < rows ? sees(min(rows, row0 + 16 * RT) - 1) : 0, least = row0 < rows ? sees(row0) : 0;
+    const uint32_t chunks = (static_cast<uint32_t>(tile_keys) + kChunk - 1) / kChunk;
+    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * blockIdx.y / tl.parts);
+    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * (blockIdx.y + 1) / tl.parts);
+
+    Query<DS> q[RT];
+    State<DT> st[RT];
+    int limit[RT];
+    const bool aligned = ((reinterpret_cast<uintptr_t>(p.Q) & 15) | (p.q.batch & 3) | (p.q.token & 3) | (p.q.head & 3)) == 0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (lane + 64 * r < D) out[lane + 64 * r] = L != 0.0f ? o[r] / L : 0.0f;
+    for (int r = 0; r < RT; ++r) {
+        const uint32_t row = row0 + 16 * r + col;
+        const bool here = row < rows;
+        const float *at = p.Q + kv::rows_base(c, p.q, b, seq) + (here ? (row / group) * p.q.token + (h * group + row % group) * p.q.head : 0);
+        q[r].load(at, here, D, p.scale, aligned);
+        st[r].clear();
+        limit[r] = here ? sees(row) : static_cast<int>(len);
+    }
+
+    const uint32_t kb = col >> 2, last16 = len ? (len - 1) / 16 : 0, log16 = c.c.log_page - 4;
+    const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld;
+    auto checked = [&](int32_t id) -> uint32_t {
+        if (static_cast<uint32_t>(id) < c.c.pages) return static_cast<uint32_t>(id);
+        kv::fail(c.err);
+        return 0;
+    };
+    int32_t k_id = 0, v_id = 0;
+    auto ids = [&](uint32_t chunk) {
+        k_id = table[min(4 * chunk + kb, last16) >> log16];
+        v_id = table[min(4 * chunk + g, last16) >> log16];
+    };
+    constexpr int VW = (DT + 3) / 4;   // tiles of V that a wave brings in
+    v4i vf[VW];
+    float ks = 0.0f, vs = 0.0f, N = power_above(0.0f);
+    auto fetch = [&](uint32_t chunk, int8_t *buf) {
+        const uint32_t in_k = (16 * min(4 * chunk + kb, last16)) & (ps - 1);
+        const int8_t *kat = c.c.k + ((static_cast<uint64_t>(checked(k_id)) * G + h) * ps + in_k + (col & 3)) * D;
+#pragma unroll
+        for (int i = 0; i < DS; ++i) {   // operand (tile t, step s) is piece t * DS + s
+            const uint32_t piece = wave + 4 * i, t = piece / DS, s = piece % DS, d = 64 * s + 16 * g;
+            lds::dma16(kat + 4 * t * D + (d < D ? d : 0), buf + piece * 1024);
+        }
+        const uint64_t unit_v = static_cast<uint64_t>(checked(v_id)) * G + h;
+        const uint32_t in_v = (16 * min(4 * chunk + g, last16)) & (ps - 1);
+        const int8_t *vat = c.c.v + (unit_v * D + col) * ps + in_v;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            const uint32_t t = wave + 4 * i;
+            if (16 * t < D) vf[i] = *reinterpret_cast<const v4i *>(vat + static_cast<uint64_t>(16 * t) * ps);
+        }
+        ks = c.c.ks[unit_v];
+        vs = c.c.vs[unit_v];
+    };
+    auto turn_v = [&](int8_t *buf) {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            const uint32_t t = wave + 4 * i;
+            if (16 * t >= D) continue;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                v2h x[4];
+                halves_of(vf[i][2 * k], x[0], x[1]);
+                halves_of(vf[i][2 * k + 1], x[2], x[3]);
+                const v8h a = {x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
+                *reinterpret_cast<v8h *>(buf + kK + (2 * t + k) * 1024 + lane * 16) = a;
+            }
+        }
+    };
+    if (begin < end) {
+        ids(begin);
+        fetch(begin, lds);
+        turn_v(lds);
+        ids(min(begin + 1, end - 1));
+        lds::wait_vmcnt<0>();
+        __syncthreads();
+    }
+    for (uint32_t chunk = begin; chunk < end; ++chunk) {
+        int8_t *now = lds + ((chunk - begin) & 1) * kBuf, *next = lds + ((chunk - begin + 1) & 1) * kBuf;
+        const float ck = ks, v_scale = vs;
+        const bool more = chunk + 1 < end;
+        if (more) {
+            fetch(chunk + 1, next);
+            ids(min(chunk + 2, end - 1));
+        }
+        const bool work = static_cast<int>(kChunk * chunk) < wave_keys;
+        v8h hi[RT][2], lo[RT][2];
+        if (work) {
+            v4i kf[4][DS];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int s = 0; s < DS; ++s) kf[t][s] = *reinterpret_cast<const v4i *>(now + (t * DS + s) * 1024 + lane * 16);
+            const float above = groups_max(power_above(v_scale)), N_now = fmaxf(N, above);
+            const float beta = N / N_now, fv = v_scale * up_over(N_now);
+            N = N_now;
+            const int first = static_cast<int>(kChunk * chunk + 16 * g);
+            const bool all = static_cast<int>(kChunk * chunk + kChunk) <= least;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                v4f f[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    v4i a0 = {}, a1 = {}, a2 = {};
+#pragma unroll
+                    for (int s = 0; s < DS; ++s) {
+                        a0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][s], q[r].digit[0][s], a0, 0, 0, 0);
+                        a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][s], q[r].digit[1][s], a1, 0, 0, 0);
+                        a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][s], q[r].digit[2][s], a2, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        f[t][i] = fmaf(static_cast<float>(a0[i] * 256 + a1[i]), 256.0f, static_cast<float>(a2[i]));
+                }
+                if (all) weigh<DT, false>(st[r], f, q[r].factor * ck, fv, beta, 16, hi[r], lo[r]);
+                else weigh<DT, true>(st[r], f, q[r].factor * ck, fv, beta, limit[r] - first, hi[r], lo[r]);
+            }
+        }
+        if (more) turn_v(next);
+        if (work) {
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                if (16 * t >= static_cast<int>(D)) continue;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const v8h a = *reinterpret_cast<const v8h *>(now + kK + (2 * t + k) * 1024 + lane * 16);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        st[r].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo[r][k], st[r].o[t], 0, 0, 0);
+                        st[r].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi[r][k], st[r].o[t], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        lds::wait_vmcnt<0>();
+        __syncthreads();
+    }
+
+    const bool out_aligned = ((reinterpret_cast<uintptr_t>(p.O) & 15) | (p.o.batch & 3) | (p.o.token & 3) | (p.o.head & 3)) == 0;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const uint32_t row = row0 + 16 * r + col;
+        const float l = groups_sum(st[r].l);
+        const float by = l != 0.0f ? N * 6.103515625e-05f / l : 0.0f;   // 2^-14
+        if (row >= rows) continue;
+        if (tl.parts == 1) {
+            float *at = p.O + kv::rows_base(c, p.o, b, seq) + (row / group) * p.o.token + (h * group + row % group) * p.o.head + 4 * g;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                if (16 * t >= static_cast<int>(D)) continue;
+                const v4f x = st[r].o[t] * by;
+                if (out_aligned) *reinterpret_cast<v4f *>(at + 16 * t) = x;
+                else
+                    for (int i = 0; i < 4; ++i) at[16 * t + i] = x[i];
+            }
+        } else {
+            float *at = ws + (((static_cast<uint64_t>(unit) * G + h) * tl.parts + blockIdx.y) * M + (row - tile * M)) * (D + 4);
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+                if (16 * t < static_cast<int>(D)) *reinterpret_cast<v4f *>(at + 4 * g + 16 * t) = st[r].o[t] * by;
+            if (g == 0) {
+                at[D] = st[r].m;
+                at[D + 1] = l;
+            }
+        }
+    }
+}
+
+// A tile's key ranges together, one wave for a row.
+template <uint32_t M>
+__global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, const float *ws)
+{
+    const KvCall &c = p.call;
+    const uint32_t lane = threadIdx.x & 63, G = c.c.kv_heads, h = blockIdx.x % G, unit = blockIdx.x / G, D = c.c.head_dim;
+    const uint32_t group = p.heads / G;
+    uint32_t b, tile, len;
+    kv::Seq seq;
+    if (!find_tile<M>(p, tl, group, unit, b, tile) || !tile_sequence(p, tl, group, b, seq, len)) return;
+    const uint32_t in = blockIdx.y * 4 + (threadIdx.x >> 6), row = tile * M + in;
+    if (static_cast<uint64_t>(tile) * M + in >= static_cast<uint64_t>(seq.n) * group) return;
+    const uint64_t step = static_cast<uint64_t>(M) * (D + 4);
+    const float *at = ws + ((static_cast<uint64_t>(unit) * G + h) * tl.parts * M + in) * (D + 4);
+    float *out = p.O + kv::rows_base(c, p.o, b, seq) + (row / group) * p.o.token + (h * group + row % group) * p.o.head;
+    join_parts(at, step, tl.parts, D, lane, out);
 }
 
 constexpr uint32_t kStreamRows = 32;
 
 struct Plan {
-    Split stream;
+    bool stream = false, tiled = false;   // kernels of the call: sequences of few rows, of many
+    Split split{};
     uint32_t slots = 0, rows = 0;   // of the stream kernel: slots a kv head, rows a slot at most
-    size_t ws = 0;
+    Tiles tiles{};
+    uint32_t tile_rows = 0;
+    size_t stream_ws = 0, ws = 0;
 };
 Plan plan_of(const KvAttn &p)
 {
     Plan r;
-    const uint32_t G = p.call.c.kv_heads, group = p.heads / G;
+    const KvCall &c = p.call;
+    const uint32_t G = c.c.kv_heads, group = p.heads / G, D = c.c.head_dim;
     const uint64_t most = static_cast<uint64_t>(p.max_tokens) * group;
-    r.rows = static_cast<uint32_t>(std::min<uint64_t>(most, kStreamRows));
-    r.stream.target = (2 * p.cus + G - 1) / G;
-    r.stream.min_per = 4;
-    r.stream.low_rows = 0;
-    r.stream.high_rows = kStreamRows;
-    r.slots = r.stream.target + p.call.batch;
-    const bool splits = p.max_kv > r.stream.min_per * kChunk;
-    if (!splits) r.slots = p.call.batch;
-    else r.ws = static_cast<size_t>(r.slots) * G * r.rows * (p.call.c.head_dim + 2) * sizeof(float);
+    r.tiled = most > kStreamRows;
+    // Without seq_start all sequences have max_tokens.
+    r.stream = !r.tiled || c.seq_start;
+    if (r.stream) {
+        r.rows = static_cast<uint32_t>(std::min<uint64_t>(most, kStreamRows));
+        r.split.target = (2 * p.cus + G - 1) / G;
+        r.split.min_per = 4;
+        r.split.low_rows = 0;
+        r.split.high_rows = kStreamRows;
+        r.slots = r.split.target + c.batch;
+        if (p.max_kv <= r.split.min_per * kChunk) r.slots = c.batch;   // none splits
+        else r.stream_ws = (static_cast<size_t>(r.slots) * G * r.rows * (D + 2) * sizeof(float) + 15) / 16 * 16;
+    }
+    r.ws = r.stream_ws;
+    if (r.tiled) {
+        r.tile_rows = most <= 64 || D > 128 ? 64 : 128;
+        r.tiles.low_rows = r.stream ? kStreamRows : 0;
+        r.tiles.per_seq = static_cast<uint32_t>((most + r.tile_rows - 1) / r.tile_rows);
+        r.tiles.count = c.seq_start ? static_cast<uint32_t>(static_cast<uint64_t>(c.tokens) * group / r.tile_rows) + c.batch
+                                    : r.tiles.per_seq * c.batch;
+        const uint64_t grid = static_cast<uint64_t>(r.tiles.count) * G;
+        const uint32_t chunks = (p.max_kv + kChunk - 1) / kChunk;
+        r.tiles.parts = grid >= p.cus ? 1 : std::max<uint32_t>(1, std::min<uint64_t>(2 * p.cus / grid, chunks / 8));
+        if (r.tiles.parts > 1) r.ws += static_cast<size_t>(grid) * r.tiles.parts * r.tile_rows * (D + 4) * sizeof(float);
+    }
     return r;
 }
 
 template <int DP, int RT>
 void launch_stream(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 {
-    kv_attention_stream<DP, RT><<<dim3(pl.slots, p.call.c.kv_heads), 256, 0, s>>>(p, pl.stream, ws, pl.rows);
+    kv_attention_stream<DP, RT><<<dim3(pl.slots, p.call.c.kv_heads), 256, 0, s>>>(p, pl.split, ws, pl.rows);
+}
+template <int DP, int RT>
+void launch_tile(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
+{
+    constexpr uint32_t bytes = 2 * (4 * (DP / 64) * 1024 + (DP / 16) * 2048);
+    if (bytes > 60 * 1024)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_attention_tile<DP, RT>),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const uint32_t grid = pl.tiles.count * p.call.c.kv_heads;
+    kv_attention_tile<DP, RT><<<dim3(grid, pl.tiles.parts), 256, bytes, s>>>(p, pl.tiles, ws);
+    if (pl.tiles.parts > 1) kv_attention_join<64 * RT><<<dim3(grid, 16 * RT), 256, 0, s>>>(p, pl.tiles, ws);
 }
 template <int DP>
-void launch_stream_rows(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
+void launch(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 {
-    if (pl.rows <= 16) launch_stream<DP, 1>(s, p, pl, ws);
-    else launch_stream<DP, 2>(s, p, pl, ws);
-}
-
-// One wave per token and query head; lane = key for the scores, lane = head
-// dimension for the products with V.  Sequences of more rows than low_rows.
-__global__ __launch_bounds__(64) void kv_attention_simple(KvAttn p, uint32_t low_rows)
-{
-    __shared__ float q[256], w[64], ws[64];
-    __shared__ uint32_t pages[64];
-    const KvCall &c = p.call;
-    const uint32_t lane = threadIdx.x, h = blockIdx.y;
-    if (blockIdx.x == 0 && h == 0) kv::check_all(c, false, p.max_kv);
-    uint32_t b, i;
-    if (!c.seq_start) {
-        const uint32_t n = c.tokens / c.batch;
-        b = blockIdx.x / n;
-        i = blockIdx.x % n;
-    } else {
-        uint32_t before = 0;
-        for (uint32_t k = 0; k < c.batch; k += 64)
-            before += __popcll(__ballot(k + lane < c.batch && static_cast<uint32_t>(c.seq_start[k + lane]) <= blockIdx.x));
-        if (!before) return;
-        b = before - 1;
-        i = blockIdx.x - static_cast<uint32_t>(c.seq_start[b]);
+    if (pl.stream) {
+        if (pl.rows <= 16) launch_stream<DP, 1>(s, p, pl, ws);
+        else launch_stream<DP, 2>(s, p, pl, ws);
+        if (pl.stream_ws)
+            kv_attention_merge<<<dim3(p.call.batch, p.call.c.kv_heads, pl.rows), 64, 0, s>>>(p, pl.split, ws, pl.rows);
     }
-    const kv::Seq s = kv::sequence(c, b);
-    const int32_t len = c.lengths[b];
-    if (!s.ok || i >= s.n || len < 0 || static_cast<uint32_t>(len) > p.max_kv || s.n * (p.heads / c.c.kv_heads) <= low_rows) return;
-    const int64_t see = p.causal ? static_cast<int64_t>(len) - s.n + i + 1 : len;
-    const uint32_t keys = see > 0 ? static_cast<uint32_t>(see) : 0;
-    const uint32_t D = c.c.head_dim, ps = c.c.page_size, kh = h / (p.heads / c.c.kv_heads);
-    const float *qr = p.Q + kv::rows_base(c, p.q, b, s) + i * p.q.token + h * p.q.head;
-    for (uint32_t d = lane; d < D; d += 64) q[d] = qr[d];
-    __syncthreads();
-    float m = -__builtin_inff(), l = 0.0f, o[4] = {};
-    const float factor = p.scale * 1.4426950408889634f;   // the softmax in powers of two
-    for (uint32_t k0 = 0; k0 < keys; k0 += 64) {
-        const uint32_t key = k0 + lane;
-        float score = -__builtin_inff();
-        w[lane] = 0.0f;
-        if (key < keys) {
-            const uint32_t page = kv::page_of(c, b, key >> c.c.log_page);
-            const uint64_t unit = static_cast<uint64_t>(page) * c.c.kv_heads + kh;
-            pages[lane] = page;
-            const uint32_t *row = reinterpret_cast<const uint32_t *>(c.c.k + (unit * ps + (key & (ps - 1))) * D);
-            float dot = 0.0f;
-            for (uint32_t d = 0; d < D; d += 4) {
-                const uint32_t x = row[d / 4];
-                for (int e = 0; e < 4; ++e) dot = fmaf(q[d + e], static_cast<float>(static_cast<int8_t>(x >> (8 * e))), dot);
-            }
-            score = dot * c.c.ks[unit] * factor;
-            ws[lane] = c.c.vs[unit];
-        }
-        float top = score;
-        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-        const float now = fmaxf(m, top);
-        const float a = now == -__builtin_inff() ? 0.0f : now;   // no finite score yet
-        const float e = key < keys ? exp2f(score - a) : 0.0f, keep = exp2f(m - a);
-        float sum = e;
-        for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-        l = l * keep + sum;
-        m = now;
-        if (key < keys) w[lane] = e * ws[lane];
-        __syncthreads();
-        const uint32_t n = min(64u, keys - k0);
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t d = lane + 64 * r;
-            if (d >= D) continue;
-            float acc = o[r] * keep;
-            for (uint32_t k = 0; k < n; ++k) {
-                const uint64_t unit = static_cast<uint64_t>(pages[k]) * c.c.kv_heads + kh;
-                acc = fmaf(w[k], static_cast<float>(c.c.v[(unit * D + d) * ps + ((k0 + k) & (ps - 1))]), acc);
-            }
-            o[r] = acc;
-        }
-        __syncthreads();
-    }
-    float *out = p.O + kv::rows_base(c, p.o, b, s) + i * p.o.token + h * p.o.head;
-    for (int r = 0; r < 4; ++r) {
-        const uint32_t d = lane + 64 * r;
-        if (d < D) out[d] = keys ? o[r] / l : 0.0f;
+    if (pl.tiled) {
+        float *rest = ws + pl.stream_ws / sizeof(float);
+        if constexpr (DP > 128) launch_tile<DP, 1>(s, p, pl, rest);
+        else if (pl.tile_rows == 64) launch_tile<DP, 1>(s, p, pl, rest);
+        else launch_tile<DP, 2>(s, p, pl, rest);
     }
 }
 
@@ -624,7 +852,8 @@ std::string kv_attention_route(const KvAttn &p)
 {
     const Plan pl = plan_of(p);
     char text[96];
-    std::snprintf(text, sizeof(text), "stream slots=%u rows=%u", pl.slots, pl.rows);
+    std::snprintf(text, sizeof(text), "stream=%u rows=%u tile=%u parts=%u", pl.stream ? pl.slots : 0, pl.rows,
+                  pl.tile_rows, pl.tiles.parts);
     return text;
 }
 
@@ -634,13 +863,9 @@ void kv_attention(hipStream_t s, const KvAttn &p, void *ws)
 {
     const Plan pl = plan_of(p);
     float *part = static_cast<float *>(ws);
-    const uint32_t D = p.call.c.head_dim;
-    if (D <= 64) launch_stream_rows<64>(s, p, pl, part);
-    else if (D <= 128) launch_stream_rows<128>(s, p, pl, part);
-    else launch_stream_rows<256>(s, p, pl, part);
-    if (pl.ws) kv_attention_merge<<<dim3(p.call.batch, p.call.c.kv_heads, pl.rows), 64, 0, s>>>(p, pl.stream, part, pl.rows);
-    if (static_cast<uint64_t>(p.max_tokens) * (p.heads / p.call.c.kv_heads) > kStreamRows)
-        kv_attention_simple<<<dim3(p.call.tokens, p.heads), 64, 0, s>>>(p, kStreamRows);
+    if (p.call.c.head_dim <= 64) launch<64>(s, p, pl, part);
+    else if (p.call.c.head_dim <= 128) launch<128>(s, p, pl, part);
+    else launch<256>(s, p, pl, part);
 }
 
 }  // namespace k
