@@ -81,6 +81,11 @@ __device__ __forceinline__ float power_above(float scale)
     const uint32_t bits = __float_as_uint(scale == scale ? scale : 0.0f);
     return fminf(fmaxf(__uint_as_float((bits + 0x7fffffu) & 0x7f800000u), 7.888609052210118e-31f), 1.7014118346046923e38f);
 }
+// a / b of two powers of two with a <= b; 0 below 2^-126.
+__device__ __forceinline__ float power_ratio(float a, float b)
+{
+    return __int_as_float(max(0, 0x3f800000 + __float_as_int(a) - __float_as_int(b)));
+}
 // 2^14 / N, exact.
 __device__ __forceinline__ float up_over(float n) { return __uint_as_float((268u << 23) - __float_as_uint(n)); }
 
@@ -278,196 +283,394 @@ __device__ __forceinline__ void weigh(State<DT> &st, v4f f[4], float ck, float f
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: a workgroup of four waves takes up to 16 RT rows and a range of
-// the keys, its waves every fourth chunk, codes straight from memory into the
-// operands.  K of the next chunk is on its way while the softmax and P . V
-// of this one run, V while the next scores do.
+// Few rows (a token or a few of grouped heads): the codes are read once and
+// bound the kernel.  A workgroup takes the rows and a range of the keys, its
+// waves every WAVES-th chunk of 64.  Each wave copies a chunk's K and V codes
+// into LDS of its own with 64-byte runs for every four lanes (read straight into
+// operands, where neighbouring lanes hold different keys, the same loads took
+// four times the cycles of the address unit: 10 TB/s even from cache), and asks for
+// the next chunk as soon as the operands have left LDS, so 16 KiB a wave are
+// under way; pages and scales come through scalar loads and disturb no count.
+// Both products run on the int8 matrix cores, no code converted: the 16
+// operand rows of a product are 4 rows times 4 base-256 digits, row 4 r + d,
+// so one product gives a lane the four digit sums of one result:
+//   q digits x K codes   lane (r = g, c): row r, key 4 c + t of tile t;
+//   p digits x V codes   lane (r = g, c): row r, dimension 16 t + c of tile t.
+// A weight is the whole number p * v_scale * 2^26 / N, p = 2^(s - m) for a
+// reference m that s may pass by 4, N a power of two that v_scale may not
+// pass; sums stay whole numbers until m or N has to move, then they are added
+// to f32 sums in LDS.
 // ---------------------------------------------------------------------------
 
-template <int DP, int RT>
-__global__ __launch_bounds__(256, DP * RT <= 128 ? 2 : 1) void kv_attention_stream(KvAttn p, Split sp, float *ws, uint32_t ws_rows)
+constexpr float kDigits4 = 2139060000.0f;   // four digits hold 127 * (2^24 + 2^16 + 2^8 + 1) = 2139062143
+constexpr float kAhead = 4.0f;
+constexpr uint32_t kMostChunks = 2000;      // 64 keys add at most 64 * 128 * 127 to a sum: 2064 fit
+
+// Maximum / sum over the 16 lanes of a row.
+template <int CTRL>
+__device__ __forceinline__ float dpp_row(float x)
 {
-    constexpr int DS = DP / 64, DT = DP / 16, R = 16 * RT;
-    __shared__ float sh_o[4][R][68];
-    __shared__ float sh_m[4][R], sh_l[4][R];
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float row_max(float x)
+{
+    x = fmaxf(x, dpp_row<0x128>(x));   // row_ror:8
+    x = fmaxf(x, dpp_row<0x124>(x));
+    x = fmaxf(x, dpp_row<0x122>(x));
+    return fmaxf(x, dpp_row<0x121>(x));
+}
+__device__ __forceinline__ float row_sum(float x)
+{
+    x += dpp_row<0x128>(x);
+    x += dpp_row<0x124>(x);
+    x += dpp_row<0x122>(x);
+    return x + dpp_row<0x121>(x);
+}
+// Sum of four digit sums, digit i counting 256^i.
+__device__ __forceinline__ float digits_sum(const v4i &a)
+{
+    return fmaf(static_cast<float>(a[3] * 256 + a[2]), 65536.0f, static_cast<float>(a[1] * 256 + a[0]));
+}
+__device__ __forceinline__ float digits_sum_wide(const v4i &a)   // sums over many chunks
+{
+    const float hi = fmaf(static_cast<float>(a[3]), 256.0f, static_cast<float>(a[2]));
+    return fmaf(hi, 65536.0f, fmaf(static_cast<float>(a[1]), 256.0f, static_cast<float>(a[0])));
+}
+
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T *at)   // a wave's address, memory that the kernel does not write
+{
+    return *(const __attribute__((address_space(4))) T *)at;
+}
+// At most n copies under way; n is one of the tile counts of DP.
+template <int DP, bool FULL>
+__device__ __forceinline__ void wait_copies(uint32_t n)
+{
+    if constexpr (FULL) lds::wait_vmcnt<DP / 16>();
+    else if constexpr (DP == 64) lds::wait_vmcnt<1>();
+    else if constexpr (DP == 128) {
+        if (n >= 6) lds::wait_vmcnt<6>();
+        else lds::wait_vmcnt<5>();
+    } else {
+        if (n >= 12) lds::wait_vmcnt<12>();
+        else lds::wait_vmcnt<9>();
+    }
+}
+
+// Bytes of dynamic LDS: a chunk's K and V a wave, its digits and its f32 sums.
+template <int DP, int RT, int WAVES>
+constexpr uint32_t few_lds()
+{
+    return WAVES * (128 * DP + 1024 + RT * DP * 16);
+}
+
+template <int DP, int RT, bool FULL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) void kv_attention_few(KvAttn p, Split sp, float *ws, uint32_t ws_rows)
+{
+    constexpr int DS = DP / 64, DT = DP / 16, R = 4 * RT;
+    extern __shared__ __align__(1024) int8_t lds[];
+    __shared__ float sh_m[WAVES][R], sh_l[WAVES][R];
     const KvCall &c = p.call;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, col = lane & 15;
-    const uint32_t h = blockIdx.y, D = c.c.head_dim, ps = c.c.page_size, group = p.heads / c.c.kv_heads;
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t h = blockIdx.y, G = c.c.kv_heads, D = FULL ? DP : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
+    int8_t *k_lds = lds + wave * 128 * DP, *v_lds = k_lds + 64 * DP;
+    uint32_t *sh_p = reinterpret_cast<uint32_t *>(lds + WAVES * 128 * DP) + wave * 256;
+    float *sh_o_all = reinterpret_cast<float *>(lds + WAVES * (128 * DP + 1024)), *sh_o = sh_o_all + wave * RT * DT * 64;
     if (blockIdx.x == 0 && h == 0) kv::check_all(c, false, p.max_kv);
     uint32_t slot = blockIdx.x;
     Slot sl;
     if (!find_slot(p, sp, false, slot, sl)) return;
-    const kv::Seq seq = kv::sequence(c, sl.b);
-    const uint32_t len = static_cast<uint32_t>(c.lengths[sl.b]), rows = seq.n * group;
-    const uint32_t begin = sl.part * sl.per, end = min(sl.chunks, begin + sl.per);
+    const uint32_t b = __builtin_amdgcn_readfirstlane(sl.b), parts = __builtin_amdgcn_readfirstlane(sl.parts);
+    const kv::Seq seq = kv::sequence(c, b);
+    const uint32_t n = __builtin_amdgcn_readfirstlane(seq.n), rows = n * group;
+    const int len = __builtin_amdgcn_readfirstlane(c.lengths[b]);
+    const uint32_t begin = __builtin_amdgcn_readfirstlane(sl.part * sl.per);
+    const uint32_t end = __builtin_amdgcn_readfirstlane(min(sl.chunks, sl.part * sl.per + sl.per));
 
-    Query<DS> q[RT];
-    State<DT> st[RT];
-    int limit[RT];   // keys that the lane's row sees
-    int least = static_cast<int>(len);
+    // Pages of a chunk's four blocks of 16 keys (blocks behind the last are
+    // the last) and, of the chunk in LDS, their scales.
+    const uint32_t last16 = len ? (len - 1) / 16 : 0, log16 = c.c.log_page - 4, tiles = D / 16;
+    const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld;
+    bool strange = false;   // a page outside the pool: page 0 is read in its place
+    uint64_t unit[4];
+    float ks4[4], vs4[4];
+    auto pages = [&](uint32_t chunk) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int32_t id = scalar_load(table + (min(4 * chunk + j, last16) >> log16));
+            const bool in = static_cast<uint32_t>(id) < c.c.pages;
+            strange |= !in;
+            unit[j] = static_cast<uint64_t>(static_cast<uint32_t>(in ? id : 0)) * G + h;
+        }
+    };
+    auto scales = [&]() {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            ks4[j] = scalar_load(c.c.ks + unit[j]);
+            vs4[j] = scalar_load(c.c.vs + unit[j]);
+        }
+    };
+    auto of_block = [&](uint32_t j, const auto &x) {
+        const auto a = x[0], b = x[1], c = x[2], d = x[3];   // values: an index would put the array into memory
+        return j & 2 ? (j & 1 ? d : c) : (j & 1 ? b : a);
+    };
+    // K: a block's 16 keys are 16 D bytes in a row.  The 16-byte pieces of a key
+    // are swapped by its place, so that the operands' reads, at keys 4 apart, spread over the banks.
+    constexpr uint32_t kSwap = FULL ? DP / 16 - 1 : 0;
+    auto copy_k = [&](uint32_t chunk) {
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+            if (!FULL && i >= static_cast<int>(tiles)) break;
+            if constexpr (FULL) {
+                constexpr int kPer = DP / 64;   // copies of a block
+                const uint32_t j = i / kPer, in = (16 * min(4 * chunk + j, last16)) & (ps - 1);
+                const uint32_t piece = 64 * (i % kPer) + lane, key = piece / (DP / 16), at = piece % (DP / 16);
+                lds::dma16(c.c.k + (unit[j] * ps + in + key) * DP + 16 * (at ^ ((4 * j + key / 4) & kSwap)), k_lds + 1024 * i);
+            } else {
+                const uint32_t piece = 64 * i + lane, j = piece / D, in = (16 * min(4 * chunk + j, last16)) & (ps - 1);
+                lds::dma16(c.c.k + (of_block(j, unit) * ps + in) * D + 16 * (piece - j * D), k_lds + 1024 * i);
+            }
+        }
+    };
+    // V: a dimension's keys of a page are a row; where a page is 16 or 32 keys,
+    // rows of neighbouring dimensions follow each other.  Lane -> dimension
+    // and block of 16 keys so that lanes in a row read bytes in a row; the blocks of a
+    // row are swapped for the banks too.
+    const uint32_t low = min(c.c.log_page, 6u) - 4, low_mask = (1u << low) - 1;
+    const uint32_t v_dim = (lane >> low) & 15;
+    const uint32_t v_block = (lane >> (4 + low)) << low | ((lane & low_mask) ^ ((v_dim >> (4 - low)) & low_mask));
+    const uint32_t v_at = 16 * ((g >> low) << (4 + low) | col << low | ((g & low_mask) ^ ((col >> (4 - low)) & low_mask)));
+    auto copy_v = [&](uint32_t chunk) {
+        const uint32_t in = (16 * min(4 * chunk + v_block, last16)) & (ps - 1);
+        const int8_t *from = c.c.v + (of_block(v_block, unit) * D + v_dim) * ps + in;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+            if (FULL || t < static_cast<int>(tiles)) lds::dma16(from + static_cast<uint64_t>(16 * t) * ps, v_lds + 1024 * t);
+    };
+    uint32_t chunk = begin + wave;
+    const bool any = len && chunk < end;
+    if (any) {
+        pages(chunk);
+        copy_k(chunk);
+        copy_v(chunk);
+        scales();
+        pages(min(chunk + WAVES, end - 1));
+    }
+
+    // Queries: lane (operand row 4 r + d, group g) holds digit d of row r's elements 64 s + 16 g .. + 15.
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.Q) & 15) | (p.q.batch & 3) | (p.q.token & 3) | (p.q.head & 3)) == 0;
+    v4i q[RT][DS];
+    float factor[RT], m[RT], l[RT];   // of row g: score in powers of two = sum * factor * k_scale
+    int limit[RT];                    // keys that row g sees
+    v4i acc[RT][DT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        const uint32_t row = 16 * r + col, i = row / group;
+        const uint32_t row = 4 * r + (col >> 2), i = row / group;
         const bool here = row < rows;
-        const float *at = p.Q + kv::rows_base(c, p.q, sl.b, seq) + (here ? i * p.q.token + (h * group + row % group) * p.q.head : 0);
-        q[r].load(at, here, D, p.scale, aligned);
-        st[r].clear();
-        limit[r] = p.causal && here ? max(0, static_cast<int>(len) - static_cast<int>(seq.n) + static_cast<int>(i) + 1)
-                                    : static_cast<int>(len);
-    }
-    if (p.causal) least = max(0, static_cast<int>(len) - static_cast<int>(seq.n) + 1);
-
-    // Page of the 16 keys that this lane loads K from (kb) and V and the scales (g).
-    const uint32_t kb = col >> 2;
-    const uint32_t last16 = len ? (len - 1) / 16 : 0, log16 = c.c.log_page - 4;
-    const int32_t *table = c.c.table + static_cast<uint64_t>(sl.b) * c.c.table_ld;
-    auto page_at = [&](uint32_t block) -> int32_t { return table[min(block, last16) >> log16]; };
-    auto checked = [&](int32_t id) -> uint32_t {
-        if (static_cast<uint32_t>(id) < c.c.pages) return static_cast<uint32_t>(id);
-        kv::fail(c.err);
-        return 0;
-    };
-    v4i kf[4][DS], vf[DT];
-    float ks = 0.0f, vs = 0.0f, N = power_above(0.0f);
-    int32_t k_id = 0, v_id = 0;
-    auto load_k = [&](uint32_t chunk) {   // and the scales
-        const uint32_t in = (16 * min(4 * chunk + kb, last16)) & (ps - 1);
-        const int8_t *at = c.c.k + ((static_cast<uint64_t>(checked(k_id)) * c.c.kv_heads + h) * ps + in + (col & 3)) * D;
+        const float *at = p.Q + kv::rows_base(c, p.q, b, seq) + (here ? i * p.q.token + (h * group + row % group) * p.q.head : 0);
+        float x[DS * 16];
+        uint32_t most = 0;
 #pragma unroll
         for (int s = 0; s < DS; ++s) {
             const uint32_t d = 64 * s + 16 * g;
-            const int8_t *from = at + (d < D ? d : 0);   // times digits that are zero
 #pragma unroll
-            for (int t = 0; t < 4; ++t) kf[t][s] = *reinterpret_cast<const v4i *>(from + 4 * t * D);
+            for (int w = 0; w < 4; ++w) {
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (here && d < D) {
+                    const float *e = at + d + 4 * w;
+                    v = aligned ? *reinterpret_cast<const float4 *>(e) : make_float4(e[0], e[1], e[2], e[3]);
+                }
+                x[16 * s + 4 * w] = v.x;
+                x[16 * s + 4 * w + 1] = v.y;
+                x[16 * s + 4 * w + 2] = v.z;
+                x[16 * s + 4 * w + 3] = v.w;
+            }
         }
-        const uint64_t unit = static_cast<uint64_t>(checked(v_id)) * c.c.kv_heads + h;
-        ks = c.c.ks[unit];
-        vs = c.c.vs[unit];
-    };
-    auto load_v = [&](uint32_t chunk) {
-        const uint32_t in = (16 * min(4 * chunk + g, last16)) & (ps - 1);
-        const int8_t *at = c.c.v + ((static_cast<uint64_t>(checked(v_id)) * c.c.kv_heads + h) * D + col) * ps + in;
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
-            if (16 * t < static_cast<int>(D)) vf[t] = *reinterpret_cast<const v4i *>(at + static_cast<uint64_t>(16 * t) * ps);
-    };
-    auto ids = [&](uint32_t chunk) {
-        k_id = page_at(4 * chunk + kb);
-        v_id = page_at(4 * chunk + g);
+        for (int e = 0; e < DS * 16; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
+        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
+        const float up = most < 0x0f800000u ? 7.922816251426434e28f : 1.0f;   // below 2^-96: times 2^96
+        const float S = most ? kDigits4 / (__uint_as_float(most) * up) : 1.0f;
+        const float f = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : p.scale * 1.4426950408889634f / S / up;
+        // Lane (operand row 4 r + d) has row r's factor; the products leave row g in group g.
+        factor[r] = __shfl(f, 4 * static_cast<int>(g));
+        const uint32_t d = col & 3, pick = 0x0c0c0000u | (4 + d) << 8 | d;
+#pragma unroll
+        for (int s = 0; s < DS; ++s)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t u[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    u[e] = (static_cast<uint32_t>(static_cast<int>(rintf(x[16 * s + 4 * w + e] * up * S))) + 0x80808080u) ^ 0x80808080u;
+                q[r][s][w] = static_cast<int>(__builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], pick),
+                                                                    __builtin_amdgcn_perm(u[1], u[0], pick), 0x05040100u));
+            }
+        const uint32_t mine = 4 * r + g;
+        limit[r] = p.causal && mine < rows ? max(0, len - static_cast<int>(n) + static_cast<int>(mine / group) + 1) : len;
+        m[r] = kNegInf;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            acc[r][t] = v4i{0, 0, 0, 0};
+            sh_o[(r * DT + t) * 64 + lane] = 0.0f;
+        }
+    }
+    const int least = p.causal ? max(0, len - static_cast<int>(n) + 1) : len;   // every row sees the keys below
+    float N = power_above(0.0f);
+    uint32_t since = 0;
+    // Whole sums to the f32 ones, both by `by`.
+    auto gather = [&](int r, float by) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            if (!FULL && 16 * t >= static_cast<int>(D)) continue;
+            float &o = sh_o[(r * DT + t) * 64 + lane];
+            o = (o + digits_sum_wide(acc[r][t])) * by;
+            acc[r][t] = v4i{0, 0, 0, 0};
+        }
     };
 
-    auto step = [&](uint32_t chunk, auto more) {
-        v4f f[RT][4];
+    auto step = [&](auto more) {
+        const uint32_t kb = col >> 2;
+        const float ks = of_block(kb, ks4), scale = of_block(kb, vs4);
+        const int first = static_cast<int>(kChunk * chunk + 4 * col);
+        const bool all = static_cast<int>(kChunk * chunk + kChunk) <= least;
+        wait_copies<DP, FULL>(tiles);   // V's may be under way
+        v4i kf[4][DS];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                v4i a0 = {}, a1 = {}, a2 = {};
-#pragma unroll
-                for (int s = 0; s < DS; ++s) {
-                    a0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][s], q[r].digit[0][s], a0, 0, 0, 0);
-                    a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][s], q[r].digit[1][s], a1, 0, 0, 0);
-                    a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][s], q[r].digit[2][s], a2, 0, 0, 0);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)   // |a0| <= 256 * 127 * 127: a0 * 256 + a1 fits
-                    f[r][t][i] = fmaf(static_cast<float>(a0[i] * 256 + a1[i]), 256.0f, static_cast<float>(a2[i]));
+            for (int s = 0; s < DS; ++s) {
+                const uint32_t piece = FULL ? (4 * s + g) ^ (col & kSwap) : 4 * s + g < tiles ? 4 * s + g : 0;   // times zeros
+                kf[t][s] = *reinterpret_cast<const v4i *>(k_lds + (4 * col + t) * D + 16 * piece);
             }
-        const float ck = ks, v_scale = vs;
-        const float above = groups_max(power_above(v_scale)), N_now = fmaxf(N, above);
-        const float beta = N / N_now, fv = v_scale * up_over(N_now);
-        N = N_now;
-        if (more) load_k(chunk + 4);   // v_id is the next chunk's already
-        v8h hi[RT][2], lo[RT][2];
-        const int first = static_cast<int>(kChunk * chunk + 16 * g);
-        if (static_cast<int>(kChunk * chunk + kChunk) <= least) {
+        __builtin_amdgcn_s_waitcnt(lds::waitcnt_imm(63, 7, 0));
+        if (more) copy_k(chunk + WAVES);
+        float f[RT][4], top[RT];
+        bool move = false;
 #pragma unroll
-            for (int r = 0; r < RT; ++r) weigh<DT, false>(st[r], f[r], q[r].factor * ck, fv, beta, 16, hi[r], lo[r]);
-        } else {
+        for (int r = 0; r < RT; ++r) {
+            top[r] = kNegInf;
 #pragma unroll
-            for (int r = 0; r < RT; ++r) weigh<DT, true>(st[r], f[r], q[r].factor * ck, fv, beta, limit[r] - first, hi[r], lo[r]);
+            for (int t = 0; t < 4; ++t) {
+                v4i a = {0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < DS; ++s) a = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[r][s], kf[t][s], a, 0, 0, 0);
+                f[r][t] = digits_sum(a);
+            }
+            const float ck = factor[r] * ks;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) f[r][t] *= ck;
+            if (all) {
+                top[r] = fmaxf(fmaxf(f[r][0], f[r][1]), fmaxf(f[r][2], f[r][3]));
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) top[r] = fmaxf(top[r], first + t < limit[r] ? f[r][t] : kNegInf);
+            }
+            move |= top[r] > m[r] + kAhead;
+        }
+        move |= scale > N;
+        if (__any(move) || ++since >= kMostChunks) {
+            // N is one for the wave's rows, with a factor of two to spare.
+            const float need = groups_max(row_max(power_above(scale))), N_now = need > N ? fminf(2.0f * need, 1.7014118346046923e38f) : N;
+            const float beta = power_ratio(N, N_now);
+            N = N_now;
+            since = 0;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const float now = fmaxf(m[r], row_max(top[r]));
+                const float alpha = now > m[r] ? __builtin_amdgcn_exp2f(m[r] - now) : 1.0f;
+                gather(r, alpha * beta);
+                l[r] *= alpha;
+                m[r] = now;
+            }
+        }
+        const float fv = scale * __uint_as_float((280u << 23) - __float_as_uint(N));   // 2^26 / N
+        v4i pd[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const float base = m[r] == kNegInf ? 0.0f : m[r];
+            uint32_t u[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                float e = __builtin_amdgcn_exp2f(f[r][t] - base), x = fmaf(e, fv, 0.5f);
+                if (!all && first + t >= limit[r]) e = x = 0.0f;
+                l[r] += e;
+                u[t] = (static_cast<uint32_t>(static_cast<int>(x)) + 0x80808080u) ^ 0x80808080u;
+            }
+            // A scale that is no number shows in l: whole numbers cannot.
+            if (all || first < limit[r]) l[r] = fmaf(fv, 0.0f, l[r]);
+            const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), e = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
+            const uint32_t d = __builtin_amdgcn_perm(u[1], u[0], 0x07030602u), k = __builtin_amdgcn_perm(u[3], u[2], 0x07030602u);
+            uint32_t *to = sh_p + 64 * g + col;
+            to[0] = __builtin_amdgcn_perm(e, a, 0x05040100u);
+            to[16] = __builtin_amdgcn_perm(e, a, 0x07060302u);
+            to[32] = __builtin_amdgcn_perm(k, d, 0x05040100u);
+            to[48] = __builtin_amdgcn_perm(k, d, 0x07060302u);
+            __builtin_amdgcn_wave_barrier();
+            pd[r] = *reinterpret_cast<const v4i *>(sh_p + 16 * col + 4 * g);
+            __builtin_amdgcn_wave_barrier();
+        }
+        if (more) wait_copies<DP, FULL>(tiles);   // the next K's may be under way
+        else lds::wait_vmcnt<0>();
+        v4i vf[DT];
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+            if (FULL || t < static_cast<int>(tiles)) vf[t] = *reinterpret_cast<const v4i *>(v_lds + 1024 * t + v_at);
+        __builtin_amdgcn_s_waitcnt(lds::waitcnt_imm(63, 7, 0));
+        if (more) {
+            copy_v(chunk + WAVES);
+            scales();
+            pages(min(chunk + 2 * WAVES, end - 1));
         }
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            if (16 * t >= static_cast<int>(D)) continue;
-            v8h a[2];
+            if (!FULL && t >= static_cast<int>(tiles)) continue;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                v2h x, y;
-                halves_of(vf[t][w], x, y);
-                a[w / 2][4 * (w & 1)] = x[0];
-                a[w / 2][4 * (w & 1) + 1] = x[1];
-                a[w / 2][4 * (w & 1) + 2] = y[0];
-                a[w / 2][4 * (w & 1) + 3] = y[1];
-            }
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    st[r].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[k], lo[r][k], st[r].o[t], 0, 0, 0);
-                    st[r].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[k], hi[r][k], st[r].o[t], 0, 0, 0);
-                }
+            for (int r = 0; r < RT; ++r) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[r], vf[t], acc[r][t], 0, 0, 0);
         }
-        if (more) {
-            load_v(chunk + 4);
-            ids(min(chunk + 8, end - 1));
-        }
+        chunk += WAVES;
     };
-    uint32_t chunk = begin + wave;
-    if (len && chunk < end) {
-        ids(chunk);
-        load_k(chunk);
-        load_v(chunk);
-        ids(min(chunk + 4, end - 1));
-        for (; chunk + 4 < end; chunk += 4) step(chunk, std::true_type{});
-        step(chunk, std::false_type{});
+    if (any) {
+        while (chunk + WAVES < end) step(std::true_type{});
+        step(std::false_type{});
     }
+    if (strange) kv::fail(c.err);
 
     // The waves' parts together: each is o / l, weighed by l 2^(m - max m).
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        st[r].l = groups_sum(st[r].l);
-        if (g == 0) {
-            sh_m[wave][16 * r + col] = st[r].m;
-            sh_l[wave][16 * r + col] = st[r].l;
+        const float sum = row_sum(l[r]);
+        gather(r, sum != 0.0f ? N * 1.4901161193847656e-08f / sum : 0.0f);   // 2^-26
+        if (col == 0) {
+            sh_m[wave][4 * r + g] = m[r];
+            sh_l[wave][4 * r + g] = sum;
         }
     }
-    const uint64_t part_at = (static_cast<uint64_t>(slot) * c.c.kv_heads + h) * ws_rows;
-    const bool whole = sl.parts == 1;
-    float *ws_o = ws + part_at * (D + 2);
+    __syncthreads();
+    float *ws_o = ws + (static_cast<uint64_t>(slot) * G + h) * ws_rows * (D + 2);
+    const uint32_t count = min(rows, static_cast<uint32_t>(R));
+    for (uint32_t e = threadIdx.x; e < count * DP; e += 64 * WAVES) {
+        const uint32_t row = e / DP, d = e % DP;
+        if (!FULL && d >= D) continue;
+        float M = kNegInf, L = 0.0f, o = 0.0f;
 #pragma unroll
-    for (int d0 = 0; d0 < DP; d0 += 64) {
-        if (d0 >= static_cast<int>(D)) continue;
-        __syncthreads();
+        for (int w = 0; w < WAVES; ++w) M = fmaxf(M, sh_m[w][row]);
+        const float base = M == kNegInf ? 0.0f : M;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const float by = st[r].l != 0.0f ? N * 6.103515625e-05f / st[r].l : 0.0f;   // 2^-14
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                *reinterpret_cast<v4f *>(&sh_o[wave][16 * r + col][16 * t + 4 * g]) = st[r].o[d0 / 16 + t] * by;
+        for (int w = 0; w < WAVES; ++w) {
+            const float x = sh_l[w][row] * __builtin_amdgcn_exp2f(sh_m[w][row] - base);
+            L += x;
+            o = fmaf(x, sh_o_all[((w * RT + row / 4) * DT + d / 16) * 64 + 16 * (row & 3) + (d & 15)], o);
         }
-        __syncthreads();
-        const uint32_t d = d0 + lane;
-        for (uint32_t row = wave; row < min(rows, static_cast<uint32_t>(R)); row += 4) {
-            float M = kNegInf, L = 0.0f, o = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) M = fmaxf(M, sh_m[w][row]);
-            const float base = M == kNegInf ? 0.0f : M;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float x = sh_l[w][row] * __builtin_amdgcn_exp2f(sh_m[w][row] - base);
-                L += x;
-                o = fmaf(x, sh_o[w][row][lane], o);
-            }
-            o = L != 0.0f ? o / L : 0.0f;
-            if (d < D) {
-                if (whole)
-                    p.O[kv::rows_base(c, p.o, sl.b, seq) + row / group * p.o.token + (h * group + row % group) * p.o.head + d] = o;
-                else
-                    ws_o[row * (D + 2) + d] = o;
-            }
-            if (!whole && d0 == 0 && lane < 2) ws_o[row * (D + 2) + D + lane] = lane ? L : M;
+        o = L != 0.0f ? o / L : 0.0f;
+        if (parts == 1) {
+            p.O[kv::rows_base(c, p.o, b, seq) + row / group * p.o.token + (h * group + row % group) * p.o.head + d] = o;
+        } else {
+            ws_o[row * (D + 2) + d] = o;
+            if (d < 2) ws_o[row * (D + 2) + D + d] = d ? L : M;
         }
     }
 }
@@ -677,7 +880,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tile(KvAttn p, Tiles tl, 
 #pragma unroll
                 for (int s = 0; s < DS; ++s) kf[t][s] = *reinterpret_cast<const v4i *>(now + (t * DS + s) * 1024 + lane * 16);
             const float above = groups_max(power_above(v_scale)), N_now = fmaxf(N, above);
-            const float beta = N / N_now, fv = v_scale * up_over(N_now);
+            const float beta = power_ratio(N, N_now), fv = v_scale * up_over(N_now);
             N = N_now;
             const int first = static_cast<int>(kChunk * chunk + 16 * g);
             const bool all = static_cast<int>(kChunk * chunk + kChunk) <= least;
@@ -769,15 +972,16 @@ __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, con
     join_parts(at, step, tl.parts, D, lane, out);
 }
 
-constexpr uint32_t kStreamRows = 32;
+// Rows that the kernel of few rows has registers for.
+uint32_t few_rows(uint32_t D) { return D > 128 ? 8 : 16; }
 
 struct Plan {
-    bool stream = false, tiled = false;   // kernels of the call: sequences of few rows, of many
+    bool few = false, tiled = false;   // kernels of the call: sequences of few rows, of many
     Split split{};
-    uint32_t slots = 0, rows = 0;   // of the stream kernel: slots a kv head, rows a slot at most
+    uint32_t slots = 0, rows = 0;   // of the kernel of few rows: slots a kv head, rows a slot at most
     Tiles tiles{};
     uint32_t tile_rows = 0;
-    size_t stream_ws = 0, ws = 0;
+    size_t few_ws = 0, ws = 0;
 };
 Plan plan_of(const KvAttn &p)
 {
@@ -785,23 +989,24 @@ Plan plan_of(const KvAttn &p)
     const KvCall &c = p.call;
     const uint32_t G = c.c.kv_heads, group = p.heads / G, D = c.c.head_dim;
     const uint64_t most = static_cast<uint64_t>(p.max_tokens) * group;
-    r.tiled = most > kStreamRows;
+    const uint32_t at_most = few_rows(D);
+    r.tiled = most > at_most;
     // Without seq_start all sequences have max_tokens.
-    r.stream = !r.tiled || c.seq_start;
-    if (r.stream) {
-        r.rows = static_cast<uint32_t>(std::min<uint64_t>(most, kStreamRows));
+    r.few = !r.tiled || c.seq_start;
+    if (r.few) {
+        r.rows = static_cast<uint32_t>(std::min<uint64_t>(most, at_most));
         r.split.target = (2 * p.cus + G - 1) / G;
         r.split.min_per = 4;
         r.split.low_rows = 0;
-        r.split.high_rows = kStreamRows;
+        r.split.high_rows = at_most;
         r.slots = r.split.target + c.batch;
         if (p.max_kv <= r.split.min_per * kChunk) r.slots = c.batch;   // none splits
-        else r.stream_ws = (static_cast<size_t>(r.slots) * G * r.rows * (D + 2) * sizeof(float) + 15) / 16 * 16;
+        else r.few_ws = (static_cast<size_t>(r.slots) * G * r.rows * (D + 2) * sizeof(float) + 15) / 16 * 16;
     }
-    r.ws = r.stream_ws;
+    r.ws = r.few_ws;
     if (r.tiled) {
         r.tile_rows = most <= 64 || D > 128 ? 64 : 128;
-        r.tiles.low_rows = r.stream ? kStreamRows : 0;
+        r.tiles.low_rows = r.few ? at_most : 0;
         r.tiles.per_seq = static_cast<uint32_t>((most + r.tile_rows - 1) / r.tile_rows);
         r.tiles.count = c.seq_start ? static_cast<uint32_t>(static_cast<uint64_t>(c.tokens) * group / r.tile_rows) + c.batch
                                     : r.tiles.per_seq * c.batch;
@@ -814,9 +1019,15 @@ Plan plan_of(const KvAttn &p)
 }
 
 template <int DP, int RT>
-void launch_stream(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
+void launch_few(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 {
-    kv_attention_stream<DP, RT><<<dim3(pl.slots, p.call.c.kv_heads), 256, 0, s>>>(p, pl.split, ws, pl.rows);
+    constexpr int W = DP > 128 ? 2 : 4;
+    constexpr uint32_t bytes = few_lds<DP, RT, W>();
+    const bool full = p.call.c.head_dim == DP;
+    const auto kernel = full ? kv_attention_few<DP, RT, true, W> : kv_attention_few<DP, RT, false, W>;
+    if (bytes > 60 * 1024)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    kernel<<<dim3(pl.slots, p.call.c.kv_heads), 64 * W, bytes, s>>>(p, pl.split, ws, pl.rows);
 }
 template <int DP, int RT>
 void launch_tile(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
@@ -832,14 +1043,15 @@ void launch_tile(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 template <int DP>
 void launch(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 {
-    if (pl.stream) {
-        if (pl.rows <= 16) launch_stream<DP, 1>(s, p, pl, ws);
-        else launch_stream<DP, 2>(s, p, pl, ws);
-        if (pl.stream_ws)
+    if (pl.few) {
+        if (pl.rows <= 4) launch_few<DP, 1>(s, p, pl, ws);
+        else if (pl.rows <= 8) launch_few<DP, 2>(s, p, pl, ws);
+        else if constexpr (DP <= 128) launch_few<DP, 4>(s, p, pl, ws);
+        if (pl.few_ws)
             kv_attention_merge<<<dim3(p.call.batch, p.call.c.kv_heads, pl.rows), 64, 0, s>>>(p, pl.split, ws, pl.rows);
     }
     if (pl.tiled) {
-        float *rest = ws + pl.stream_ws / sizeof(float);
+        float *rest = ws + pl.few_ws / sizeof(float);
         if constexpr (DP > 128) launch_tile<DP, 1>(s, p, pl, rest);
         else if (pl.tile_rows == 64) launch_tile<DP, 1>(s, p, pl, rest);
         else launch_tile<DP, 2>(s, p, pl, rest);
@@ -852,7 +1064,7 @@ std::string kv_attention_route(const KvAttn &p)
 {
     const Plan pl = plan_of(p);
     char text[96];
-    std::snprintf(text, sizeof(text), "stream=%u rows=%u tile=%u parts=%u", pl.stream ? pl.slots : 0, pl.rows,
+    std::snprintf(text, sizeof(text), "few=%u rows=%u tile=%u parts=%u", pl.few ? pl.slots : 0, pl.rows,
                   pl.tile_rows, pl.tiles.parts);
     return text;
 }
