@@ -90,31 +90,29 @@ __device__ __forceinline__ float power_ratio(float a, float b)
 __device__ __forceinline__ float up_over(float n) { return __uint_as_float((268u << 23) - __float_as_uint(n)); }
 
 // ---------------------------------------------------------------------------
-// Which workgroup does what.  kv_len is on the device, so the host gives a
-// grid of `target + batch` slots for each kv head and the workgroups share the
-// keys out themselves: `per` chunks each, so that all sequences together take
+// Which workgroup does what.  kv_len is on the device.  With enough sequences
+// and heads a slot is a sequence (whole); else the host gives a grid of
+// `target + batch` slots for each kv head and the workgroups share the keys out
+// themselves: `per` chunks each, so that all sequences together take
 // `target` slots and their ragged ends at most one more each.
 // ---------------------------------------------------------------------------
 
 struct Split {
-    uint32_t target, min_per;    // slots aimed at; least chunks of a slot
+    uint32_t whole;                 // slot = sequence
+    uint32_t target, min_per;       // slots aimed at; least chunks of a slot
     uint32_t low_rows, high_rows;   // sequences with rows in (low, high] are this kernel's
 };
 struct Slot {
     uint32_t b, part, parts, per, chunks;
 };
 
-__device__ __forceinline__ uint32_t wave_total(uint32_t v)
-{
-    for (int o = 1; o < 64; o <<= 1) v += static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o));
-    return v;
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v)   // inclusive
+// Inclusive sums over the first `count` lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t count)
 {
     const uint32_t lane = threadIdx.x & 63;
-    for (int o = 1; o < 64; o <<= 1) {
+    for (uint32_t o = 1; o < 64 && o < count; o <<= 1) {
         const uint32_t x = static_cast<uint32_t>(__shfl_up(static_cast<int>(v), o));
-        if (lane >= static_cast<uint32_t>(o)) v += x;
+        if (lane >= o) v += x;
     }
     return v;
 }
@@ -131,19 +129,33 @@ __device__ __forceinline__ uint32_t chunks_of(const KvAttn &p, const Split &sp, 
         return 0;
     return max(1u, (static_cast<uint32_t>(len) + kChunk - 1) / kChunk);
 }
-// The slot's share, or (of_b) sequence b's parts and first slot; by each wave.
+// The slot's share, or (of_b) sequence r.b's parts and first slot; by each wave.
 __device__ __forceinline__ bool find_slot(const KvAttn &p, const Split &sp, bool of_b, uint32_t &slot, Slot &r)
 {
     const uint32_t lane = threadIdx.x & 63, batch = p.call.batch;
+    if (sp.whole || batch == 1) {
+        if (sp.whole) r.b = slot;
+        else r.b = 0;
+        r.chunks = chunks_of(p, sp, r.b);
+        r.per = sp.whole ? r.chunks : max(sp.min_per, (r.chunks + sp.target - 1) / sp.target);
+        r.parts = r.chunks ? (r.chunks + r.per - 1) / r.per : 0;
+        if (of_b) slot = 0;
+        r.part = sp.whole ? 0 : slot;
+        return r.part < r.parts;
+    }
     uint64_t total = 0;
-    for (uint32_t i = 0; i < batch; i += 64) total += wave_total(chunks_of(p, sp, i + lane));
+    for (uint32_t i = 0; i < batch; i += 64) {
+        const uint32_t n = min(64u, batch - i);
+        total += static_cast<uint32_t>(__shfl(static_cast<int>(wave_scan(chunks_of(p, sp, i + lane), n)), n - 1));
+    }
     const uint64_t share = (total + sp.target - 1) / sp.target;
     r.per = max(sp.min_per, static_cast<uint32_t>(share));
     uint32_t before = 0;
     for (uint32_t i = 0; i < batch; i += 64) {
+        const uint32_t n = min(64u, batch - i);
         const uint32_t c = chunks_of(p, sp, i + lane), parts = (c + r.per - 1) / r.per;
-        const uint32_t upto = wave_scan(parts);
-        const uint64_t hit = of_b ? (r.b - i < 64 ? 1ull << (r.b - i) : 0) : __ballot(before + upto > slot);
+        const uint32_t upto = wave_scan(parts, n);
+        const uint64_t hit = of_b ? (r.b - i < 64 ? 1ull << (r.b - i) : 0) : __ballot(lane < n && before + upto > slot);
         if (hit) {
             const int at = __ffsll(static_cast<unsigned long long>(hit)) - 1;
             const uint32_t first = before + static_cast<uint32_t>(__shfl(static_cast<int>(upto - parts), at));
@@ -154,7 +166,7 @@ __device__ __forceinline__ bool find_slot(const KvAttn &p, const Split &sp, bool
             r.part = slot - first;
             return r.parts > 0;
         }
-        before += static_cast<uint32_t>(__shfl(static_cast<int>(upto), 63));
+        before += static_cast<uint32_t>(__shfl(static_cast<int>(upto), n - 1));
     }
     return false;
 }
@@ -426,10 +438,10 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
                 constexpr int kPer = DP / 64;   // copies of a block
                 const uint32_t j = i / kPer, in = (16 * min(4 * chunk + j, last16)) & (ps - 1);
                 const uint32_t piece = 64 * (i % kPer) + lane, key = piece / (DP / 16), at = piece % (DP / 16);
-                lds::dma16(c.c.k + (unit[j] * ps + in + key) * DP + 16 * (at ^ ((4 * j + key / 4) & kSwap)), k_lds + 1024 * i);
+                lds::dma16_nt(c.c.k + (unit[j] * ps + in + key) * DP + 16 * (at ^ ((4 * j + key / 4) & kSwap)), k_lds + 1024 * i);
             } else {
                 const uint32_t piece = 64 * i + lane, j = piece / D, in = (16 * min(4 * chunk + j, last16)) & (ps - 1);
-                lds::dma16(c.c.k + (of_block(j, unit) * ps + in) * D + 16 * (piece - j * D), k_lds + 1024 * i);
+                lds::dma16_nt(c.c.k + (of_block(j, unit) * ps + in) * D + 16 * (piece - j * D), k_lds + 1024 * i);
             }
         }
     };
@@ -446,7 +458,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
         const int8_t *from = c.c.v + (of_block(v_block, unit) * D + v_dim) * ps + in;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
-            if (FULL || t < static_cast<int>(tiles)) lds::dma16(from + static_cast<uint64_t>(16 * t) * ps, v_lds + 1024 * t);
+            if (FULL || t < static_cast<int>(tiles)) lds::dma16_nt(from + static_cast<uint64_t>(16 * t) * ps, v_lds + 1024 * t);
     };
     uint32_t chunk = begin + wave;
     const bool any = len && chunk < end;
@@ -676,30 +688,57 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
 }
 
 // Parts of a row, `step` floats apart, each o / l with its m and l behind it:
-// weighed by l 2^(m - max m).  One wave.
-__device__ __forceinline__ void join_parts(const float *at, uint64_t step, uint32_t parts, uint32_t D, uint32_t lane, float *out)
+// weighed by l 2^(m - max m).  A workgroup a row: the weights first, a part a
+// thread, then the sums, threads over the dimensions and every few parts.
+constexpr uint32_t kJoinThreads = 512, kMostParts = 1024;
+__device__ __forceinline__ void join_parts(const float *at, uint64_t step, uint32_t parts, uint32_t D, float *out)
 {
-    float M = kNegInf, L = 0.0f, o[4] = {};
-    for (uint32_t i = lane; i < parts; i += 64) M = fmaxf(M, at[i * step + D]);
-    for (int x = 32; x; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
-    const float base = M == kNegInf ? 0.0f : M;
-    for (uint32_t i = 0; i < parts; ++i) {
-        const float x = at[i * step + D + 1] * __builtin_amdgcn_exp2f(at[i * step + D] - base);
-        L += x;
+    __shared__ float weight[kMostParts], sums[kJoinThreads], red[2][kJoinThreads / 64];
+    const uint32_t tid = threadIdx.x, wave = tid >> 6;
+    float m[kMostParts / kJoinThreads], l[kMostParts / kJoinThreads], M = kNegInf, L = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (lane + 64 * r < D) o[r] = fmaf(x, at[i * step + lane + 64 * r], o[r]);
+    for (uint32_t k = 0; k < kMostParts / kJoinThreads; ++k) {
+        const uint32_t i = tid + k * kJoinThreads;
+        m[k] = i < parts ? at[i * step + D] : kNegInf;
+        l[k] = i < parts ? at[i * step + D + 1] : 0.0f;
+        M = fmaxf(M, m[k]);
     }
+    for (int x = 32; x; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
+    if ((tid & 63) == 0) red[0][wave] = M;
+    __syncthreads();
+    for (uint32_t w = 0; w < kJoinThreads / 64; ++w) M = fmaxf(M, red[0][w]);
+    const float base = M == kNegInf ? 0.0f : M;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (lane + 64 * r < D) out[lane + 64 * r] = L != 0.0f ? o[r] / L : 0.0f;
+    for (uint32_t k = 0; k < kMostParts / kJoinThreads; ++k) {
+        const float x = l[k] * __builtin_amdgcn_exp2f(m[k] - base);
+        weight[tid + k * kJoinThreads] = x;
+        L += x;
+    }
+    for (int x = 32; x; x >>= 1) L += __shfl_xor(L, x);
+    if ((tid & 63) == 0) red[1][wave] = L;
+    __syncthreads();
+    L = 0.0f;
+    for (uint32_t w = 0; w < kJoinThreads / 64; ++w) L += red[1][w];
+    const uint32_t width = D <= 64 ? 64 : D <= 128 ? 128 : 256, every = kJoinThreads / width, d = tid % width;
+    float o = 0.0f;
+    if (d < D) {
+#pragma unroll 8
+        for (uint32_t i = tid / width; i < parts; i += every) o = fmaf(weight[i], at[i * step + d], o);
+    }
+    sums[tid] = o;
+    __syncthreads();
+    if (tid < D) {
+        o = 0.0f;
+        for (uint32_t k = 0; k < every; ++k) o += sums[tid + k * width];
+        out[tid] = L != 0.0f ? o / L : 0.0f;
+    }
 }
 
-// A sequence's parts together, one wave for a row.
-__global__ __launch_bounds__(64) void kv_attention_merge(KvAttn p, Split sp, const float *ws, uint32_t ws_rows)
+// A sequence's parts together.
+__global__ __launch_bounds__(kJoinThreads) void kv_attention_merge(KvAttn p, Split sp, const float *ws, uint32_t ws_rows)
 {
     const KvCall &c = p.call;
-    const uint32_t lane = threadIdx.x, h = blockIdx.y, row = blockIdx.z, D = c.c.head_dim, group = p.heads / c.c.kv_heads;
+    const uint32_t h = blockIdx.y, row = blockIdx.z, D = c.c.head_dim, group = p.heads / c.c.kv_heads;
     Slot sl;
     sl.b = blockIdx.x;
     uint32_t slot = 0;
@@ -708,7 +747,7 @@ __global__ __launch_bounds__(64) void kv_attention_merge(KvAttn p, Split sp, con
     if (row >= seq.n * group) return;
     const uint64_t step = static_cast<uint64_t>(c.c.kv_heads) * ws_rows * (D + 2);
     const float *at = ws + ((static_cast<uint64_t>(slot) * c.c.kv_heads + h) * ws_rows + row) * (D + 2);
-    join_parts(at, step, sl.parts, D, lane,
+    join_parts(at, step, sl.parts, D,
                p.O + kv::rows_base(c, p.o, sl.b, seq) + row / group * p.o.token + (h * group + row % group) * p.o.head);
 }
 
@@ -954,22 +993,21 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tile(KvAttn p, Tiles tl, 
     }
 }
 
-// A tile's key ranges together, one wave for a row.
+// A tile's key ranges together.
 template <uint32_t M>
-__global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, const float *ws)
+__global__ __launch_bounds__(kJoinThreads) void kv_attention_join(KvAttn p, Tiles tl, const float *ws)
 {
     const KvCall &c = p.call;
-    const uint32_t lane = threadIdx.x & 63, G = c.c.kv_heads, h = blockIdx.x % G, unit = blockIdx.x / G, D = c.c.head_dim;
-    const uint32_t group = p.heads / G;
+    const uint32_t G = c.c.kv_heads, h = blockIdx.x % G, unit = blockIdx.x / G, D = c.c.head_dim, group = p.heads / G;
     uint32_t b, tile, len;
     kv::Seq seq;
     if (!find_tile<M>(p, tl, group, unit, b, tile) || !tile_sequence(p, tl, group, b, seq, len)) return;
-    const uint32_t in = blockIdx.y * 4 + (threadIdx.x >> 6), row = tile * M + in;
-    if (static_cast<uint64_t>(tile) * M + in >= static_cast<uint64_t>(seq.n) * group) return;
+    const uint32_t row = tile * M + blockIdx.y;
+    if (static_cast<uint64_t>(tile) * M + blockIdx.y >= static_cast<uint64_t>(seq.n) * group) return;
     const uint64_t step = static_cast<uint64_t>(M) * (D + 4);
-    const float *at = ws + ((static_cast<uint64_t>(unit) * G + h) * tl.parts * M + in) * (D + 4);
-    float *out = p.O + kv::rows_base(c, p.o, b, seq) + (row / group) * p.o.token + (h * group + row % group) * p.o.head;
-    join_parts(at, step, tl.parts, D, lane, out);
+    const float *at = ws + ((static_cast<uint64_t>(unit) * G + h) * tl.parts * M + blockIdx.y) * (D + 4);
+    join_parts(at, step, tl.parts, D,
+               p.O + kv::rows_base(c, p.o, b, seq) + (row / group) * p.o.token + (h * group + row % group) * p.o.head);
 }
 
 // Rows that the kernel of few rows has registers for.
@@ -995,13 +1033,19 @@ Plan plan_of(const KvAttn &p)
     r.few = !r.tiled || c.seq_start;
     if (r.few) {
         r.rows = static_cast<uint32_t>(std::min<uint64_t>(most, at_most));
-        r.split.target = (2 * p.cus + G - 1) / G;
+        r.split.target = std::min((2 * p.cus + G - 1) / G, kMostParts);
         r.split.min_per = 4;
+        // A sequence and kv head as one workgroup: 9 us and 1.05 us for each 256
+        // keys, or the codes at 6.2 TB/s; split: 14 us with the join, codes at 5.0
+        // (8 heads of 128, 4096 keys: 1 sequence 25.5 and 15.0 us, 16 sequences
+        // 30.1 and 32.0; 32 heads, 8 sequences 43.6 and 57.6).  Sequences are taken to be
+        // 0.6 of max_kv long.
+        const double mb = 1.2e-6 * c.batch * G * D * p.max_kv;
+        r.split.whole = std::max(9.0 + 1.05 * ((p.max_kv + 255) / 256), mb / 6.2) <= 14.0 + mb / 5.0;
         r.split.low_rows = 0;
         r.split.high_rows = at_most;
-        r.slots = r.split.target + c.batch;
-        if (p.max_kv <= r.split.min_per * kChunk) r.slots = c.batch;   // none splits
-        else r.few_ws = (static_cast<size_t>(r.slots) * G * r.rows * (D + 2) * sizeof(float) + 15) / 16 * 16;
+        r.slots = r.split.whole ? c.batch : r.split.target + c.batch;
+        if (!r.split.whole) r.few_ws = (static_cast<size_t>(r.slots) * G * r.rows * (D + 2) * sizeof(float) + 15) / 16 * 16;
     }
     r.ws = r.few_ws;
     if (r.tiled) {
@@ -1038,7 +1082,7 @@ void launch_tile(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
                                   hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     const uint32_t grid = pl.tiles.count * p.call.c.kv_heads;
     kv_attention_tile<DP, RT><<<dim3(grid, pl.tiles.parts), 256, bytes, s>>>(p, pl.tiles, ws);
-    if (pl.tiles.parts > 1) kv_attention_join<64 * RT><<<dim3(grid, 16 * RT), 256, 0, s>>>(p, pl.tiles, ws);
+    if (pl.tiles.parts > 1) kv_attention_join<64 * RT><<<dim3(grid, 64 * RT), kJoinThreads, 0, s>>>(p, pl.tiles, ws);
 }
 template <int DP>
 void launch(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
@@ -1048,7 +1092,7 @@ void launch(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
         else if (pl.rows <= 8) launch_few<DP, 2>(s, p, pl, ws);
         else if constexpr (DP <= 128) launch_few<DP, 4>(s, p, pl, ws);
         if (pl.few_ws)
-            kv_attention_merge<<<dim3(p.call.batch, p.call.c.kv_heads, pl.rows), 64, 0, s>>>(p, pl.split, ws, pl.rows);
+            kv_attention_merge<<<dim3(p.call.batch, p.call.c.kv_heads, pl.rows), kJoinThreads, 0, s>>>(p, pl.split, ws, pl.rows);
     }
     if (pl.tiled) {
         float *rest = ws + pl.few_ws / sizeof(float);
