@@ -369,11 +369,12 @@ __device__ __forceinline__ void wait_copies(uint32_t n)
     }
 }
 
-// Bytes of dynamic LDS: a chunk's K and V a wave, its digits and its f32 sums.
+// Bytes of dynamic LDS: a chunk's K and V a wave, its digits and its f32
+// sums; the queries.
 template <int DP, int RT, int WAVES>
 constexpr uint32_t few_lds()
 {
-    return WAVES * (128 * DP + 1024 + RT * DP * 16);
+    return WAVES * (128 * DP + 1024 + RT * DP * 16) + RT * (DP / 64) * 1024;
 }
 
 template <int DP, int RT, bool FULL, int WAVES>
@@ -381,7 +382,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
 {
     constexpr int DS = DP / 64, DT = DP / 16, R = 4 * RT;
     extern __shared__ __align__(1024) int8_t lds[];
-    __shared__ float sh_m[WAVES][R], sh_l[WAVES][R];
+    __shared__ float sh_m[WAVES][R], sh_l[WAVES][R], sh_f[R];
     const KvCall &c = p.call;
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -395,25 +396,33 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
     if (!find_slot(p, sp, false, slot, sl)) return;
     const uint32_t b = __builtin_amdgcn_readfirstlane(sl.b), parts = __builtin_amdgcn_readfirstlane(sl.parts);
     const kv::Seq seq = kv::sequence(c, b);
-    const uint32_t n = __builtin_amdgcn_readfirstlane(seq.n), rows = n * group;
+    const uint32_t n = __builtin_amdgcn_readfirstlane(seq.n), rows = n * group, row0 = blockIdx.z * R;
+    if (row0 >= rows) return;
     const int len = __builtin_amdgcn_readfirstlane(c.lengths[b]);
-    const uint32_t begin = __builtin_amdgcn_readfirstlane(sl.part * sl.per);
-    const uint32_t end = __builtin_amdgcn_readfirstlane(min(sl.chunks, sl.part * sl.per + sl.per));
+    // Even parts of the keys.
+    const uint32_t chunks = __builtin_amdgcn_readfirstlane(sl.chunks), part = __builtin_amdgcn_readfirstlane(sl.part);
+    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * part / parts);
+    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * (part + 1) / parts);
 
     // Pages of a chunk's four blocks of 16 keys (blocks behind the last are
     // the last) and, of the chunk in LDS, their scales.
     const uint32_t last16 = len ? (len - 1) / 16 : 0, log16 = c.c.log_page - 4, tiles = D / 16;
     const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld;
     bool strange = false;   // a page outside the pool: page 0 is read in its place
-    uint64_t unit[4];
+    int32_t id[4] = {};
+    uint64_t unit[4] = {};
     float ks4[4], vs4[4];
+    // Asked for a chunk ahead: `pages` waits for nothing, `units` for them.
     auto pages = [&](uint32_t chunk) {
 #pragma unroll
+        for (int j = 0; j < 4; ++j) id[j] = scalar_load(table + (min(4 * chunk + j, last16) >> log16));
+    };
+    auto units = [&]() {
+#pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int32_t id = scalar_load(table + (min(4 * chunk + j, last16) >> log16));
-            const bool in = static_cast<uint32_t>(id) < c.c.pages;
+            const bool in = static_cast<uint32_t>(id[j]) < c.c.pages;
             strange |= !in;
-            unit[j] = static_cast<uint64_t>(static_cast<uint32_t>(in ? id : 0)) * G + h;
+            unit[j] = static_cast<uint64_t>(static_cast<uint32_t>(in ? id[j] : 0)) * G + h;
         }
     };
     auto scales = [&]() {
@@ -462,89 +471,115 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
     };
     uint32_t chunk = begin + wave;
     const bool any = len && chunk < end;
+    if (any) pages(chunk);
+    // The rows' queries to LDS (where the f32 sums will be), all loads at once.
+    const bool aligned = ((reinterpret_cast<uintptr_t>(p.Q) & 15) | (p.q.batch & 3) | (p.q.token & 3) | (p.q.head & 3)) == 0;
+    constexpr int kLoads = (R * DP / 4 + 64 * WAVES - 1) / (64 * WAVES);
+    float4 *sh_x = reinterpret_cast<float4 *>(sh_o_all);
+    const float *q_base = p.Q + kv::rows_base(c, p.q, b, seq) + h * group * p.q.head;
+    float4 raw[kLoads];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+        const uint32_t e = threadIdx.x + k * 64 * WAVES, r = e / (DP / 4), d = 4 * (e % (DP / 4)), row = row0 + r, i = row / group;
+        raw[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r < R && row < rows && d < D) {
+            const float *at = q_base + i * p.q.token + (row - i * group) * p.q.head + d;
+            raw[k] = aligned ? *reinterpret_cast<const float4 *>(at) : make_float4(at[0], at[1], at[2], at[3]);
+        }
+    }
+    if (any) units();
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+        const uint32_t e = threadIdx.x + k * 64 * WAVES;
+        if (e < R * DP / 4) sh_x[e] = raw[k];
+    }
     if (any) {
-        pages(chunk);
         copy_k(chunk);
         copy_v(chunk);
         scales();
         pages(min(chunk + WAVES, end - 1));
     }
+    __syncthreads();
 
-    // Queries: lane (operand row 4 r + d, group g) holds digit d of row r's elements 64 s + 16 g .. + 15.
-    const bool aligned = ((reinterpret_cast<uintptr_t>(p.Q) & 15) | (p.q.batch & 3) | (p.q.token & 3) | (p.q.head & 3)) == 0;
-    v4i q[RT][DS];
-    float factor[RT], m[RT], l[RT];   // of row g: score in powers of two = sum * factor * k_scale
-    int limit[RT];                    // keys that row g sees
-    v4i acc[RT][DT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        const uint32_t row = 4 * r + (col >> 2), i = row / group;
-        const bool here = row < rows;
-        const float *at = p.Q + kv::rows_base(c, p.q, b, seq) + (here ? i * p.q.token + (h * group + row % group) * p.q.head : 0);
-        float x[DS * 16];
+    // Queries: lane (operand row 4 r + d, group g) holds digit d of row r's
+    // elements 64 s + 16 g .. + 15.  The waves share the (r, s) out and hand
+    // them over in LDS.
+    v4i *sh_q = reinterpret_cast<v4i *>(lds + WAVES * (128 * DP + 1024 + RT * DP * 16));
+#pragma unroll 1
+    for (uint32_t task = wave; task < RT * DS; task += WAVES) {
+        const uint32_t r = task / DS, s = task % DS;
+        const float4 *at = sh_x + (4 * r + (col >> 2)) * (DP / 4) + 4 * g;
         uint32_t most = 0;
-#pragma unroll
-        for (int s = 0; s < DS; ++s) {
-            const uint32_t d = 64 * s + 16 * g;
+        float x[16];
+#pragma unroll 1
+        for (uint32_t k = 1; k <= DS; ++k) {   // the task's own step last
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (here && d < D) {
-                    const float *e = at + d + 4 * w;
-                    v = aligned ? *reinterpret_cast<const float4 *>(e) : make_float4(e[0], e[1], e[2], e[3]);
-                }
-                x[16 * s + 4 * w] = v.x;
-                x[16 * s + 4 * w + 1] = v.y;
-                x[16 * s + 4 * w + 2] = v.z;
-                x[16 * s + 4 * w + 3] = v.w;
+                const float4 v = at[16 * ((s + k) % DS) + w];
+                x[4 * w] = v.x;
+                x[4 * w + 1] = v.y;
+                x[4 * w + 2] = v.z;
+                x[4 * w + 3] = v.w;
             }
-        }
 #pragma unroll
-        for (int e = 0; e < DS * 16; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+            for (int e = 0; e < 16; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+        }
         most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
         most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
         const float up = most < 0x0f800000u ? 7.922816251426434e28f : 1.0f;   // below 2^-96: times 2^96
         const float S = most ? kDigits4 / (__uint_as_float(most) * up) : 1.0f;
-        const float f = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : p.scale * 1.4426950408889634f / S / up;
-        // Lane (operand row 4 r + d) has row r's factor; the products leave row g in group g.
-        factor[r] = __shfl(f, 4 * static_cast<int>(g));
+        if (s == 0 && g == 0 && (col & 3) == 0)
+            sh_f[4 * r + (col >> 2)] = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : p.scale * 1.4426950408889634f / S / up;
         const uint32_t d = col & 3, pick = 0x0c0c0000u | (4 + d) << 8 | d;
+        v4i digits;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                u[e] = (static_cast<uint32_t>(static_cast<int>(rintf(x[4 * w + e] * up * S))) + 0x80808080u) ^ 0x80808080u;
+            digits[w] = static_cast<int>(__builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], pick),
+                                                               __builtin_amdgcn_perm(u[1], u[0], pick), 0x05040100u));
+        }
+        sh_q[task * 64 + lane] = digits;
+    }
+    __syncthreads();
+    // With 16 rows the queries stay in LDS: a register spilled in the loop would
+    // wait for the copies under way.
+    constexpr bool kHeld = RT < 4;
+    v4i q[kHeld ? RT : 1][DS], acc[RT][DT];
+    float factor[RT], m[RT], l[RT];   // of row g: score in powers of two = sum * factor * k_scale
+    int limit[RT];                    // keys that row g sees
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
 #pragma unroll
         for (int s = 0; s < DS; ++s)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t u[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    u[e] = (static_cast<uint32_t>(static_cast<int>(rintf(x[16 * s + 4 * w + e] * up * S))) + 0x80808080u) ^ 0x80808080u;
-                q[r][s][w] = static_cast<int>(__builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], pick),
-                                                                    __builtin_amdgcn_perm(u[1], u[0], pick), 0x05040100u));
-            }
-        const uint32_t mine = 4 * r + g;
+            if (kHeld) q[r][s] = sh_q[(r * DS + s) * 64 + lane];
+        factor[r] = sh_f[4 * r + g];
+        const uint32_t mine = row0 + 4 * r + g;
         limit[r] = p.causal && mine < rows ? max(0, len - static_cast<int>(n) + static_cast<int>(mine / group) + 1) : len;
         m[r] = kNegInf;
         l[r] = 0.0f;
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            acc[r][t] = v4i{0, 0, 0, 0};
-            sh_o[(r * DT + t) * 64 + lane] = 0.0f;
-        }
+        for (int t = 0; t < DT; ++t) acc[r][t] = v4i{0, 0, 0, 0};
     }
-    const int least = p.causal ? max(0, len - static_cast<int>(n) + 1) : len;   // every row sees the keys below
+    const int least = p.causal ? max(0, len - static_cast<int>(n) + static_cast<int>(row0 / group) + 1) : len;   // every row sees the keys below
     float N = power_above(0.0f);
     uint32_t since = 0;
+    bool begun = false, kept = false;   // the whole sums, the f32 sums hold something
     // Whole sums to the f32 ones, both by `by`.
     auto gather = [&](int r, float by) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
             if (!FULL && 16 * t >= static_cast<int>(D)) continue;
             float &o = sh_o[(r * DT + t) * 64 + lane];
-            o = (o + digits_sum_wide(acc[r][t])) * by;
+            o = ((kept ? o : 0.0f) + digits_sum_wide(acc[r][t])) * by;
             acc[r][t] = v4i{0, 0, 0, 0};
         }
     };
 
-    auto step = [&](auto more) {
+    for (bool more = any; more;) {
+        more = chunk + WAVES < end;
         const uint32_t kb = col >> 2;
         const float ks = of_block(kb, ks4), scale = of_block(kb, vs4);
         const int first = static_cast<int>(kChunk * chunk + 4 * col);
@@ -559,17 +594,24 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
                 kf[t][s] = *reinterpret_cast<const v4i *>(k_lds + (4 * col + t) * D + 16 * piece);
             }
         __builtin_amdgcn_s_waitcnt(lds::waitcnt_imm(63, 7, 0));
-        if (more) copy_k(chunk + WAVES);
+        if (more) {
+            units();
+            copy_k(chunk + WAVES);
+        }
         float f[RT][4], top[RT];
         bool move = false;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             top[r] = kNegInf;
+            constexpr int H = kHeld ? 1 : 0;
+            if (!kHeld)
+#pragma unroll
+                for (int s = 0; s < DS; ++s) q[0][s] = sh_q[(r * DS + s) * 64 + lane];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 v4i a = {0, 0, 0, 0};
 #pragma unroll
-                for (int s = 0; s < DS; ++s) a = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[r][s], kf[t][s], a, 0, 0, 0);
+                for (int s = 0; s < DS; ++s) a = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[H * r][s], kf[t][s], a, 0, 0, 0);
                 f[r][t] = digits_sum(a);
             }
             const float ck = factor[r] * ks;
@@ -594,11 +636,13 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
             for (int r = 0; r < RT; ++r) {
                 const float now = fmaxf(m[r], row_max(top[r]));
                 const float alpha = now > m[r] ? __builtin_amdgcn_exp2f(m[r] - now) : 1.0f;
-                gather(r, alpha * beta);
+                if (begun) gather(r, alpha * beta);
                 l[r] *= alpha;
                 m[r] = now;
             }
+            kept = begun;
         }
+        begun = true;
         const float fv = scale * __uint_as_float((280u << 23) - __float_as_uint(N));   // 2^26 / N
         v4i pd[RT];
 #pragma unroll
@@ -644,10 +688,6 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
             for (int r = 0; r < RT; ++r) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[r], vf[t], acc[r][t], 0, 0, 0);
         }
         chunk += WAVES;
-    };
-    if (any) {
-        while (chunk + WAVES < end) step(std::true_type{});
-        step(std::false_type{});
     }
     if (strange) kv::fail(c.err);
 
@@ -663,7 +703,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
     }
     __syncthreads();
     float *ws_o = ws + (static_cast<uint64_t>(slot) * G + h) * ws_rows * (D + 2);
-    const uint32_t count = min(rows, static_cast<uint32_t>(R));
+    const uint32_t count = min(rows - row0, static_cast<uint32_t>(R));
     for (uint32_t e = threadIdx.x; e < count * DP; e += 64 * WAVES) {
         const uint32_t row = e / DP, d = e % DP;
         if (!FULL && d >= D) continue;
@@ -678,11 +718,12 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
             o = fmaf(x, sh_o_all[((w * RT + row / 4) * DT + d / 16) * 64 + 16 * (row & 3) + (d & 15)], o);
         }
         o = L != 0.0f ? o / L : 0.0f;
+        const uint32_t at = row0 + row;
         if (parts == 1) {
-            p.O[kv::rows_base(c, p.o, b, seq) + row / group * p.o.token + (h * group + row % group) * p.o.head + d] = o;
+            p.O[kv::rows_base(c, p.o, b, seq) + at / group * p.o.token + (h * group + at % group) * p.o.head + d] = o;
         } else {
-            ws_o[row * (D + 2) + d] = o;
-            if (d < 2) ws_o[row * (D + 2) + D + d] = d ? L : M;
+            ws_o[at * (D + 2) + d] = o;
+            if (d < 2) ws_o[at * (D + 2) + D + d] = d ? L : M;
         }
     }
 }
@@ -798,11 +839,11 @@ __device__ __forceinline__ bool tile_sequence(const KvAttn &p, const Tiles &tl, 
     return seq.ok && n >= 0 && len <= p.max_kv && seq.n <= p.max_tokens && static_cast<uint64_t>(seq.n) * group > tl.low_rows;
 }
 
-template <int DP, int RT>
-__global__ __launch_bounds__(256, 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
+template <int DP, int RT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 && DP <= 128 ? 4 : 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
 {
     constexpr int DS = DP / 64, DT = DP / 16;
-    constexpr uint32_t M = 64 * RT;
+    constexpr uint32_t M = 16 * RT * WAVES;
     constexpr uint32_t kK = 4 * DS * 1024, kV = DT * 2048, kBuf = kK + kV;   // bytes of a chunk's operands
     extern __shared__ __align__(1024) int8_t lds[];
     const KvCall &c = p.call;
@@ -857,23 +898,23 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tile(KvAttn p, Tiles tl, 
         k_id = table[min(4 * chunk + kb, last16) >> log16];
         v_id = table[min(4 * chunk + g, last16) >> log16];
     };
-    constexpr int VW = (DT + 3) / 4;   // tiles of V that a wave brings in
+    constexpr int VW = (DT + WAVES - 1) / WAVES, KW = (4 * DS + WAVES - 1) / WAVES;   // tiles of V, pieces of K that a wave brings in
     v4i vf[VW];
     float ks = 0.0f, vs = 0.0f, N = power_above(0.0f);
     auto fetch = [&](uint32_t chunk, int8_t *buf) {
         const uint32_t in_k = (16 * min(4 * chunk + kb, last16)) & (ps - 1);
         const int8_t *kat = c.c.k + ((static_cast<uint64_t>(checked(k_id)) * G + h) * ps + in_k + (col & 3)) * D;
 #pragma unroll
-        for (int i = 0; i < DS; ++i) {   // operand (tile t, step s) is piece t * DS + s
-            const uint32_t piece = wave + 4 * i, t = piece / DS, s = piece % DS, d = 64 * s + 16 * g;
-            lds::dma16(kat + 4 * t * D + (d < D ? d : 0), buf + piece * 1024);
+        for (int i = 0; i < KW; ++i) {   // operand (tile t, step s) is piece t * DS + s
+            const uint32_t piece = wave + WAVES * i, t = piece / DS, s = piece % DS, d = 64 * s + 16 * g;
+            if (4 * DS % WAVES == 0 || piece < 4 * DS) lds::dma16(kat + 4 * t * D + (d < D ? d : 0), buf + piece * 1024);
         }
         const uint64_t unit_v = static_cast<uint64_t>(checked(v_id)) * G + h;
         const uint32_t in_v = (16 * min(4 * chunk + g, last16)) & (ps - 1);
         const int8_t *vat = c.c.v + (unit_v * D + col) * ps + in_v;
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
-            const uint32_t t = wave + 4 * i;
+            const uint32_t t = wave + WAVES * i;
             if (16 * t < D) vf[i] = *reinterpret_cast<const v4i *>(vat + static_cast<uint64_t>(16 * t) * ps);
         }
         ks = c.c.ks[unit_v];
@@ -882,7 +923,7 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tile(KvAttn p, Tiles tl, 
     auto turn_v = [&](int8_t *buf) {
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
-            const uint32_t t = wave + 4 * i;
+            const uint32_t t = wave + WAVES * i;
             if (16 * t >= D) continue;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -913,11 +954,6 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tile(KvAttn p, Tiles tl, 
         const bool work = static_cast<int>(kChunk * chunk) < wave_keys;
         v8h hi[RT][2], lo[RT][2];
         if (work) {
-            v4i kf[4][DS];
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int s = 0; s < DS; ++s) kf[t][s] = *reinterpret_cast<const v4i *>(now + (t * DS + s) * 1024 + lane * 16);
             const float above = groups_max(power_above(v_scale)), N_now = fmaxf(N, above);
             const float beta = power_ratio(N, N_now), fv = v_scale * up_over(N_now);
             N = N_now;
@@ -931,9 +967,10 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tile(KvAttn p, Tiles tl, 
                     v4i a0 = {}, a1 = {}, a2 = {};
 #pragma unroll
                     for (int s = 0; s < DS; ++s) {
-                        a0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][s], q[r].digit[0][s], a0, 0, 0, 0);
-                        a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][s], q[r].digit[1][s], a1, 0, 0, 0);
-                        a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][s], q[r].digit[2][s], a2, 0, 0, 0);
+                        const v4i k = *reinterpret_cast<const v4i *>(now + (t * DS + s) * 1024 + lane * 16);
+                        a0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[r].digit[0][s], a0, 0, 0, 0);
+                        a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[r].digit[1][s], a1, 0, 0, 0);
+                        a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[r].digit[2][s], a2, 0, 0, 0);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -993,25 +1030,46 @@ __global__ __launch_bounds__(256, 2) void kv_attention_tile(KvAttn p, Tiles tl, 
     }
 }
 
-// A tile's key ranges together.
+// A tile's key ranges, at most 64, together: a wave a row, a range's weight a lane.
 template <uint32_t M>
-__global__ __launch_bounds__(kJoinThreads) void kv_attention_join(KvAttn p, Tiles tl, const float *ws)
+__global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, const float *ws)
 {
     const KvCall &c = p.call;
     const uint32_t G = c.c.kv_heads, h = blockIdx.x % G, unit = blockIdx.x / G, D = c.c.head_dim, group = p.heads / G;
     uint32_t b, tile, len;
     kv::Seq seq;
     if (!find_tile<M>(p, tl, group, unit, b, tile) || !tile_sequence(p, tl, group, b, seq, len)) return;
-    const uint32_t row = tile * M + blockIdx.y;
-    if (static_cast<uint64_t>(tile) * M + blockIdx.y >= static_cast<uint64_t>(seq.n) * group) return;
+    const uint32_t lane = threadIdx.x & 63, in = blockIdx.y * 4 + (threadIdx.x >> 6), row = tile * M + in;
+    if (static_cast<uint64_t>(tile) * M + in >= static_cast<uint64_t>(seq.n) * group) return;
     const uint64_t step = static_cast<uint64_t>(M) * (D + 4);
-    const float *at = ws + ((static_cast<uint64_t>(unit) * G + h) * tl.parts * M + blockIdx.y) * (D + 4);
-    join_parts(at, step, tl.parts, D,
-               p.O + kv::rows_base(c, p.o, b, seq) + (row / group) * p.o.token + (h * group + row % group) * p.o.head);
+    const float *at = ws + ((static_cast<uint64_t>(unit) * G + h) * tl.parts * M + in) * (D + 4);
+    const float m = lane < tl.parts ? at[lane * step + D] : kNegInf, l = lane < tl.parts ? at[lane * step + D + 1] : 0.0f;
+    float top = m;
+    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    const float weight = l * __builtin_amdgcn_exp2f(m - (top == kNegInf ? 0.0f : top));
+    float sum = weight, o[4] = {};
+    for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+    for (uint32_t i = 0; i < tl.parts; ++i) {
+        const float w = __shfl(weight, i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (lane + 64 * r < D) o[r] = fmaf(w, at[i * step + lane + 64 * r], o[r]);
+    }
+    float *out = p.O + kv::rows_base(c, p.o, b, seq) + (row / group) * p.o.token + (h * group + row % group) * p.o.head;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (lane + 64 * r < D) out[lane + 64 * r] = sum != 0.0f ? o[r] / sum : 0.0f;
 }
 
-// Rows that the kernel of few rows has registers for.
-uint32_t few_rows(uint32_t D) { return D > 128 ? 8 : 16; }
+// Rows that the kernel of few rows takes: one workgroup's, or two's where all
+// sequences' keys together are few.  (20 rows of 8 heads of 128, 3001 keys:
+// 1 sequence 17 us against 27 in tiles, 4 of 700 to 3001 keys 23 and 29, 4 of 3001 keys 37 and 29.)
+uint32_t few_rows(const KvAttn &p)
+{
+    const uint32_t one = p.call.c.head_dim > 128 ? 8 : 16;
+    const double keys = (p.call.seq_start ? 0.6 : 1.0) * p.call.batch * p.call.c.kv_heads * p.max_kv;
+    return keys <= 65536 ? 2 * one : one;
+}
 
 struct Plan {
     bool few = false, tiled = false;   // kernels of the call: sequences of few rows, of many
@@ -1027,13 +1085,19 @@ Plan plan_of(const KvAttn &p)
     const KvCall &c = p.call;
     const uint32_t G = c.c.kv_heads, group = p.heads / G, D = c.c.head_dim;
     const uint64_t most = static_cast<uint64_t>(p.max_tokens) * group;
-    const uint32_t at_most = few_rows(D);
+    const uint32_t at_most = few_rows(p);
     r.tiled = most > at_most;
-    // Without seq_start all sequences have max_tokens.
-    r.few = !r.tiled || c.seq_start;
+    // Without seq_start all sequences have max_tokens.  Beside sequences of many
+    // rows the few-row ones have a launch of their own where they may be many;
+    // some more tiles cost less than that (6 sequences of 4 heads: 22 us).
+    r.few = !r.tiled || (c.seq_start && static_cast<uint64_t>(c.batch) * G >= p.cus / 2);
     if (r.few) {
         r.rows = static_cast<uint32_t>(std::min<uint64_t>(most, at_most));
-        r.split.target = std::min((2 * p.cus + G - 1) / G, kMostParts);
+        // Slots for as many workgroups as run at a time (16 rows take the LDS
+        // of a CU), the ragged ends among them.
+        const uint32_t tile = D > 128 ? (r.rows <= 4 ? 4 : 8) : r.rows <= 4 ? 4 : r.rows <= 8 ? 8 : 16;
+        const uint32_t at_once = (tile == 16 ? 1 : 2) * p.cus / (G * ((r.rows + tile - 1) / tile));
+        r.split.target = std::min(std::max(at_once > c.batch ? at_once - c.batch / 2 : at_once / 2, 1u), kMostParts);
         r.split.min_per = 4;
         // A sequence and kv head as one workgroup: 9 us and 1.05 us for each 256
         // keys, or the codes at 6.2 TB/s; split: 14 us with the join, codes at 5.0
@@ -1044,7 +1108,11 @@ Plan plan_of(const KvAttn &p)
         r.split.whole = std::max(9.0 + 1.05 * ((p.max_kv + 255) / 256), mb / 6.2) <= 14.0 + mb / 5.0;
         r.split.low_rows = 0;
         r.split.high_rows = at_most;
-        r.slots = r.split.whole ? c.batch : r.split.target + c.batch;
+        // No more slots than parts of the longest: a workgroup without work takes its turn too.
+        r.slots = r.split.whole ? c.batch
+                                : static_cast<uint32_t>(std::min<uint64_t>(
+                                      r.split.target + c.batch,
+                                      static_cast<uint64_t>(c.batch) * ((p.max_kv + r.split.min_per * kChunk - 1) / (r.split.min_per * kChunk))));
         if (!r.split.whole) r.few_ws = (static_cast<size_t>(r.slots) * G * r.rows * (D + 2) * sizeof(float) + 15) / 16 * 16;
     }
     r.ws = r.few_ws;
@@ -1056,7 +1124,7 @@ Plan plan_of(const KvAttn &p)
                                     : r.tiles.per_seq * c.batch;
         const uint64_t grid = static_cast<uint64_t>(r.tiles.count) * G;
         const uint32_t chunks = (p.max_kv + kChunk - 1) / kChunk;
-        r.tiles.parts = grid >= p.cus ? 1 : std::max<uint32_t>(1, std::min<uint64_t>(2 * p.cus / grid, chunks / 8));
+        r.tiles.parts = grid >= p.cus ? 1 : std::max<uint32_t>(1, std::min<uint64_t>(std::min<uint64_t>(64, 2 * p.cus / grid), chunks / 8));
         if (r.tiles.parts > 1) r.ws += static_cast<size_t>(grid) * r.tiles.parts * r.tile_rows * (D + 4) * sizeof(float);
     }
     return r;
@@ -1071,34 +1139,34 @@ void launch_few(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
     const auto kernel = full ? kv_attention_few<DP, RT, true, W> : kv_attention_few<DP, RT, false, W>;
     if (bytes > 60 * 1024)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    kernel<<<dim3(pl.slots, p.call.c.kv_heads), 64 * W, bytes, s>>>(p, pl.split, ws, pl.rows);
+    const uint32_t tiles = (pl.rows + 4 * RT - 1) / (4 * RT);
+    kernel<<<dim3(pl.slots, p.call.c.kv_heads, tiles), 64 * W, bytes, s>>>(p, pl.split, ws, pl.rows);
 }
-template <int DP, int RT>
+template <int DP, int RT, int WAVES>
 void launch_tile(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 {
     constexpr uint32_t bytes = 2 * (4 * (DP / 64) * 1024 + (DP / 16) * 2048);
     if (bytes > 60 * 1024)
-        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_attention_tile<DP, RT>),
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_attention_tile<DP, RT, WAVES>),
                                   hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     const uint32_t grid = pl.tiles.count * p.call.c.kv_heads;
-    kv_attention_tile<DP, RT><<<dim3(grid, pl.tiles.parts), 256, bytes, s>>>(p, pl.tiles, ws);
-    if (pl.tiles.parts > 1) kv_attention_join<64 * RT><<<dim3(grid, 64 * RT), kJoinThreads, 0, s>>>(p, pl.tiles, ws);
+    kv_attention_tile<DP, RT, WAVES><<<dim3(grid, pl.tiles.parts), 64 * WAVES, bytes, s>>>(p, pl.tiles, ws);
+    if (pl.tiles.parts > 1) kv_attention_join<16 * RT * WAVES><<<dim3(grid, 4 * RT * WAVES), 256, 0, s>>>(p, pl.tiles, ws);
 }
 template <int DP>
 void launch(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 {
     if (pl.few) {
         if (pl.rows <= 4) launch_few<DP, 1>(s, p, pl, ws);
-        else if (pl.rows <= 8) launch_few<DP, 2>(s, p, pl, ws);
+        else if (DP > 128 || pl.rows <= 8) launch_few<DP, 2>(s, p, pl, ws);
         else if constexpr (DP <= 128) launch_few<DP, 4>(s, p, pl, ws);
         if (pl.few_ws)
             kv_attention_merge<<<dim3(p.call.batch, p.call.c.kv_heads, pl.rows), kJoinThreads, 0, s>>>(p, pl.split, ws, pl.rows);
     }
     if (pl.tiled) {
         float *rest = ws + pl.few_ws / sizeof(float);
-        if constexpr (DP > 128) launch_tile<DP, 1>(s, p, pl, rest);
-        else if (pl.tile_rows == 64) launch_tile<DP, 1>(s, p, pl, rest);
-        else launch_tile<DP, 2>(s, p, pl, rest);
+        if (DP > 128 || pl.tile_rows == 64) launch_tile<DP, 1, 4>(s, p, pl, rest);
+        else if constexpr (DP <= 128) launch_tile<DP, 2, 4>(s, p, pl, rest);
     }
 }
 
