@@ -11,7 +11,7 @@
 //   new codes = round(x * f32(1 / s)), half away from zero, in +-127.
 // One page and kv head is one workgroup: it alone reads and writes that
 // page's codes and scale, so nothing is atomic and results do not depend on
-// order.  The new tokens' f32 values are read once and stay in registers
+// order; K and V are workgroups of their own, Q's rows others.  The new tokens' f32 values are read once and stay in registers
 // between the largest magnitude and the codes.
 #include "device_math.hpp"
 #include "kv_common.hpp"
@@ -107,115 +107,106 @@ __device__ __forceinline__ PageScale page_scale(uint32_t largest, bool kept, flo
     return r;
 }
 
-// Thread e of m * D / 2 pairs has pair e % (D / 2) of token e / (D / 2); pairs
-// per thread: PAIRS.  Codes go through LDS (dynamic, page_size * D bytes) so
-// that the cache is written 16 bytes at a time.
-template <int T, int PAIRS>
-__global__ __launch_bounds__(T) void kv_append_kernel(KvAppend p, Rates rates, uint32_t half_magic)
+// Elements of pair j of a row, in the first half of the turned ones or beside each other.
+__device__ __forceinline__ uint2 pair_at(const KvAppend &p, uint32_t j)
 {
-    extern __shared__ __align__(16) int8_t tile[];
-    __shared__ uint32_t red[2][T / 64];
+    const uint32_t turns = p.rope_dim / 2;
+    return p.rotation == 1 && j < turns ? make_uint2(j, j + turns) : make_uint2(2 * j, 2 * j + 1);
+}
+
+// Workgroups of a call: 2 units * kv_heads that append (even: K, odd: V of a
+// page and head), then those that turn Q, which are cut as their number asks.
+struct AppendGrid {
+    uint32_t units, q_splits, half_magic;
+};
+
+// One page and head of K or V.  Thread e of m * D / 2 pairs has pair e % (D /
+// 2) of token e / (D / 2); PAIRS of a thread.  Codes go through LDS (dynamic,
+// page_size * D bytes) so that the cache is written 16 bytes at a time.
+template <int T, int PAIRS, bool V>
+__device__ __forceinline__ void append_page(const KvAppend &p, const Rates &rates, uint32_t magic, uint32_t b, const kv::Piece &pc,
+                                            uint32_t h, int8_t *tile, uint32_t *red)
+{
     const KvCall &c = p.call;
-    const uint32_t h = blockIdx.y, tid = threadIdx.x;
-    if (blockIdx.x == 0 && h == 0) kv::check_all(c, true, kv::capacity(c));
-    uint32_t b;
-    kv::Piece pc;
-    if (!kv::find_piece(c, blockIdx.x, b, pc)) return;
-    const uint32_t D = c.c.head_dim, half = D / 2, ps = c.c.page_size, turns = p.rotation ? p.rope_dim / 2 : 0;
-    const uint32_t pairs = pc.m * half;
-    const uint64_t position = static_cast<uint64_t>(c.lengths[b]) + pc.first;
+    const uint32_t tid = threadIdx.x, D = c.c.head_dim, half = D / 2, ps = c.c.page_size, pairs = pc.m * half;
     const uint64_t unit = static_cast<uint64_t>(pc.page) * c.c.kv_heads + h;
-    const float *K = p.K + kv::rows_base(c, p.k, b, pc.seq) + pc.first * p.k.token + h * p.k.head;
-    const float *V = p.V + kv::rows_base(c, p.v, b, pc.seq) + pc.first * p.v.token + h * p.v.head;
-    const float k_before = c.c.ks[unit], v_before = c.c.vs[unit];
-    const uint32_t group = p.heads / c.c.kv_heads;
+    const KvRows &rows = V ? p.v : p.k;
+    const float *in = (V ? p.V : p.K) + kv::rows_base(c, rows, b, pc.seq) + pc.first * rows.token + h * rows.head;
+    float *scales = V ? c.c.vs : c.c.ks;
+    const float before = scales[unit];
+    const uint64_t position = static_cast<uint64_t>(c.lengths[b]) + pc.first;
+    const uint32_t turns = !V && p.rotation ? p.rope_dim / 2 : 0;
 
-    float2 kx[PAIRS], vx[PAIRS];
-    uint32_t k_most = 0, v_most = 0;
+    float2 x[PAIRS];
+    uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
         const uint32_t e = tid + i * T;
-        kx[i] = vx[i] = make_float2(0.0f, 0.0f);
+        x[i] = make_float2(0.0f, 0.0f);
         if (e >= pairs) continue;
-        const uint32_t t = __umulhi(e, half_magic), j = e - t * half;
-        const bool turn = j < turns;
-        const uint32_t d0 = turn && p.rotation == 1 ? j : 2 * j, d1 = turn && p.rotation == 1 ? j + turns : 2 * j + 1;
-        const float *kr = K + t * p.k.token, *vr = V + t * p.v.token;
-        kx[i] = make_float2(kr[d0], kr[d1]);
-        vx[i] = make_float2(vr[2 * j], vr[2 * j + 1]);
-        float cs = 1.0f, sn = 0.0f;
-        if (turn) {
+        const uint32_t t = __umulhi(e, magic), j = e - t * half;
+        const uint2 d = V ? make_uint2(2 * j, 2 * j + 1) : pair_at(p, j);
+        const float *row = in + t * rows.token;
+        x[i] = make_float2(row[d.x], row[d.y]);
+    }
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+        const uint32_t e = tid + i * T, t = __umulhi(e, magic), j = e - t * half;
+        if (!V && e < pairs && j < turns) {
+            float cs, sn;
             cos_sin_turns(static_cast<double>(position + t) * rates.turns[j], cs, sn);
-            kx[i] = turned(kx[i], cs, sn);
+            x[i] = turned(x[i], cs, sn);
         }
-        k_most = max(k_most, max(__float_as_uint(kx[i].x) & 0x7fffffffu, __float_as_uint(kx[i].y) & 0x7fffffffu));
-        v_most = max(v_most, max(__float_as_uint(vx[i].x) & 0x7fffffffu, __float_as_uint(vx[i].y) & 0x7fffffffu));
-        for (uint32_t g = 0; g < group; ++g) {
-            const uint32_t qh = h * group + g;
-            const float *qr = p.Q + kv::rows_base(c, p.q, b, pc.seq) + (pc.first + t) * p.q.token + qh * p.q.head;
-            float *qo = p.Q_out + kv::rows_base(c, p.o, b, pc.seq) + (pc.first + t) * p.o.token + qh * p.o.head;
-            float2 x = make_float2(qr[d0], qr[d1]);
-            if (turn) x = turned(x, cs, sn);
-            qo[d0] = x.x;
-            qo[d1] = x.y;
-        }
+        most = max(most, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
     }
-    k_most = block_largest<T>(k_most, red[0]);
-    v_most = block_largest<T>(v_most, red[1]);
-    const bool kept = pc.slot > 0;
-    const PageScale ks = page_scale(k_most, kept, k_before), vs = page_scale(v_most, kept, v_before);
+    const PageScale s = page_scale(block_largest<T>(most, red), pc.slot > 0, before);
+    if (tid == 0) scales[unit] = s.scale;
+    if (s.scale != s.scale) return;   // under a NaN scale the codes stay
 
-    // K: [slot][D], the new tokens' bytes are one run.
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
         const uint32_t e = tid + i * T;
         if (e >= pairs) continue;
-        const uint32_t t = __umulhi(e, half_magic), j = e - t * half;
-        const bool first_half = j < turns && p.rotation == 1;
-        tile[t * D + (first_half ? j : 2 * j)] = static_cast<int8_t>(code_of(kx[i].x, ks.inv));
-        tile[t * D + (first_half ? j + turns : 2 * j + 1)] = static_cast<int8_t>(code_of(kx[i].y, ks.inv));
+        const uint32_t t = __umulhi(e, magic), j = e - t * half;
+        const int8_t c0 = static_cast<int8_t>(code_of(x[i].x, s.inv)), c1 = static_cast<int8_t>(code_of(x[i].y, s.inv));
+        if (V) {
+            tile[2 * j * ps + pc.slot + t] = c0;
+            tile[(2 * j + 1) * ps + pc.slot + t] = c1;
+        } else {
+            const uint2 d = pair_at(p, j);
+            tile[t * D + d.x] = c0;
+            tile[t * D + d.y] = c1;
+        }
     }
     __syncthreads();
-    uint4 *kp = reinterpret_cast<uint4 *>(c.c.k + unit * ps * D);
     const uint4 *tp = reinterpret_cast<const uint4 *>(tile);
-    const uint32_t row16 = D / 16;
-    const uint32_t k_bytes16 = ks.scale == ks.scale ? pc.m * row16 : 0;   // under a NaN scale the codes stay
-    for (uint32_t e = tid; e < k_bytes16; e += T) kp[pc.slot * row16 + e] = tp[e];
-    if (ks.ratio != 1.0f)
-        for (uint32_t e = tid; e < pc.slot * row16; e += T) {
-            const uint4 o = kp[e];
-            kp[e] = make_uint4(rescaled4(o.x, ks.ratio), rescaled4(o.y, ks.ratio), rescaled4(o.z, ks.ratio), rescaled4(o.w, ks.ratio));
-        }
-    __syncthreads();
-
-    // V: [D][slot], rows of page_size bytes of which the new tokens are a part.
-#pragma unroll
-    for (int i = 0; i < PAIRS; ++i) {
-        const uint32_t e = tid + i * T;
-        if (e >= pairs) continue;
-        const uint32_t t = __umulhi(e, half_magic), j = e - t * half;
-        tile[2 * j * ps + pc.slot + t] = static_cast<int8_t>(code_of(vx[i].x, vs.inv));
-        tile[(2 * j + 1) * ps + pc.slot + t] = static_cast<int8_t>(code_of(vx[i].y, vs.inv));
+    uint4 *to = reinterpret_cast<uint4 *>((V ? c.c.v : c.c.k) + unit * ps * D);
+    if (!V) {   // [slot][D]: the new tokens' bytes are one run
+        const uint32_t row16 = D / 16;
+        for (uint32_t e = tid; e < pc.m * row16; e += T) to[pc.slot * row16 + e] = tp[e];
+        if (s.ratio != 1.0f)
+            for (uint32_t e = tid; e < pc.slot * row16; e += T) {
+                const uint4 o = to[e];
+                to[e] = make_uint4(rescaled4(o.x, s.ratio), rescaled4(o.y, s.ratio), rescaled4(o.z, s.ratio), rescaled4(o.w, s.ratio));
+            }
+        return;
     }
-    __syncthreads();
-    uint4 *vp = reinterpret_cast<uint4 *>(c.c.v + unit * ps * D);
+    // [D][slot]: rows of page_size bytes of which the new tokens are a part.
     const uint32_t log16 = c.c.log_page - 4, end = pc.slot + pc.m;
-    const uint32_t from16 = vs.ratio != 1.0f ? 0 : pc.slot / 16, to16 = (end + 15) / 16, n16 = to16 - from16;
-    const uint32_t v_bytes16 = vs.scale == vs.scale ? D * n16 : 0;
-    for (uint32_t e = tid; e < v_bytes16; e += T) {
-        const uint32_t d = e / n16, s16 = from16 + e % n16, s0 = 16 * s16;
-        const uint32_t at = (d << log16) + s16;
+    const uint32_t from16 = s.ratio != 1.0f ? 0 : pc.slot / 16, n16 = (end + 15) / 16 - from16;
+    for (uint32_t e = tid; e < D * n16; e += T) {
+        const uint32_t d = e / n16, s16 = from16 + e % n16, s0 = 16 * s16, at = (d << log16) + s16;
         const uint4 fresh = tp[at];
         if (s0 >= pc.slot && s0 + 16 <= end) {
-            vp[at] = fresh;
+            to[at] = fresh;
             continue;
         }
-        const uint4 old = vp[at];
+        const uint4 old = to[at];
         const uint32_t o4[4] = {old.x, old.y, old.z, old.w}, f4[4] = {fresh.x, fresh.y, fresh.z, fresh.w};
         uint32_t r4[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const uint32_t moved = vs.ratio != 1.0f ? rescaled4(o4[w], vs.ratio) : o4[w];
+            const uint32_t moved = s.ratio != 1.0f ? rescaled4(o4[w], s.ratio) : o4[w];
             r4[w] = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -223,58 +214,150 @@ __global__ __launch_bounds__(T) void kv_append_kernel(KvAppend p, Rates rates, u
                 r4[w] |= (slot < pc.slot ? moved : slot < end ? f4[w] : o4[w]) & m;
             }
         }
-        vp[at] = make_uint4(r4[0], r4[1], r4[2], r4[3]);
+        to[at] = make_uint4(r4[0], r4[1], r4[2], r4[3]);
     }
-    if (tid == 0) {
-        c.c.ks[unit] = ks.scale;
-        c.c.vs[unit] = vs.scale;
+}
+
+// Queries: a thread has one pair of a token and turns it in some of the heads.
+template <int T>
+__device__ __forceinline__ void turn_queries(const KvAppend &p, const Rates &rates, uint32_t magic, uint32_t block, uint32_t splits)
+{
+    const KvCall &c = p.call;
+    const uint32_t half = c.c.head_dim / 2, per = (p.heads + splits - 1) / splits;
+    const uint64_t e = static_cast<uint64_t>(block / splits) * T + threadIdx.x;
+    uint32_t row, j;
+    if (e < 65536) {
+        row = __umulhi(static_cast<uint32_t>(e), magic);
+        j = static_cast<uint32_t>(e) - row * half;
+    } else {
+        row = static_cast<uint32_t>(e / half);
+        j = static_cast<uint32_t>(e % half);
     }
+    if (row >= c.tokens) return;
+    uint32_t b;
+    if (!c.seq_start) {
+        b = row / (c.tokens / c.batch);
+    } else {   // the last sequence that begins here or before
+        uint32_t lo = 0, hi = c.batch;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (static_cast<uint32_t>(c.seq_start[mid]) <= row) lo = mid + 1;
+            else hi = mid;
+        }
+        if (!lo) return;
+        b = lo - 1;
+    }
+    const kv::Seq seq = kv::sequence(c, b);
+    const int64_t past = c.lengths[b];
+    const uint32_t i = row - seq.row;
+    if (!seq.ok || i >= seq.n || past < 0 || past + seq.n > static_cast<int64_t>(kv::capacity(c))) return;   // check_all told
+    const uint2 d = pair_at(p, j);
+    float cs = 1.0f, sn = 0.0f;
+    const bool turn = p.rotation && j < p.rope_dim / 2;
+    if (turn) cos_sin_turns(static_cast<double>(past + i) * rates.turns[j], cs, sn);
+    const uint32_t h0 = block % splits * per, h1 = min(p.heads, h0 + per);
+    const float *in = p.Q + kv::rows_base(c, p.q, b, seq) + i * p.q.token;
+    float *out = p.Q_out + kv::rows_base(c, p.o, b, seq) + i * p.o.token;
+    for (uint32_t h = h0; h < h1; h += 8) {
+        float2 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (h + k < h1) x[k] = make_float2(in[(h + k) * p.q.head + d.x], in[(h + k) * p.q.head + d.y]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (h + k >= h1) continue;
+            if (turn) x[k] = turned(x[k], cs, sn);
+            out[(h + k) * p.o.head + d.x] = x[k].x;
+            out[(h + k) * p.o.head + d.y] = x[k].y;
+        }
+    }
+}
+
+template <int T, int PAIRS>
+__global__ __launch_bounds__(T) void kv_append_kernel(KvAppend p, Rates rates, AppendGrid grid)
+{
+    extern __shared__ __align__(16) int8_t tile[];
+    __shared__ uint32_t red[T / 64];
+    const KvCall &c = p.call;
+    if (blockIdx.x == 0) kv::check_all(c, true, kv::capacity(c));
+    const uint32_t appends = 2 * grid.units * c.c.kv_heads;
+    if (blockIdx.x >= appends) {
+        turn_queries<T>(p, rates, grid.half_magic, blockIdx.x - appends, grid.q_splits);
+        return;
+    }
+    const uint32_t rest = blockIdx.x / 2, h = rest % c.c.kv_heads;
+    uint32_t b;
+    kv::Piece pc;
+    if (!kv::find_piece(c, rest / c.c.kv_heads, b, pc)) return;
+    if (blockIdx.x & 1) append_page<T, PAIRS, true>(p, rates, grid.half_magic, b, pc, h, tile, red);
+    else append_page<T, PAIRS, false>(p, rates, grid.half_magic, b, pc, h, tile, red);
 }
 
 constexpr int kReadThreads = 256;
 
-// One page and kv head to f32 rows.  V's codes pass through LDS (dynamic,
-// page_size rows of D + 4 bytes) to turn [D][slot] into rows.
-__global__ __launch_bounds__(kReadThreads) void kv_read_kernel(KvRead p)
+// One page and head of K or V to f32 rows.  V's codes pass through LDS (dynamic,
+// page_size rows of D + 4 bytes) to turn [D][slot] into rows.  VEC: rows that
+// begin at 16 bytes.
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+
+template <bool VEC>
+__device__ __forceinline__ void store4(float *to, uint32_t w, float scale)
+{
+    float4 x;
+    x.x = static_cast<float>(static_cast<int8_t>(w)) * scale;
+    x.y = static_cast<float>(static_cast<int8_t>(w >> 8)) * scale;
+    x.z = static_cast<float>(static_cast<int8_t>(w >> 16)) * scale;
+    x.w = static_cast<float>(static_cast<int8_t>(w >> 24)) * scale;
+    if (VEC) {
+        // Past the caches: the rows are more than they hold where time counts.
+        __builtin_nontemporal_store(f32x4{x.x, x.y, x.z, x.w}, reinterpret_cast<f32x4 *>(to));
+    } else {
+        to[0] = x.x;
+        to[1] = x.y;
+        to[2] = x.z;
+        to[3] = x.w;
+    }
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(kReadThreads) void kv_read_kernel(KvRead p, uint32_t magic)
 {
     extern __shared__ __align__(16) int8_t tile[];
     const KvCall &c = p.call;
+    const bool values = blockIdx.z || !p.K;
     const uint32_t h = blockIdx.y, tid = threadIdx.x;
-    if (blockIdx.x == 0 && h == 0) kv::check_all(c, true, kv::capacity(c));
+    if (blockIdx.x == 0 && h == 0 && blockIdx.z == 0) kv::check_all(c, true, kv::capacity(c));
     uint32_t b;
     kv::Piece pc;
     if (!kv::find_piece(c, blockIdx.x, b, pc)) return;
     const uint32_t D = c.c.head_dim, ps = c.c.page_size, quads = D / 4;
     const uint64_t unit = static_cast<uint64_t>(pc.page) * c.c.kv_heads + h;
-    if (p.K) {
+    if (!values) {
         const float scale = c.c.ks[unit];
         const uint32_t *codes = reinterpret_cast<const uint32_t *>(c.c.k + (unit * ps + pc.slot) * D);
         float *out = p.K + kv::rows_base(c, p.k, b, pc.seq) + pc.first * p.k.token + h * p.k.head;
+#pragma unroll 4
         for (uint32_t e = tid; e < pc.m * quads; e += kReadThreads) {
-            const uint32_t t = e / quads, d = 4 * (e % quads), w = codes[e];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                out[t * p.k.token + d + i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i))) * scale;
+            const uint32_t t = __umulhi(e, magic);
+            store4<VEC>(out + t * p.k.token + 4 * (e - t * quads), codes[e], scale);
         }
+        return;
     }
-    if (p.V) {
-        const float scale = c.c.vs[unit];
-        const uint32_t *codes = reinterpret_cast<const uint32_t *>(c.c.v + unit * ps * D);
-        const uint32_t from4 = pc.slot / 4, n4 = (pc.slot + pc.m + 3) / 4 - from4, row = D + 4;
-        for (uint32_t e = tid; e < D * n4; e += kReadThreads) {
-            const uint32_t d = e / n4, s4 = from4 + e % n4, w = codes[d * (ps / 4) + s4];
+    const float scale = c.c.vs[unit];
+    const uint32_t *codes = reinterpret_cast<const uint32_t *>(c.c.v + unit * ps * D);
+    const uint32_t from4 = pc.slot / 4, n4 = (pc.slot + pc.m + 3) / 4 - from4, row = D + 4;
+#pragma unroll 4
+    for (uint32_t e = tid; e < D * n4; e += kReadThreads) {
+        const uint32_t d = e / n4, s4 = from4 + e % n4, w = codes[d * (ps / 4) + s4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tile[(4 * s4 + i) * row + d] = static_cast<int8_t>(w >> (8 * i));
-        }
-        __syncthreads();
-        float *out = p.V + kv::rows_base(c, p.v, b, pc.seq) + pc.first * p.v.token + h * p.v.head;
-        for (uint32_t e = tid; e < pc.m * quads; e += kReadThreads) {
-            const uint32_t t = e / quads, d = 4 * (e % quads);
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(tile + (pc.slot + t) * row + d);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                out[t * p.v.token + d + i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i))) * scale;
-        }
+        for (int i = 0; i < 4; ++i) tile[(4 * s4 + i) * row + d] = static_cast<int8_t>(w >> (8 * i));
+    }
+    __syncthreads();
+    float *out = p.V + kv::rows_base(c, p.v, b, pc.seq) + pc.first * p.v.token + h * p.v.head;
+#pragma unroll 4
+    for (uint32_t e = tid; e < pc.m * quads; e += kReadThreads) {
+        const uint32_t t = __umulhi(e, magic), d = 4 * (e - t * quads);
+        store4<VEC>(out + t * p.v.token + d, *reinterpret_cast<const uint32_t *>(tile + (pc.slot + t) * row + d), scale);
     }
 }
 
@@ -312,7 +395,15 @@ void launch_append(hipStream_t s, const KvAppend &p, const Rates &rates, uint32_
 {
     const size_t lds = static_cast<size_t>(p.call.c.page_size) * p.call.c.head_dim;
     allow_lds(kv_append_kernel<T, PAIRS>, lds);
-    kv_append_kernel<T, PAIRS><<<dim3(kv::unit_count(p.call), p.call.c.kv_heads), T, lds, s>>>(p, rates, magic);
+    AppendGrid g{kv::unit_count(p.call), 1, magic};
+    uint64_t blocks = 2ull * g.units * p.call.c.kv_heads;
+    if (p.heads) {
+        const uint64_t q = (static_cast<uint64_t>(p.call.tokens) * (p.call.c.head_dim / 2) + T - 1) / T;
+        // Enough workgroups for two a CU, of one head each at least.
+        g.q_splits = static_cast<uint32_t>(std::min<uint64_t>(p.heads, (511 + q) / q));
+        blocks += q * g.q_splits;
+    }
+    kv_append_kernel<T, PAIRS><<<static_cast<uint32_t>(blocks), T, lds, s>>>(p, rates, g);
 }
 }  // namespace
 
@@ -335,8 +426,14 @@ void kv_read(hipStream_t s, const KvRead &p)
 {
     const KvCall &c = p.call;
     const size_t lds = p.V ? static_cast<size_t>(c.c.page_size) * (c.c.head_dim + 4) : 0;
-    allow_lds(kv_read_kernel, lds);
-    kv_read_kernel<<<dim3(kv::unit_count(c), c.c.kv_heads), kReadThreads, lds, s>>>(p);
+    auto vectors = [](const float *at, const KvRows &r) {
+        return !at || !((reinterpret_cast<uintptr_t>(at) & 15) | (r.batch & 3) | (r.token & 3) | (r.head & 3));
+    };
+    const auto kernel = vectors(p.K, p.k) && vectors(p.V, p.v) ? kv_read_kernel<true> : kv_read_kernel<false>;
+    allow_lds(kernel, lds);
+    const uint32_t quads = c.c.head_dim / 4;
+    const uint32_t magic = static_cast<uint32_t>((0x100000000ull + quads - 1) / quads);   // exact below 2^16
+    kernel<<<dim3(kv::unit_count(c), c.c.kv_heads, p.K && p.V ? 2 : 1), kReadThreads, lds, s>>>(p, magic);
 }
 
 }  // namespace k
