@@ -1124,6 +1124,7 @@ k::KvAppend kv_append_params(vnpu_stream_t *s, const vnpu_kv_append_i8_args_t &a
     const KvTensor vt = kv_rows(a.v_batch_stride, a.v_token_stride, a.v_head_stride, G, D, a.batch, a.tokens, ragged, false);
     p.k = kt.rows;
     p.v = vt.rows;
+    uint64_t q_span = 0, qo_span = 0;
     if (a.Q) {
         require(a.heads && a.heads % G == 0 && a.heads <= 65535, "kv heads is a multiple of kv_heads");
         const KvTensor qt = kv_rows(a.q_batch_stride, a.q_token_stride, a.q_head_stride, a.heads, D, a.batch, a.tokens, ragged, false);
@@ -1134,8 +1135,13 @@ k::KvAppend kv_append_params(vnpu_stream_t *s, const vnpu_kv_append_i8_args_t &a
         p.q = qt.rows;
         p.o = ot.rows;
         if (!same || a.rotation != VNPU_ROTATE_NONE) p.heads = a.heads;
-        p.Q_out = src.out(a.Q_out, ot.span);
-        p.Q = same ? p.Q_out : src.in(a.Q, qt.span);
+        q_span = qt.span;
+        qo_span = ot.span;
+    }
+    require(k::kv_append_fits(p), "kv_append too large");
+    if (a.Q) {
+        p.Q_out = src.out(a.Q_out, qo_span);
+        p.Q = a.Q_out == a.Q ? p.Q_out : src.in(a.Q, q_span);
     }
     p.K = src.in(a.K, kt.span);
     p.V = src.in(a.V, vt.span);
@@ -1169,6 +1175,7 @@ k::KvAttn kv_attention_params(vnpu_stream_t *s, const vnpu_kv_attention_i8_args_
     p.causal = a.causal != 0;
     p.scale = a.scale > 0.0f ? a.scale : 1.0f / std::sqrt(static_cast<float>(D));
     p.cus = s->device ? std::max(1u, s->device->cu_count) : 256;
+    require(k::kv_attention_fits(p), "kv_attention too large");
     p.O = src.out(a.O, ot.span);
     p.Q = same ? p.O : src.in(a.Q, qt.span);
     return p;
@@ -1194,6 +1201,7 @@ k::KvRead kv_read_params(vnpu_stream_t *s, const vnpu_kv_read_f32_args_t &a, con
     const KvTensor vt = kv_rows(a.v_batch_stride, a.v_token_stride, a.v_head_stride, G, D, a.batch, a.tokens, ragged, a.V != nullptr);
     p.k = kt.rows;
     p.v = vt.rows;
+    require(k::kv_read_fits(p), "kv_read too large");
     p.K = a.K ? src.out(a.K, kt.span) : nullptr;
     p.V = a.V ? src.out(a.V, vt.span) : nullptr;
     return p;

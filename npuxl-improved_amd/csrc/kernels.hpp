@@ -289,6 +289,11 @@ struct KvRead {
     float *K = nullptr, *V = nullptr;
     KvRows k, v;
 };
+// Whether a call's grid can be launched; nothing else may be asked of one that
+// cannot.
+bool kv_append_fits(const KvAppend &p);
+bool kv_read_fits(const KvRead &p);
+bool kv_attention_fits(const KvAttn &p);
 void kv_append(hipStream_t s, const KvAppend &p);
 void kv_read(hipStream_t s, const KvRead &p);
 // ws holds kv_attention_ws_bytes(p) bytes (0: none is used).

@@ -1181,6 +1181,15 @@ std::string kv_attention_route(const KvAttn &p)
     return text;
 }
 
+// A grid's work-items count in 32 bits.
+bool kv_attention_fits(const KvAttn &p)
+{
+    const Plan pl = plan_of(p);
+    return static_cast<uint64_t>(pl.slots) * 256 < (1ull << 32) &&
+           static_cast<uint64_t>(p.call.batch) * kJoinThreads < (1ull << 32) &&
+           static_cast<uint64_t>(pl.tiles.count) * p.call.c.kv_heads * 256 < (1ull << 32);
+}
+
 size_t kv_attention_ws_bytes(const KvAttn &p) { return plan_of(p).ws; }
 
 void kv_attention(hipStream_t s, const KvAttn &p, void *ws)

@@ -378,9 +378,6 @@ Rates rates_of(float theta, uint32_t dim, float scaling)
     return r;
 }
 
-}  // namespace
-
-namespace {
 // Pages of 256 tokens and heads of 256 take more LDS than a kernel has unasked.
 template <typename Kernel>
 void allow_lds(Kernel kernel, size_t bytes)
@@ -390,12 +387,19 @@ void allow_lds(Kernel kernel, size_t bytes)
                                   static_cast<int>(bytes));
 }
 
-template <int T, int PAIRS>
-void launch_append(hipStream_t s, const KvAppend &p, const Rates &rates, uint32_t magic)
+// Threads of a workgroup and the pairs that each has, for the pairs of a page's
+// new tokens: at most page_size * D / 2 = 32768.
+uint32_t append_pairs(const KvCall &c)
 {
-    const size_t lds = static_cast<size_t>(p.call.c.page_size) * p.call.c.head_dim;
-    allow_lds(kv_append_kernel<T, PAIRS>, lds);
-    AppendGrid g{kv::unit_count(p.call), 1, magic};
+    return std::min(c.seq_start ? c.tokens : c.tokens / c.batch, c.c.page_size) * (c.c.head_dim / 2);
+}
+uint32_t append_threads(const KvCall &c) { return append_pairs(c) <= 4096 ? 256 : 1024; }
+
+uint64_t append_blocks(const KvAppend &p, AppendGrid &g)
+{
+    const uint64_t T = append_threads(p.call);
+    g.units = kv::unit_count(p.call);
+    g.q_splits = 1;
     uint64_t blocks = 2ull * g.units * p.call.c.kv_heads;
     if (p.heads) {
         const uint64_t q = (static_cast<uint64_t>(p.call.tokens) * (p.call.c.head_dim / 2) + T - 1) / T;
@@ -403,23 +407,37 @@ void launch_append(hipStream_t s, const KvAppend &p, const Rates &rates, uint32_
         g.q_splits = static_cast<uint32_t>(std::min<uint64_t>(p.heads, (511 + q) / q));
         blocks += q * g.q_splits;
     }
-    kv_append_kernel<T, PAIRS><<<static_cast<uint32_t>(blocks), T, lds, s>>>(p, rates, g);
+    return blocks;
+}
+
+template <int T, int PAIRS>
+void launch_append(hipStream_t s, const KvAppend &p, uint32_t blocks, const AppendGrid &grid)
+{
+    const size_t lds = static_cast<size_t>(p.call.c.page_size) * p.call.c.head_dim;
+    allow_lds(kv_append_kernel<T, PAIRS>, lds);
+    const Rates rates = p.rotation ? rates_of(p.theta, p.rope_dim, p.scaling) : Rates{};
+    kv_append_kernel<T, PAIRS><<<blocks, T, lds, s>>>(p, rates, grid);
 }
 }  // namespace
 
+// A grid's work-items count in 32 bits.
+bool kv_append_fits(const KvAppend &p)
+{
+    AppendGrid g;
+    return append_blocks(p, g) * append_threads(p.call) < (1ull << 32);
+}
+bool kv_read_fits(const KvRead &p) { return static_cast<uint64_t>(kv::unit_count(p.call)) * kReadThreads < (1ull << 32); }
+
 void kv_append(hipStream_t s, const KvAppend &p)
 {
-    const KvCall &c = p.call;
-    const Rates rates = p.rotation ? rates_of(p.theta, p.rope_dim, p.scaling) : Rates{};
-    const uint32_t half = c.c.head_dim / 2;
-    const uint32_t magic = static_cast<uint32_t>((0x100000000ull + half - 1) / half);   // exact below 2^16
-    // Pairs of a page's new tokens: at most page_size * D / 2 = 32768.
-    const uint32_t most = std::min(c.seq_start ? c.tokens : c.tokens / c.batch, c.c.page_size) * half;
-    if (most <= 256) launch_append<256, 1>(s, p, rates, magic);
-    else if (most <= 1024) launch_append<256, 4>(s, p, rates, magic);
-    else if (most <= 4096) launch_append<256, 16>(s, p, rates, magic);
-    else if (most <= 16384) launch_append<1024, 16>(s, p, rates, magic);
-    else launch_append<1024, 32>(s, p, rates, magic);
+    AppendGrid g;
+    const uint32_t blocks = static_cast<uint32_t>(append_blocks(p, g)), half = p.call.c.head_dim / 2, most = append_pairs(p.call);
+    g.half_magic = static_cast<uint32_t>((0x100000000ull + half - 1) / half);   // exact below 2^16
+    if (most <= 256) launch_append<256, 1>(s, p, blocks, g);
+    else if (most <= 1024) launch_append<256, 4>(s, p, blocks, g);
+    else if (most <= 4096) launch_append<256, 16>(s, p, blocks, g);
+    else if (most <= 16384) launch_append<1024, 16>(s, p, blocks, g);
+    else launch_append<1024, 32>(s, p, blocks, g);
 }
 
 void kv_read(hipStream_t s, const KvRead &p)

@@ -38,16 +38,6 @@ __device__ __forceinline__ uint64_t rows_base(const KvCall &c, const KvRows &r, 
     return c.seq_start ? s.row * r.token : b * r.batch;
 }
 
-// The page of sequence b's tokens pg * page_size and on; 0 and an error where
-// the table names none.
-__device__ __forceinline__ uint32_t page_of(const KvCall &c, uint32_t b, uint32_t pg)
-{
-    const int32_t id = c.c.table[static_cast<uint64_t>(b) * c.c.table_ld + pg];
-    if (static_cast<uint32_t>(id) < c.c.pages) return static_cast<uint32_t>(id);
-    fail(c.err);
-    return 0;
-}
-
 // Append and read work page by page.  The pages that sequences touch are not
 // known to the host: sequence b of n tokens touches at most n / page_size + 2,
 // so its units are given room for that many.  unit -> (b, which of its pages);

@@ -97,3 +97,34 @@ def test_null_arguments():
 
 def test_route_of_a_call():
     assert route(*attention()[:1], **attention()[1]).endswith("ws=0")
+
+
+@pytest.mark.parametrize("make,bad,fine", [
+    (append, dict(batch=1 << 20, tokens=1 << 20, Q=None, Q_out=None, cache=cache(kv_heads=16)), dict(cache=cache(kv_heads=2))),
+    (append, dict(batch=1, tokens=1 << 28, heads=64, cache=cache(kv_heads=1, head_dim=256)), dict(heads=8, tokens=1 << 20)),
+    (attention, dict(batch=1 << 24, tokens=1 << 24, heads=1, cache=cache(kv_heads=1)), dict(batch=1 << 22, tokens=1 << 22)),
+    (attention, dict(batch=1, tokens=1 << 26, heads=64, cache=cache(kv_heads=64)), dict(tokens=1 << 24)),
+    (read, dict(batch=1 << 24, tokens=1 << 24), dict(batch=1 << 20, tokens=1 << 20)),
+])
+def test_grids_that_cannot_be_launched_are_refused(make, bad, fine):
+    """2^32 threads and more in one dimension: pages of a call, sequences, tiles of rows."""
+    opcode, fields = make(**bad)
+    assert not taken(opcode, fields)
+    assert taken(opcode, {**fields, **fine})
+
+
+def test_routes_over_sizes():
+    """One workgroup for a sequence and head, keys split over workgroups, tiles, tiles with split keys, both."""
+    def text(max_kv, batch=1, tokens=1, seq_start=None):
+        c = cache(kv_heads=8, head_dim=128, table_ld=1 << 16)
+        opcode, f = attention(c, batch=batch, tokens=tokens, max_kv=max_kv, seq_start=seq_start)
+        return dict(x.split("=") for x in route(opcode, **f).split())
+
+    assert text(500)["few"] == "1" and text(500)["ws"] == "0"
+    assert int(text(100000)["few"]) > 1 and int(text(100000)["ws"]) > 0
+    assert text(4096, batch=64, tokens=64)["few"] == "64" and text(4096, batch=64, tokens=64)["ws"] == "0"
+    assert text(4096, tokens=64)["few"] == "0" and text(4096, tokens=64)["tile"] == "64"
+    assert text(4096, tokens=4096)["tile"] == "128" and text(4096, tokens=4096)["parts"] == "1"
+    assert int(text(4096, tokens=100)["parts"]) > 1 and int(text(4096, tokens=100)["ws"]) > 0
+    mixed = text(4096, batch=64, tokens=300, seq_start=P)
+    assert mixed["few"] != "0" and mixed["tile"] != "0"
