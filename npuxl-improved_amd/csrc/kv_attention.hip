@@ -24,6 +24,7 @@
 #include "lds_dma.hpp"
 
 #include <algorithm>
+#include <type_traits>
 #include <cstdio>
 
 namespace vnpu {
@@ -242,33 +243,28 @@ struct State {
     }
 };
 
-// Scores f (sums of digits, keys 16 g + 4 t + i) to weights: the softmax step
-// and the two f16 parts of p * v_scale.  seen: this lane's keys below it count.
-// beta: N before over N now.
-template <int DT, bool MASK>
-__device__ __forceinline__ void weigh(State<DT> &st, v4f f[4], float ck, float fv, float beta, int seen, v8h hi[2], v8h lo[2])
+// The largest of a lane's scores f (sums of digits, keys 16 g + 4 t + i).
+// seen: this lane's keys below it count.
+template <bool MASK>
+__device__ __forceinline__ float largest(const v4f f[4], float ck, int seen)
 {
     float top = kNegInf;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, !MASK || 4 * t + i < seen ? f[t][i] : kNegInf);
-    // k scales are not negative: the largest sum is the largest score of the lane.
-    top = MASK && seen <= 0 ? kNegInf : top * ck;
-    const float now = fmaxf(st.m, groups_max(top));
-    const float base = now == kNegInf ? 0.0f : now;
-    const float alpha = __builtin_amdgcn_exp2f(st.m - base);
-    // 1 for rows whose maximum stays; o is left alone where all do.
-    if (__any(now > st.m) || beta != 1.0f) {
-        const float a = now > st.m ? alpha : 1.0f;
-        st.l *= a;
+    // k scales are not negative: the largest sum is the largest score.
+    return MASK && seen <= 0 ? kNegInf : top * ck;
+}
+
+// Scores of tiles 2 half and 2 half + 1 to weights: the two f16 parts of
+// p * v_scale, p added to the lane's sum.
+template <bool MASK>
+__device__ __forceinline__ void weigh(float &sum, const v4f f[4], int half, float ck, float base, float fv, int seen, v8h &hi, v8h &lo)
+{
 #pragma unroll
-        for (int t = 0; t < DT; ++t) st.o[t] *= a * beta;
-        st.m = now;
-    }
-    float sum = 0.0f;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int u = 0; u < 2; ++u) {
+        const int t = 2 * half + u;
         v4f p;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -285,13 +281,12 @@ __device__ __forceinline__ void weigh(State<DT> &st, v4f f[4], float ck, float f
             }
             const v2h h = __builtin_convertvector(x, v2h);
             const v2h r = __builtin_convertvector(x - __builtin_convertvector(h, v2f), v2h);
-            hi[t / 2][4 * (t & 1) + i] = h[0];
-            hi[t / 2][4 * (t & 1) + i + 1] = h[1];
-            lo[t / 2][4 * (t & 1) + i] = r[0];
-            lo[t / 2][4 * (t & 1) + i + 1] = r[1];
+            hi[4 * u + i] = h[0];
+            hi[4 * u + i + 1] = h[1];
+            lo[4 * u + i] = r[0];
+            lo[4 * u + i + 1] = r[1];
         }
     }
-    st.l += sum;
 }
 
 // ---------------------------------------------------------------------------
@@ -839,8 +834,8 @@ __device__ __forceinline__ bool tile_sequence(const KvAttn &p, const Tiles &tl, 
     return seq.ok && n >= 0 && len <= p.max_kv && seq.n <= p.max_tokens && static_cast<uint64_t>(seq.n) * group > tl.low_rows;
 }
 
-template <int DP, int RT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 && DP <= 128 ? 4 : 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
+template <int DP, int RT, bool FULL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
 {
     constexpr int DS = DP / 64, DT = DP / 16;
     constexpr uint32_t M = 16 * RT * WAVES;
@@ -943,62 +938,91 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 && DP <= 128 ? 4 : 2) void k
         lds::wait_vmcnt<0>();
         __syncthreads();
     }
-    for (uint32_t chunk = begin; chunk < end; ++chunk) {
+    auto step = [&](uint32_t chunk, auto works, auto masks) {
+        constexpr bool WORK = decltype(works)::value, MASK = decltype(masks)::value;
         int8_t *now = lds + ((chunk - begin) & 1) * kBuf, *next = lds + ((chunk - begin + 1) & 1) * kBuf;
-        const float ck = ks, v_scale = vs;
+        const float k_scale = ks, v_scale = vs;
         const bool more = chunk + 1 < end;
         if (more) {
             fetch(chunk + 1, next);
             ids(min(chunk + 2, end - 1));
         }
-        const bool work = static_cast<int>(kChunk * chunk) < wave_keys;
-        v8h hi[RT][2], lo[RT][2];
-        if (work) {
+        if constexpr (WORK) {
             const float above = groups_max(power_above(v_scale)), N_now = fmaxf(N, above);
             const float beta = power_ratio(N, N_now), fv = v_scale * up_over(N_now);
             N = N_now;
             const int first = static_cast<int>(kChunk * chunk + 16 * g);
-            const bool all = static_cast<int>(kChunk * chunk + kChunk) <= least;
+            v4f f[RT][4];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                v4f f[4];
+            for (int t = 0; t < 4; ++t) {
+                v4i a[RT][3];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    v4i a0 = {}, a1 = {}, a2 = {};
+                for (int s = 0; s < DS; ++s) {
+                    const v4i k = *reinterpret_cast<const v4i *>(now + (t * DS + s) * 1024 + lane * 16);
 #pragma unroll
-                    for (int s = 0; s < DS; ++s) {
-                        const v4i k = *reinterpret_cast<const v4i *>(now + (t * DS + s) * 1024 + lane * 16);
-                        a0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[r].digit[0][s], a0, 0, 0, 0);
-                        a1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[r].digit[1][s], a1, 0, 0, 0);
-                        a2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[r].digit[2][s], a2, 0, 0, 0);
-                    }
+                    for (int d = 0; d < 3; ++d)
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
+                            a[r][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, q[r].digit[d][s], s ? a[r][d] : v4i{}, 0, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        f[t][i] = fmaf(static_cast<float>(a0[i] * 256 + a1[i]), 256.0f, static_cast<float>(a2[i]));
-                }
-                if (all) weigh<DT, false>(st[r], f, q[r].factor * ck, fv, beta, 16, hi[r], lo[r]);
-                else weigh<DT, true>(st[r], f, q[r].factor * ck, fv, beta, limit[r] - first, hi[r], lo[r]);
+                        f[r][t][i] = fmaf(static_cast<float>(a[r][0][i] * 256 + a[r][1][i]), 256.0f, static_cast<float>(a[r][2][i]));
             }
-        }
-        if (more) turn_v(next);
-        if (work) {
+            float ck[RT], base[RT], top[RT];
+            bool move = beta != 1.0f;
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                if (16 * t >= static_cast<int>(D)) continue;
+            for (int r = 0; r < RT; ++r) {
+                ck[r] = q[r].factor * k_scale;
+                top[r] = fmaxf(st[r].m, groups_max(largest<MASK>(f[r], ck[r], limit[r] - first)));
+                base[r] = top[r] == kNegInf ? 0.0f : top[r];
+                move = move || top[r] > st[r].m;
+            }
+            if (__any(move)) {   // else o is left alone
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const v8h a = *reinterpret_cast<const v8h *>(now + kK + (2 * t + k) * 1024 + lane * 16);
+                for (int r = 0; r < RT; ++r) {
+                    // 1 for rows whose maximum stays.
+                    const float alpha = top[r] > st[r].m ? __builtin_amdgcn_exp2f(st[r].m - base[r]) : 1.0f;
+                    st[r].l *= alpha;
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        st[r].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo[r][k], st[r].o[t], 0, 0, 0);
-                        st[r].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi[r][k], st[r].o[t], 0, 0, 0);
-                    }
+                    for (int t = 0; t < DT; ++t) st[r].o[t] *= alpha * beta;
+                    st[r].m = top[r];
                 }
             }
+            // The products of the first half's weights go beside the second half's exponentials.
+            v8h hi[RT][2], lo[RT][2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) weigh<MASK>(st[r].l, f[r], k, ck[r], base[r], fv, limit[r] - first, hi[r][k], lo[r][k]);
+            }
+            if (more) turn_v(next);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    if (!FULL && 16 * t >= static_cast<int>(D)) continue;
+                    const v8h v = *reinterpret_cast<const v8h *>(now + kK + (2 * t + k) * 1024 + lane * 16);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) st[r].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo[r][k], st[r].o[t], 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) st[r].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi[r][k], st[r].o[t], 0, 0, 0);
+                }
+        } else if (more) {
+            turn_v(next);
         }
         lds::wait_vmcnt<0>();
         __syncthreads();
-    }
+    };
+    // Chunks that every row of the wave sees, that some see, that are other waves'.
+    const uint32_t all_end = min(max(static_cast<uint32_t>(least) / kChunk, begin), end);
+    const uint32_t wave_end = min(max((static_cast<uint32_t>(wave_keys) + kChunk - 1) / kChunk, all_end), end);
+    uint32_t chunk = begin;
+    for (; chunk < all_end; ++chunk) step(chunk, std::true_type(), std::false_type());
+    for (; chunk < wave_end; ++chunk) step(chunk, std::true_type(), std::true_type());
+    for (; chunk < end; ++chunk) step(chunk, std::false_type(), std::false_type());
 
     const bool out_aligned = ((reinterpret_cast<uintptr_t>(p.O) & 15) | (p.o.batch & 3) | (p.o.token & 3) | (p.o.head & 3)) == 0;
 #pragma unroll
@@ -1146,11 +1170,11 @@ template <int DP, int RT, int WAVES>
 void launch_tile(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 {
     constexpr uint32_t bytes = 2 * (4 * (DP / 64) * 1024 + (DP / 16) * 2048);
+    const auto kernel = p.call.c.head_dim == DP ? kv_attention_tile<DP, RT, true, WAVES> : kv_attention_tile<DP, RT, false, WAVES>;
     if (bytes > 60 * 1024)
-        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kv_attention_tile<DP, RT, WAVES>),
-                                  hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     const uint32_t grid = pl.tiles.count * p.call.c.kv_heads;
-    kv_attention_tile<DP, RT, WAVES><<<dim3(grid, pl.tiles.parts), 64 * WAVES, bytes, s>>>(p, pl.tiles, ws);
+    kernel<<<dim3(grid, pl.tiles.parts), 64 * WAVES, bytes, s>>>(p, pl.tiles, ws);
     if (pl.tiles.parts > 1) kv_attention_join<16 * RT * WAVES><<<dim3(grid, 4 * RT * WAVES), 256, 0, s>>>(p, pl.tiles, ws);
 }
 template <int DP>
