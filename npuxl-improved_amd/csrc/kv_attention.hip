@@ -844,7 +844,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
     const KvCall &c = p.call;
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t G = c.c.kv_heads, h = blockIdx.x % G, D = c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
+    const uint32_t G = c.c.kv_heads, h = blockIdx.x % G, D = FULL ? DP : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
     if (blockIdx.x == 0 && blockIdx.y == 0) kv::check_all(c, false, p.max_kv);
     // The last tiles of a causal sequence have the most keys: they come first.
     uint32_t b, tile, len;
@@ -896,17 +896,20 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
     constexpr int VW = (DT + WAVES - 1) / WAVES, KW = (4 * DS + WAVES - 1) / WAVES;   // tiles of V, pieces of K that a wave brings in
     v4i vf[VW];
     float ks = 0.0f, vs = 0.0f, N = power_above(0.0f);
+    // A page's codes, of all heads, are less than 2^32 bytes.
+    const uint32_t page_bytes = G * ps * D;
+    const int8_t *k_lane = c.c.k + static_cast<uint64_t>(h * ps + (col & 3)) * D, *v_lane = c.c.v + static_cast<uint64_t>(h * D + col) * ps;
     auto fetch = [&](uint32_t chunk, int8_t *buf) {
         const uint32_t in_k = (16 * min(4 * chunk + kb, last16)) & (ps - 1);
-        const int8_t *kat = c.c.k + ((static_cast<uint64_t>(checked(k_id)) * G + h) * ps + in_k + (col & 3)) * D;
+        const int8_t *kat = k_lane + (static_cast<uint64_t>(checked(k_id)) * page_bytes + in_k * D);
 #pragma unroll
         for (int i = 0; i < KW; ++i) {   // operand (tile t, step s) is piece t * DS + s
             const uint32_t piece = wave + WAVES * i, t = piece / DS, s = piece % DS, d = 64 * s + 16 * g;
             if (4 * DS % WAVES == 0 || piece < 4 * DS) lds::dma16(kat + 4 * t * D + (d < D ? d : 0), buf + piece * 1024);
         }
-        const uint64_t unit_v = static_cast<uint64_t>(checked(v_id)) * G + h;
-        const uint32_t in_v = (16 * min(4 * chunk + g, last16)) & (ps - 1);
-        const int8_t *vat = c.c.v + (unit_v * D + col) * ps + in_v;
+        const uint32_t in_v = (16 * min(4 * chunk + g, last16)) & (ps - 1), id = checked(v_id);
+        const uint64_t unit_v = static_cast<uint64_t>(id) * G + h;
+        const int8_t *vat = v_lane + (static_cast<uint64_t>(id) * page_bytes + in_v);
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
             const uint32_t t = wave + WAVES * i;
