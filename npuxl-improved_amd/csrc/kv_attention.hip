@@ -798,7 +798,8 @@ __global__ __launch_bounds__(kJoinThreads) void kv_attention_merge(KvAttn p, Spl
 struct Tiles {
     uint32_t per_seq;      // tiles a sequence (without seq_start)
     uint32_t count;        // room for tiles a kv head
-    uint32_t parts;        // key ranges of a tile
+    uint32_t parts;        // key ranges of a tile at most
+    uint32_t per;          // chunks of a range at most
     uint32_t low_rows;     // sequences with more rows are this kernel's
 };
 
@@ -834,6 +835,21 @@ __device__ __forceinline__ bool tile_sequence(const KvAttn &p, const Tiles &tl, 
     return seq.ok && n >= 0 && len <= p.max_kv && seq.n <= p.max_tokens && static_cast<uint64_t>(seq.n) * group > tl.low_rows;
 }
 
+// Keys that a row sees; chunks of a tile and the ranges that share them evenly.
+__device__ __forceinline__ int keys_of(const KvAttn &p, uint32_t len, uint32_t n, uint32_t row, uint32_t group)
+{
+    return p.causal ? max(0, static_cast<int>(len) - static_cast<int>(n) + static_cast<int>(row / group) + 1) : static_cast<int>(len);
+}
+template <uint32_t M>
+__device__ __forceinline__ uint32_t tile_chunks(const KvAttn &p, uint32_t len, uint32_t n, uint32_t tile, uint32_t group)
+{
+    return (static_cast<uint32_t>(keys_of(p, len, n, min(n * group, tile * M + M) - 1, group)) + kChunk - 1) / kChunk;
+}
+__device__ __forceinline__ uint32_t ranges_of(const Tiles &tl, uint32_t chunks)
+{
+    return tl.parts == 1 ? 1 : max(1u, (chunks + tl.per - 1) / tl.per);
+}
+
 template <int DP, int RT, bool FULL, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
 {
@@ -857,15 +873,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
     const uint32_t rows = __builtin_amdgcn_readfirstlane(seq.n) * group, n = __builtin_amdgcn_readfirstlane(seq.n);
     if (static_cast<uint64_t>(tile) * M >= rows) return;
     const uint32_t row0 = tile * M + wave * 16 * RT;   // the wave's first
-    auto sees = [&](uint32_t row) -> int {
-        return p.causal ? max(0, static_cast<int>(len) - static_cast<int>(n) + static_cast<int>(row / group) + 1) : static_cast<int>(len);
-    };
-    // Keys of the tile, of the wave; below `least` every row of the wave sees all.
-    const int tile_keys = sees(min(rows, tile * M + M) - 1);
+    const uint32_t chunks = tile_chunks<M>(p, len, n, tile, group), ranges = ranges_of(tl, chunks);
+    if (blockIdx.y >= ranges) return;
+    auto sees = [&](uint32_t row) { return keys_of(p, len, n, row, group); };
+    // Keys of the wave; below `least` every row of the wave sees all.
     const int wave_keys = row0 < rows ? sees(min(rows, row0 + 16 * RT) - 1) : 0, least = row0 < rows ? sees(row0) : 0;
-    const uint32_t chunks = (static_cast<uint32_t>(tile_keys) + kChunk - 1) / kChunk;
-    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * blockIdx.y / tl.parts);
-    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * (blockIdx.y + 1) / tl.parts);
+    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * blockIdx.y / ranges);
+    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * (blockIdx.y + 1) / ranges);
 
     Query<DS> q[RT];
     State<DT> st[RT];
@@ -1034,7 +1048,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
         const float l = groups_sum(st[r].l);
         const float by = l != 0.0f ? N * 6.103515625e-05f / l : 0.0f;   // 2^-14
         if (row >= rows) continue;
-        if (tl.parts == 1) {
+        if (ranges == 1) {
             float *at = p.O + kv::rows_base(c, p.o, b, seq) + (row / group) * p.o.token + (h * group + row % group) * p.o.head + 4 * g;
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
@@ -1068,15 +1082,18 @@ __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, con
     if (!find_tile<M>(p, tl, group, unit, b, tile) || !tile_sequence(p, tl, group, b, seq, len)) return;
     const uint32_t lane = threadIdx.x & 63, in = blockIdx.y * 4 + (threadIdx.x >> 6), row = tile * M + in;
     if (static_cast<uint64_t>(tile) * M + in >= static_cast<uint64_t>(seq.n) * group) return;
+    const uint32_t ranges = ranges_of(tl, tile_chunks<M>(p, len, seq.n, tile, group));
+    if (ranges == 1) return;   // written by the tile itself
     const uint64_t step = static_cast<uint64_t>(M) * (D + 4);
     const float *at = ws + ((static_cast<uint64_t>(unit) * G + h) * tl.parts * M + in) * (D + 4);
-    const float m = lane < tl.parts ? at[lane * step + D] : kNegInf, l = lane < tl.parts ? at[lane * step + D + 1] : 0.0f;
+    const float m = lane < ranges ? at[lane * step + D] : kNegInf, l = lane < ranges ? at[lane * step + D + 1] : 0.0f;
     float top = m;
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
     const float weight = l * __builtin_amdgcn_exp2f(m - (top == kNegInf ? 0.0f : top));
     float sum = weight, o[4] = {};
     for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-    for (uint32_t i = 0; i < tl.parts; ++i) {
+#pragma unroll 4
+    for (uint32_t i = 0; i < ranges; ++i) {
         const float w = __shfl(weight, i);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -1090,12 +1107,12 @@ __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, con
 
 // Rows that the kernel of few rows takes: one workgroup's, or two's where all
 // sequences' keys together are few.  (20 rows of 8 heads of 128, 3001 keys:
-// 1 sequence 17 us against 27 in tiles, 4 of 700 to 3001 keys 23 and 29, 4 of 3001 keys 37 and 29.)
+// 1 sequence 17 us against 21 in tiles, 4 of 700 to 3001 keys 23 and 23, 4 of 3001 keys 37 and 24.)
 uint32_t few_rows(const KvAttn &p)
 {
     const uint32_t one = p.call.c.head_dim > 128 ? 8 : 16;
     const double keys = (p.call.seq_start ? 0.6 : 1.0) * p.call.batch * p.call.c.kv_heads * p.max_kv;
-    return keys <= 65536 ? 2 * one : one;
+    return keys <= 32768 ? 2 * one : one;
 }
 
 struct Plan {
@@ -1144,14 +1161,28 @@ Plan plan_of(const KvAttn &p)
     }
     r.ws = r.few_ws;
     if (r.tiled) {
-        r.tile_rows = most <= 64 || D > 128 ? 64 : 128;
         r.tiles.low_rows = r.few ? at_most : 0;
-        r.tiles.per_seq = static_cast<uint32_t>((most + r.tile_rows - 1) / r.tile_rows);
-        r.tiles.count = c.seq_start ? static_cast<uint32_t>(static_cast<uint64_t>(c.tokens) * group / r.tile_rows) + c.batch
-                                    : r.tiles.per_seq * c.batch;
-        const uint64_t grid = static_cast<uint64_t>(r.tiles.count) * G;
+        auto tiles_of = [&](uint32_t rows) {   // of all kv heads
+            r.tile_rows = rows;
+            r.tiles.per_seq = static_cast<uint32_t>((most + rows - 1) / rows);
+            r.tiles.count = c.seq_start ? static_cast<uint32_t>(static_cast<uint64_t>(c.tokens) * group / rows) + c.batch
+                                        : r.tiles.per_seq * c.batch;
+            return static_cast<uint64_t>(r.tiles.count) * G;
+        };
+        // 128 rows share K and V of a chunk where the card has more of such tiles
+        // than run at a time (32 heads of 128, causal: 4096 tokens of 8 kv heads
+        // 248 us against 273 with 64 rows, 2048 of 32 kv heads 96 and 87).
+        uint64_t grid = D <= 128 ? tiles_of(128) : 0;
+        if (grid <= 2 * p.cus) grid = tiles_of(64);
+        // Key ranges of 4 chunks at least for a workgroup a CU, of 8 for as many as
+        // run at a time (32 tiles, 47 chunks: 8 ranges 24 us, 5 29 us; 64 chunks: 8
+        // ranges 30 us, 10 35 us).  Where sequences differ the shorter have fewer.
+        const uint64_t at_once = (D > 128 ? 1 : 3) * p.cus;
         const uint32_t chunks = (p.max_kv + kChunk - 1) / kChunk;
-        r.tiles.parts = grid >= p.cus ? 1 : std::max<uint32_t>(1, std::min<uint64_t>(std::min<uint64_t>(64, 2 * p.cus / grid), chunks / 8));
+        const uint64_t parts = std::max(std::min<uint64_t>(p.cus / grid, chunks / 4),
+                                        std::min<uint64_t>(at_once * (c.seq_start ? 5 : 3) / (3 * grid), chunks / (c.seq_start ? 5 : 8)));
+        r.tiles.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(parts, 1), 64));
+        r.tiles.per = (chunks + r.tiles.parts - 1) / r.tiles.parts;
         if (r.tiles.parts > 1) r.ws += static_cast<size_t>(grid) * r.tiles.parts * r.tile_rows * (D + 4) * sizeof(float);
     }
     return r;

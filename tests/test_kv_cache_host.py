@@ -124,7 +124,8 @@ def test_routes_over_sizes():
     assert int(text(100000)["few"]) > 1 and int(text(100000)["ws"]) > 0
     assert text(4096, batch=64, tokens=64)["few"] == "64" and text(4096, batch=64, tokens=64)["ws"] == "0"
     assert text(4096, tokens=64)["few"] == "0" and text(4096, tokens=64)["tile"] == "64"
-    assert text(4096, tokens=4096)["tile"] == "128" and text(4096, tokens=4096)["parts"] == "1"
+    assert text(4096, tokens=4096)["tile"] == "64" and text(4096, tokens=4096)["parts"] == "1"
+    assert text(1 << 14, tokens=1 << 14)["tile"] == "128" and text(1 << 14, tokens=1 << 14)["parts"] == "1"
     assert int(text(4096, tokens=100)["parts"]) > 1 and int(text(4096, tokens=100)["ws"]) > 0
     mixed = text(4096, batch=64, tokens=300, seq_start=P)
     assert mixed["few"] != "0" and mixed["tile"] != "0"
