@@ -1071,8 +1071,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
     }
 }
 
-// A tile's key ranges, at most 64, together: a wave a row, a range's weight a lane.
-template <uint32_t M>
+// A tile's key ranges, at most 64, together: kJoinRows rows a wave, a range's
+// weight a lane.  Lanes behind head_dim load its last element: loads under a
+// condition are waited for one by one (20 us instead of 7).
+constexpr int kJoinRows = 2;
+template <uint32_t M, int DS>
 __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, const float *ws)
 {
     const KvCall &c = p.call;
@@ -1080,29 +1083,45 @@ __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, con
     uint32_t b, tile, len;
     kv::Seq seq;
     if (!find_tile<M>(p, tl, group, unit, b, tile) || !tile_sequence(p, tl, group, b, seq, len)) return;
-    const uint32_t lane = threadIdx.x & 63, in = blockIdx.y * 4 + (threadIdx.x >> 6), row = tile * M + in;
+    const uint32_t lane = threadIdx.x & 63, in = (blockIdx.y * 4 + (threadIdx.x >> 6)) * kJoinRows, row = tile * M + in;
     if (static_cast<uint64_t>(tile) * M + in >= static_cast<uint64_t>(seq.n) * group) return;
-    const uint32_t ranges = ranges_of(tl, tile_chunks<M>(p, len, seq.n, tile, group));
+    const uint32_t ranges = __builtin_amdgcn_readfirstlane(ranges_of(tl, tile_chunks<M>(p, len, seq.n, tile, group)));
     if (ranges == 1) return;   // written by the tile itself
     const uint64_t step = static_cast<uint64_t>(M) * (D + 4);
-    const float *at = ws + ((static_cast<uint64_t>(unit) * G + h) * tl.parts * M + in) * (D + 4);
-    const float m = lane < ranges ? at[lane * step + D] : kNegInf, l = lane < ranges ? at[lane * step + D + 1] : 0.0f;
-    float top = m;
-    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-    const float weight = l * __builtin_amdgcn_exp2f(m - (top == kNegInf ? 0.0f : top));
-    float sum = weight, o[4] = {};
-    for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-#pragma unroll 4
-    for (uint32_t i = 0; i < ranges; ++i) {
-        const float w = __shfl(weight, i);
+    const float *first = ws + (static_cast<uint64_t>(unit) * G + h) * tl.parts * step;
+    const float *at[kJoinRows];
+    float m[kJoinRows], l[kJoinRows], weight[kJoinRows], sum[kJoinRows], o[kJoinRows][DS] = {};
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (lane + 64 * r < D) o[r] = fmaf(w, at[i * step + lane + 64 * r], o[r]);
+    for (int k = 0; k < kJoinRows; ++k) {   // a row behind the last is the last again
+        at[k] = first + static_cast<uint64_t>(min(row + k, seq.n * group - 1) - tile * M) * (D + 4);
+        m[k] = at[k][min(lane, ranges - 1) * step + D];
+        l[k] = at[k][min(lane, ranges - 1) * step + D + 1];
     }
-    float *out = p.O + kv::rows_base(c, p.o, b, seq) + (row / group) * p.o.token + (h * group + row % group) * p.o.head;
+    uint32_t d[DS];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (lane + 64 * r < D) out[lane + 64 * r] = sum != 0.0f ? o[r] / sum : 0.0f;
+    for (int r = 0; r < DS; ++r) d[r] = min(lane + 64 * r, D - 1);
+#pragma unroll
+    for (int k = 0; k < kJoinRows; ++k) {
+        const float top = groups_max(row_max(m[k]));
+        weight[k] = lane < ranges ? l[k] * __builtin_amdgcn_exp2f(m[k] - (top == kNegInf ? 0.0f : top)) : 0.0f;
+        sum[k] = groups_sum(row_sum(weight[k]));
+    }
+#pragma unroll 4
+    for (uint32_t i = 0; i < ranges; ++i)
+#pragma unroll
+        for (int k = 0; k < kJoinRows; ++k) {
+            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight[k]), i));
+#pragma unroll
+            for (int r = 0; r < DS; ++r) o[k][r] = fmaf(w, at[k][i * step + d[r]], o[k][r]);
+        }
+#pragma unroll
+    for (int k = 0; k < kJoinRows; ++k) {
+        const uint32_t to = min(row + k, seq.n * group - 1);
+        float *out = p.O + kv::rows_base(c, p.o, b, seq) + (to / group) * p.o.token + (h * group + to % group) * p.o.head;
+#pragma unroll
+        for (int r = 0; r < DS; ++r)
+            if (lane + 64 * r < D) out[lane + 64 * r] = sum[k] != 0.0f ? o[k][r] / sum[k] : 0.0f;
+    }
 }
 
 // Rows that the kernel of few rows takes: one workgroup's, or two's where all
@@ -1209,7 +1228,7 @@ void launch_tile(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     const uint32_t grid = pl.tiles.count * p.call.c.kv_heads;
     kernel<<<dim3(grid, pl.tiles.parts), 64 * WAVES, bytes, s>>>(p, pl.tiles, ws);
-    if (pl.tiles.parts > 1) kv_attention_join<16 * RT * WAVES><<<dim3(grid, 4 * RT * WAVES), 256, 0, s>>>(p, pl.tiles, ws);
+    if (pl.tiles.parts > 1) kv_attention_join<16 * RT * WAVES, DP / 64><<<dim3(grid, 4 * RT * WAVES / kJoinRows), 256, 0, s>>>(p, pl.tiles, ws);
 }
 template <int DP>
 void launch(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
