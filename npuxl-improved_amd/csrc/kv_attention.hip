@@ -183,23 +183,29 @@ struct Query {
         const uint32_t g = (threadIdx.x & 63) >> 4;
         float x[DS * 16];
         uint32_t most = 0;
+        // Loads under a condition would be waited for one by one.
+        auto at = [&](int s) { return row + (64 * s + 16 * g < D ? 64 * s + 16 * g : 0); };
+        if (aligned) {
 #pragma unroll
-        for (int s = 0; s < DS; ++s) {
-            const uint32_t d = 64 * s + 16 * g;
-            const bool in = here && d < D;
+            for (int s = 0; s < DS; ++s)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (in) {
-                    const float *at = row + d + 4 * w;
-                    v = aligned ? *reinterpret_cast<const float4 *>(at) : make_float4(at[0], at[1], at[2], at[3]);
+                for (int w = 0; w < 4; ++w) {
+                    const float4 v = *reinterpret_cast<const float4 *>(at(s) + 4 * w);
+                    x[16 * s + 4 * w] = v.x;
+                    x[16 * s + 4 * w + 1] = v.y;
+                    x[16 * s + 4 * w + 2] = v.z;
+                    x[16 * s + 4 * w + 3] = v.w;
                 }
-                x[16 * s + 4 * w] = v.x;
-                x[16 * s + 4 * w + 1] = v.y;
-                x[16 * s + 4 * w + 2] = v.z;
-                x[16 * s + 4 * w + 3] = v.w;
-            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < DS; ++s)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[16 * s + i] = at(s)[i];
         }
+#pragma unroll
+        for (int s = 0; s < DS; ++s)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[16 * s + i] = here && 64 * s + 16 * g < D ? x[16 * s + i] : 0.0f;
 #pragma unroll
         for (int i = 0; i < DS * 16; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
         // Bits of magnitudes order as floats do, infinity and NaN above all.
@@ -927,7 +933,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
             const uint32_t t = wave + WAVES * i;
-            if (16 * t < D) vf[i] = *reinterpret_cast<const v4i *>(vat + static_cast<uint64_t>(16 * t) * ps);
+            vf[i] = *reinterpret_cast<const v4i *>(vat + static_cast<uint64_t>(FULL ? 16 * t : min(16 * t, D - 16)) * ps);
         }
         ks = c.c.ks[unit_v];
         vs = c.c.vs[unit_v];
@@ -936,7 +942,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
             const uint32_t t = wave + WAVES * i;
-            if (16 * t >= D) continue;
+            if (!FULL && 16 * t >= D) continue;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 v2h x[4];
