@@ -481,12 +481,12 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
     float4 raw[kLoads];
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
-        const uint32_t e = threadIdx.x + k * 64 * WAVES, r = e / (DP / 4), d = 4 * (e % (DP / 4)), row = row0 + r, i = row / group;
-        raw[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (r < R && row < rows && d < D) {
-            const float *at = q_base + i * p.q.token + (row - i * group) * p.q.head + d;
-            raw[k] = aligned ? *reinterpret_cast<const float4 *>(at) : make_float4(at[0], at[1], at[2], at[3]);
-        }
+        // Loads under a condition would be waited for one by one.
+        const uint32_t e = threadIdx.x + k * 64 * WAVES, r = e / (DP / 4), d = 4 * (e % (DP / 4));
+        const uint32_t row = min(row0 + r, rows - 1), i = row / group;
+        const float *at = q_base + i * p.q.token + (row - i * group) * p.q.head + min(d, D - 4);
+        raw[k] = aligned ? *reinterpret_cast<const float4 *>(at) : make_float4(at[0], at[1], at[2], at[3]);
+        if (row0 + r >= rows || d >= D) raw[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
     if (any) units();
 #pragma unroll
@@ -737,12 +737,25 @@ __device__ __forceinline__ void join_parts(const float *at, uint64_t step, uint3
 {
     __shared__ float weight[kMostParts], sums[kJoinThreads], red[2][kJoinThreads / 64];
     const uint32_t tid = threadIdx.x, wave = tid >> 6;
-    float m[kMostParts / kJoinThreads], l[kMostParts / kJoinThreads], M = kNegInf, L = 0.0f;
+    // The statistics and each thread's first parts are asked for together; what
+    // is behind the last part is that one again, its weight 0.
+    constexpr uint32_t kFirst = 16;
+    const uint32_t width = D <= 64 ? 64 : D <= 128 ? 128 : 256, every = kJoinThreads / width, d = min(tid % width, D - 1);
+    float m[kMostParts / kJoinThreads], l[kMostParts / kJoinThreads], x[kFirst], M = kNegInf, L = 0.0f;
 #pragma unroll
     for (uint32_t k = 0; k < kMostParts / kJoinThreads; ++k) {
-        const uint32_t i = tid + k * kJoinThreads;
-        m[k] = i < parts ? at[i * step + D] : kNegInf;
-        l[k] = i < parts ? at[i * step + D + 1] : 0.0f;
+        const float *part = at + min(tid + k * kJoinThreads, parts - 1) * step + D;
+        m[k] = part[0];
+        l[k] = part[1];
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kFirst; ++k) x[k] = at[min(tid / width + k * every, parts - 1) * step + d];
+#pragma unroll
+    for (uint32_t k = 0; k < kMostParts / kJoinThreads; ++k) {
+        if (tid + k * kJoinThreads >= parts) {
+            m[k] = kNegInf;
+            l[k] = 0.0f;
+        }
         M = fmaxf(M, m[k]);
     }
     for (int x = 32; x; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
@@ -761,12 +774,14 @@ __device__ __forceinline__ void join_parts(const float *at, uint64_t step, uint3
     __syncthreads();
     L = 0.0f;
     for (uint32_t w = 0; w < kJoinThreads / 64; ++w) L += red[1][w];
-    const uint32_t width = D <= 64 ? 64 : D <= 128 ? 128 : 256, every = kJoinThreads / width, d = tid % width;
     float o = 0.0f;
-    if (d < D) {
-#pragma unroll 8
-        for (uint32_t i = tid / width; i < parts; i += every) o = fmaf(weight[i], at[i * step + d], o);
+#pragma unroll
+    for (uint32_t k = 0; k < kFirst; ++k) {
+        const uint32_t i = tid / width + k * every;
+        o = fmaf(i < parts ? weight[i] : 0.0f, x[k], o);
     }
+#pragma unroll 8
+    for (uint32_t i = tid / width + kFirst * every; i < parts; i += every) o = fmaf(weight[i], at[i * step + d], o);
     sums[tid] = o;
     __syncthreads();
     if (tid < D) {
