@@ -1184,12 +1184,13 @@ Plan plan_of(const KvAttn &p)
         r.split.target = std::min(std::max(at_once > c.batch ? at_once - c.batch / 2 : at_once / 2, 1u), kMostParts);
         r.split.min_per = 4;
         // A sequence and kv head as one workgroup: 9 us and 1.05 us for each 256
-        // keys, or the codes at 6.2 TB/s; split: 14 us with the join, codes at 5.0
-        // (8 heads of 128, 4096 keys: 1 sequence 25.5 and 15.0 us, 16 sequences
-        // 30.1 and 32.0; 32 heads, 8 sequences 43.6 and 57.6).  Sequences are taken to be
-        // 0.6 of max_kv long.
-        const double mb = 1.2e-6 * c.batch * G * D * p.max_kv;
-        r.split.whole = std::max(9.0 + 1.05 * ((p.max_kv + 255) / 256), mb / 6.2) <= 14.0 + mb / 5.0;
+        // keys of the longest, or the codes at 6.4 TB/s; split: 12 us with the join
+        // and the codes (8 heads of 128, 4096 keys: 1 sequence 24.7 and 10.9 us, 16 sequences
+        // 28.4 and 30.6; 32 heads, 8 sequences 42.0 and 52.6; 8 heads, 16 sequences of 100 to
+        // 8000 keys 47.3 and 39.2).  Sequences are taken to be 0.8 of max_kv long, with
+        // seq_start 0.6.
+        const double mb = (c.seq_start ? 1.2e-6 : 1.6e-6) * c.batch * G * D * p.max_kv;
+        r.split.whole = std::max(9.0 + 1.05 * ((p.max_kv + 255) / 256), mb / 6.4) <= 12.0 + mb / 6.4;
         r.split.low_rows = 0;
         r.split.high_rows = at_most;
         // No more slots than parts of the longest: a workgroup without work takes its turn too.
