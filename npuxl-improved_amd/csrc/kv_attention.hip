@@ -7,7 +7,8 @@
 // head) are its tokens times the query heads of the group, row r = token r / g,
 // head r % g, so grouped heads share every code that is read.
 //
-// Both products run on the matrix cores with the codes as they are:
+// Both products run on the matrix cores with the codes as they are.  Calls of
+// many rows (the kernel of few rows has its own forms, see there):
 //   Q . K   int8: a query row is the whole number rint(q * S), S = 8355700 /
 //           max|q|, in three balanced base-256 digits (24 bits), so three
 //           v_mfma_i32_16x16x64_i8 give the sum without a rounding;
@@ -313,6 +314,12 @@ __device__ __forceinline__ void weigh(float &sum, const v4f f[4], int half, floa
 // reference m that s may pass by 4, N a power of two that v_scale may not
 // pass; sums stay whole numbers until m or N has to move, then they are added
 // to f32 sums in LDS.
+// Bound by the codes from HBM where there are enough of them (32 heads of 128, 8
+// sequences of 4096 keys: 42 us, 6.4 TB/s of codes; a large read reaches 6.2 to
+// 6.7; 64 sequences of 100 to 8000 keys, 32 heads to 8: 106 us, 5.6 TB/s; one of
+// 131072 keys: 43 us and 4.5 us of join), by the latency of launch, page,
+// copy and join where not (one sequence of 128 keys 5.2 us, of 4096 10.9 us).
+// Not temporal copies: 67 -> 56 us at the first size, which nothing reads twice.
 // ---------------------------------------------------------------------------
 
 constexpr float kDigits4 = 2139060000.0f;   // four digits hold 127 * (2^24 + 2^16 + 2^8 + 1) = 2139062143
@@ -731,7 +738,9 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
 
 // Parts of a row, `step` floats apart, each o / l with its m and l behind it:
 // weighed by l 2^(m - max m).  A workgroup a row: the weights first, a part a
-// thread, then the sums, threads over the dimensions and every few parts.
+// thread, then the sums, threads over the dimensions and every few parts.  The
+// latency of what other dies have just written bounds it: 4.6 us for 65 parts of 32 rows,
+// 7.6 us with the sums asked for after the weights.
 constexpr uint32_t kJoinThreads = 512, kMostParts = 1024;
 __device__ __forceinline__ void join_parts(const float *at, uint64_t step, uint32_t parts, uint32_t D, float *out)
 {
@@ -814,6 +823,16 @@ __global__ __launch_bounds__(kJoinThreads) void kv_attention_merge(KvAttn p, Spl
 // into LDS in operand order, its V codes pass through registers to be turned into
 // f16 once for the four waves; both of the next chunk are on their way while
 // this one is computed, and one barrier a chunk hands the buffers over.
+// Bound by the vector instructions: 64 keys of 32 rows take a wave 112 matrix
+// instructions (16 cycles each) and about 530 others (4 cycles, exponentials 16):
+// three conversions and sums for a score's digits, ten for a weight and its two
+// halves.  Two waves a SIMD fill 69 % of its vector issue and 43 % of its matrix
+// cores.  A step has few branches, so that its products and exponentials
+// mix: with the rows one after another and conditions inside, 306 us instead of 256.
+// 4096 tokens on themselves, causal, 32 heads of 128: 238 us, 577 TFLOP/s (a
+// large f16 product of the library, which needs 2 of these 5 matrix
+// instructions, 1109); heads of 64 165 us, of 256 (half the heads and tokens) 115 us.
+// Workgroups of 8 waves and 256 rows: 254 us and worse where tiles are few.
 // ---------------------------------------------------------------------------
 
 struct Tiles {
@@ -1094,7 +1113,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
 
 // A tile's key ranges, at most 64, together: kJoinRows rows a wave, a range's
 // weight a lane.  Lanes behind head_dim load its last element: loads under a
-// condition are waited for one by one (20 us instead of 7).
+// condition are waited for one by one (10.8 us instead of 7.9 for 220 tiles of 64 rows
+// and up to 5 ranges).
 constexpr int kJoinRows = 2;
 template <uint32_t M, int DS>
 __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, const float *ws)
@@ -1210,16 +1230,18 @@ Plan plan_of(const KvAttn &p)
                                         : r.tiles.per_seq * c.batch;
             return static_cast<uint64_t>(r.tiles.count) * G;
         };
+        const uint32_t chunks = (p.max_kv + kChunk - 1) / kChunk;
         // 128 rows share K and V of a chunk where the card has more of such tiles
         // than run at a time (32 heads of 128, causal: 4096 tokens of 8 kv heads
-        // 248 us against 273 with 64 rows, 2048 of 32 kv heads 96 and 87).
+        // 248 us against 273 with 64 rows, 2048 of 32 kv heads 96 and 87), or a few
+        // even ones with keys for 16 chunks a range (512 tokens of 4096, 8 kv heads: 76 us
+        // against 79; a ragged batch of 3 x 200 tokens 97 against 79).
         uint64_t grid = D <= 128 ? tiles_of(128) : 0;
-        if (grid <= 2 * p.cus) grid = tiles_of(64);
+        if (grid <= 2 * p.cus && (c.seq_start || grid >= p.cus || grid * (chunks / 16) < 2 * p.cus)) grid = tiles_of(64);
         // Key ranges of 4 chunks at least for a workgroup a CU, of 8 for as many as
         // run at a time (32 tiles, 47 chunks: 8 ranges 24 us, 5 29 us; 64 chunks: 8
         // ranges 30 us, 10 35 us).  Where sequences differ the shorter have fewer.
-        const uint64_t at_once = (D > 128 ? 1 : 3) * p.cus;
-        const uint32_t chunks = (p.max_kv + kChunk - 1) / kChunk;
+        const uint64_t at_once = (D > 128 ? 1 : r.tile_rows == 128 ? 2 : 3) * p.cus;
         const uint64_t parts = std::max(std::min<uint64_t>(p.cus / grid, chunks / 4),
                                         std::min<uint64_t>(at_once * (c.seq_start ? 5 : 3) / (3 * grid), chunks / (c.seq_start ? 5 : 8)));
         r.tiles.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(parts, 1), 64));

@@ -9,10 +9,16 @@
 //   s = max(n0 ? s0 : 0, f32(a * f32(1 / 127))) for n0 tokens kept from before,
 //   kept codes -> round(code * f32(s0 / s)) where s > s0,
 //   new codes = round(x * f32(1 / s)), half away from zero, in +-127.
-// One page and kv head is one workgroup: it alone reads and writes that
-// page's codes and scale, so nothing is atomic and results do not depend on
-// order; K and V are workgroups of their own, Q's rows others.  The new tokens' f32 values are read once and stay in registers
-// between the largest magnitude and the codes.
+// One page and kv head of K or V is one workgroup: it alone reads and writes
+// those codes and their scale, so nothing is atomic and results do not depend on
+// order.  The new tokens' f32 values are read once and stay in registers between
+// the largest magnitude and the codes.  Q's rows are workgroups of their own behind
+// them: the three used to be one, 62 us for 2048 tokens of 32 and 8 heads of
+// 128, now 24 us, 4.2 TB/s of rows in and out and codes (a large copy: 4.9 TB/s).
+// A token each for 8 sequences takes 4.4 us, a launch and its latency.
+//
+// Read: one page and kv head of K or V is one workgroup; f32 rows, four times the
+// codes, bound it: 8 x 2048 tokens of 8 heads of 128 in 27.7 us, 6.1 TB/s.
 #include "device_math.hpp"
 #include "kv_common.hpp"
 
@@ -121,9 +127,13 @@ struct AppendGrid {
 };
 
 // One page and head of K or V.  Thread e of m * D / 2 pairs has pair e % (D /
-// 2) of token e / (D / 2); PAIRS of a thread.  Codes go through LDS (dynamic,
-// page_size * D bytes) so that the cache is written 16 bytes at a time.
-template <int T, int PAIRS, bool V>
+// 2) of token e / (D / 2); PAIRS of a thread, and where that may not be enough
+// (ROUNDS: the host does not know how many tokens a ragged sequence has) rounds of
+// as many, of which all but the last are read again for their codes (64 sequences of
+// 1 to 6 tokens, pages of 256: 10 us instead of 41 with room for whole pages;
+// 2048 tokens of one sequence: 24 us without rounds, 26 with).  Codes go through LDS
+// (dynamic, page_size * D bytes) so that the cache is written 16 bytes at a time.
+template <int T, int PAIRS, bool ROUNDS, bool V>
 __device__ __forceinline__ void append_page(const KvAppend &p, const Rates &rates, uint32_t magic, uint32_t b, const kv::Piece &pc,
                                             uint32_t h, int8_t *tile, uint32_t *red)
 {
@@ -138,45 +148,59 @@ __device__ __forceinline__ void append_page(const KvAppend &p, const Rates &rate
     const uint32_t turns = !V && p.rotation ? p.rope_dim / 2 : 0;
 
     float2 x[PAIRS];
-    uint32_t most = 0;
+    auto load = [&](uint32_t from) {
 #pragma unroll
-    for (int i = 0; i < PAIRS; ++i) {
-        const uint32_t e = tid + i * T;
-        x[i] = make_float2(0.0f, 0.0f);
-        if (e >= pairs) continue;
-        const uint32_t t = __umulhi(e, magic), j = e - t * half;
-        const uint2 d = V ? make_uint2(2 * j, 2 * j + 1) : pair_at(p, j);
-        const float *row = in + t * rows.token;
-        x[i] = make_float2(row[d.x], row[d.y]);
-    }
-#pragma unroll
-    for (int i = 0; i < PAIRS; ++i) {
-        const uint32_t e = tid + i * T, t = __umulhi(e, magic), j = e - t * half;
-        if (!V && e < pairs && j < turns) {
-            float cs, sn;
-            cos_sin_turns(static_cast<double>(position + t) * rates.turns[j], cs, sn);
-            x[i] = turned(x[i], cs, sn);
+        for (int i = 0; i < PAIRS; ++i) {
+            const uint32_t e = from + tid + i * T;
+            x[i] = make_float2(0.0f, 0.0f);
+            if (e >= pairs) continue;
+            const uint32_t t = __umulhi(e, magic), j = e - t * half;
+            const uint2 d = V ? make_uint2(2 * j, 2 * j + 1) : pair_at(p, j);
+            const float *row = in + t * rows.token;
+            x[i] = make_float2(row[d.x], row[d.y]);
         }
-        most = max(most, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
+        if (V) return;
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+            const uint32_t e = from + tid + i * T, t = __umulhi(e, magic), j = e - t * half;
+            if (e < pairs && j < turns) {
+                float cs, sn;
+                cos_sin_turns(static_cast<double>(position + t) * rates.turns[j], cs, sn);
+                x[i] = turned(x[i], cs, sn);
+            }
+        }
+    };
+    uint32_t most = 0, from = 0;
+    for (;; from += PAIRS * T) {
+        load(from);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i)
+            most = max(most, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
+        if (!ROUNDS || from + PAIRS * T >= pairs) break;
     }
     const PageScale s = page_scale(block_largest<T>(most, red), pc.slot > 0, before);
     if (tid == 0) scales[unit] = s.scale;
     if (s.scale != s.scale) return;   // under a NaN scale the codes stay
 
+    for (;;) {
 #pragma unroll
-    for (int i = 0; i < PAIRS; ++i) {
-        const uint32_t e = tid + i * T;
-        if (e >= pairs) continue;
-        const uint32_t t = __umulhi(e, magic), j = e - t * half;
-        const int8_t c0 = static_cast<int8_t>(code_of(x[i].x, s.inv)), c1 = static_cast<int8_t>(code_of(x[i].y, s.inv));
-        if (V) {
-            tile[2 * j * ps + pc.slot + t] = c0;
-            tile[(2 * j + 1) * ps + pc.slot + t] = c1;
-        } else {
-            const uint2 d = pair_at(p, j);
-            tile[t * D + d.x] = c0;
-            tile[t * D + d.y] = c1;
+        for (int i = 0; i < PAIRS; ++i) {
+            const uint32_t e = from + tid + i * T;
+            if (e >= pairs) continue;
+            const uint32_t t = __umulhi(e, magic), j = e - t * half;
+            const int8_t c0 = static_cast<int8_t>(code_of(x[i].x, s.inv)), c1 = static_cast<int8_t>(code_of(x[i].y, s.inv));
+            if (V) {
+                tile[2 * j * ps + pc.slot + t] = c0;
+                tile[(2 * j + 1) * ps + pc.slot + t] = c1;
+            } else {
+                const uint2 d = pair_at(p, j);
+                tile[t * D + d.x] = c0;
+                tile[t * D + d.y] = c1;
+            }
         }
+        if (!ROUNDS || !from) break;
+        from -= PAIRS * T;
+        load(from);
     }
     __syncthreads();
     const uint4 *tp = reinterpret_cast<const uint4 *>(tile);
@@ -273,7 +297,7 @@ __device__ __forceinline__ void turn_queries(const KvAppend &p, const Rates &rat
     }
 }
 
-template <int T, int PAIRS>
+template <int T, int PAIRS, bool ROUNDS>
 __global__ __launch_bounds__(T) void kv_append_kernel(KvAppend p, Rates rates, AppendGrid grid)
 {
     extern __shared__ __align__(16) int8_t tile[];
@@ -289,8 +313,8 @@ __global__ __launch_bounds__(T) void kv_append_kernel(KvAppend p, Rates rates, A
     uint32_t b;
     kv::Piece pc;
     if (!kv::find_piece(c, rest / c.c.kv_heads, b, pc)) return;
-    if (blockIdx.x & 1) append_page<T, PAIRS, true>(p, rates, grid.half_magic, b, pc, h, tile, red);
-    else append_page<T, PAIRS, false>(p, rates, grid.half_magic, b, pc, h, tile, red);
+    if (blockIdx.x & 1) append_page<T, PAIRS, ROUNDS, true>(p, rates, grid.half_magic, b, pc, h, tile, red);
+    else append_page<T, PAIRS, ROUNDS, false>(p, rates, grid.half_magic, b, pc, h, tile, red);
 }
 
 constexpr int kReadThreads = 256;
@@ -387,11 +411,19 @@ void allow_lds(Kernel kernel, size_t bytes)
                                   static_cast<int>(bytes));
 }
 
-// Threads of a workgroup and the pairs that each has, for the pairs of a page's
-// new tokens: at most page_size * D / 2 = 32768.
-uint32_t append_pairs(const KvCall &c)
+// Pairs of a page's new tokens: at most (page_size * D / 2 = 32768 or less), and
+// what to make room for: of ragged sequences what a page has if they have up to
+// twice as many tokens as the mean, where all would be more than 4 of a thread.
+uint32_t append_most(const KvCall &c)
 {
     return std::min(c.seq_start ? c.tokens : c.tokens / c.batch, c.c.page_size) * (c.c.head_dim / 2);
+}
+uint32_t append_pairs(const KvCall &c)
+{
+    const uint32_t most = append_most(c);
+    if (!c.seq_start || most <= 1024) return most;
+    const uint64_t twice = 2ull * ((c.tokens + c.batch - 1) / c.batch) * (c.c.head_dim / 2);
+    return static_cast<uint32_t>(std::min<uint64_t>(most, twice));
 }
 uint32_t append_threads(const KvCall &c) { return append_pairs(c) <= 4096 ? 256 : 1024; }
 
@@ -410,13 +442,13 @@ uint64_t append_blocks(const KvAppend &p, AppendGrid &g)
     return blocks;
 }
 
-template <int T, int PAIRS>
+template <int T, int PAIRS, bool ROUNDS>
 void launch_append(hipStream_t s, const KvAppend &p, uint32_t blocks, const AppendGrid &grid)
 {
     const size_t lds = static_cast<size_t>(p.call.c.page_size) * p.call.c.head_dim;
-    allow_lds(kv_append_kernel<T, PAIRS>, lds);
+    allow_lds(kv_append_kernel<T, PAIRS, ROUNDS>, lds);
     const Rates rates = p.rotation ? rates_of(p.theta, p.rope_dim, p.scaling) : Rates{};
-    kv_append_kernel<T, PAIRS><<<blocks, T, lds, s>>>(p, rates, grid);
+    kv_append_kernel<T, PAIRS, ROUNDS><<<blocks, T, lds, s>>>(p, rates, grid);
 }
 }  // namespace
 
@@ -433,11 +465,14 @@ void kv_append(hipStream_t s, const KvAppend &p)
     AppendGrid g;
     const uint32_t blocks = static_cast<uint32_t>(append_blocks(p, g)), half = p.call.c.head_dim / 2, most = append_pairs(p.call);
     g.half_magic = static_cast<uint32_t>((0x100000000ull + half - 1) / half);   // exact below 2^16
-    if (most <= 256) launch_append<256, 1>(s, p, blocks, g);
-    else if (most <= 1024) launch_append<256, 4>(s, p, blocks, g);
-    else if (most <= 4096) launch_append<256, 16>(s, p, blocks, g);
-    else if (most <= 16384) launch_append<1024, 16>(s, p, blocks, g);
-    else launch_append<1024, 32>(s, p, blocks, g);
+    const bool fit = append_most(p.call) <= (most <= 256 ? 256u : most <= 1024 ? 1024u : most <= 4096 ? 4096u : 16384u);
+    if (most <= 256 && fit) launch_append<256, 1, false>(s, p, blocks, g);
+    else if (most <= 1024 && fit) launch_append<256, 4, false>(s, p, blocks, g);
+    else if (most <= 1024) launch_append<256, 4, true>(s, p, blocks, g);
+    else if (most <= 4096 && fit) launch_append<256, 16, false>(s, p, blocks, g);
+    else if (most <= 4096) launch_append<256, 16, true>(s, p, blocks, g);
+    else if (fit) launch_append<1024, 16, false>(s, p, blocks, g);
+    else launch_append<1024, 16, true>(s, p, blocks, g);
 }
 
 void kv_read(hipStream_t s, const KvRead &p)

@@ -102,6 +102,15 @@ def test_append_one_token_each(gpu, batch):
     append_case(gpu, 8, 2, 128, 16, past, [1] * batch, ragged=True, with_q=False)
 
 
+@pytest.mark.parametrize("d,page,n", [(64, 128, [200] + [1] * 39), (128, 256, [1] * 7 + [300] + [2] * 8),
+                                      (256, 256, [300, 200]), (80, 256, [6] * 20 + [256, 0, 5])])
+@pytest.mark.parametrize("rotation", [0, 1, 2])
+def test_append_one_long_among_short(gpu, d, page, n, rotation):
+    """Ragged sequences with many times the mean's tokens: a page's tokens are taken in several rounds."""
+    append_case(gpu, 4, 2, d, page, [(53 * b) % 300 for b in range(len(n))], n, rotation=rotation)
+    append_case(gpu, 4, 2, d, page, [page * (b % 2) for b in range(len(n))], n, rotation=rotation, with_q=False, layout="wide")
+
+
 def test_append_far_positions_and_bases(gpu):
     append_case(gpu, 2, 1, 128, 256, [131000, 70000], [9, 300])
     append_case(gpu, 2, 1, 128, 256, [131000, 70000], [9, 300], theta=500000.0, scaling=0.125, rotation=2)
