@@ -826,10 +826,10 @@ __global__ __launch_bounds__(kJoinThreads) void kv_attention_merge(KvAttn p, Spl
 // Bound by the vector instructions: 64 keys of 32 rows take a wave 112 matrix
 // instructions (16 cycles each) and about 530 others (4 cycles, exponentials 16):
 // three conversions and sums for a score's digits, ten for a weight and its two
-// halves.  Two waves a SIMD fill 69 % of its vector issue and 43 % of its matrix
+// halves.  Two waves a SIMD fill 73 % of its vector issue and 47 % of its matrix
 // cores.  A step has few branches, so that its products and exponentials
 // mix: with the rows one after another and conditions inside, 306 us instead of 256.
-// 4096 tokens on themselves, causal, 32 heads of 128: 238 us, 577 TFLOP/s (a
+// 4096 tokens on themselves, causal, 32 heads of 128: 239 us, 576 TFLOP/s (a
 // large f16 product of the library, which needs 2 of these 5 matrix
 // instructions, 1109); heads of 64 165 us, of 256 (half the heads and tokens) 115 us.
 // Workgroups of 8 waves and 256 rows: 254 us and worse where tiles are few.
