@@ -496,9 +496,11 @@ typedef struct vnpu_memset_args_t {
 /*                                                                           */
 /* k, v and the scales must be device memory; table, the length arrays and   */
 /* the f32 tensors may be host memory, staged as everywhere.  Lengths and    */
-/* pages are read on the GPU: a negative or too long length, a seq_start     */
-/* that decreases or passes `tokens`, or a page outside [0, pages) of a      */
-/* token that the call touches fails the stream at its next sync             */
+/* pages are read on the GPU: a negative or too long length (of any          */
+/* sequence, one without tokens too), a seq_start that decreases or passes   */
+/* `tokens`, more tokens or keys than max_tokens or max_kv say, or a page    */
+/* outside [0, pages) of a token that the call touches fails the stream at   */
+/* its next sync                                                             */
 /* (VNPU_ERR_DEVICE_ERROR); nothing outside the given buffers is touched,    */
 /* and what such a call wrote is unspecified.                                */
 /* ----------------------------------------------------------------------- */

@@ -1082,8 +1082,9 @@ k::KvCall kv_call_params(vnpu_stream_t *s, const vnpu_kv_cache_t &c, const int32
             "kv page_size is 16, 32, 64, 128 or 256");
     require(c.head_dim && c.head_dim <= 256 && c.head_dim % 16 == 0, "kv head_dim is a multiple of 16 up to 256");
     require(!((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15), "kv codes are 16-byte aligned");
-    // Pages and positions are int32 on the device, grids 16 bits in y.
-    require(c.pages <= 0x7fffffffu && c.table_ld <= 0x7fffffffu / c.page_size && c.kv_heads <= 65535, "kv cache too large");
+    // Pages and positions are int32 on the device (a step past the last key
+    // too), grids 16 bits in y.
+    require(c.pages <= 0x7fffffffu && c.table_ld <= (1u << 30) / c.page_size && c.kv_heads <= 65535, "kv cache too large");
     require(batch && tokens && batch <= (1u << 24) && tokens <= (1u << 28), "invalid kv batch or tokens");
     require(seq_start || tokens % batch == 0, "kv tokens is a multiple of batch without seq_start");
     k::KvCall p;

@@ -398,7 +398,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
     int8_t *k_lds = lds + wave * 128 * DP, *v_lds = k_lds + 64 * DP;
     uint32_t *sh_p = reinterpret_cast<uint32_t *>(lds + WAVES * 128 * DP) + wave * 256;
     float *sh_o_all = reinterpret_cast<float *>(lds + WAVES * (128 * DP + 1024)), *sh_o = sh_o_all + wave * RT * DT * 64;
-    if (blockIdx.x == 0 && h == 0) kv::check_all(c, false, p.max_kv);
+    if (blockIdx.x == 0 && h == 0) kv::check_all(c, false, p.max_kv, p.max_tokens);
     uint32_t slot = blockIdx.x;
     Slot sl;
     if (!find_slot(p, sp, false, slot, sl)) return;
@@ -901,7 +901,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t G = c.c.kv_heads, h = blockIdx.x % G, D = FULL ? DP : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
-    if (blockIdx.x == 0 && blockIdx.y == 0) kv::check_all(c, false, p.max_kv);
+    if (blockIdx.x == 0 && blockIdx.y == 0) kv::check_all(c, false, p.max_kv, p.max_tokens);
     // The last tiles of a causal sequence have the most keys: they come first.
     uint32_t b, tile, len;
     kv::Seq seq;

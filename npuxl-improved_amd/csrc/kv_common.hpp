@@ -74,13 +74,13 @@ inline uint32_t unit_count(const KvCall &c)
 
 // Every sequence's rows and lengths, looked over by one workgroup of a call so
 // that what no workgroup meets is an error too.  extra: the call's tokens count
-// towards the length (append, read).
-__device__ __forceinline__ void check_all(const KvCall &c, bool extra, uint32_t limit)
+// towards the length (append, read).  most: tokens of a sequence.
+__device__ __forceinline__ void check_all(const KvCall &c, bool extra, uint32_t limit, uint32_t most)
 {
     for (uint32_t b = threadIdx.x; b < c.batch; b += blockDim.x) {
         const Seq s = sequence(c, b);
         const int64_t len = c.lengths ? c.lengths[b] : 0;
-        if (!s.ok || len < 0 || len + (extra ? static_cast<int64_t>(s.n) : 0) > static_cast<int64_t>(limit)) fail(c.err);
+        if (!s.ok || s.n > most || len < 0 || len + (extra ? static_cast<int64_t>(s.n) : 0) > static_cast<int64_t>(limit)) fail(c.err);
     }
 }
 

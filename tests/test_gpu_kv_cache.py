@@ -424,6 +424,20 @@ def test_bad_arrays_fail_the_stream(own, op, bad):
     assert np.all(out[T:] == 7)
 
 
+@pytest.mark.parametrize("n,told", [([3, 1, 2], 2), ([40, 1, 2], 39), ([1, 200, 1], 1)])
+def test_more_tokens_than_told_fail_the_stream(own, n, told):
+    """A sequence with more tokens than max_tokens says, met by either kernel or by none."""
+    c = kv.Cache(np.random.default_rng(1), 3, 2, 64, 16, 20)
+    cache, _ = kv.upload(own, c)
+    T = sum(n)
+    q, o = own.alloc(T * 4 * 64 * 4), own.alloc(T * 4 * 64 * 4)
+    lengths, start = own.upload(np.array([300, 250, 200], np.int32)), own.upload(kv.starts(n))
+    f = dict(cache=cache, Q=q, O=o, kv_len=lengths.ptr, seq_start=start.ptr, batch=3, tokens=T, heads=4, causal=1)
+    run(own, (abi.OP_KV_ATTENTION_I8, dict(f, max_tokens=max(n))))
+    assert own.submit([own.command(abi.OP_KV_ATTENTION_I8, **dict(f, max_tokens=told))]) == abi.OK
+    assert own.sync() == abi.ERR_DEVICE_ERROR
+
+
 def test_refused_commands_fail_the_stream(own):
     c = kv.Cache(np.random.default_rng(1), 1, 1, 64, 16, 2)
     cache, _ = kv.upload(own, c)

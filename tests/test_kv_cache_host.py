@@ -113,6 +113,13 @@ def test_grids_that_cannot_be_launched_are_refused(make, bad, fine):
     assert taken(opcode, {**fields, **fine})
 
 
+@pytest.mark.parametrize("make", [append, attention, read])
+@pytest.mark.parametrize("page", [16, 256])
+def test_rooms_of_more_than_a_billion_tokens_are_refused(make, page):
+    assert taken(*make(cache(page_size=page, table_ld=(1 << 30) // page)))
+    assert not taken(*make(cache(page_size=page, table_ld=(1 << 30) // page + 1)))
+
+
 def test_routes_over_sizes():
     """One workgroup for a sequence and head, keys split over workgroups, tiles, tiles with split keys, both."""
     def text(max_kv, batch=1, tokens=1, seq_start=None):
