@@ -90,6 +90,8 @@ __device__ __forceinline__ float power_ratio(float a, float b)
 }
 // 2^14 / N, exact.
 __device__ __forceinline__ float up_over(float n) { return __uint_as_float((268u << 23) - __float_as_uint(n)); }
+// 1 / N of a power of two from 2^-126 to 2^126, exact.
+__device__ __forceinline__ float over_power(float n) { return __uint_as_float((254u << 23) - __float_as_uint(n)); }
 
 // ---------------------------------------------------------------------------
 // Which workgroup does what.  kv_len is on the device.  With enough sequences
@@ -310,21 +312,34 @@ __device__ __forceinline__ void weigh(float &sum, const v4f f[4], int half, floa
 // so one product gives a lane the four digit sums of one result:
 //   q digits x K codes   lane (r = g, c): row r, key 4 c + t of tile t;
 //   p digits x V codes   lane (r = g, c): row r, dimension 16 t + c of tile t.
-// A weight is the whole number p * v_scale * 2^26 / N, p = 2^(s - m) for a
-// reference m that s may pass by 4, N a power of two that v_scale may not
-// pass; sums stay whole numbers until m or N has to move, then they are added
-// to f32 sums in LDS.
+// A weight w = p * v_scale / N, p = 2^(s - m) for a reference m that s may pass by
+// 4, N a power of two that v_scale may not pass, becomes the whole number rint(w *
+// 2^k), k such that the largest of the row's weights in these 64 keys has 31 bits:
+// a chunk's sums are whole numbers of their own unit, then added to f32 sums.  What
+// the rounding left is four digits more, under 2^-31 of the unit, and goes through
+// the product again where it is more than 2^-22 of some weight: one key with nearly
+// all of the weight, or a page of large values, takes nothing from the others.
+// (In one unit for all chunks, that of the largest weight so far, whole sums could
+// stay on the matrix cores, 3 to 6 % faster, with 16 rows 52 us instead of 68 for 16
+// sequences of 4096 keys, but weights 2^-26 below it were lost: 7 % of a result
+// whose first of 4096 keys has 99.99 % of the weight and zeros for values.)
 // Bound by the codes from HBM where there are enough of them (32 heads of 128, 8
-// sequences of 4096 keys: 42 us, 6.4 TB/s of codes; a large read reaches 6.2 to
-// 6.7; 64 sequences of 100 to 8000 keys, 32 heads to 8: 106 us, 5.6 TB/s; one of
+// sequences of 4096 keys: 42 us, 6.3 TB/s of codes; a large read reaches 6.2 to
+// 6.7; 64 sequences of 100 to 8000 keys, 32 heads to 8: 110 us, 5.4 TB/s; one of
 // 131072 keys: 43 us and 4.5 us of join), by the latency of launch, page,
-// copy and join where not (one sequence of 128 keys 5.2 us, of 4096 10.9 us).
+// copy and join where not (one sequence of 128 keys 5.4 us, of 4096 11.3 us).
 // Not temporal copies: 67 -> 56 us at the first size, which nothing reads twice.
 // ---------------------------------------------------------------------------
 
 constexpr float kDigits4 = 2139060000.0f;   // four digits hold 127 * (2^24 + 2^16 + 2^8 + 1) = 2139062143
 constexpr float kAhead = 4.0f;
-constexpr uint32_t kMostChunks = 2000;      // 64 keys add at most 64 * 128 * 127 to a sum: 2064 fit
+// Biased exponent e for whole numbers of up to 31 bits: x * 2^(157 - e), x at most
+// `largest`, fits four digits (2139062143 / 2^30 is 2 less 65793 / 2^23; 0x10400 is 66560).
+// Below 2^-96 e stays, so that 2^(e - 157) is a normal number.
+__device__ __forceinline__ uint32_t digits_exponent(float largest)
+{
+    return max((__float_as_uint(largest) + 0x10400u) >> 23, 31u);
+}
 
 // Maximum / sum over the 16 lanes of a row.
 template <int CTRL>
@@ -346,15 +361,10 @@ __device__ __forceinline__ float row_sum(float x)
     x += dpp_row<0x122>(x);
     return x + dpp_row<0x121>(x);
 }
-// Sum of four digit sums, digit i counting 256^i.
+// Sum of four digit sums over 64 keys or 256 dimensions, digit i counting 256^i.
 __device__ __forceinline__ float digits_sum(const v4i &a)
 {
     return fmaf(static_cast<float>(a[3] * 256 + a[2]), 65536.0f, static_cast<float>(a[1] * 256 + a[0]));
-}
-__device__ __forceinline__ float digits_sum_wide(const v4i &a)   // sums over many chunks
-{
-    const float hi = fmaf(static_cast<float>(a[3]), 256.0f, static_cast<float>(a[2]));
-    return fmaf(hi, 65536.0f, fmaf(static_cast<float>(a[1]), 256.0f, static_cast<float>(a[0])));
 }
 
 template <typename T>
@@ -555,7 +565,8 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
     // With 16 rows the queries stay in LDS: a register spilled in the loop would
     // wait for the copies under way.
     constexpr bool kHeld = RT < 4;
-    v4i q[kHeld ? RT : 1][DS], acc[RT][DT];
+    v4i q[kHeld ? RT : 1][DS];
+    float o[RT][DT];                  // row g, dimension 16 t + col, in N
     float factor[RT], m[RT], l[RT];   // of row g: score in powers of two = sum * factor * k_scale
     int limit[RT];                    // keys that row g sees
 #pragma unroll
@@ -569,21 +580,27 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
         m[r] = kNegInf;
         l[r] = 0.0f;
 #pragma unroll
-        for (int t = 0; t < DT; ++t) acc[r][t] = v4i{0, 0, 0, 0};
+        for (int t = 0; t < DT; ++t) o[r][t] = 0.0f;
     }
     const int least = p.causal ? max(0, len - static_cast<int>(n) + static_cast<int>(row0 / group) + 1) : len;   // every row sees the keys below
     float N = power_above(0.0f);
-    uint32_t since = 0;
-    bool begun = false, kept = false;   // the whole sums, the f32 sums hold something
-    // Whole sums to the f32 ones, both by `by`.
-    auto gather = [&](int r, float by) {
+    // Four whole numbers of this lane's keys as digits through LDS: operand row 4 r + d
+    // of the product with V.
+    auto operand = [&](const int x[4]) {
+        uint32_t u[4];
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            if (!FULL && 16 * t >= static_cast<int>(D)) continue;
-            float &o = sh_o[(r * DT + t) * 64 + lane];
-            o = ((kept ? o : 0.0f) + digits_sum_wide(acc[r][t])) * by;
-            acc[r][t] = v4i{0, 0, 0, 0};
-        }
+        for (int t = 0; t < 4; ++t) u[t] = (static_cast<uint32_t>(x[t]) + 0x80808080u) ^ 0x80808080u;
+        const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), e = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
+        const uint32_t d = __builtin_amdgcn_perm(u[1], u[0], 0x07030602u), k = __builtin_amdgcn_perm(u[3], u[2], 0x07030602u);
+        uint32_t *to = sh_p + 64 * g + col;
+        to[0] = __builtin_amdgcn_perm(e, a, 0x05040100u);
+        to[16] = __builtin_amdgcn_perm(e, a, 0x07060302u);
+        to[32] = __builtin_amdgcn_perm(k, d, 0x05040100u);
+        to[48] = __builtin_amdgcn_perm(k, d, 0x07060302u);
+        __builtin_amdgcn_wave_barrier();
+        const v4i got = *reinterpret_cast<const v4i *>(sh_p + 16 * col + 4 * g);
+        __builtin_amdgcn_wave_barrier();
+        return got;
     };
 
     for (bool more = any; more;) {
@@ -634,48 +651,52 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
             move |= top[r] > m[r] + kAhead;
         }
         move |= scale > N;
-        if (__any(move) || ++since >= kMostChunks) {
+        if (__any(move)) {
             // N is one for the wave's rows, with a factor of two to spare.
-            const float need = groups_max(row_max(power_above(scale))), N_now = need > N ? fminf(2.0f * need, 1.7014118346046923e38f) : N;
+            const float need = groups_max(row_max(power_above(scale))), N_now = need > N ? fminf(2.0f * need, 8.507059173023462e37f) : N;   // to 2^126
             const float beta = power_ratio(N, N_now);
             N = N_now;
-            since = 0;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 const float now = fmaxf(m[r], row_max(top[r]));
                 const float alpha = now > m[r] ? __builtin_amdgcn_exp2f(m[r] - now) : 1.0f;
-                if (begun) gather(r, alpha * beta);
                 l[r] *= alpha;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) o[r][t] *= alpha * beta;
                 m[r] = now;
             }
-            kept = begun;
         }
-        begun = true;
-        const float fv = scale * __uint_as_float((280u << 23) - __float_as_uint(N));   // 2^26 / N
+        const float fv = scale * over_power(N);
         v4i pd[RT];
+        float unit[RT];   // of the chunk's whole numbers, in N; f becomes what their rounding left
+        bool again[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const float base = m[r] == kNegInf ? 0.0f : m[r];
-            uint32_t u[4];
+            float w[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                float e = __builtin_amdgcn_exp2f(f[r][t] - base), x = fmaf(e, fv, 0.5f);
-                if (!all && first + t >= limit[r]) e = x = 0.0f;
+                float e = __builtin_amdgcn_exp2f(f[r][t] - base);
+                w[t] = e * fv;
+                if (!all && first + t >= limit[r]) e = w[t] = 0.0f;
                 l[r] += e;
-                u[t] = (static_cast<uint32_t>(static_cast<int>(x)) + 0x80808080u) ^ 0x80808080u;
             }
             // A scale that is no number shows in l: whole numbers cannot.
             if (all || first < limit[r]) l[r] = fmaf(fv, 0.0f, l[r]);
-            const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), e = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
-            const uint32_t d = __builtin_amdgcn_perm(u[1], u[0], 0x07030602u), k = __builtin_amdgcn_perm(u[3], u[2], 0x07030602u);
-            uint32_t *to = sh_p + 64 * g + col;
-            to[0] = __builtin_amdgcn_perm(e, a, 0x05040100u);
-            to[16] = __builtin_amdgcn_perm(e, a, 0x07060302u);
-            to[32] = __builtin_amdgcn_perm(k, d, 0x05040100u);
-            to[48] = __builtin_amdgcn_perm(k, d, 0x07060302u);
-            __builtin_amdgcn_wave_barrier();
-            pd[r] = *reinterpret_cast<const v4i *>(sh_p + 16 * col + 4 * g);
-            __builtin_amdgcn_wave_barrier();
+            const uint32_t e = digits_exponent(row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))));
+            const float up = __uint_as_float((284u - e) << 23);
+            unit[r] = __uint_as_float((e - 30u) << 23);
+            int x[4];
+            bool lost = false;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float y = w[t] * up, whole = rintf(y);
+                x[t] = static_cast<int>(whole);
+                f[r][t] = y - whole;
+                lost |= fabsf(f[r][t]) > y * 2.384185791015625e-07f;   // 2^-22
+            }
+            again[r] = __any(lost);
+            pd[r] = operand(x);
         }
         if (more) wait_copies<DP, FULL>(tiles);   // the next K's may be under way
         else lds::wait_vmcnt<0>();
@@ -693,7 +714,25 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
         for (int t = 0; t < DT; ++t) {
             if (!FULL && t >= static_cast<int>(tiles)) continue;
 #pragma unroll
-            for (int r = 0; r < RT; ++r) acc[r][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[r], vf[t], acc[r][t], 0, 0, 0);
+            for (int r = 0; r < RT; ++r) {
+                const v4i sums = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[r], vf[t], v4i{0, 0, 0, 0}, 0, 0, 0);
+                o[r][t] = fmaf(digits_sum(sums), unit[r], o[r][t]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            if (!again[r]) continue;
+            int x[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) x[t] = static_cast<int>(rintf(f[r][t] * 2147483648.0f));   // 2^31; f is 1/2 at most
+            const v4i rest = operand(x);
+            const float below = unit[r] * 4.656612873077393e-10f;   // 2^-31
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                if (!FULL && t >= static_cast<int>(tiles)) continue;
+                const v4i sums = __builtin_amdgcn_mfma_i32_16x16x64_i8(rest, vf[t], v4i{0, 0, 0, 0}, 0, 0, 0);
+                o[r][t] = fmaf(digits_sum(sums), below, o[r][t]);
+            }
         }
         chunk += WAVES;
     }
@@ -703,7 +742,10 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const float sum = row_sum(l[r]);
-        gather(r, sum != 0.0f ? N * 1.4901161193847656e-08f / sum : 0.0f);   // 2^-26
+        const float by = sum != 0.0f ? N / sum : 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+            if (FULL || 16 * t < static_cast<int>(D)) sh_o[(r * DT + t) * 64 + lane] = o[r][t] * by;
         if (col == 0) {
             sh_m[wave][4 * r + g] = m[r];
             sh_l[wave][4 * r + g] = sum;
