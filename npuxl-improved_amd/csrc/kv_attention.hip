@@ -313,7 +313,7 @@ __device__ __forceinline__ void weigh(float &sum, const v4f f[4], int half, floa
 //   q digits x K codes   lane (r = g, c): row r, key 4 c + t of tile t;
 //   p digits x V codes   lane (r = g, c): row r, dimension 16 t + c of tile t.
 // A weight w = p * v_scale / N, p = 2^(s - m) for a reference m that s may pass by
-// 4, N a power of two that v_scale may not pass, becomes the whole number rint(w *
+// 4, N a power of two that no v_scale seen by the row passes, becomes the whole number rint(w *
 // 2^k), k such that the largest of the row's weights in these 64 keys has 31 bits:
 // a chunk's sums are whole numbers of their own unit, then added to f32 sums.  What
 // the rounding left is four digits more, under 2^-31 of the unit, and goes through
@@ -396,7 +396,7 @@ constexpr uint32_t few_lds()
 }
 
 template <int DP, int RT, bool FULL, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) void kv_attention_few(KvAttn p, Split sp, float *ws, uint32_t ws_rows)
+__global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) void kv_attention_few(KvAttn p, Split sp, float *ws, uint32_t ws_rows)
 {
     constexpr int DS = DP / 64, DT = DP / 16, R = 4 * RT;
     extern __shared__ __align__(1024) int8_t lds[];
@@ -567,7 +567,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
     constexpr bool kHeld = RT < 4;
     v4i q[kHeld ? RT : 1][DS];
     float o[RT][DT];                  // row g, dimension 16 t + col, in N
-    float factor[RT], m[RT], l[RT];   // of row g: score in powers of two = sum * factor * k_scale
+    float factor[RT], m[RT], l[RT], N[RT];   // of row g: score in powers of two = sum * factor * k_scale
     int limit[RT];                    // keys that row g sees
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -579,11 +579,11 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
         limit[r] = p.causal && mine < rows ? max(0, len - static_cast<int>(n) + static_cast<int>(mine / group) + 1) : len;
         m[r] = kNegInf;
         l[r] = 0.0f;
+        N[r] = power_above(0.0f);
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[r][t] = 0.0f;
     }
     const int least = p.causal ? max(0, len - static_cast<int>(n) + static_cast<int>(row0 / group) + 1) : len;   // every row sees the keys below
-    float N = power_above(0.0f);
     // Four whole numbers of this lane's keys as digits through LDS: operand row 4 r + d
     // of the product with V.
     auto operand = [&](const int x[4]) {
@@ -609,6 +609,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
         const float ks = of_block(kb, ks4), scale = of_block(kb, vs4);
         const int first = static_cast<int>(kChunk * chunk + 4 * col);
         const bool all = static_cast<int>(kChunk * chunk + kChunk) <= least;
+        auto seen = [&](int r) { return all || first < limit[r]; };   // keys of this lane's page
         wait_copies<DP, FULL>(tiles);   // V's may be under way
         v4i kf[4][DS];
 #pragma unroll
@@ -648,16 +649,17 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
 #pragma unroll
                 for (int t = 0; t < 4; ++t) top[r] = fmaxf(top[r], first + t < limit[r] ? f[r][t] : kNegInf);
             }
-            move |= top[r] > m[r] + kAhead;
+            // A page that the row does not see counts for nothing.
+            move |= top[r] > m[r] + kAhead || (seen(r) && scale > N[r]);
         }
-        move |= scale > N;
         if (__any(move)) {
-            // N is one for the wave's rows, with a factor of two to spare.
-            const float need = groups_max(row_max(power_above(scale))), N_now = need > N ? fminf(2.0f * need, 8.507059173023462e37f) : N;   // to 2^126
-            const float beta = power_ratio(N, N_now);
-            N = N_now;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
+                // With a factor of two to spare, up to 2^126.
+                const float need = row_max(power_above(seen(r) ? scale : 0.0f));
+                const float N_now = need > N[r] ? fminf(2.0f * need, 8.507059173023462e37f) : N[r];
+                const float beta = power_ratio(N[r], N_now);
+                N[r] = N_now;
                 const float now = fmaxf(m[r], row_max(top[r]));
                 const float alpha = now > m[r] ? __builtin_amdgcn_exp2f(m[r] - now) : 1.0f;
                 l[r] *= alpha;
@@ -666,13 +668,12 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
                 m[r] = now;
             }
         }
-        const float fv = scale * over_power(N);
         v4i pd[RT];
         float unit[RT];   // of the chunk's whole numbers, in N; f becomes what their rounding left
         bool again[RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            const float base = m[r] == kNegInf ? 0.0f : m[r];
+            const float base = m[r] == kNegInf ? 0.0f : m[r], fv = scale * over_power(N[r]);
             float w[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -682,7 +683,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
                 l[r] += e;
             }
             // A scale that is no number shows in l: whole numbers cannot.
-            if (all || first < limit[r]) l[r] = fmaf(fv, 0.0f, l[r]);
+            if (seen(r)) l[r] = fmaf(fv, 0.0f, l[r]);
             const uint32_t e = digits_exponent(row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))));
             const float up = __uint_as_float((284u - e) << 23);
             unit[r] = __uint_as_float((e - 30u) << 23);
@@ -742,7 +743,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 512 && DP <= 128 ? 2 : 1) vo
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const float sum = row_sum(l[r]);
-        const float by = sum != 0.0f ? N / sum : 0.0f;
+        const float by = sum != 0.0f ? N[r] / sum : 0.0f;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
             if (FULL || 16 * t < static_cast<int>(D)) sh_o[(r * DT + t) * 64 + lane] = o[r][t] * by;

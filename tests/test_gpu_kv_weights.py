@@ -70,6 +70,8 @@ def check(s, c, q, kv_len, n, heads, causal=1, scale=0.0, nan=None, in_rows=None
             want, bound = rows_of(c, b, h, h // (heads // G), q[at:at + m, h], int(kv_len[b]), causal, used, last)
             rows = np.ones(m, bool) if nan is None else ~nan[at:at + m, h]
             assert np.all(np.isnan(got[~rows]))
+            if not rows.any():
+                continue
             off = np.abs(got[rows] - want[rows])
             over = ~(off <= bound[rows])
             assert not over.any(), (b, h, np.argwhere(over)[:3].tolist(), float((off / bound[rows]).max()),
@@ -147,3 +149,40 @@ def test_quiet_pages_beside_loud_ones(gpu, n, heads, kv_heads, d, page, ratio):
         c.k[loud] = (-100 * u).astype(np.int8)
     check(gpu, c, q, kv_len, [n, n], heads, scale=90.0 / d, causal=0)   # about e^-90 of the others
     check(gpu, c, q, kv_len, [n, n], heads, scale=20.0 / d, causal=0)
+
+
+@pytest.mark.parametrize("what,value", [("vs", 1e6), ("vs", 1e30), ("vs", np.inf), ("vs", np.nan), ("ks", 1e20), ("ks", np.nan)])
+@pytest.mark.parametrize("n,heads,kv_heads,d,page", [(2, 4, 2, 64, 16), (7, 2, 1, 128, 16), (16, 1, 1, 80, 16), (8, 2, 2, 256, 16)])
+def test_pages_that_a_row_does_not_see(gpu, n, heads, kv_heads, d, page, what, value):
+    """Earlier tokens of a causal call have nothing of a later one's scales; infinite ones give NaN to those that see them."""
+    rng = np.random.default_rng(6)
+    kv_len = [16 * page + 1, 2 * page + n - n % page + 1, page * (-(-n // page))]
+    kv_len = [max(x, n) for x in kv_len]
+    c = kv.Cache(rng, 3, kv_heads, d, page, -(-max(kv_len) // page))
+    q = rng.standard_normal((3 * n, heads, d)).astype(np.float32)
+    nan = np.zeros((3 * n, heads), bool)
+    for b, length in enumerate(kv_len):
+        last = (length - 1) // page
+        getattr(c, what)[c.table[b, last]] = value
+        sees = length - n + np.arange(n) >= last * page
+        if not np.isfinite(value):
+            nan[b * n:(b + 1) * n] = sees[:, None]
+        elif what == "ks":   # scores as they are elsewhere for the rows that see it
+            q[b * n:(b + 1) * n][sees] *= np.float32(1e-20)
+    with np.errstate(all="ignore"):
+        check(gpu, c, q, kv_len, [n] * 3, heads, nan=nan)
+
+
+@pytest.mark.parametrize("n", [1, 3, 12])
+@pytest.mark.parametrize("spread", [2, 6, 14])
+def test_scales_and_scores_over_orders_of_magnitude(gpu, n, spread):
+    """Random scales of both sides, scores from flat to picking one key."""
+    for seed, factor in enumerate((0.3, 3.0, 20.0)):
+        rng = np.random.default_rng(seed)
+        kv_len = [900, 65 + n, n]
+        c = kv.Cache(rng, 3, 2, 64, 32, 29)
+        c.vs *= (10.0 ** rng.uniform(-spread, 1, c.vs.shape)).astype(np.float32)
+        c.ks *= (2.0 ** rng.uniform(-3, 1, c.ks.shape)).astype(np.float32)
+        q = (factor * rng.standard_normal((3 * n, 4, 64))).astype(np.float32)
+        check(gpu, c, q, kv_len, [n] * 3, 4)
+        check(gpu, c, q[:sum([n, n, 1])], kv_len, [n, n, 1], 4)
