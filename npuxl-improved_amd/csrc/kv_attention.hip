@@ -12,9 +12,10 @@
 //   Q . K   int8: a query row is the whole number rint(q * S), S = 8355700 /
 //           max|q|, in three balanced base-256 digits (24 bits), so three
 //           v_mfma_i32_16x16x64_i8 give the sum without a rounding;
-//   P . V   f16: a code is exact in f16, a weight times its page's scale over a
-//           power of two N >= all scales so far is hi + lo, two f16 (22 bits),
-//           and two v_mfma_f32_16x16x32_f16 sum in f32.
+//   P . V   f16: a code is exact in f16, a weight times its page's scale over the
+//           row's unit U is hi + lo, two f16 (22 bits, and 2^-25 where those end),
+//           and two v_mfma_f32_16x16x32_f16 sum in f32.  U is a power of two that
+//           follows the largest product of the row in each chunk, up and down.
 // The scores are computed transposed (keys x rows) with the keys of a 64-key
 // chunk dealt to the tiles so that lane (group g, row) ends with keys 16g ..
 // 16g + 15 of its row: those are the operand of P . V as they stand, and their
@@ -88,8 +89,6 @@ __device__ __forceinline__ float power_ratio(float a, float b)
 {
     return __int_as_float(max(0, 0x3f800000 + __float_as_int(a) - __float_as_int(b)));
 }
-// 2^14 / N, exact.
-__device__ __forceinline__ float up_over(float n) { return __uint_as_float((268u << 23) - __float_as_uint(n)); }
 // 1 / N of a power of two from 2^-126 to 2^126, exact.
 __device__ __forceinline__ float over_power(float n) { return __uint_as_float((254u << 23) - __float_as_uint(n)); }
 
@@ -238,15 +237,24 @@ struct Query {
 };
 
 // The running softmax of a lane's row and its part of O^T: dimensions 16 t +
-// 4 g + i.  o counts in N / 2^14; l is this lane's part of the sum.
+// 4 g + i.  o counts in 2^-shift = U / 2^14; l is this lane's part of the sum.
+// The largest p * v_scale of the row's chunk lies between 2^-12 U and 2 U: below, U
+// comes down after it, so that its smaller weights keep their bits, unless o, which
+// holds what was summed before, would pass 2^100.  The reference m is one that
+// scores may pass by kAhead, as for few rows.  (Scores of normal numbers: one chunk in
+// 40 moves something for one of a wave's 32 rows, 243 us for 4096 tokens against 237 with a
+// U that only grew; 8 times as far apart every chunk does, 267 against 228.  Within 2^-6
+// a fifth of the chunks did for ordinary scores: 259.)
+constexpr float kAhead = 4.0f, kMostShift = 114.0f;
 template <int DT>
 struct State {
     v4f o[DT];
-    float m, l;
+    float m, l, shift;
     __device__ __forceinline__ void clear()
     {
         m = kNegInf;
         l = 0.0f;
+        shift = kMostShift;
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -332,7 +340,6 @@ __device__ __forceinline__ void weigh(float &sum, const v4f f[4], int half, floa
 // ---------------------------------------------------------------------------
 
 constexpr float kDigits4 = 2139060000.0f;   // four digits hold 127 * (2^24 + 2^16 + 2^8 + 1) = 2139062143
-constexpr float kAhead = 4.0f;
 // Biased exponent e for whole numbers of up to 31 bits: x * 2^(157 - e), x at most
 // `largest`, fits four digits (2139062143 / 2^30 is 2 less 65793 / 2^23; 0x10400 is 66560).
 // Below 2^-96 e stays, so that 2^(e - 157) is a normal number.
@@ -867,14 +874,14 @@ __global__ __launch_bounds__(kJoinThreads) void kv_attention_merge(KvAttn p, Spl
 // f16 once for the four waves; both of the next chunk are on their way while
 // this one is computed, and one barrier a chunk hands the buffers over.
 // Bound by the vector instructions: 64 keys of 32 rows take a wave 112 matrix
-// instructions (16 cycles each) and about 530 others (4 cycles, exponentials 16):
+// instructions (16 cycles each) and about 490 others (4 cycles, exponentials 16):
 // three conversions and sums for a score's digits, ten for a weight and its two
 // halves.  Two waves a SIMD fill 73 % of its vector issue and 47 % of its matrix
 // cores.  A step has few branches, so that its products and exponentials
 // mix: with the rows one after another and conditions inside, 306 us instead of 256.
-// 4096 tokens on themselves, causal, 32 heads of 128: 239 us, 576 TFLOP/s (a
+// 4096 tokens on themselves, causal, 32 heads of 128: 243 us, 566 TFLOP/s (a
 // large f16 product of the library, which needs 2 of these 5 matrix
-// instructions, 1109); heads of 64 165 us, of 256 (half the heads and tokens) 115 us.
+// instructions, 1109); heads of 64 161 us, of 256 (half the heads and tokens) 100 us.
 // Workgroups of 8 waves and 256 rows: 254 us and worse where tiles are few.
 // ---------------------------------------------------------------------------
 
@@ -934,7 +941,7 @@ __device__ __forceinline__ uint32_t ranges_of(const Tiles &tl, uint32_t chunks)
 }
 
 template <int DP, int RT, bool FULL, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
+__global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
 {
     constexpr int DS = DP / 64, DT = DP / 16;
     constexpr uint32_t M = 16 * RT * WAVES;
@@ -992,7 +999,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
     };
     constexpr int VW = (DT + WAVES - 1) / WAVES, KW = (4 * DS + WAVES - 1) / WAVES;   // tiles of V, pieces of K that a wave brings in
     v4i vf[VW];
-    float ks = 0.0f, vs = 0.0f, N = power_above(0.0f);
+    float ks = 0.0f, vs = 0.0f;
     // A page's codes, of all heads, are less than 2^32 bytes.
     const uint32_t page_bytes = G * ps * D;
     const int8_t *k_lane = c.c.k + static_cast<uint64_t>(h * ps + (col & 3)) * D, *v_lane = c.c.v + static_cast<uint64_t>(h * D + col) * ps;
@@ -1048,9 +1055,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
             ids(min(chunk + 2, end - 1));
         }
         if constexpr (WORK) {
-            const float above = groups_max(power_above(v_scale)), N_now = fmaxf(N, above);
-            const float beta = power_ratio(N, N_now), fv = v_scale * up_over(N_now);
-            N = N_now;
+            // The lane's 16 keys are of one page.  What is multiplied with its scale stays finite
+            // whatever U is: a row with a U so far below it has no weight there.
+            const float power = __builtin_amdgcn_fmed3f(__builtin_amdgcn_logf(v_scale), -100.0f, 127.0f);
+            const float most_shift = 126.0f - fmaxf(power, 0.0f);
             const int first = static_cast<int>(kChunk * chunk + 16 * g);
             v4f f[RT][4];
 #pragma unroll
@@ -1072,31 +1080,57 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
                         f[r][t][i] = fmaf(static_cast<float>(a[r][0][i] * 256 + a[r][1][i]), 256.0f, static_cast<float>(a[r][2][i]));
             }
             float ck[RT], base[RT], top[RT];
-            bool move = beta != 1.0f;
+            bool move = false;
+            uint32_t covered = 0xffffu;   // rows with a product of 2^-12 U or more, or none at all
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 ck[r] = q[r].factor * k_scale;
-                top[r] = fmaxf(st[r].m, groups_max(largest<MASK>(f[r], ck[r], limit[r] - first)));
-                base[r] = top[r] == kNegInf ? 0.0f : top[r];
-                move = move || top[r] > st[r].m;
+                top[r] = largest<MASK>(f[r], ck[r], limit[r] - first);   // of the lane's keys
+                const float over = top[r] - st[r].m + (power - 14.0f + st[r].shift);   // log2 of the largest product / U
+                move = move || top[r] > st[r].m + kAhead || over > 1.0f;
+                const uint64_t rows_of = __ballot(over >= -12.0f || (MASK && limit[r] <= static_cast<int>(kChunk * chunk)));
+                const uint32_t halves = static_cast<uint32_t>(rows_of | rows_of >> 32);
+                covered &= halves | halves >> 16;
             }
-            if (__any(move)) {   // else o is left alone
+            if (__any(move) || covered != 0xffffu) {   // else o is left alone
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    // 1 for rows whose maximum stays.
-                    const float alpha = top[r] > st[r].m ? __builtin_amdgcn_exp2f(st[r].m - base[r]) : 1.0f;
+                    const float now = fmaxf(st[r].m, groups_max(top[r]));
+                    const float alpha = now > st[r].m ? __builtin_amdgcn_exp2f(st[r].m - now) : 1.0f;
+                    const float need = groups_max(top[r] + power) - now;
+                    // A row without keys or numbers keeps its unit.
+                    float to = st[r].shift;
+                    if (need > 15.0f - to) to = 10.0f - ceilf(need);   // U up: 2^-4 U is the largest now
+                    const bool low = need < 2.0f - to;
+                    if (__any(low)) {
+                        float held = 0.0f;
+#pragma unroll
+                        for (int t = 0; t < DT; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) held = fmaxf(held, fabsf(st[r].o[t][i]));
+                        const float room = 226.0f - static_cast<float>(__float_as_uint(groups_max(held)) >> 23);
+                        if (low) to = fminf(fminf(8.0f - ceilf(fmaxf(need, -200.0f)), to + fmaxf(0.0f, room)), kMostShift);   // 2^-6 U
+                    }
+                    const float by = ldexpf(alpha, static_cast<int>(to - st[r].shift));
                     st[r].l *= alpha;
 #pragma unroll
-                    for (int t = 0; t < DT; ++t) st[r].o[t] *= alpha * beta;
-                    st[r].m = top[r];
+                    for (int t = 0; t < DT; ++t) st[r].o[t] *= by;
+                    st[r].m = now;
+                    st[r].shift = to;
                 }
+            }
+            float fv[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                base[r] = st[r].m == kNegInf ? 0.0f : st[r].m;
+                fv[r] = ldexpf(v_scale, static_cast<int>(fminf(st[r].shift, most_shift)));
             }
             // The products of the first half's weights go beside the second half's exponentials.
             v8h hi[RT][2], lo[RT][2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
 #pragma unroll
-                for (int r = 0; r < RT; ++r) weigh<MASK>(st[r].l, f[r], k, ck[r], base[r], fv, limit[r] - first, hi[r][k], lo[r][k]);
+                for (int r = 0; r < RT; ++r) weigh<MASK>(st[r].l, f[r], k, ck[r], base[r], fv[r], limit[r] - first, hi[r][k], lo[r][k]);
             }
             if (more) turn_v(next);
 #pragma unroll
@@ -1129,14 +1163,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
     for (int r = 0; r < RT; ++r) {
         const uint32_t row = row0 + 16 * r + col;
         const float l = groups_sum(st[r].l);
-        const float by = l != 0.0f ? N * 6.103515625e-05f / l : 0.0f;   // 2^-14
+        const float by = l != 0.0f ? 1.0f / l : 0.0f;
+        const int down = -static_cast<int>(st[r].shift);
+        auto result = [&](int t) { return v4f{ldexpf(st[r].o[t][0] * by, down), ldexpf(st[r].o[t][1] * by, down), ldexpf(st[r].o[t][2] * by, down), ldexpf(st[r].o[t][3] * by, down)}; };
         if (row >= rows) continue;
         if (ranges == 1) {
             float *at = p.O + kv::rows_base(c, p.o, b, seq) + (row / group) * p.o.token + (h * group + row % group) * p.o.head + 4 * g;
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
                 if (16 * t >= static_cast<int>(D)) continue;
-                const v4f x = st[r].o[t] * by;
+                const v4f x = result(t);
                 if (out_aligned) *reinterpret_cast<v4f *>(at + 16 * t) = x;
                 else
                     for (int i = 0; i < 4; ++i) at[16 * t + i] = x[i];
@@ -1145,7 +1181,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void kv_attention_tile(KvAttn p, Til
             float *at = ws + (((static_cast<uint64_t>(unit) * G + h) * tl.parts + blockIdx.y) * M + (row - tile * M)) * (D + 4);
 #pragma unroll
             for (int t = 0; t < DT; ++t)
-                if (16 * t < static_cast<int>(D)) *reinterpret_cast<v4f *>(at + 4 * g + 16 * t) = st[r].o[t] * by;
+                if (16 * t < static_cast<int>(D)) *reinterpret_cast<v4f *>(at + 4 * g + 16 * t) = result(t);
             if (g == 0) {
                 at[D] = st[r].m;
                 at[D + 1] = l;

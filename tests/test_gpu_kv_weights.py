@@ -19,7 +19,7 @@ def rows_of(c, b, h, kv_head, q, kv_len, causal, scale, last):
     roundings of exponential and products, 2^-22 as digits or halves.  Sums over keys, of numerator and denominator:
     a rounding for every 16 keys of each, 16 more for waves, parts and the division.  All of them relative to the row's own
     sum of p |v|.  Behind these the last place of the weights' parts: `last` of the largest p * scale among the same 64 keys
-    for each."""
+    for each; and exponentials below 2^-126 are 0."""
     k, v = (x[kv_head] for x in c.values(b, kv_len))
     m, n, D = q.shape[0], kv_len, c.head_dim
     s = q.astype(np.float64) @ k.T * scale
@@ -44,7 +44,8 @@ def rows_of(c, b, h, kv_head, q, kv_len, causal, scale, last):
     w = np.pad(p * vs, ((0, 0), (0, pad))).reshape(m, -1, 64).max(axis=2)
     codes = np.abs(np.where(vs[:, None] > 0, v / np.where(vs > 0, vs, 1)[:, None], 0))
     codes = np.pad(codes, ((0, pad), (0, 0))).reshape(-1, 64, D).sum(axis=1)
-    return np.where(some[:, None], o, 0), rel[:, None] * mass + last * (w @ codes)
+    bound = rel[:, None] * mass + last * (w @ codes) + 2.0**-126 * (see @ np.abs(v))
+    return np.where(some[:, None], o, 0), bound
 
 
 def check(s, c, q, kv_len, n, heads, causal=1, scale=0.0, nan=None, in_rows=None, **more):
@@ -61,8 +62,9 @@ def check(s, c, q, kv_len, n, heads, causal=1, scale=0.0, nan=None, in_rows=None
     assert s.sync() == abi.OK
     out = s.download(y, np.float32, q.shape)
     kv.free(s, bufs, start, lens, x, y)
-    # Four digits and four of the remainder for up to 16 rows of a kv head (8 above 128 dimensions), else two f16 parts.
-    last = 2.0**-56 if not ragged and n[0] * heads // G <= (16 if D <= 128 else 8) else 2.0**-32
+    # Four digits and four of the remainder for up to 16 rows of a kv head (8 above 128 dimensions).  Else two f16 parts in a
+    # unit that the largest product is at most 2^12 below: half of 2^-24 of 2^14.
+    last = 2.0**-56 if not ragged and n[0] * heads // G <= (16 if D <= 128 else 8) else 2.0**-27
     at, worst = 0, 0.0
     for b, m in enumerate(n):
         for h in range(heads):
@@ -103,7 +105,8 @@ PLACES = {"first": lambda n: 0, "second_chunk": lambda n: min(n - 1, 70), "last"
 @pytest.mark.parametrize("place", list(PLACES))
 @pytest.mark.parametrize("silent", [True, False])
 @pytest.mark.parametrize("n,heads,kv_heads,d", [(1, 2, 2, 128), (1, 8, 2, 64), (2, 8, 2, 80), (3, 8, 2, 128), (1, 4, 1, 256),
-                                                (2, 4, 1, 192), (4, 4, 1, 128), (5, 2, 1, 112)])
+                                                (2, 4, 1, 192), (4, 4, 1, 128), (5, 2, 1, 112),
+                                                (70, 2, 1, 64), (130, 1, 1, 128), (33, 2, 2, 80), (40, 2, 2, 256)])
 def test_one_key_with_most_of_the_weight(gpu, n, heads, kv_heads, d, silent, place, weight):
     """The others, before and behind it, keep what their own small weights give, also where its values are all zero."""
     rng = np.random.default_rng(9)
@@ -134,7 +137,7 @@ def test_one_key_with_most_of_the_weight_of_a_long_sequence(gpu, silent, weight)
 
 @pytest.mark.parametrize("ratio", [1e2, 1e4, 1e6, 1e8, 1e20])
 @pytest.mark.parametrize("n,heads,kv_heads,d,page", [(1, 4, 2, 128, 16), (3, 4, 1, 64, 64), (1, 4, 4, 256, 16),
-                                                     (4, 4, 1, 80, 32)])
+                                                     (4, 4, 1, 80, 32), (70, 2, 1, 64, 16), (70, 2, 1, 128, 64), (33, 1, 1, 256, 16)])
 def test_quiet_pages_beside_loud_ones(gpu, n, heads, kv_heads, d, page, ratio):
     """Pages of large values with next to no weight leave the others theirs, in the same 64 keys and in others."""
     rng = np.random.default_rng(3)
@@ -152,7 +155,8 @@ def test_quiet_pages_beside_loud_ones(gpu, n, heads, kv_heads, d, page, ratio):
 
 
 @pytest.mark.parametrize("what,value", [("vs", 1e6), ("vs", 1e30), ("vs", np.inf), ("vs", np.nan), ("ks", 1e20), ("ks", np.nan)])
-@pytest.mark.parametrize("n,heads,kv_heads,d,page", [(2, 4, 2, 64, 16), (7, 2, 1, 128, 16), (16, 1, 1, 80, 16), (8, 2, 2, 256, 16)])
+@pytest.mark.parametrize("n,heads,kv_heads,d,page", [(2, 4, 2, 64, 16), (7, 2, 1, 128, 16), (16, 1, 1, 80, 16), (8, 2, 2, 256, 16),
+                                                     (70, 2, 1, 64, 16), (200, 1, 1, 128, 64), (70, 1, 1, 256, 16)])
 def test_pages_that_a_row_does_not_see(gpu, n, heads, kv_heads, d, page, what, value):
     """Earlier tokens of a causal call have nothing of a later one's scales; infinite ones give NaN to those that see them."""
     rng = np.random.default_rng(6)
@@ -173,7 +177,7 @@ def test_pages_that_a_row_does_not_see(gpu, n, heads, kv_heads, d, page, what, v
         check(gpu, c, q, kv_len, [n] * 3, heads, nan=nan)
 
 
-@pytest.mark.parametrize("n", [1, 3, 12])
+@pytest.mark.parametrize("n", [1, 3, 12, 70])
 @pytest.mark.parametrize("spread", [2, 6, 14])
 def test_scales_and_scores_over_orders_of_magnitude(gpu, n, spread):
     """Random scales of both sides, scores from flat to picking one key."""
