@@ -689,8 +689,8 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) vo
                 if (!all && first + t >= limit[r]) e = w[t] = 0.0f;
                 l[r] += e;
             }
-            // A scale that is no number shows in l: whole numbers cannot.
-            if (seen(r)) l[r] = fmaf(fv, 0.0f, l[r]);
+            // A scale that is infinite or no number shows in l: whole numbers and weights of 0 cannot.
+            if (seen(r)) l[r] = fmaf(fv + ks, 0.0f, l[r]);
             const uint32_t e = digits_exponent(row_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]))));
             const float up = __uint_as_float((284u - e) << 23);
             unit[r] = __uint_as_float((e - 30u) << 23);
@@ -1048,7 +1048,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attenti
     auto step = [&](uint32_t chunk, auto works, auto masks) {
         constexpr bool WORK = decltype(works)::value, MASK = decltype(masks)::value;
         int8_t *now = lds + ((chunk - begin) & 1) * kBuf, *next = lds + ((chunk - begin + 1) & 1) * kBuf;
-        const float k_scale = ks, v_scale = vs;
+        const float k_scale = fmaf(ks, 0.0f, ks), v_scale = vs;   // infinite as NaN: scores of minus infinity are none
         const bool more = chunk + 1 < end;
         if (more) {
             fetch(chunk + 1, next);

@@ -154,7 +154,7 @@ def test_quiet_pages_beside_loud_ones(gpu, n, heads, kv_heads, d, page, ratio):
     check(gpu, c, q, kv_len, [n, n], heads, scale=20.0 / d, causal=0)
 
 
-@pytest.mark.parametrize("what,value", [("vs", 1e6), ("vs", 1e30), ("vs", np.inf), ("vs", np.nan), ("ks", 1e20), ("ks", np.nan)])
+@pytest.mark.parametrize("what,value", [("vs", 1e6), ("vs", 1e30), ("vs", np.inf), ("vs", np.nan), ("ks", 1e20), ("ks", np.nan), ("ks", np.inf)])
 @pytest.mark.parametrize("n,heads,kv_heads,d,page", [(2, 4, 2, 64, 16), (7, 2, 1, 128, 16), (16, 1, 1, 80, 16), (8, 2, 2, 256, 16),
                                                      (70, 2, 1, 64, 16), (200, 1, 1, 128, 64), (70, 1, 1, 256, 16)])
 def test_pages_that_a_row_does_not_see(gpu, n, heads, kv_heads, d, page, what, value):
