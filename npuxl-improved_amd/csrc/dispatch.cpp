@@ -112,6 +112,19 @@ public:
         outs_.emplace_back(static_cast<void *>(p), d, bytes);
         return static_cast<T *>(d);
     }
+    // Two outputs with gaps.  Host ranges that meet are staged as one: of two
+    // copies back the later would put old contents over the other's results.
+    template <typename T>
+    std::pair<T *, T *> inout2(T *p, size_t bytes, T *q, size_t q_bytes)
+    {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+        const bool apart = a + bytes <= b || b + q_bytes <= a;
+        if (!p || !q || !bytes || !q_bytes || apart || is_device_pointer(p) || is_device_pointer(q))
+            return {inout(p, bytes), inout(q, q_bytes)};
+        const uintptr_t lo = std::min(a, b), hi = std::max(a + bytes, b + q_bytes);
+        char *d = inout(reinterpret_cast<char *>(lo), hi - lo);
+        return {reinterpret_cast<T *>(d + (a - lo)), reinterpret_cast<T *>(d + (b - lo))};
+    }
     void finish()
     {
         for (auto &o : outs_)
@@ -1071,6 +1084,11 @@ struct KvSource {
     {
         return stager ? stager->inout(p, count * sizeof(float)) : device(p, "kv tensor in host memory");
     }
+    std::pair<float *, float *> outs(float *p, uint64_t count, float *q, uint64_t q_count) const
+    {
+        if (stager) return stager->inout2(p, count * sizeof(float), q, q_count * sizeof(float));
+        return {p ? out(p, count) : nullptr, q ? out(q, q_count) : nullptr};
+    }
 };
 
 k::KvCall kv_call_params(vnpu_stream_t *s, const vnpu_kv_cache_t &c, const int32_t *lengths, const int32_t *seq_start,
@@ -1203,8 +1221,7 @@ k::KvRead kv_read_params(vnpu_stream_t *s, const vnpu_kv_read_f32_args_t &a, con
     p.k = kt.rows;
     p.v = vt.rows;
     require(k::kv_read_fits(p), "kv_read too large");
-    p.K = a.K ? src.out(a.K, kt.span) : nullptr;
-    p.V = a.V ? src.out(a.V, vt.span) : nullptr;
+    std::tie(p.K, p.V) = src.outs(a.K, kt.span, a.V, vt.span);
     return p;
 }
 
