@@ -190,3 +190,36 @@ def test_scales_and_scores_over_orders_of_magnitude(gpu, n, spread):
         q = (factor * rng.standard_normal((3 * n, 4, 64))).astype(np.float32)
         check(gpu, c, q, kv_len, [n] * 3, 4)
         check(gpu, c, q[:sum([n, n, 1])], kv_len, [n, n, 1], 4)
+
+
+@pytest.mark.parametrize("weight", [0.9, 0.99, 0.9945, 0.9999])
+@pytest.mark.parametrize("batch,n,kv_heads,d,kv_len", [
+    (16, 1, 8, 128, 131072),   # a workgroup a sequence and head
+    (1, 4, 8, 64, 131072),     # keys split over workgroups
+    (96, 64, 8, 64, 16384),    # tiles, whole
+    (2, 70, 1, 256, 30000)])   # tiles, keys split
+def test_weights_that_only_count_together(gpu, batch, n, kv_heads, d, kv_len, weight):
+    """Weights of less than half a step of the largest each, and together a part of the sum.  Only the heaviest key has
+    values, so that the result shows the sum of weights alone: relative error a rounding for each of 64 steps
+    (exponentials, products, the kept sums of lanes, waves and parts, the division) and the score's 8 roundings.  All sequences share
+    two pages, the second is used again and again."""
+    page = 256
+    k, v = np.zeros((2, kv_heads, page, d), np.int8), np.zeros((2, kv_heads, d, page), np.int8)
+    u = np.random.default_rng(5).choice([-1, 1], d)
+    k[0, :, 0], v[0, :, :, 0] = 100 * u, -50
+    table = np.ones((batch, -(-kv_len // page)), np.int32)
+    table[:, 0] = 0
+    scales, q = np.full((2, kv_heads), 2.0**-7, np.float32), np.broadcast_to(u, (batch * n, kv_heads, d)).astype(np.float32)
+    scale = np.float32(np.log(weight / (1 - weight) * kv_len) / (d * 100 * 2.0**-7))
+    bufs = [gpu.upload(x) for x in (k, v, scales, table, q, np.full(batch, kv_len, np.int32))]
+    cache = abi.KvCache(k=bufs[0].ptr, v=bufs[1].ptr, k_scales=bufs[2].ptr, v_scales=bufs[2].ptr, table=bufs[3].ptr, pages=2,
+                        page_size=page, kv_heads=kv_heads, head_dim=d, table_ld=table.shape[1])
+    out = gpu.alloc(q.nbytes)
+    gpu.run(abi.OP_KV_ATTENTION_I8, cache=cache, Q=bufs[4], O=out, kv_len=bufs[5], batch=batch, tokens=batch * n,
+            heads=kv_heads, scale=scale)
+    got = gpu.download(out, np.float32, q.shape)
+    score = float(scale) * d * 100 * 2.0**-7
+    want = -50 * 2.0**-7 / (1 + (kv_len - 1) * np.exp(-score))
+    off = float(np.abs(got / want - 1).max())
+    assert off <= EPS * (64 + 2 * 8 * score), off
+    kv.free(gpu, *bufs, out)
