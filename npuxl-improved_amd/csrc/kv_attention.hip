@@ -252,9 +252,9 @@ struct Query {
 // holds what was summed before, would pass 2^100.  The reference m is one that
 // scores may pass by kAhead, as for few rows.  (Scores of normal numbers: one chunk in
 // 40 moves something for one of a wave's 32 rows, 243 us for 4096 tokens against 237 with a
-// U that only grew; 8 times as far apart every chunk does, 267 against 228.  Within 2^-6
+// U that only grew; 8 times as far apart every chunk does, 280 against 228.  Within 2^-6
 // a fifth of the chunks did for ordinary scores: 259.)
-constexpr float kAhead = 4.0f, kMostShift = 114.0f;
+constexpr float kAhead = 4.0f, kMostShift = 114.0f, kFar = 12.0f, kJump = 8.0f;
 template <int DT>
 struct State {
     v4f o[DT];
@@ -1111,7 +1111,19 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attenti
                     const float need = groups_max(top[r] + power) - now;
                     // A row without keys or numbers keeps its unit.
                     float to = st[r].shift;
-                    if (need > 15.0f - to) to = 10.0f - ceilf(need);   // U up: 2^-4 U is the largest now
+                    // U up: 2^-4 U is the largest now, so that the next ones may be larger; 2 U where it
+                    // is far above what came before and above others of its chunk: their last bits count.
+                    const bool jump = need > 15.0f + kJump - to;
+                    bool far = false;
+                    if (__any(jump)) {
+                        float least = f[r][0][0];
+#pragma unroll
+                        for (int t = 0; t < 4; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) least = fminf(least, f[r][t][i]);
+                        far = jump && -groups_max(-fmaf(least, ck[r], power)) - now < need - kFar;
+                    }
+                    if (need > 15.0f - to) to = (far ? 15.0f : 10.0f) - ceilf(need);
                     const bool low = need < 2.0f - to;
                     if (__any(low)) {
                         float held = 0.0f;

@@ -48,7 +48,7 @@ def rows_of(c, b, h, kv_head, q, kv_len, causal, scale, last):
     return np.where(some[:, None], o, 0), bound
 
 
-def check(s, c, q, kv_len, n, heads, causal=1, scale=0.0, nan=None, in_rows=None, **more):
+def check(s, c, q, kv_len, n, heads, causal=1, scale=0.0, nan=None, last=None, **more):
     """Runs one call over uniform or ragged sequences and compares every row; returns the largest share of its bound."""
     D, G, batch = c.head_dim, c.kv_heads, len(n)
     used = scale if scale > 0 else float(np.float32(1.0) / np.sqrt(np.float32(D)))
@@ -64,7 +64,7 @@ def check(s, c, q, kv_len, n, heads, causal=1, scale=0.0, nan=None, in_rows=None
     kv.free(s, bufs, start, lens, x, y)
     # Four digits and four of the remainder for up to 16 rows of a kv head (8 above 128 dimensions).  Else two f16 parts in a
     # unit that the largest product is at most 2^12 below: half of 2^-24 of 2^14.
-    last = 2.0**-56 if not ragged and n[0] * heads // G <= (16 if D <= 128 else 8) else 2.0**-27
+    last = last or (2.0**-56 if not ragged and n[0] * heads // G <= (16 if D <= 128 else 8) else 2.0**-27)
     at, worst = 0, 0.0
     for b, m in enumerate(n):
         for h in range(heads):
@@ -133,6 +133,21 @@ def test_one_key_with_most_of_the_weight_of_a_long_sequence(gpu, silent, weight)
     if silent:
         c.v[c.table[:, 0], :, :, 0] = 0
     check(gpu, c, q, kv_len, [1] * 16, 8, scale=scale)
+
+
+@pytest.mark.parametrize("power", range(20, 33, 2))
+@pytest.mark.parametrize("n,heads,kv_heads,d", [(1, 2, 2, 128), (70, 2, 1, 64), (70, 1, 1, 128), (33, 1, 1, 256)])
+def test_the_chunk_of_a_key_without_values(gpu, n, heads, kv_heads, d, power):
+    """The first key has all but 2^-power of the weight and no values; the few others, all alike, round the same way.  In
+    tiles the unit has the largest product between 2^14 and 2^15 then: half of 2^-24 is 2^-39 of it."""
+    rng = np.random.default_rng(power)
+    kv_len = [64, 30, 200]
+    c = kv.Cache(rng, 3, kv_heads, d, 16, 13)
+    c.v[:] = np.maximum(np.abs(c.v), 1)
+    q, scale = lean(rng, c, [n] * 3, heads, 1 - 2.0**-power, PLACES["first"], kv_len, noise=0)
+    c.k[np.abs(c.k) != 100] = 0
+    c.v[c.table[:, 0], :, :, 0] = 0
+    check(gpu, c, q, kv_len, [n] * 3, heads, scale=scale, causal=0, last=2.0**-39 if n > 1 else None)
 
 
 @pytest.mark.parametrize("ratio", [1e2, 1e4, 1e6, 1e8, 1e20])
