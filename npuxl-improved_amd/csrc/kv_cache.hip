@@ -37,10 +37,11 @@ struct Rates {
 };
 
 // cos and sin of 2 pi t.  t less its nearest quarter leaves |x| <= pi / 4, where
-// the Taylor series to x^14 and x^13 are within 2e-14: the f32 results are the
-// correctly rounded ones but for about one in 10^6.  f64 because t is
-// exact to 2^-53 of itself only there: position 100000 in f32 would be off by
-// 0.006 rad.
+// the Taylor series to x^14 and x^13 are within 2e-14.  f64 because t is
+// exact to some 2^-52 of itself only there: position 100000 in f32 would be off by
+// 0.006 rad.  That error grows with the position: of the f32 results 1 in 10^5 is not the
+// correctly rounded one up to position 10000, 1 in 14000 at 100000, 1 in 2000 at 10^6
+// (theta 10000, 64 and 128 dimensions), all within half a step and 2^-10 of one to there.
 __device__ __forceinline__ void cos_sin_turns(double t, float &c, float &s)
 {
     const double quarter = rint(4.0 * t);
@@ -98,6 +99,10 @@ __device__ __forceinline__ uint32_t block_largest(uint32_t v, uint32_t *red)
     return r;
 }
 
+// A product with f32(1 / 127), not a division: that is what a division by a constant
+// becomes in torch on a GPU, so that a program there makes the same codes from the same
+// values.  It is within a step of largest / 127, which QUANTIZE_I8 takes: its scale of the same values
+// may differ in the last bit.
 struct PageScale {
     float scale, ratio, inv;
 };
