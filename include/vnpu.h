@@ -478,9 +478,10 @@ typedef struct vnpu_memset_args_t {
 /* A page holds page_size consecutive tokens of one sequence; row b of the   */
 /* table names the pages of sequence b in order, so token i of it is slot    */
 /* i % page_size of page table[b][i / page_size].  A cached value is its     */
-/* int8 code times the scale of its (page, kv head); keys and values have    */
-/* scales of their own.  V is stored with the tokens of a page side by side, */
-/* which is the operand order of the product with the softmax weights.       */
+/* int8 code times the scale of its (page, kv head), which is not negative;  */
+/* keys and values have scales of their own.  V is stored with the tokens of */
+/* a page side by side, which is the operand order of the product with the   */
+/* softmax weights.                                                          */
 /*                                                                           */
 /* The new (or read) tokens of a call are `tokens` rows.  With seq_start     */
 /* ([batch + 1], not decreasing) rows seq_start[b] .. seq_start[b + 1] - 1   */
@@ -529,7 +530,10 @@ typedef struct vnpu_kv_cache_t {
  * codes are round-half-away(x * (1 / scale)) in +-127.  A scale below 2^-126
  * is 0 (codes 0); an infinity or NaN among a page's new values makes its
  * scale NaN and leaves its codes.  A page that two sequences of one call
- * write to has unspecified contents afterwards. */
+ * write to has unspecified contents afterwards.  Rounding anew adds up to half a
+ * step each time: a page written at once is within half a step of its scale, one
+ * written token by token within 1 to 3 (root mean square 0.29 and 0.36 to 0.39
+ * steps for normal numbers, up to 1.0 where they grow by 2 % a token). */
 typedef struct vnpu_kv_append_i8_args_t {
     vnpu_kv_cache_t cache;
     const float *Q;             /* optional: queries to turn */
@@ -555,10 +559,15 @@ typedef struct vnpu_kv_append_i8_args_t {
  * head h / (heads / kv_heads).  Query i of the n of sequence b sees keys
  * j < kv_len[b] (kv_len counts the new tokens once they are appended) and,
  * causal, j <= kv_len[b] - n + i; one that sees none gives zeros.  Q may be
- * O, with the same strides.  Sums and softmax statistics are f32; queries
- * and weights enter the products with 22 bits or more (about 1e-7 of
- * the result).  A query row with an infinity or NaN, or one that sees a page
- * with such a scale, gives NaN.  Calls that split the keys of a sequence
+ * O, with the same strides.  Sums and softmax statistics are f32.  A query
+ * element enters the products to 2^-23 of the row's largest; a weight times its
+ * page's scale to 2^-22 of itself, and not beyond 2^-27 of the largest such
+ * product of the row among the same 64 keys (2^-39 where one key is far above all
+ * others; up to 16 rows, tokens times query heads, of a kv head: 2^-60): the
+ * error is some 1e-7 of the sum of weight * |value| that the row sees, whatever
+ * other pages hold.  A query row with an infinity or NaN, or one that sees a page
+ * with such a scale, gives NaN.  max_tokens and max_kv choose how the work is laid
+ * out, and with it the last digits.  Calls that split the keys of a sequence
  * over workgroups keep partial results in `workspace` (device memory of
  * vnpu_kv_attention_workspace bytes or more, 16-byte aligned, of no other
  * call that may run at the same time), or with NULL in the stream's own. */

@@ -20,7 +20,7 @@
 // chunk dealt to the tiles so that lane (group g, row) ends with keys 16g ..
 // 16g + 15 of its row: those are the operand of P . V as they stand, and their
 // V codes are 16 consecutive bytes of a page.  No value crosses a lane in the
-// loop but the row's maximum.
+// loop but where a row's maximum or unit moves.
 #include "device_math.hpp"
 #include "kv_common.hpp"
 #include "lds_dma.hpp"
@@ -330,9 +330,9 @@ __device__ __forceinline__ void weigh(float &sum, const v4f f[4], int half, floa
 //   q digits x K codes   lane (r = g, c): row r, key 4 c + t of tile t;
 //   p digits x V codes   lane (r = g, c): row r, dimension 16 t + c of tile t.
 // A weight w = p * v_scale / N, p = 2^(s - m) for a reference m that s may pass by
-// 4, N a power of two that no v_scale seen by the row passes, becomes the whole number rint(w *
-// 2^k), k such that the largest of the row's weights in these 64 keys has 31 bits:
-// a chunk's sums are whole numbers of their own unit, then added to f32 sums.  What
+// 4, N a power of two that no v_scale seen by the row passes, becomes the whole
+// number rint(w * 2^k), k such that the largest of the row's weights in these 64
+// keys has 31 bits: a chunk's sums are whole numbers of their own unit, then added to f32 sums.  What
 // the rounding left is four digits more, under 2^-31 of the unit, and goes through
 // the product again where it is more than 2^-22 of some weight: one key with nearly
 // all of the weight, or a page of large values, takes nothing from the others.
@@ -1273,7 +1273,8 @@ __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, con
 
 // Rows that the kernel of few rows takes: one workgroup's, or two's where all
 // sequences' keys together are few.  (20 rows of 8 heads of 128, 3001 keys:
-// 1 sequence 17 us against 21 in tiles, 4 of 700 to 3001 keys 23 and 23, 4 of 3001 keys 37 and 24.)
+// 1 sequence 17.4 us and 16.7 in tiles, heads of 64 14.3 and 14.7, 12 rows of 256 22.9 and
+// 24.0; 4 of 700 to 3001 keys 25.0 and 18.7, 4 of 3001 keys 42.1 and 20.3.)
 uint32_t few_rows(const KvAttn &p)
 {
     const uint32_t one = p.call.c.head_dim > 128 ? 8 : 16;
@@ -1311,10 +1312,12 @@ Plan plan_of(const KvAttn &p)
         r.split.min_per = 4;
         // A sequence and kv head as one workgroup: 9 us and 1.05 us for each 256
         // keys of the longest, or the codes at 6.4 TB/s; split: 12 us with the join
-        // and the codes (8 heads of 128, 4096 keys: 1 sequence 24.7 and 10.9 us, 16 sequences
-        // 28.4 and 30.6; 32 heads, 8 sequences 42.0 and 52.6; 8 heads, 16 sequences of 100 to
-        // 8000 keys 47.3 and 39.2).  Sequences are taken to be 0.8 of max_kv long, with
-        // seq_start 0.6.
+        // and the codes (8 heads of 128, 4096 keys: 1 sequence 27.9 and 11.1 us, 16 sequences
+        // 29.3 and 29.9; 32 heads, 8 sequences 43.0 and 54.8; 8 heads, 16 sequences of 100 to
+        // 8000 keys 51.2 and 38.8; 1 sequence of 768 keys 9.6 and 10.9, of 1024 11.1 and 11.0).
+        // Sequences are taken to be 0.8 of max_kv long, with seq_start 0.6.  It does not know
+        // that more rows and larger heads take longer for a chunk (16 sequences of 4096 keys,
+        // 16 rows on 8 heads of 128: 67 whole as it says, 56 split).
         const double mb = (c.seq_start ? 1.2e-6 : 1.6e-6) * c.batch * G * D * p.max_kv;
         r.split.whole = std::max(9.0 + 1.05 * ((p.max_kv + 255) / 256), mb / 6.4) <= 12.0 + mb / 6.4;
         r.split.low_rows = 0;
@@ -1339,14 +1342,14 @@ Plan plan_of(const KvAttn &p)
         const uint32_t chunks = (p.max_kv + kChunk - 1) / kChunk;
         // 128 rows share K and V of a chunk where the card has more of such tiles
         // than run at a time (32 heads of 128, causal: 4096 tokens of 8 kv heads
-        // 248 us against 273 with 64 rows, 2048 of 32 kv heads 96 and 87), or a few
+        // 248 us against 254 with 64 rows, 2048 of 32 kv heads 84 and 81), or a few
         // even ones with keys for 16 chunks a range (512 tokens of 4096, 8 kv heads: 76 us
-        // against 79; a ragged batch of 3 x 200 tokens 97 against 79).
+        // against 79; a ragged batch of 1 to 331 tokens, 4 kv heads of 80, 43 against 35).
         uint64_t grid = D <= 128 ? tiles_of(128) : 0;
         if (grid <= 2 * p.cus && (c.seq_start || grid >= p.cus || grid * (chunks / 16) < 2 * p.cus)) grid = tiles_of(64);
         // Key ranges of 4 chunks at least for a workgroup a CU, of 8 for as many as
-        // run at a time (32 tiles, 47 chunks: 8 ranges 24 us, 5 29 us; 64 chunks: 8
-        // ranges 30 us, 10 35 us).  Where sequences differ the shorter have fewer.
+        // run at a time (32 tiles, 47 chunks: 8 ranges 20.5 us, 5 24.2, 10 22.1; 64 chunks: 8
+        // ranges 23.7 us, 5 28.8, 10 26.2).  Where sequences differ the shorter have fewer.
         const uint64_t at_once = (D > 128 ? 1 : r.tile_rows == 128 ? 2 : 3) * p.cus;
         const uint64_t parts = std::max(std::min<uint64_t>(p.cus / grid, chunks / 4),
                                         std::min<uint64_t>(at_once * (c.seq_start ? 5 : 3) / (3 * grid), chunks / (c.seq_start ? 5 : 8)));
