@@ -887,7 +887,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv_attention_merge(KvAttn p, Spl
 // Bound by the vector instructions: 64 keys of 32 rows take a wave 112 matrix
 // instructions (16 cycles each) and about 490 others (4 cycles, exponentials 16):
 // three conversions and sums for a score's digits, ten for a weight and its two
-// halves.  Two waves a SIMD fill 73 % of its vector issue and 47 % of its matrix
+// halves.  Two waves a SIMD fill 70 % of its vector issue and 47 % of its matrix
 // cores.  A step has few branches, so that its products and exponentials
 // mix: with the rows one after another and conditions inside, 306 us instead of 256.
 // 4096 tokens on themselves, causal, 32 heads of 128: 243 us, 566 TFLOP/s (a
