@@ -192,15 +192,33 @@ typedef enum vnpu_opcode_t {
      * invalid commands. */
     VNPU_OP_KV_APPEND_I8    = 64,
     VNPU_OP_KV_ATTENTION_I8 = 65,
-    VNPU_OP_KV_READ_F32     = 66
+    VNPU_OP_KV_READ_F32     = 66,
+    /* MI355X extension (additive): 4-bit weights, positions with several axes
+     * and a prompt that a batch shares.  67 to 79 stay invalid commands. */
+    VNPU_OP_MATMUL_I4              = 80,
+    VNPU_OP_ROPE_AXES_F32          = 81,
+    VNPU_OP_KV_PREFIX_ATTENTION_I8 = 82
 } vnpu_opcode_t;
 
-/* MI355X extension: position rotation of VNPU_OP_KV_APPEND_I8. */
+/* MI355X extension: position rotation of VNPU_OP_KV_APPEND_I8 and
+ * VNPU_OP_ROPE_AXES_F32. */
 typedef enum vnpu_rotation_t {
     VNPU_ROTATE_NONE        = 0,
     VNPU_ROTATE_HALF        = 1,   /* pairs (j, j + rope_dim / 2), as ROPE_F32 */
     VNPU_ROTATE_INTERLEAVED = 2    /* pairs (2j, 2j + 1) */
 } vnpu_rotation_t;
+
+/* MI355X extension: how VNPU_OP_ROPE_AXES_F32 deals pairs to axes. */
+typedef enum vnpu_axes_order_t {
+    VNPU_AXES_BLOCKS = 0,   /* the first sections[0] pairs are axis 0's, the next sections[1] axis 1's, ... */
+    VNPU_AXES_TURNS  = 1    /* pair by pair in turn; an axis that has all its pairs is passed over */
+} vnpu_axes_order_t;
+
+/* MI355X extension: the frequencies of VNPU_OP_ROPE_AXES_F32. */
+typedef enum vnpu_axes_ladders_t {
+    VNPU_AXES_ONE_LADDER  = 0,   /* pair j: theta_base^(-j / pairs), whichever axis it is */
+    VNPU_AXES_OWN_LADDERS = 1    /* the i-th pair of axis a: theta_base^(-i / sections[a]) */
+} vnpu_axes_ladders_t;
 
 /* reference include/vnpu.h:186-197 */
 typedef struct vnpu_config_t {
@@ -285,6 +303,7 @@ typedef struct vnpu_stream vnpu_stream_t;
 typedef struct vnpu_event vnpu_event_t;
 typedef struct vnpu_buffer vnpu_buffer_t;
 typedef struct vnpu_packed_weights vnpu_packed_weights_t;
+typedef struct vnpu_packed_weights_i4 vnpu_packed_weights_i4_t;   /* MI355X extension */
 typedef struct vnpu_cluster vnpu_cluster_t;
 typedef struct vnpu_remote_node vnpu_remote_node_t;
 typedef struct vnpu_weight_handle vnpu_weight_handle_t;
@@ -604,6 +623,90 @@ typedef struct vnpu_kv_read_f32_args_t {
     uint32_t v_batch_stride, v_token_stride, v_head_stride;
 } vnpu_kv_read_f32_args_t;
 
+/* MI355X extension (additive): products with 4-bit weights.
+ * C[m][n] = epi(sum over k of A[m][k] * w[k][n] + bias[n]), w[k][n] = (code -
+ * zero[k / group_size][n]) * scale[k / group_size][n] as packed.  Differences code
+ * - zero are whole numbers and enter exactly; an element of A enters to 2^-29 of
+ * the largest of its row among the same 128 of K (up to 16 rows) or to 2^-22 of
+ * itself (2^-38 of the largest of its row where that is more); sums
+ * are f32 or wider, each group's scaled once.  A row of A with an infinity or NaN
+ * gives NaN in all of its results.  SILU, GELU_TANH and GELU_ERF are the
+ * functions themselves to some 2^-21 of the result (not the polynomials of the int8
+ * and f32 products). `workspace`: as in vnpu_kv_attention_i8_args_t, its bytes
+ * from vnpu_matmul_i4_workspace. */
+typedef struct vnpu_matmul_i4_args_t {
+    const float *A;             /* MxK, lda */
+    vnpu_packed_weights_i4_t *B;   /* from vnpu_pack_weights_i4 */
+    const float *bias;          /* optional [N] */
+    float *C;                   /* MxN, ldc; no part of A, bias or the weights */
+    void *workspace;            /* optional */
+    uint64_t workspace_bytes;
+    uint32_t M;
+    uint32_t K;
+    uint32_t N;
+    uint32_t lda;               /* 0 = dense */
+    uint32_t ldc;
+    uint32_t epilogue;          /* vnpu_epilogue_t */
+    uint32_t unit;
+    uint32_t reserved0;
+} vnpu_matmul_i4_args_t;
+
+/* MI355X extension (additive): rotary positions with up to four axes (time,
+ * height and width of images and video).  Of a head's head_dim elements
+ * the first 2 * pairs, pairs = sections[0] + .. + sections[axes - 1], are pairs
+ * as `rotation` says (HALF: (j, j + pairs)); pair j of token t, of axis a, is turned
+ * by positions[a * position_ld + t] * scaling * its frequency: (x, y) -> (x cos - y
+ * sin, x sin + y cos), angles, cosines and products in 64 bits, each result
+ * rounded once.  Elements behind are copied.  Token t of `tokens` is token t %
+ * (tokens / batch) of sequence t / (tokens / batch), with strides and their
+ * defaults as in the KV commands without seq_start.  Q_out may be Q and K_out K,
+ * with the same strides (in place); outputs overlap nothing else.  Positions may be
+ * negative: those of opposite sign turn back, which is the gradient too.  Positions,
+ * Q and K may be host memory, staged as everywhere. */
+typedef struct vnpu_rope_axes_f32_args_t {
+    const float *Q;             /* optional, with Q_out */
+    float *Q_out;
+    const float *K;             /* optional, with K_out */
+    float *K_out;
+    const int32_t *positions;   /* [axes][position_ld] */
+    uint32_t batch;             /* 0 = 1 */
+    uint32_t tokens;            /* of all sequences */
+    uint32_t heads;             /* of Q */
+    uint32_t kv_heads;          /* of K */
+    uint32_t head_dim;          /* even, up to 256 */
+    uint32_t position_ld;       /* 0 = tokens */
+    uint32_t q_batch_stride, q_token_stride, q_head_stride;
+    uint32_t o_batch_stride, o_token_stride, o_head_stride;      /* of Q_out */
+    uint32_t k_batch_stride, k_token_stride, k_head_stride;
+    uint32_t ko_batch_stride, ko_token_stride, ko_head_stride;   /* of K_out */
+    uint32_t axes;              /* 1 to 4 */
+    uint32_t sections[4];       /* pairs of each axis, none 0 */
+    uint32_t order;             /* vnpu_axes_order_t */
+    uint32_t ladders;           /* vnpu_axes_ladders_t */
+    uint32_t rotation;          /* VNPU_ROTATE_HALF or VNPU_ROTATE_INTERLEAVED */
+    float theta_base;           /* <= 0 means 10000 */
+    float scaling;              /* <= 0 means 1 */
+} vnpu_rope_axes_f32_args_t;
+
+/* MI355X extension (additive): KV_ATTENTION_I8 of a batch whose sequences all begin
+ * with the same prefix_len cached tokens, which are read once for all of them.
+ * Token j < prefix_len of every sequence is in the pages of prefix_table, the
+ * others are in the sequence's row of attention.cache.table as always; entries of
+ * that row below prefix_len / page_size are not read.  prefix_len is a whole
+ * number of pages; 0 makes it KV_ATTENTION_I8 (prefix_table may be NULL).  kv_len
+ * and max_kv count the prefix.  A sequence with new tokens has kv_len >=
+ * prefix_len, causal ones kv_len - new tokens >= prefix_len (no new token lies in
+ * the prefix); others fail the stream at its next sync.  kv_len of a sequence
+ * without new tokens is not looked at.  Arguments, results and precision are those
+ * of KV_ATTENTION_I8, up to the order of f32 sums; the workspace is of
+ * vnpu_kv_prefix_attention_workspace bytes. */
+typedef struct vnpu_kv_prefix_attention_i8_args_t {
+    vnpu_kv_attention_i8_args_t attention;
+    const int32_t *prefix_table;   /* [prefix_len / page_size] */
+    uint32_t prefix_len;
+    uint32_t reserved0;
+} vnpu_kv_prefix_attention_i8_args_t;
+
 /* The fixed 208-byte command packet: reference include/vnpu.h:447-468. */
 typedef struct vnpu_command_t {
     uint32_t opcode;
@@ -627,6 +730,9 @@ typedef struct vnpu_command_t {
         vnpu_kv_append_i8_args_t kv_append;
         vnpu_kv_attention_i8_args_t kv_attention;
         vnpu_kv_read_f32_args_t kv_read;
+        vnpu_matmul_i4_args_t matmul_i4;
+        vnpu_rope_axes_f32_args_t rope_axes;
+        vnpu_kv_prefix_attention_i8_args_t kv_prefix_attention;
         uint8_t raw[192];
     } args;
 } vnpu_command_t;
@@ -957,10 +1063,53 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_kv_read_f32(vnpu_stream_t *stream,
 VNPU_API uint64_t VNPU_CALL vnpu_kv_attention_workspace(const vnpu_device_t *device,
                                                         const vnpu_kv_attention_i8_args_t *args);
 
-/* MI355X extension (additive): enqueues KV_* commands (no others) and does
+/* MI355X extension (additive): 4-bit weights to device memory in the layout of
+ * MATMUL_I4's kernels.  B: codes 0 to 15, two a byte, the lower half first; as
+ * [K][ldb] bytes (row k holds its N codes) or, trans_b, [N][ldb] (row n holds its K
+ * codes); ldb counts bytes, 0 = the row's codes / 2 rounded up.  scales [groups][N]
+ * f32; zeros [groups][N] uint8 of 0 to 15, NULL = all 8; groups = ceil(K /
+ * group_size).  group_size is 32, 64, a multiple of 128, or 0 for one group a column.
+ * Host or device memory.  Synchronous.  A zero above 15 is
+ * VNPU_ERR_INVALID_ARGUMENT. */
+VNPU_API vnpu_status_t VNPU_CALL vnpu_pack_weights_i4(vnpu_device_t *device,
+                                                      const uint8_t *B,
+                                                      const float *scales,
+                                                      const uint8_t *zeros,
+                                                      uint32_t K,
+                                                      uint32_t N,
+                                                      uint32_t group_size,
+                                                      uint32_t ldb,
+                                                      uint32_t trans_b,
+                                                      vnpu_packed_weights_i4_t **out_weights);
+VNPU_API void VNPU_CALL vnpu_packed_weights_i4_destroy(vnpu_packed_weights_i4_t *weights);
+/* group_size as given (K where that was 0); bytes of device memory. */
+VNPU_API vnpu_status_t VNPU_CALL vnpu_packed_weights_i4_info(const vnpu_packed_weights_i4_t *weights,
+                                                             uint32_t *K,
+                                                             uint32_t *N,
+                                                             uint32_t *group_size,
+                                                             uint64_t *bytes);
+
+/* MI355X extension (additive): submit one command + sync, as the wrappers above. */
+VNPU_API vnpu_status_t VNPU_CALL vnpu_matmul_i4(vnpu_stream_t *stream,
+                                                const vnpu_matmul_i4_args_t *args);
+VNPU_API vnpu_status_t VNPU_CALL vnpu_rope_axes_f32(vnpu_stream_t *stream,
+                                                    const vnpu_rope_axes_f32_args_t *args);
+VNPU_API vnpu_status_t VNPU_CALL vnpu_kv_prefix_attention_i8(vnpu_stream_t *stream,
+                                                             const vnpu_kv_prefix_attention_i8_args_t *args);
+
+/* MI355X extension (additive): bytes of workspace that such a call needs on this
+ * device (0: none, or a call that is refused), from its sizes, strides and which
+ * pointers are given. */
+VNPU_API uint64_t VNPU_CALL vnpu_matmul_i4_workspace(const vnpu_device_t *device,
+                                                     const vnpu_matmul_i4_args_t *args);
+VNPU_API uint64_t VNPU_CALL vnpu_kv_prefix_attention_workspace(const vnpu_device_t *device,
+                                                               const vnpu_kv_prefix_attention_i8_args_t *args);
+
+/* MI355X extension (additive): enqueues KV_*, MATMUL_I4 and ROPE_AXES_F32 commands
+ * (no others) and does
  * nothing else: no allocation, no event, no synchronization, so a caller may
  * capture it into a HIP graph of the stream.  Every pointer must be device
- * memory, and a KV_ATTENTION_I8 that needs a workspace must be given one; each
+ * memory, and a command that needs a workspace must be given one; each
  * captured graph that may run beside another needs one of its own.  Returns
  * VNPU_ERR_INVALID_ARGUMENT with nothing enqueued where a command is refused. */
 VNPU_API vnpu_status_t VNPU_CALL vnpu_kv_enqueue_noalloc(vnpu_stream_t *stream,
@@ -1006,6 +1155,9 @@ VNPU_STATIC_ASSERT(sizeof(vnpu_kv_cache_t) == 64, "kv cache");
 VNPU_STATIC_ASSERT(sizeof(vnpu_kv_append_i8_args_t) == 192, "kv append args");
 VNPU_STATIC_ASSERT(sizeof(vnpu_kv_attention_i8_args_t) == 168, "kv attention args");
 VNPU_STATIC_ASSERT(sizeof(vnpu_kv_read_f32_args_t) == 128, "kv read args");
+VNPU_STATIC_ASSERT(sizeof(vnpu_matmul_i4_args_t) == 80, "matmul_i4 args");
+VNPU_STATIC_ASSERT(sizeof(vnpu_rope_axes_f32_args_t) == 152, "rope_axes args");
+VNPU_STATIC_ASSERT(sizeof(vnpu_kv_prefix_attention_i8_args_t) == 184, "kv prefix attention args");
 #endif
 
 #endif /* VNPU_H */

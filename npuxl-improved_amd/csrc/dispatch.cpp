@@ -1200,13 +1200,29 @@ k::KvAttn kv_attention_params(vnpu_stream_t *s, const vnpu_kv_attention_i8_args_
     return p;
 }
 
-// The workspace that the caller gave; null: none given.
-void *kv_given_workspace(const vnpu_kv_attention_i8_args_t &a, size_t need)
+// KV_PREFIX_ATTENTION_I8 with a prefix: the call over what lies behind it, and the prefix's table.
+k::KvAttn kv_prefix_params(vnpu_stream_t *s, const vnpu_kv_prefix_attention_i8_args_t &a, const KvSource &src,
+                           const int32_t *&prefix_table)
 {
-    if (!a.workspace || !need) return nullptr;
-    require(a.workspace_bytes >= need && !(reinterpret_cast<uintptr_t>(a.workspace) & 15) && is_device_pointer(a.workspace),
-            "kv workspace too small, unaligned or in host memory");
-    return a.workspace;
+    const uint32_t ps = a.attention.cache.page_size;
+    require(a.prefix_table && ps && a.prefix_len % ps == 0, "a kv prefix is whole pages of a table");
+    k::KvAttn p = kv_attention_params(s, a.attention, src);
+    require(a.prefix_len <= p.max_kv, "a kv prefix is longer than max_kv or the table");
+    p.call.skip = a.prefix_len;
+    p.max_kv = std::max(1u, p.max_kv - a.prefix_len);
+    p.partial = 1;
+    prefix_table = src.in(a.prefix_table, a.prefix_len / ps);
+    require(k::kv_prefix_attention_fits(p, prefix_table), "kv_prefix_attention too large");
+    return p;
+}
+
+// The workspace that the caller gave; null: none given.
+void *given_workspace(void *ws, uint64_t bytes, size_t need)
+{
+    if (!ws || !need) return nullptr;
+    require(bytes >= need && !(reinterpret_cast<uintptr_t>(ws) & 15) && is_device_pointer(ws),
+            "workspace too small, unaligned or in host memory");
+    return ws;
 }
 
 k::KvRead kv_read_params(vnpu_stream_t *s, const vnpu_kv_read_f32_args_t &a, const KvSource &src)
@@ -1262,7 +1278,7 @@ void exec_kv(vnpu_stream_t *s, const vnpu_command_t &cmd, ExecStats &st)
         const auto &a = cmd.args.kv_attention;
         const k::KvAttn p = kv_attention_params(s, a, {&sg});
         const size_t need = k::kv_attention_ws_bytes(p);
-        void *ws = kv_given_workspace(a, need);
+        void *ws = given_workspace(a.workspace, a.workspace_bytes, need);
         if (!ws) ws = s->ensure_workspace(need);
         k::kv_attention(s->hip, p, ws);
         max_kv = p.max_kv;
@@ -1272,6 +1288,173 @@ void exec_kv(vnpu_stream_t *s, const vnpu_command_t &cmd, ExecStats &st)
     VNPU_HIP(hipGetLastError());
     sg.finish();
     account_kv(cmd, max_kv, st);
+}
+
+// ---------------------------------------------------------------------------
+// 4-bit weights and positions with several axes (no reference counterpart),
+// checked and staged as the KV commands are.
+// ---------------------------------------------------------------------------
+
+k::I4Gemm matmul_i4_params(vnpu_stream_t *s, const vnpu_matmul_i4_args_t &a, const KvSource &src)
+{
+    const vnpu_packed_weights_i4_t *w = a.B;
+    require(a.A && w && a.C && a.M && a.K && a.N, "invalid matmul_i4 arguments");
+    require(a.epilogue <= VNPU_EPILOGUE_GELU_ERF, "invalid matmul_i4 epilogue");
+    k::I4Gemm p;
+    p.M = a.M; p.N = a.N; p.K = a.K;
+    p.lda = a.lda ? a.lda : a.K;
+    p.ldc = a.ldc ? a.ldc : a.N;
+    require(p.lda >= a.K && p.ldc >= a.N, "invalid matmul_i4 leading dimensions");
+    p.KB = cdiv(a.K, 128u);
+    p.Np = cdiv(a.N, 16u) * 16;
+    p.epilogue = a.epilogue;
+    p.cus = s->device ? std::max(1u, s->device->cu_count) : 256;
+    require(a.K <= (1u << 30) && a.N <= (1u << 30) && k::matmul_i4_fits(p), "matmul_i4 too large");
+    if (src.sizes_only) {
+        p.A = a.A;
+        return p;
+    }
+    require(w->K == a.K && w->N == a.N, "packed weight shape mismatch");
+    require(w->device->hip_device == s->device->hip_device, "packed weights live on another device");
+    p.codes = w->codes;
+    p.scales = w->scales;
+    p.zeros = w->zeros;
+    p.slots = w->slots;
+    p.groups_of_block = w->groups_of_block;
+    p.blocks_of_group = w->blocks_of_group;
+    p.A = src.in(a.A, static_cast<uint64_t>(a.M - 1) * p.lda + a.K);
+    p.bias = src.in(a.bias, a.N);
+    p.C = src.out(a.C, static_cast<uint64_t>(a.M - 1) * p.ldc + a.N);
+    return p;
+}
+
+k::RopeAxes rope_axes_params(const vnpu_rope_axes_f32_args_t &a, const KvSource &src)
+{
+    require((a.Q || a.K) && !a.Q == !a.Q_out && !a.K == !a.K_out && a.positions, "invalid rope_axes arguments");
+    require(a.rotation == VNPU_ROTATE_HALF || a.rotation == VNPU_ROTATE_INTERLEAVED, "invalid rope_axes rotation");
+    require(a.order <= VNPU_AXES_TURNS && a.ladders <= VNPU_AXES_OWN_LADDERS, "invalid rope_axes order or ladders");
+    require(a.head_dim && a.head_dim <= 256 && a.head_dim % 2 == 0, "rope_axes head_dim is even, up to 256");
+    require(a.axes >= 1 && a.axes <= 4, "rope_axes has 1 to 4 axes");
+    k::RopeAxes p;
+    p.batch = a.batch ? a.batch : 1;
+    p.tokens = a.tokens;
+    p.head_dim = a.head_dim;
+    require(a.tokens && a.tokens <= (1u << 28) && a.tokens % p.batch == 0, "rope_axes tokens is a multiple of batch");
+    p.position_ld = a.position_ld ? a.position_ld : a.tokens;
+    require(p.position_ld >= a.tokens, "invalid rope_axes position_ld");
+    for (uint32_t i = 0; i < a.axes; ++i) {
+        require(a.sections[i] && a.sections[i] <= 128, "rope_axes sections are not 0");
+        p.pairs += a.sections[i];
+    }
+    require(2 * p.pairs <= a.head_dim, "rope_axes sections are more than a head");
+    p.half = a.rotation == VNPU_ROTATE_HALF;
+    const double theta = a.theta_base > 0.0f ? a.theta_base : 10000.0, scaling = a.scaling > 0.0f ? a.scaling : 1.0;
+    uint32_t used[4] = {}, axis = 0;
+    for (uint32_t j = 0; j < p.pairs; ++j) {
+        while (used[axis] == a.sections[axis]) axis = (axis + 1) % a.axes;
+        const double power = a.ladders == VNPU_AXES_OWN_LADDERS ? static_cast<double>(used[axis]) / a.sections[axis]
+                                                                : static_cast<double>(j) / p.pairs;
+        p.axis[j] = static_cast<uint8_t>(axis);
+        p.turns[j] = scaling * std::pow(theta, -power) / 6.283185307179586476925;
+        ++used[axis];
+        if (a.order == VNPU_AXES_TURNS) axis = (axis + 1) % a.axes;
+    }
+    auto side = [&](const float *in, float *out, uint32_t heads, const uint32_t from[3], const uint32_t to[3], k::KvRows &in_rows,
+                    k::KvRows &out_rows) -> std::pair<uint64_t, uint64_t> {
+        if (!in) return {0, 0};
+        require(heads && heads <= 65535, "invalid rope_axes heads");
+        const KvTensor i = kv_rows(from[0], from[1], from[2], heads, a.head_dim, p.batch, a.tokens, false, false);
+        const KvTensor o = kv_rows(to[0], to[1], to[2], heads, a.head_dim, p.batch, a.tokens, false, true);
+        require(out != in || (i.rows.batch == o.rows.batch && i.rows.token == o.rows.token && i.rows.head == o.rows.head),
+                "rope_axes turns in place with the same strides only");
+        in_rows = i.rows;
+        out_rows = o.rows;
+        return {i.span, o.span};
+    };
+    const uint32_t qs[3] = {a.q_batch_stride, a.q_token_stride, a.q_head_stride}, os[3] = {a.o_batch_stride, a.o_token_stride, a.o_head_stride};
+    const uint32_t ks[3] = {a.k_batch_stride, a.k_token_stride, a.k_head_stride}, kos[3] = {a.ko_batch_stride, a.ko_token_stride, a.ko_head_stride};
+    const auto q_span = side(a.Q, a.Q_out, a.heads, qs, os, p.q, p.qo), k_span = side(a.K, a.K_out, a.kv_heads, ks, kos, p.k, p.ko);
+    p.heads = a.Q ? a.heads : 0;
+    p.kv_heads = a.K ? a.kv_heads : 0;
+    require(k::rope_axes_fits(p), "rope_axes too large");
+    p.positions = src.in(a.positions, static_cast<uint64_t>(a.axes - 1) * p.position_ld + a.tokens);
+    std::tie(p.Q_out, p.K_out) = src.outs(a.Q_out, q_span.second, a.K_out, k_span.second);
+    p.Q = a.Q == a.Q_out ? p.Q_out : src.in(a.Q, q_span.first);
+    p.K = a.K == a.K_out ? p.K_out : src.in(a.K, k_span.first);
+    return p;
+}
+
+// As account_kv; the prefix is read once.
+void account_kv_prefix(const vnpu_kv_prefix_attention_i8_args_t &a, uint64_t max_own, ExecStats &st)
+{
+    const auto &t = a.attention;
+    const uint64_t qn = static_cast<uint64_t>(t.tokens) * t.heads * t.cache.head_dim;
+    st.bytes_read += qn * 4 + 2ull * (a.prefix_len + t.batch * max_own) * t.cache.kv_heads * t.cache.head_dim;
+    st.bytes_written += qn * 4;
+    st.flops += 4 * qn * (a.prefix_len + max_own);
+}
+
+void account_serving(const vnpu_command_t &cmd, ExecStats &st)
+{
+    if (cmd.opcode == VNPU_OP_MATMUL_I4) {
+        const auto &a = cmd.args.matmul_i4;
+        const uint64_t mk = static_cast<uint64_t>(a.M) * a.K, mn = static_cast<uint64_t>(a.M) * a.N;
+        st.bytes_read += 4 * mk + a.B->bytes + (a.bias ? 4ull * a.N : 0);
+        st.bytes_written += 4 * mn;
+        st.flops += 2 * mk * a.N;
+    } else if (cmd.opcode == VNPU_OP_ROPE_AXES_F32) {
+        const auto &a = cmd.args.rope_axes;
+        const uint64_t turned = static_cast<uint64_t>(a.tokens) * ((a.Q ? a.heads : 0) + (a.K ? a.kv_heads : 0)) * a.head_dim;
+        st.bytes_read += 4 * turned + 4ull * a.axes * a.tokens;
+        st.bytes_written += 4 * turned;
+        st.flops += 3 * turned;
+    }
+}
+
+void exec_matmul_i4(vnpu_stream_t *s, const vnpu_command_t &cmd, uint32_t flags, ExecStats &st)
+{
+    const auto &a = cmd.args.matmul_i4;
+    Stager sg(s->hip, s);
+    const k::I4Gemm p = matmul_i4_params(s, a, {&sg});
+    const size_t need = k::matmul_i4_ws_bytes(p);
+    void *ws = given_workspace(a.workspace, a.workspace_bytes, need);
+    if (!ws) ws = s->ensure_workspace(need);
+    st.unit = choose_unit(a.unit, false, flags);
+    k::matmul_i4(s->hip, p, ws);
+    VNPU_HIP(hipGetLastError());
+    sg.finish();
+    account_serving(cmd, st);
+}
+
+void exec_kv_prefix(vnpu_stream_t *s, const vnpu_command_t &cmd, ExecStats &st)
+{
+    const auto &a = cmd.args.kv_prefix_attention;
+    vnpu_command_t plain{};   // what it is without a prefix
+    plain.opcode = VNPU_OP_KV_ATTENTION_I8;
+    plain.args.kv_attention = a.attention;
+    if (!a.prefix_len) {
+        exec_kv(s, plain, st);
+        return;
+    }
+    Stager sg(s->hip, s);
+    const int32_t *table = nullptr;
+    const k::KvAttn p = kv_prefix_params(s, a, {&sg}, table);
+    const size_t need = k::kv_prefix_attention_ws_bytes(p, table);
+    void *ws = given_workspace(a.attention.workspace, a.attention.workspace_bytes, need);
+    if (!ws) ws = s->ensure_workspace(need);
+    k::kv_prefix_attention(s->hip, p, table, ws);
+    VNPU_HIP(hipGetLastError());
+    sg.finish();
+    account_kv_prefix(a, p.max_kv, st);
+}
+
+void exec_rope_axes(vnpu_stream_t *s, const vnpu_command_t &cmd, ExecStats &st)
+{
+    Stager sg(s->hip, s);
+    k::rope_axes(s->hip, rope_axes_params(cmd.args.rope_axes, {&sg}));
+    VNPU_HIP(hipGetLastError());
+    sg.finish();
+    account_serving(cmd, st);
 }
 
 void exec_copy(vnpu_stream_t *s, const vnpu_copy_args_t &a, ExecStats &st)
@@ -1341,12 +1524,67 @@ uint64_t kv_attention_workspace(const vnpu_device_t *dev, const vnpu_kv_attentio
     return k::kv_attention_ws_bytes(kv_attention_params(&on, a, {nullptr, true}));
 }
 
+uint64_t kv_prefix_attention_workspace(const vnpu_device_t *dev, const vnpu_kv_prefix_attention_i8_args_t &a)
+{
+    if (!a.prefix_len) return kv_attention_workspace(dev, a.attention);
+    vnpu_stream_t on;   // carries the device only
+    on.device = const_cast<vnpu_device_t *>(dev);
+    const int32_t *table = nullptr;
+    const k::KvAttn p = kv_prefix_params(&on, a, {nullptr, true}, table);
+    return k::kv_prefix_attention_ws_bytes(p, table);
+}
+
+uint64_t matmul_i4_workspace(const vnpu_device_t *dev, const vnpu_matmul_i4_args_t &a)
+{
+    vnpu_stream_t on;   // carries the device only
+    on.device = const_cast<vnpu_device_t *>(dev);
+    return k::matmul_i4_ws_bytes(matmul_i4_params(&on, a, {nullptr, true}));
+}
+
 void enqueue_kv_noalloc(vnpu_stream_t *s, const vnpu_command_t *commands, uint64_t count, ExecStats &st)
 {
     for (int pass = 0; pass < 2; ++pass)   // all are checked before one is enqueued
         for (uint64_t i = 0; i < count; ++i) {
-            const vnpu_command_t &cmd = commands[i];
-            require(is_kv_opcode(cmd.opcode), "only KV commands run without allocation");
+            vnpu_command_t cmd = commands[i];
+            if (cmd.opcode == VNPU_OP_KV_PREFIX_ATTENTION_I8 && !cmd.args.kv_prefix_attention.prefix_len) {
+                const vnpu_kv_attention_i8_args_t plain = cmd.args.kv_prefix_attention.attention;
+                cmd.opcode = VNPU_OP_KV_ATTENTION_I8;
+                cmd.args.kv_attention = plain;
+            }
+            require(is_kv_opcode(cmd.opcode) || is_serving_opcode(cmd.opcode), "this command does not run without allocation");
+            if (cmd.opcode == VNPU_OP_MATMUL_I4) {
+                const auto &a = cmd.args.matmul_i4;
+                const k::I4Gemm p = matmul_i4_params(s, a, {});
+                const size_t need = k::matmul_i4_ws_bytes(p);
+                void *ws = given_workspace(a.workspace, a.workspace_bytes, need);
+                require(ws || !need, "this matmul_i4 needs a workspace");
+                if (!pass) continue;
+                k::matmul_i4(s->hip, p, ws);
+                VNPU_HIP(hipGetLastError());
+                account_serving(cmd, st);
+                continue;
+            }
+            if (cmd.opcode == VNPU_OP_ROPE_AXES_F32) {
+                const k::RopeAxes p = rope_axes_params(cmd.args.rope_axes, {});
+                if (!pass) continue;
+                k::rope_axes(s->hip, p);
+                VNPU_HIP(hipGetLastError());
+                account_serving(cmd, st);
+                continue;
+            }
+            if (cmd.opcode == VNPU_OP_KV_PREFIX_ATTENTION_I8) {
+                const auto &a = cmd.args.kv_prefix_attention;
+                const int32_t *table = nullptr;
+                const k::KvAttn p = kv_prefix_params(s, a, {}, table);
+                const size_t need = k::kv_prefix_attention_ws_bytes(p, table);
+                void *ws = given_workspace(a.attention.workspace, a.attention.workspace_bytes, need);
+                require(ws, "this kv_prefix_attention needs a workspace");
+                if (!pass) continue;
+                k::kv_prefix_attention(s->hip, p, table, ws);
+                VNPU_HIP(hipGetLastError());
+                account_kv_prefix(a, p.max_kv, st);
+                continue;
+            }
             uint64_t max_kv = 0;
             if (cmd.opcode == VNPU_OP_KV_APPEND_I8) {
                 const k::KvAppend p = kv_append_params(s, cmd.args.kv_append, {});
@@ -1354,7 +1592,7 @@ void enqueue_kv_noalloc(vnpu_stream_t *s, const vnpu_command_t *commands, uint64
             } else if (cmd.opcode == VNPU_OP_KV_ATTENTION_I8) {
                 const k::KvAttn p = kv_attention_params(s, cmd.args.kv_attention, {});
                 const size_t need = k::kv_attention_ws_bytes(p);
-                void *ws = kv_given_workspace(cmd.args.kv_attention, need);
+                void *ws = given_workspace(cmd.args.kv_attention.workspace, cmd.args.kv_attention.workspace_bytes, need);
                 require(ws || !need, "this kv_attention needs a workspace");
                 if (pass) k::kv_attention(s->hip, p, ws);
                 max_kv = p.max_kv;
@@ -1444,6 +1682,15 @@ void execute_command(vnpu_device_t *dev, vnpu_stream_t *s, const vnpu_command_t 
     case VNPU_OP_KV_ATTENTION_I8:
     case VNPU_OP_KV_READ_F32:
         exec_kv(s, cmd, st);
+        return;
+    case VNPU_OP_MATMUL_I4:
+        exec_matmul_i4(s, cmd, flags, st);
+        return;
+    case VNPU_OP_ROPE_AXES_F32:
+        exec_rope_axes(s, cmd, st);
+        return;
+    case VNPU_OP_KV_PREFIX_ATTENTION_I8:
+        exec_kv_prefix(s, cmd, st);
         return;
     default:
         throw ArgError("invalid opcode");
@@ -1539,6 +1786,67 @@ void destroy_packed(vnpu_packed_weights_t *w)
     delete w;
 }
 
+// Null: a zero above 15.
+vnpu_packed_weights_i4_t *pack_weights_i4(vnpu_device_t *dev, const uint8_t *B, const float *scales, const uint8_t *zeros,
+                                          uint32_t K, uint32_t N, uint32_t group, uint32_t ldb, uint32_t trans_b)
+{
+    VNPU_HIP(hipSetDevice(dev->hip_device));
+    std::unique_ptr<vnpu_packed_weights_i4_t, void (*)(vnpu_packed_weights_i4_t *)> w(
+        new vnpu_packed_weights_i4_t(), destroy_packed_i4);
+    w->device = dev;
+    w->K = K;
+    w->N = N;
+    w->group = group ? group : K;
+    w->KB = cdiv(K, 128u);
+    w->Np = cdiv(N, 16u) * 16;
+    const uint32_t groups = group ? cdiv(K, group) : 1;
+    if (group == 32 || group == 64) w->groups_of_block = 128 / group;
+    else w->blocks_of_group = group ? group / 128 : w->KB;
+    w->slots = w->groups_of_block > 1 ? w->KB * w->groups_of_block : groups;
+    const uint64_t code_bytes = static_cast<uint64_t>(w->Np / 16) * w->KB * 1024, count = static_cast<uint64_t>(w->Np) * w->slots;
+    const uint64_t zero_bytes = zeros ? count : 0;
+    w->bytes = code_bytes + 4 * count + zero_bytes;
+    VNPU_HIP(hipMalloc(&w->codes, code_bytes));
+    VNPU_HIP(hipMalloc(&w->scales, 4 * count));
+    if (zeros) VNPU_HIP(hipMalloc(&w->zeros, zero_bytes));
+    uint32_t *bad_dev = nullptr, bad = 0;
+    VNPU_HIP(hipMalloc(&bad_dev, sizeof(bad)));
+    std::unique_ptr<uint32_t, hipError_t (*)(void *)> bad_guard(bad_dev, hipFree);
+    hipStream_t st = nullptr;
+    VNPU_HIP(hipStreamCreate(&st));
+    std::unique_ptr<std::remove_pointer<hipStream_t>::type, hipError_t (*)(hipStream_t)> st_guard(st, hipStreamDestroy);
+    const uint64_t row = ((trans_b ? K : N) + 1) / 2, ld = ldb ? ldb : row;
+    Stager sg(st);
+    const uint8_t *Bd = sg.in(B, span(trans_b ? N : K, row, ld, 1));
+    const float *sd = sg.in(scales, static_cast<size_t>(groups) * N * 4);
+    const uint8_t *zd = sg.in(zeros, zeros ? static_cast<size_t>(groups) * N : 0);
+    VNPU_HIP(hipMemcpyAsync(bad_dev, &bad, sizeof(bad), hipMemcpyHostToDevice, st));
+    k::I4Weights to;
+    to.codes = w->codes;
+    to.zeros = w->zeros;
+    to.scales = w->scales;
+    to.KB = w->KB;
+    to.Np = w->Np;
+    to.slots = w->slots;
+    k::pack_i4(st, Bd, sd, zd, K, N, groups, static_cast<uint32_t>(ld), trans_b, to, bad_dev);
+    VNPU_HIP(hipGetLastError());
+    VNPU_HIP(hipMemcpyAsync(&bad, bad_dev, sizeof(bad), hipMemcpyDeviceToHost, st));
+    VNPU_HIP(hipStreamSynchronize(st));
+    sg.finish();
+    if (bad) return nullptr;
+    dev->dma_bytes.fetch_add(static_cast<uint64_t>(K) * N);
+    return w.release();
+}
+
+void destroy_packed_i4(vnpu_packed_weights_i4_t *w)
+{
+    if (!w) return;
+    if (w->codes) (void)hipFree(w->codes);
+    if (w->scales) (void)hipFree(w->scales);
+    if (w->zeros) (void)hipFree(w->zeros);
+    delete w;
+}
+
 void release_device_tables(vnpu_device_t *dev)
 {
     {
@@ -1600,6 +1908,32 @@ extern "C" VNPU_API int32_t VNPU_CALL vnpu_debug_route(const vnpu_command_t *cmd
                 (void)vnpu::kv_read_params(&on, cmd->args.kv_read, sizes);
                 std::snprintf(out, size, "read");
             }
+            return VNPU_OK;
+        }
+        if (cmd->opcode == VNPU_OP_MATMUL_I4) {   // the weights are not looked at
+            vnpu_stream_t on;
+            const vnpu::k::I4Gemm p = vnpu::matmul_i4_params(&on, cmd->args.matmul_i4, {nullptr, true});
+            std::snprintf(out, size, "%s ws=%zu", vnpu::k::matmul_i4_route(p).c_str(), vnpu::k::matmul_i4_ws_bytes(p));
+            return VNPU_OK;
+        }
+        if (cmd->opcode == VNPU_OP_KV_PREFIX_ATTENTION_I8) {
+            const vnpu_kv_prefix_attention_i8_args_t &a = cmd->args.kv_prefix_attention;
+            vnpu_stream_t on;
+            if (!a.prefix_len) {
+                const vnpu::k::KvAttn p = vnpu::kv_attention_params(&on, a.attention, {nullptr, true});
+                std::snprintf(out, size, "%s ws=%zu", vnpu::k::kv_attention_route(p).c_str(),
+                              vnpu::k::kv_attention_ws_bytes(p));
+                return VNPU_OK;
+            }
+            const int32_t *table = nullptr;
+            const vnpu::k::KvAttn p = vnpu::kv_prefix_params(&on, a, {nullptr, true}, table);
+            std::snprintf(out, size, "%s ws=%zu", vnpu::k::kv_prefix_attention_route(p, table).c_str(),
+                          vnpu::k::kv_prefix_attention_ws_bytes(p, table));
+            return VNPU_OK;
+        }
+        if (cmd->opcode == VNPU_OP_ROPE_AXES_F32) {
+            (void)vnpu::rope_axes_params(cmd->args.rope_axes, {nullptr, true});
+            std::snprintf(out, size, "rope_axes");
             return VNPU_OK;
         }
         if (cmd->opcode == VNPU_OP_MATMUL_F32) {   // no tile mask, no requested K depth

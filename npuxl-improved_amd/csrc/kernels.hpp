@@ -265,6 +265,11 @@ struct KvCall {
     const int32_t *lengths = nullptr, *seq_start = nullptr;
     uint32_t batch = 0, tokens = 0;
     uint32_t *err = nullptr;
+    // Attention behind a shared prefix: its tokens, whole pages, which lengths count
+    // and which are not this call's.  0: none.
+    uint32_t skip = 0;
+    // The prefix itself: one sequence of every row of `every` sequences, of `length` keys.
+    uint32_t every = 1, length = 0;
 };
 struct KvAppend {
     KvCall call;
@@ -283,6 +288,10 @@ struct KvAttn {
     KvRows q, o;
     float scale = 1.0f;
     uint32_t cus = 256;
+    // Results stay in the workspace with their maximum and sum (kv_prefix_attention).
+    uint32_t partial = 0;
+    // Without seq_start, tokens of one of the sequences that are one here (0: they are not).
+    uint32_t per = 0;
 };
 struct KvRead {
     KvCall call;
@@ -299,8 +308,54 @@ void kv_read(hipStream_t s, const KvRead &p);
 // ws holds kv_attention_ws_bytes(p) bytes (0: none is used).
 size_t kv_attention_ws_bytes(const KvAttn &p);
 void kv_attention(hipStream_t s, const KvAttn &p, void *ws);
+// own: attention over what lies behind a prefix of own.call.skip tokens, which are
+// the pages of prefix_table.
+size_t kv_prefix_attention_ws_bytes(const KvAttn &own, const int32_t *prefix_table);
+bool kv_prefix_attention_fits(const KvAttn &own, const int32_t *prefix_table);
+void kv_prefix_attention(hipStream_t s, const KvAttn &own, const int32_t *prefix_table, void *ws);
+std::string kv_prefix_attention_route(const KvAttn &own, const int32_t *prefix_table);
 // Its kernels and how the work is split, by name.
 std::string kv_attention_route(const KvAttn &p);
+
+// ---- MATMUL_I4 (matmul_i4.hip) ----
+// Weights in device memory: 16 columns a strip, 128 of K a block (see there).
+struct I4Weights {
+    uint8_t *codes = nullptr, *zeros = nullptr;   // zeros null: all 8
+    float *scales = nullptr;
+    uint32_t KB = 0, Np = 0, slots = 0;   // blocks of K, padded columns, groups of a strip in scales and zeros
+};
+// bad: stored 1 where a zero is above 15.
+void pack_i4(hipStream_t s, const uint8_t *B, const float *scales, const uint8_t *zeros, uint32_t K, uint32_t N, uint32_t groups,
+             uint32_t ldb, uint32_t trans_b, const I4Weights &w, uint32_t *bad);
+struct I4Gemm {
+    const float *A = nullptr, *bias = nullptr;
+    float *C = nullptr;
+    const uint8_t *codes = nullptr, *zeros = nullptr;
+    const float *scales = nullptr;
+    uint32_t KB = 0, Np = 0, slots = 0;
+    uint32_t groups_of_block = 1, blocks_of_group = 1;   // one of them is 1
+    uint32_t M = 0, K = 0, N = 0, lda = 0, ldc = 0, epilogue = 0;
+    uint32_t cus = 256;
+};
+// ws holds matmul_i4_ws_bytes(p) bytes (0: none is used).
+bool matmul_i4_fits(const I4Gemm &p);
+size_t matmul_i4_ws_bytes(const I4Gemm &p);
+void matmul_i4(hipStream_t s, const I4Gemm &p, void *ws);
+std::string matmul_i4_route(const I4Gemm &p);
+
+// ---- ROPE_AXES_F32 (rope_axes.hip) ----
+struct RopeAxes {
+    const float *Q = nullptr, *K = nullptr;
+    float *Q_out = nullptr, *K_out = nullptr;
+    const int32_t *positions = nullptr;
+    uint32_t batch = 1, tokens = 0, heads = 0, kv_heads = 0, head_dim = 0, position_ld = 0, pairs = 0;
+    uint32_t half = 0;       // pairs (j, j + pairs), else (2 j, 2 j + 1)
+    KvRows q, qo, k, ko;
+    double turns[128];       // angle / 2 pi of position 1, of each pair
+    uint8_t axis[128];
+};
+bool rope_axes_fits(const RopeAxes &p);
+void rope_axes(hipStream_t s, const RopeAxes &p);
 
 // ---- fills (ops.hip) ----
 void fill_u8(hipStream_t s, void *dst, uint8_t value, uint64_t bytes);

@@ -134,10 +134,10 @@ __device__ __forceinline__ uint32_t chunks_of(const KvAttn &p, const Split &sp, 
 {
     if (b >= p.call.batch) return 0;
     const kv::Seq s = kv::sequence(p.call, b);
-    const int32_t len = p.call.lengths[b];
+    const int32_t len = kv::length(p.call, b);
     const uint64_t rows = static_cast<uint64_t>(s.n) * (p.heads / p.call.c.kv_heads);
     if (!s.ok || len < 0 || static_cast<uint32_t>(len) > p.max_kv || s.n > p.max_tokens || rows <= sp.low_rows ||
-        rows > sp.high_rows)
+        rows > sp.high_rows || !kv::behind_prefix(p.call, s, len, p.causal))
         return 0;
     return max(1u, (static_cast<uint32_t>(len) + kChunk - 1) / kChunk);
 }
@@ -181,6 +181,12 @@ __device__ __forceinline__ bool find_slot(const KvAttn &p, const Split &sp, bool
         before += static_cast<uint32_t>(__shfl(static_cast<int>(upto), n - 1));
     }
     return false;
+}
+
+// Token i of the sequence's queries, from its first.
+__device__ __forceinline__ uint64_t query_at(const KvAttn &p, uint32_t i)
+{
+    return p.per ? i / p.per * p.q.batch + i % p.per * p.q.token : i * p.q.token;
 }
 
 // A row's query as digits for the matrix cores: lane (group g, row) holds
@@ -424,7 +430,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) vo
     int8_t *k_lds = lds + wave * 128 * DP, *v_lds = k_lds + 64 * DP;
     uint32_t *sh_p = reinterpret_cast<uint32_t *>(lds + WAVES * 128 * DP) + wave * 256;
     float *sh_o_all = reinterpret_cast<float *>(lds + WAVES * (128 * DP + 1024)), *sh_o = sh_o_all + wave * RT * DT * 64;
-    if (blockIdx.x == 0 && h == 0) kv::check_all(c, false, p.max_kv, p.max_tokens);
+    if (blockIdx.x == 0 && h == 0) kv::check_all(c, false, p.max_kv, p.max_tokens, p.causal);
     uint32_t slot = blockIdx.x;
     Slot sl;
     if (!find_slot(p, sp, false, slot, sl)) return;
@@ -432,7 +438,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) vo
     const kv::Seq seq = kv::sequence(c, b);
     const uint32_t n = __builtin_amdgcn_readfirstlane(seq.n), rows = n * group, row0 = blockIdx.z * R;
     if (row0 >= rows) return;
-    const int len = __builtin_amdgcn_readfirstlane(c.lengths[b]);
+    const int len = __builtin_amdgcn_readfirstlane(kv::length(c, b));
     // Even parts of the keys.
     const uint32_t chunks = __builtin_amdgcn_readfirstlane(sl.chunks), part = __builtin_amdgcn_readfirstlane(sl.part);
     const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * part / parts);
@@ -441,7 +447,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) vo
     // Pages of a chunk's four blocks of 16 keys (blocks behind the last are
     // the last) and, of the chunk in LDS, their scales.
     const uint32_t last16 = len ? (len - 1) / 16 : 0, log16 = c.c.log_page - 4, tiles = D / 16;
-    const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld;
+    const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld + (c.skip >> c.c.log_page);
     bool strange = false;   // a page outside the pool: page 0 is read in its place
     int32_t id[4] = {};
     uint64_t unit[4] = {};
@@ -517,7 +523,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) vo
         // Loads under a condition would be waited for one by one.
         const uint32_t e = threadIdx.x + k * 64 * WAVES, r = e / (DP / 4), d = 4 * (e % (DP / 4));
         const uint32_t row = min(row0 + r, rows - 1), i = row / group;
-        const float *at = q_base + i * p.q.token + (row - i * group) * p.q.head + min(d, D - 4);
+        const float *at = q_base + query_at(p, i) + (row - i * group) * p.q.head + min(d, D - 4);
         raw[k] = aligned ? *reinterpret_cast<const float4 *>(at) : make_float4(at[0], at[1], at[2], at[3]);
         if (row0 + r >= rows || d >= D) raw[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
@@ -788,7 +794,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) vo
         }
         o = L != 0.0f ? o / L : 0.0f;
         const uint32_t at = row0 + row;
-        if (parts == 1) {
+        if (parts == 1 && !p.partial) {
             p.O[kv::rows_base(c, p.o, b, seq) + at / group * p.o.token + (h * group + at % group) * p.o.head + d] = o;
         } else {
             ws_o[at * (D + 2) + d] = o;
@@ -931,9 +937,10 @@ __device__ __forceinline__ bool find_tile(const KvAttn &p, const Tiles &tl, uint
 __device__ __forceinline__ bool tile_sequence(const KvAttn &p, const Tiles &tl, uint32_t group, uint32_t b, kv::Seq &seq, uint32_t &len)
 {
     seq = kv::sequence(p.call, b);
-    const int32_t n = p.call.lengths[b];
+    const int32_t n = kv::length(p.call, b);
     len = static_cast<uint32_t>(n);
-    return seq.ok && n >= 0 && len <= p.max_kv && seq.n <= p.max_tokens && static_cast<uint64_t>(seq.n) * group > tl.low_rows;
+    return seq.ok && n >= 0 && len <= p.max_kv && seq.n <= p.max_tokens && static_cast<uint64_t>(seq.n) * group > tl.low_rows &&
+           kv::behind_prefix(p.call, seq, n, p.causal);
 }
 
 // Keys that a row sees; chunks of a tile and the ranges that share them evenly.
@@ -962,7 +969,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attenti
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t G = c.c.kv_heads, h = blockIdx.x % G, D = FULL ? DP : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
-    if (blockIdx.x == 0 && blockIdx.y == 0) kv::check_all(c, false, p.max_kv, p.max_tokens);
+    if (blockIdx.x == 0 && blockIdx.y == 0) kv::check_all(c, false, p.max_kv, p.max_tokens, p.causal);
     // The last tiles of a causal sequence have the most keys: they come first.
     uint32_t b, tile, len;
     kv::Seq seq;
@@ -990,14 +997,14 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attenti
     for (int r = 0; r < RT; ++r) {
         const uint32_t row = row0 + 16 * r + col;
         const bool here = row < rows;
-        const float *at = p.Q + kv::rows_base(c, p.q, b, seq) + (here ? (row / group) * p.q.token + (h * group + row % group) * p.q.head : 0);
+        const float *at = p.Q + kv::rows_base(c, p.q, b, seq) + (here ? query_at(p, row / group) + (h * group + row % group) * p.q.head : 0);
         q[r].load(at, here, D, p.scale, aligned);
         st[r].clear();
         limit[r] = here ? sees(row) : static_cast<int>(len);
     }
 
     const uint32_t kb = col >> 2, last16 = len ? (len - 1) / 16 : 0, log16 = c.c.log_page - 4;
-    const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld;
+    const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld + (c.skip >> c.c.log_page);
     auto checked = [&](int32_t id) -> uint32_t {
         if (static_cast<uint32_t>(id) < c.c.pages) return static_cast<uint32_t>(id);
         kv::fail(c.err);
@@ -1194,7 +1201,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attenti
         const int down = -static_cast<int>(st[r].shift);
         auto result = [&](int t) { return v4f{ldexpf(st[r].o[t][0] * by, down), ldexpf(st[r].o[t][1] * by, down), ldexpf(st[r].o[t][2] * by, down), ldexpf(st[r].o[t][3] * by, down)}; };
         if (row >= rows) continue;
-        if (ranges == 1) {
+        if (ranges == 1 && !p.partial) {
             float *at = p.O + kv::rows_base(c, p.o, b, seq) + (row / group) * p.o.token + (h * group + row % group) * p.o.head + 4 * g;
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
@@ -1327,7 +1334,7 @@ Plan plan_of(const KvAttn &p)
                                 : static_cast<uint32_t>(std::min<uint64_t>(
                                       r.split.target + c.batch,
                                       static_cast<uint64_t>(c.batch) * ((p.max_kv + r.split.min_per * kChunk - 1) / (r.split.min_per * kChunk))));
-        if (!r.split.whole) r.few_ws = (static_cast<size_t>(r.slots) * G * r.rows * (D + 2) * sizeof(float) + 15) / 16 * 16;
+        if (!r.split.whole || p.partial) r.few_ws = (static_cast<size_t>(r.slots) * G * r.rows * (D + 2) * sizeof(float) + 15) / 16 * 16;
     }
     r.ws = r.few_ws;
     if (r.tiled) {
@@ -1355,7 +1362,7 @@ Plan plan_of(const KvAttn &p)
                                         std::min<uint64_t>(at_once * (c.seq_start ? 5 : 3) / (3 * grid), chunks / (c.seq_start ? 5 : 8)));
         r.tiles.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(parts, 1), 64));
         r.tiles.per = (chunks + r.tiles.parts - 1) / r.tiles.parts;
-        if (r.tiles.parts > 1) r.ws += static_cast<size_t>(grid) * r.tiles.parts * r.tile_rows * (D + 4) * sizeof(float);
+        if (r.tiles.parts > 1 || p.partial) r.ws += static_cast<size_t>(grid) * r.tiles.parts * r.tile_rows * (D + 4) * sizeof(float);
     }
     return r;
 }
@@ -1381,7 +1388,7 @@ void launch_tile(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     const uint32_t grid = pl.tiles.count * p.call.c.kv_heads;
     kernel<<<dim3(grid, pl.tiles.parts), 64 * WAVES, bytes, s>>>(p, pl.tiles, ws);
-    if (pl.tiles.parts > 1) kv_attention_join<16 * RT * WAVES, DP / 64><<<dim3(grid, 4 * RT * WAVES / kJoinRows), 256, 0, s>>>(p, pl.tiles, ws);
+    if (pl.tiles.parts > 1 && !p.partial) kv_attention_join<16 * RT * WAVES, DP / 64><<<dim3(grid, 4 * RT * WAVES / kJoinRows), 256, 0, s>>>(p, pl.tiles, ws);
 }
 template <int DP>
 void launch(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
@@ -1390,7 +1397,7 @@ void launch(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
         if (pl.rows <= 4) launch_few<DP, 1>(s, p, pl, ws);
         else if (DP > 128 || pl.rows <= 8) launch_few<DP, 2>(s, p, pl, ws);
         else if constexpr (DP <= 128) launch_few<DP, 4>(s, p, pl, ws);
-        if (pl.few_ws)
+        if (pl.few_ws && !p.partial)
             kv_attention_merge<<<dim3(p.call.batch, p.call.c.kv_heads, pl.rows), kJoinThreads, 0, s>>>(p, pl.split, ws, pl.rows);
     }
     if (pl.tiled) {
@@ -1398,6 +1405,137 @@ void launch(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
         if (DP > 128 || pl.tile_rows == 64) launch_tile<DP, 1, 4>(s, p, pl, rest);
         else if constexpr (DP <= 128) launch_tile<DP, 2, 4>(s, p, pl, rest);
     }
+}
+
+// ---------------------------------------------------------------------------
+// A shared prefix: the rows of all sequences are one sequence's against its keys,
+// each sequence's rows its own against what lies behind; both leave their results
+// in the workspace, each o / l with its maximum m and sum l, and are weighed together
+// by l 2^(m - max m).
+// ---------------------------------------------------------------------------
+
+// Where a row's results of one of the two calls are: parts of them, `step` floats apart.
+struct Found {
+    const float *at;
+    uint64_t step;
+    uint32_t parts;
+};
+struct Side {
+    KvAttn p;
+    Split split;
+    Tiles tiles;
+    uint32_t rows, tile_rows;   // rows of a slot; of a tile (0: the call has none)
+    const float *few, *tile;
+};
+__device__ __forceinline__ Found find_results(const Side &s, uint32_t b, const kv::Seq &seq, uint32_t row, uint32_t h)
+{
+    const KvCall &c = s.p.call;
+    const uint32_t G = c.c.kv_heads, D = c.c.head_dim, group = s.p.heads / G;
+    const uint64_t rows = static_cast<uint64_t>(seq.n) * group;
+    if (s.tile_rows && rows > s.tiles.low_rows) {
+        const uint32_t len = static_cast<uint32_t>(kv::length(c, b)), M = s.tile_rows, tile = row / M;
+        const uint32_t unit = c.seq_start ? static_cast<uint32_t>(static_cast<uint64_t>(seq.row) * group / M) + b + tile
+                                          : b * s.tiles.per_seq + tile;
+        const uint32_t last = min(seq.n * group, tile * M + M) - 1;
+        const uint32_t chunks = (static_cast<uint32_t>(keys_of(s.p, len, seq.n, last, group)) + kChunk - 1) / kChunk;
+        return {s.tile + ((static_cast<uint64_t>(unit) * G + h) * s.tiles.parts * M + (row - tile * M)) * (D + 4),
+                static_cast<uint64_t>(M) * (D + 4), ranges_of(s.tiles, chunks)};
+    }
+    Slot sl;
+    sl.b = b;
+    uint32_t slot = s.split.whole ? b : 0;
+    if (!find_slot(s.p, s.split, true, slot, sl)) return {s.few, 0, 0};
+    if (s.split.whole) slot = b;
+    return {s.few + ((static_cast<uint64_t>(slot) * G + h) * s.rows + row) * (D + 2), static_cast<uint64_t>(G) * s.rows * (D + 2), sl.parts};
+}
+
+// A wave a token and kv head.
+__global__ __launch_bounds__(256) void kv_attention_prefix_join(Side shared, Side own)
+{
+    const KvAttn &p = own.p;
+    const KvCall &c = p.call;
+    const uint32_t lane = threadIdx.x & 63, G = c.c.kv_heads, D = c.c.head_dim, group = p.heads / G;
+    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t t = static_cast<uint32_t>(item / G), h = static_cast<uint32_t>(item % G);
+    if (t >= c.tokens) return;
+    uint32_t b = 0;
+    if (!c.seq_start) {
+        b = t / (c.tokens / c.batch);
+    } else {   // how many sequences end at this token or before it
+        for (uint32_t i = 0; i < c.batch; i += 64) {
+            const uint32_t at = i + lane;
+            b += __popcll(__ballot(at < c.batch && static_cast<int64_t>(c.seq_start[at + 1]) <= static_cast<int64_t>(t)));
+        }
+        if (b >= c.batch) return;   // behind the last
+    }
+    const kv::Seq seq = kv::sequence(c, b), all = kv::sequence(shared.p.call, 0);
+    const int32_t len = kv::length(c, b);
+    if (!seq.ok || !all.ok || t < seq.row || t - seq.row >= seq.n || seq.n > p.max_tokens || len < 0 || static_cast<uint32_t>(len) > p.max_kv ||
+        !kv::behind_prefix(c, seq, len, p.causal))
+        return;   // check_all told
+    const uint32_t i = t - seq.row, i_all = t - all.row;
+    Found f[2] = {find_results(shared, 0, all, i_all * group, h), find_results(own, b, seq, i * group, h)};
+    float *out = p.O + kv::rows_base(c, p.o, b, seq) + i * p.o.token + static_cast<uint64_t>(h) * group * p.o.head;
+    for (uint32_t r = 0; r < group; ++r, out += p.o.head) {
+        if (r) {   // a token's rows may lie in two tiles
+            f[0] = find_results(shared, 0, all, i_all * group + r, h);
+            f[1] = find_results(own, b, seq, i * group + r, h);
+        }
+        float top = kNegInf;
+        for (int k = 0; k < 2; ++k)
+            for (uint32_t j = lane; j < f[k].parts; j += 64) top = fmaxf(top, f[k].at[j * f[k].step + D]);
+        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+        const float base = top == kNegInf ? 0.0f : top;
+        float sum = 0.0f, o[4] = {};
+        for (int k = 0; k < 2; ++k)
+            for (uint32_t j0 = 0; j0 < f[k].parts; j0 += 64) {
+                const uint32_t n = min(64u, f[k].parts - j0);
+                const float *at = f[k].at + j0 * f[k].step, *mine = at + min(lane, n - 1) * f[k].step + D;
+                const float w = lane < n ? mine[1] * __builtin_amdgcn_exp2f(mine[0] - base) : 0.0f;
+                sum += w;
+                for (uint32_t j = 0; j < n; ++j) {
+                    const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
+#pragma unroll
+                    for (uint32_t x = 0; x < 4; ++x)
+                        if (lane + 64 * x < D) o[x] = fmaf(wj, at[j * f[k].step + lane + 64 * x], o[x]);
+                }
+            }
+        for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x)
+            if (lane + 64 * x < D) out[lane + 64 * x] = sum != 0.0f ? o[x] / sum : 0.0f;
+    }
+}
+
+// The call over the prefix's keys of what own attends to behind it.
+KvAttn shared_call(const KvAttn &own, const int32_t *prefix_table)
+{
+    KvAttn p = own;
+    const KvCall &c = own.call;
+    p.call.c.table = prefix_table;
+    p.call.c.table_ld = c.skip >> c.c.log_page;
+    p.call.lengths = nullptr;
+    p.call.length = c.skip;
+    p.call.skip = 0;
+    p.call.every = c.batch;
+    p.call.batch = 1;
+    p.max_tokens = c.tokens;
+    p.max_kv = c.skip;
+    p.causal = 0;
+    p.per = c.seq_start ? 0 : c.tokens / c.batch;
+    return p;
+}
+Side side_of(const KvAttn &p, const Plan &pl, const float *ws)
+{
+    return {p, pl.split, pl.tiles, pl.rows, pl.tiled ? pl.tile_rows : 0, ws, ws + pl.few_ws / sizeof(float)};
+}
+size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+void launch_any(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
+{
+    if (p.call.c.head_dim <= 64) launch<64>(s, p, pl, ws);
+    else if (p.call.c.head_dim <= 128) launch<128>(s, p, pl, ws);
+    else launch<256>(s, p, pl, ws);
 }
 
 }  // namespace
@@ -1424,11 +1562,35 @@ size_t kv_attention_ws_bytes(const KvAttn &p) { return plan_of(p).ws; }
 
 void kv_attention(hipStream_t s, const KvAttn &p, void *ws)
 {
-    const Plan pl = plan_of(p);
-    float *part = static_cast<float *>(ws);
-    if (p.call.c.head_dim <= 64) launch<64>(s, p, pl, part);
-    else if (p.call.c.head_dim <= 128) launch<128>(s, p, pl, part);
-    else launch<256>(s, p, pl, part);
+    launch_any(s, p, plan_of(p), static_cast<float *>(ws));
+}
+
+size_t kv_prefix_attention_ws_bytes(const KvAttn &own, const int32_t *prefix_table)
+{
+    return padded(plan_of(own).ws) + padded(plan_of(shared_call(own, prefix_table)).ws);
+}
+
+bool kv_prefix_attention_fits(const KvAttn &own, const int32_t *prefix_table)
+{
+    return kv_attention_fits(own) && kv_attention_fits(shared_call(own, prefix_table)) &&
+           static_cast<uint64_t>(own.call.tokens) * own.call.c.kv_heads * 64 < (1ull << 32) - 256;
+}
+
+std::string kv_prefix_attention_route(const KvAttn &own, const int32_t *prefix_table)
+{
+    return "shared: " + kv_attention_route(shared_call(own, prefix_table)) + " own: " + kv_attention_route(own);
+}
+
+void kv_prefix_attention(hipStream_t s, const KvAttn &own, const int32_t *prefix_table, void *ws)
+{
+    const KvAttn shared = shared_call(own, prefix_table);
+    const Plan own_plan = plan_of(own), shared_plan = plan_of(shared);
+    float *own_ws = static_cast<float *>(ws), *shared_ws = own_ws + padded(own_plan.ws) / sizeof(float);
+    launch_any(s, shared, shared_plan, shared_ws);
+    launch_any(s, own, own_plan, own_ws);
+    const uint64_t items = static_cast<uint64_t>(own.call.tokens) * own.call.c.kv_heads;
+    kv_attention_prefix_join<<<static_cast<uint32_t>((items + 3) / 4), 256, 0, s>>>(side_of(shared, shared_plan, shared_ws),
+                                                                                  side_of(own, own_plan, own_ws));
 }
 
 }  // namespace k

@@ -36,34 +36,16 @@ struct Rates {
     double turns[128];
 };
 
-// cos and sin of 2 pi t.  t less its nearest quarter leaves |x| <= pi / 4, where
-// the Taylor series to x^14 and x^13 are within 2e-14.  f64 because t is
-// exact to some 2^-52 of itself only there: position 100000 in f32 would be off by
-// 0.006 rad.  That error grows with the position: of the f32 results 1 in 10^5 is not the
-// correctly rounded one up to position 10000, 1 in 14000 at 100000, 1 in 2000 at 10^6
-// (theta 10000, 64 and 128 dimensions), all within half a step and 2^-10 of one to there.
+// cos and sin of 2 pi t in f32.  Their error grows with the position: of the f32
+// results 1 in 10^5 is not the correctly rounded one up to position 10000, 1 in 14000 at
+// 100000, 1 in 2000 at 10^6 (theta 10000, 64 and 128 dimensions), all within half a step
+// and 2^-10 of one to there.
 __device__ __forceinline__ void cos_sin_turns(double t, float &c, float &s)
 {
-    const double quarter = rint(4.0 * t);
-    const double x = 6.283185307179586476925 * fma(-0.25, quarter, t);
-    const double z = x * x;
-    double pc = -1.0 / 87178291200.0, ps = 1.0 / 6227020800.0;
-    pc = fma(pc, z, 1.0 / 479001600.0);
-    ps = fma(ps, z, -1.0 / 39916800.0);
-    pc = fma(pc, z, -1.0 / 3628800.0);
-    ps = fma(ps, z, 1.0 / 362880.0);
-    pc = fma(pc, z, 1.0 / 40320.0);
-    ps = fma(ps, z, -1.0 / 5040.0);
-    pc = fma(pc, z, -1.0 / 720.0);
-    ps = fma(ps, z, 1.0 / 120.0);
-    pc = fma(pc, z, 1.0 / 24.0);
-    ps = fma(ps, z, -1.0 / 6.0);
-    pc = fma(pc, z, -0.5);
-    const double cx = fma(pc, z, 1.0), sx = fma(ps * z, x, x);
-    const int q = static_cast<int>(static_cast<long long>(quarter) & 3);
-    const double a = q & 1 ? sx : cx, b = q & 1 ? cx : sx;
-    c = static_cast<float>(q == 1 || q == 2 ? -a : a);
-    s = static_cast<float>(q >= 2 ? -b : b);
+    double cd, sd;
+    dev::cos_sin_turns(t, cd, sd);
+    c = static_cast<float>(cd);
+    s = static_cast<float>(sd);
 }
 
 __device__ __forceinline__ float2 turned(float2 x, float c, float s)

@@ -26,9 +26,22 @@ __device__ __forceinline__ Seq sequence(const KvCall &c, uint32_t b)
         const uint32_t n = c.tokens / c.batch;
         return {b * n, n, true};
     }
-    const int32_t a = c.seq_start[b], e = c.seq_start[b + 1];
+    const int32_t a = c.seq_start[b * c.every], e = c.seq_start[(b + 1) * c.every];
     return {static_cast<uint32_t>(a), static_cast<uint32_t>(e - a),
             a >= 0 && e >= a && static_cast<uint32_t>(e) <= c.tokens};
+}
+// Keys of sequence b; negative where there cannot be as many or as few.
+__device__ __forceinline__ int32_t length(const KvCall &c, uint32_t b)
+{
+    if (!c.lengths) return static_cast<int32_t>(c.length);
+    const int32_t n = c.lengths[b];
+    return n < 0 ? -1 : n - static_cast<int32_t>(c.skip);
+}
+// Behind a prefix: a sequence without rows may have any length, a causal one's new
+// tokens are keys of its own.
+__device__ __forceinline__ bool behind_prefix(const KvCall &c, const Seq &s, int32_t len, uint32_t causal)
+{
+    return !c.skip || !s.n || (len >= 0 && (!causal || static_cast<uint32_t>(len) >= s.n));
 }
 __device__ __forceinline__ uint32_t capacity(const KvCall &c) { return c.c.table_ld << c.c.log_page; }
 
@@ -75,10 +88,15 @@ inline uint32_t unit_count(const KvCall &c)
 // Every sequence's rows and lengths, looked over by one workgroup of a call so
 // that what no workgroup meets is an error too.  extra: the call's tokens count
 // towards the length (append, read).  most: tokens of a sequence.
-__device__ __forceinline__ void check_all(const KvCall &c, bool extra, uint32_t limit, uint32_t most)
+__device__ __forceinline__ void check_all(const KvCall &c, bool extra, uint32_t limit, uint32_t most, uint32_t causal = 0)
 {
     for (uint32_t b = threadIdx.x; b < c.batch; b += blockDim.x) {
         const Seq s = sequence(c, b);
+        if (c.skip) {
+            const int32_t own = length(c, b);
+            if (!s.ok || s.n > most || !behind_prefix(c, s, own, causal) || (s.n && own > static_cast<int32_t>(limit))) fail(c.err);
+            continue;
+        }
         const int64_t len = c.lengths ? c.lengths[b] : 0;
         if (!s.ok || s.n > most || len < 0 || len + (extra ? static_cast<int64_t>(s.n) : 0) > static_cast<int64_t>(limit)) fail(c.err);
     }

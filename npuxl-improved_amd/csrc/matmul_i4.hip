@@ -1,0 +1,352 @@
+// matmul_i4.hip - MATMUL_I4: f32 rows times 4-bit weights with group scales, on
+// gfx950.
+//
+//   C[m][n] = epi(sum_g scale[g][n] * sum_{k in g} A[m][k] (code[k][n] - zero[g][n]) + bias[n])
+//
+// The inner sums run on the int8 matrix cores without a rounding: 128 of a row of A
+// become whole numbers of up to 31 bits in a unit of their own (a power of two),
+// four balanced base-256 digits each, and codes are 0 to 15 as they stand.  The 16
+// operand rows of v_mfma_i32_16x16x64_i8 are 4 rows of A times 4 digits, so one
+// product gives a lane the four digit sums of one result.  Zeros enter as the
+// product's first summand, -zero * (sum of the digits), which a product with ones gives.
+//
+// Weights in device memory, strips of 16 columns and blocks of 128 of K:
+//   codes  [Np/16][KB][64][16]: byte j of lane (kg, c) holds k = 128 kb + 32 (j / 8)
+//          + 8 kg + j % 8 in its lower half and k + 64 in its upper, so that a lane's
+//          16 bytes and two masks are its operands of two products; 1 KiB a block, a
+//          strip's blocks in a row.
+//   scales [Np/16][groups][16] f32, zeros the same in bytes; padding 0.
+#include "device_math.hpp"
+#include "kernels.hpp"
+
+#include <algorithm>
+#include <cstdio>
+
+namespace vnpu {
+namespace k {
+namespace {
+
+using v4i = int __attribute__((ext_vector_type(4)));
+using v4f = float __attribute__((ext_vector_type(4)));
+
+// ---------------------------------------------------------------------------
+// Packing
+// ---------------------------------------------------------------------------
+
+__global__ __launch_bounds__(256) void pack_codes(const uint8_t *B, uint32_t K, uint32_t N, uint32_t ldb, uint32_t trans_b,
+                                                  uint8_t *codes, uint32_t KB, uint64_t pieces)
+{
+    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (at >= pieces) return;
+    const uint32_t lane = at & 63, c = lane & 15, kg = lane >> 4;
+    const uint64_t block = at >> 6;
+    const uint32_t kb = static_cast<uint32_t>(block % KB), n = static_cast<uint32_t>(block / KB) * 16 + c;
+    auto code = [&](uint32_t k) -> uint32_t {
+        if (k >= K || n >= N) return 0;
+        const uint32_t row = trans_b ? n : k, col = trans_b ? k : n;
+        return (B[static_cast<uint64_t>(row) * ldb + col / 2] >> (4 * (col & 1))) & 15;
+    };
+    uint32_t w[4] = {};
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) {
+        const uint32_t k = 128 * kb + 32 * (j / 8) + 8 * kg + j % 8;
+        w[j / 4] |= (code(k) | code(k + 64) << 4) << (8 * (j % 4));
+    }
+    reinterpret_cast<uint4 *>(codes)[at] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// groups of the caller's, slots of a strip in the packed arrays.
+__global__ __launch_bounds__(256) void pack_scales(const float *scales, const uint8_t *zeros, uint32_t groups, uint32_t slots,
+                                                   uint32_t N, float *to, uint8_t *to_zeros, uint64_t count, uint32_t *bad)
+{
+    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (at >= count) return;
+    const uint64_t row = at >> 4;
+    const uint32_t g = static_cast<uint32_t>(row % slots), n = static_cast<uint32_t>(row / slots) * 16 + (at & 15);
+    const bool in = g < groups && n < N;
+    to[at] = in ? scales[static_cast<uint64_t>(g) * N + n] : 0.0f;
+    if (!zeros) return;
+    const uint8_t z = in ? zeros[static_cast<uint64_t>(g) * N + n] : 0;
+    if (z > 15) *bad = 1;
+    to_zeros[at] = z;
+}
+
+// ---------------------------------------------------------------------------
+// Epilogue
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ float finished(float x, uint32_t epilogue)
+{
+    switch (epilogue) {
+    case 1: return x > 0.0f ? x : x != x ? x : 0.0f;
+    case 2: return x / (1.0f + expf(-x));
+    case 3: return x / (1.0f + expf(-1.5957691216057308f * fmaf(0.044715f * x * x, x, x)));   // 1 + tanh(u) = 2 / (1 + exp(-2 u))
+    case 4: return 0.5f * x * erfcf(-0.70710678118654752f * x);
+    default: return x;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: bound by the codes.
+// ---------------------------------------------------------------------------
+
+// Largest bits over the lanes of a row of A: 4 lanes side by side, 4 groups of 16.
+__device__ __forceinline__ uint32_t row_largest(uint32_t x)
+{
+    x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0xB1, 0xf, 0xf, true)));
+    x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x4E, 0xf, 0xf, true)));
+    const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return max(b[0], b[1]);
+}
+// Biased exponent e: x * 2^(157 - e) of an x no larger than these bits fits four balanced digits,
+// 127 * (2^24 + 2^16 + 2^8 + 1) = 2139062143 = 2^30 (2 - 65793 / 2^23), 0x10400 is 66560.
+// From 31 up, so that 2^(e - 157) is a normal number.
+__device__ __forceinline__ uint32_t digits_exponent(uint32_t bits) { return max((bits + 0x10400u) >> 23, 31u); }
+
+// Bytes i of four words in word i.
+__device__ __forceinline__ void planes_of(const uint32_t u[4], uint32_t p[4])
+{
+    const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), b = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(u[1], u[0], 0x07030602u), d = __builtin_amdgcn_perm(u[3], u[2], 0x07030602u);
+    p[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    p[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    p[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    p[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+// Sum of four digit sums, digit i counting 256^i.
+__device__ __forceinline__ float digits_sum(const v4i &a)
+{
+    return fmaf(static_cast<float>(a[3] * 256 + a[2]), 65536.0f, static_cast<float>(a[1] * 256 + a[0]));
+}
+
+// A workgroup has T strips and 4 RQ rows, its waves every W-th block of 128 of K.
+// GB: groups of a block (4, 2, or 1 where a group is a block or more).
+template <int RQ, int T, int GB, bool ZEROS, bool ALIGNED>
+__global__ __launch_bounds__(1024) void matmul_i4_few(I4Gemm p)
+{
+    extern __shared__ __align__(16) int8_t lds[];
+    const uint32_t lane = threadIdx.x & 63, m = (lane & 15) >> 2, d = lane & 3, kg = lane >> 4, c = lane & 15;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
+    const uint32_t strip0 = blockIdx.x * T, row0 = blockIdx.y * 4 * RQ, strips = p.Np / 16;
+    int8_t *mine = lds + wave * 2048;
+
+    const v4i *codes[T];
+    const float *scales[T];
+    const uint8_t *zeros[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        const uint64_t strip = min(strip0 + t, strips - 1);
+        codes[t] = reinterpret_cast<const v4i *>(p.codes + strip * p.KB * 1024) + lane;
+        scales[t] = p.scales + strip * p.slots * 16 + c;
+        zeros[t] = ZEROS ? p.zeros + strip * p.slots * 16 + c : nullptr;
+    }
+    const float *rows[RQ];
+#pragma unroll
+    for (int q = 0; q < RQ; ++q) rows[q] = p.A + static_cast<uint64_t>(min(row0 + 4 * q + m, p.M - 1)) * p.lda;
+
+    struct Block {
+        v4i codes[T];
+        float scale[T][GB];
+        uint8_t zero[T][GB];
+        float x[RQ][8];
+    };
+    // What is behind the last block is the last again; behind K, zeros times whatever was read.
+    auto load = [&](Block &b, uint32_t kb) {
+        kb = min(kb, p.KB - 1);
+        const uint32_t k = 128 * kb + 32 * d + 8 * kg;
+#pragma unroll
+        for (int q = 0; q < RQ; ++q) {
+            if constexpr (ALIGNED) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const v4f v = *reinterpret_cast<const v4f *>(rows[q] + (k + 4 * i < p.K ? k + 4 * i : 0));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) b.x[q][4 * i + j] = v[j];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) b.x[q][i] = rows[q][k + i < p.K ? k + i : 0];
+            }
+        }
+        const uint32_t slot = GB > 1 ? GB * kb : kb / p.blocks_of_group;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            b.codes[t] = __builtin_nontemporal_load(codes[t] + static_cast<uint64_t>(kb) * 64);
+#pragma unroll
+            for (int i = 0; i < GB; ++i) {
+                b.scale[t][i] = scales[t][(slot + i) * 16];
+                b.zero[t][i] = ZEROS ? zeros[t][(slot + i) * 16] : 8;
+            }
+        }
+    };
+
+    float acc[RQ][T] = {};   // row 4 q + kg, column c
+    auto of_row_kg = [&](float x) {   // as lane 4 kg has it
+        return __int_as_float(__builtin_amdgcn_ds_bpermute(static_cast<int>(16 * kg), __float_as_int(x)));
+    };
+    auto work = [&](const Block &b, uint32_t kb) {
+        v4i low[T], high[T];
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                low[t][i] = b.codes[t][i] & 0x0f0f0f0f;
+                high[t][i] = (b.codes[t][i] >> 4) & 0x0f0f0f0f;
+            }
+        const uint32_t k = 128 * kb + 32 * d + 8 * kg;
+#pragma unroll
+        for (int q = 0; q < RQ; ++q) {
+            float x[8];
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = k + i < p.K ? b.x[q][i] : 0.0f;
+                most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+            }
+            most = row_largest(most);
+            // Below 2^-96 the unit would not be a normal number: 2^96 times as large, and back at the end.
+            const bool tiny = most - 1u < 0x0f800000u - 1u, rare = __any(tiny);
+            float down = 1.0f;
+            if (rare) {
+                const float by = tiny ? 7.922816251426434e28f : 1.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] *= by;
+                most = tiny ? __float_as_uint(__uint_as_float(most) * by) : most;
+                down = of_row_kg(tiny ? 1.262177448353619e-29f : 1.0f);
+            }
+            const uint32_t e = digits_exponent(most);
+            const float up = __uint_as_float((284u - e) << 23);
+            uint32_t u[8], plane[2][4];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                u[i] = (static_cast<uint32_t>(static_cast<int>(rintf(x[i] * up))) + 0x80808080u) ^ 0x80808080u;   // bytes: balanced digits
+            planes_of(u, plane[0]);
+            planes_of(u + 4, plane[1]);
+            // Lane (m, d, kg) has 8 of K and all digits; as an operand it wants digit d of 32 of K.
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint2 *>(mine + ((m * 4 + i) * 4 + kg) * 32 + d * 8) = make_uint2(plane[0][i], plane[1][i]);
+            __builtin_amdgcn_wave_barrier();
+            const v4i a0 = *reinterpret_cast<const v4i *>(mine + (c * 4 + kg) * 32), a1 = *reinterpret_cast<const v4i *>(mine + (c * 4 + kg) * 32 + 16);
+            __builtin_amdgcn_wave_barrier();
+            const float own = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((e - 30u) << 23);
+            const float unit = of_row_kg(own);
+            const v4i ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101}, none = {0, 0, 0, 0};
+            auto product = [&](const v4i &x, const v4i &y, const v4i &s) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(x, y, s, 0, 0, 0); };
+            auto half = [&](const v4i &x, const v4i &y, int i, const v4i &s) {
+                const long xs = static_cast<long>(static_cast<uint32_t>(x[2 * i])) | static_cast<long>(x[2 * i + 1]) << 32;
+                const long ys = static_cast<long>(static_cast<uint32_t>(y[2 * i])) | static_cast<long>(y[2 * i + 1]) << 32;
+                return __builtin_amdgcn_mfma_i32_16x16x32_i8(xs, ys, s, 0, 0, 0);
+            };
+            auto less = [&](const v4i &sums, int zero) {
+                v4i r;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = __mul24(sums[i], -zero);
+                return r;
+            };
+            v4i sums[GB];
+            if constexpr (GB == 1) {
+                sums[0] = product(a1, ones, product(a0, ones, none));
+            } else if constexpr (GB == 2) {
+                sums[0] = product(a0, ones, none);
+                sums[1] = product(a1, ones, none);
+            } else {
+                sums[0] = half(a0, ones, 0, none);
+                sums[1] = half(a0, ones, 1, none);
+                sums[2] = half(a1, ones, 0, none);
+                sums[3] = half(a1, ones, 1, none);
+            }
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                v4i r[GB];
+                if constexpr (GB == 1) {
+                    r[0] = product(a1, high[t], product(a0, low[t], less(sums[0], b.zero[t][0])));
+                } else if constexpr (GB == 2) {
+                    r[0] = product(a0, low[t], less(sums[0], b.zero[t][0]));
+                    r[1] = product(a1, high[t], less(sums[1], b.zero[t][1]));
+                } else {
+                    r[0] = half(a0, low[t], 0, less(sums[0], b.zero[t][0]));
+                    r[1] = half(a0, low[t], 1, less(sums[1], b.zero[t][1]));
+                    r[2] = half(a1, high[t], 0, less(sums[2], b.zero[t][2]));
+                    r[3] = half(a1, high[t], 1, less(sums[3], b.zero[t][3]));
+                }
+#pragma unroll
+                for (int i = 0; i < GB; ++i) {
+                    float x = digits_sum(r[i]);
+                    if (rare) x *= down;
+                    acc[q][t] = fmaf(x, unit * b.scale[t][i], acc[q][t]);
+                }
+            }
+        }
+    };
+    Block now, next;
+    if (wave < p.KB) load(now, wave);
+    for (uint32_t kb = wave; kb < p.KB; kb += W) {
+        load(next, kb + W);
+        work(now, kb);
+        now = next;
+    }
+    // The waves' sums together, in the waves' order.
+    __syncthreads();
+    float *sums = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int q = 0; q < RQ; ++q)
+#pragma unroll
+        for (int t = 0; t < T; ++t) sums[(wave * RQ * T + q * T + t) * 64 + lane] = acc[q][t];
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < RQ * T * 64; e += blockDim.x) {
+        const uint32_t q = e / (T * 64), row = row0 + 4 * q + (e >> 4 & 3), n = (strip0 + e / 64 % T) * 16 + (e & 15);
+        if (row >= p.M || n >= p.N) continue;
+        float x = 0.0f;
+        for (uint32_t w = 0; w < W; ++w) x += sums[w * RQ * T * 64 + e];
+        if (p.bias) x += p.bias[n];
+        p.C[static_cast<uint64_t>(row) * p.ldc + n] = finished(x, p.epilogue);
+    }
+}
+
+template <int RQ, int T, int GB>
+void launch_few(hipStream_t s, const I4Gemm &p, uint32_t waves)
+{
+    const dim3 grid((p.Np / 16 + T - 1) / T, (p.M + 4 * RQ - 1) / (4 * RQ));
+    const uint32_t bytes = std::max<uint32_t>(waves * 2048, waves * RQ * T * 256);
+    const bool aligned = !((reinterpret_cast<uintptr_t>(p.A) & 15) | (p.lda & 3) | (p.K & 3));
+    const auto kernel = p.zeros ? (aligned ? matmul_i4_few<RQ, T, GB, true, true> : matmul_i4_few<RQ, T, GB, true, false>)
+                                : (aligned ? matmul_i4_few<RQ, T, GB, false, true> : matmul_i4_few<RQ, T, GB, false, false>);
+    kernel<<<grid, 64 * waves, bytes, s>>>(p);
+}
+template <int RQ, int T>
+void launch_few(hipStream_t s, const I4Gemm &p, uint32_t waves)
+{
+    if (p.groups_of_block == 4) launch_few<RQ, T, 4>(s, p, waves);
+    else if (p.groups_of_block == 2) launch_few<RQ, T, 2>(s, p, waves);
+    else launch_few<RQ, T, 1>(s, p, waves);
+}
+
+}  // namespace
+
+void pack_i4(hipStream_t s, const uint8_t *B, const float *scales, const uint8_t *zeros, uint32_t K, uint32_t N, uint32_t groups,
+             uint32_t ldb, uint32_t trans_b, const I4Weights &w, uint32_t *bad)
+{
+    const uint64_t pieces = static_cast<uint64_t>(w.Np / 16) * w.KB * 64, count = static_cast<uint64_t>(w.Np) * w.slots;
+    pack_codes<<<static_cast<uint32_t>((pieces + 255) / 256), 256, 0, s>>>(B, K, N, ldb, trans_b, w.codes, w.KB, pieces);
+    pack_scales<<<static_cast<uint32_t>((count + 255) / 256), 256, 0, s>>>(scales, zeros, groups, w.slots, N, w.scales, w.zeros, count, bad);
+}
+
+// A grid's work-items count in 32 bits in x, workgroups in 16 in y.
+bool matmul_i4_fits(const I4Gemm &p) { return p.Np / 16 < (1u << 22) && p.M <= 16u * 65535; }
+
+size_t matmul_i4_ws_bytes(const I4Gemm &) { return 0; }
+
+void matmul_i4(hipStream_t s, const I4Gemm &p, void *)
+{
+    if (p.M <= 4) launch_few<1, 1>(s, p, 16);
+    else if (p.M <= 8) launch_few<2, 1>(s, p, 16);
+    else launch_few<4, 1>(s, p, 16);
+}
+
+std::string matmul_i4_route(const I4Gemm &) { return "few"; }
+
+}  // namespace k
+}  // namespace vnpu

@@ -98,6 +98,19 @@ static uint32_t trace_category(uint32_t opcode)
     return 0;  // compute
 }
 
+// A workspace's bytes: 0 for a call that is refused.
+template <typename F>
+static uint64_t workspace_or_none(const char *name, F &&bytes) noexcept
+{
+    try {
+        return bytes();
+    } catch (const std::exception &e) {
+        debug_log("%s: %s", name, e.what());
+    } catch (...) {
+    }
+    return 0;
+}
+
 }  // namespace vnpu
 
 using namespace vnpu;
@@ -264,7 +277,9 @@ VNPU_API const char *VNPU_CALL vnpu_opcode_name(uint32_t opcode)
                                   "ATTENTION_F32", "QUANTIZE_I8", "PACK_WEIGHTS_I8",
                                   "MTP_HEAD_F32", "COPY", "MEMSET", "BARRIER"};
     static const char *kv[] = {"KV_APPEND_I8", "KV_ATTENTION_I8", "KV_READ_F32"};
+    static const char *serving[] = {"MATMUL_I4", "ROPE_AXES_F32", "KV_PREFIX_ATTENTION_I8"};
     if (is_kv_opcode(opcode)) return kv[opcode - VNPU_OP_KV_APPEND_I8];
+    if (is_serving_opcode(opcode)) return serving[opcode - VNPU_OP_MATMUL_I4];
     return opcode < sizeof(names) / sizeof(names[0]) ? names[opcode] : "UNKNOWN";
 }
 
@@ -818,16 +833,24 @@ VNPU_API uint64_t VNPU_CALL vnpu_kv_attention_workspace(const vnpu_device_t *dev
                                                         const vnpu_kv_attention_i8_args_t *args)
 {
     if (!device || !args) return 0;
-    try {
-        return kv_attention_workspace(device, *args);
-    } catch (const std::exception &e) {
-        debug_log("vnpu_kv_attention_workspace: %s", e.what());
-    } catch (...) {
-    }
-    return 0;
+    return workspace_or_none("vnpu_kv_attention_workspace", [&] { return kv_attention_workspace(device, *args); });
 }
 
-// KV_* commands for callers that cannot allocate (graph capture, serving
+VNPU_API uint64_t VNPU_CALL vnpu_kv_prefix_attention_workspace(const vnpu_device_t *device,
+                                                               const vnpu_kv_prefix_attention_i8_args_t *args)
+{
+    if (!device || !args) return 0;
+    return workspace_or_none("vnpu_kv_prefix_attention_workspace",
+                             [&] { return kv_prefix_attention_workspace(device, *args); });
+}
+
+VNPU_API uint64_t VNPU_CALL vnpu_matmul_i4_workspace(const vnpu_device_t *device, const vnpu_matmul_i4_args_t *args)
+{
+    if (!device || !args) return 0;
+    return workspace_or_none("vnpu_matmul_i4_workspace", [&] { return matmul_i4_workspace(device, *args); });
+}
+
+// KV_*, MATMUL_I4 and ROPE_AXES_F32 commands for callers that cannot allocate (graph capture, serving
 // loops): checked first, then enqueued; nothing else touches the stream.
 VNPU_API vnpu_status_t VNPU_CALL vnpu_kv_enqueue_noalloc(vnpu_stream_t *stream, const vnpu_command_t *commands,
                                                          uint64_t count)
@@ -1030,7 +1053,7 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_stream_submit(vnpu_stream_t *stream,
             }
             ExecStats st;
             vnpu_status_t rc = VNPU_OK;
-            if (cmd.opcode >= VNPU_OP_COUNT && !is_kv_opcode(cmd.opcode)) {
+            if (cmd.opcode >= VNPU_OP_COUNT && !is_kv_opcode(cmd.opcode) && !is_serving_opcode(cmd.opcode)) {
                 rc = VNPU_ERR_INVALID_COMMAND;
             } else {
                 try {
@@ -1231,6 +1254,39 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_packed_weights_info(const vnpu_packed_weig
     return VNPU_OK;
 }
 
+VNPU_API vnpu_status_t VNPU_CALL vnpu_pack_weights_i4(vnpu_device_t *device, const uint8_t *B, const float *scales,
+                                                      const uint8_t *zeros, uint32_t K, uint32_t N,
+                                                      uint32_t group_size, uint32_t ldb, uint32_t trans_b,
+                                                      vnpu_packed_weights_i4_t **out_weights)
+{
+    if (!device || !B || !scales || !out_weights || !K || !N || trans_b > 1) return VNPU_ERR_INVALID_ARGUMENT;
+    *out_weights = nullptr;
+    if (group_size && group_size != 32 && group_size != 64 && group_size % 128) return VNPU_ERR_INVALID_ARGUMENT;
+    if (K > (1u << 30) || N > (1u << 30) || (ldb && ldb < ((trans_b ? K : N) + 1) / 2)) return VNPU_ERR_INVALID_ARGUMENT;
+    // 16-byte pieces of the packed codes, as many as scales of 32 codes, count in 32 bits.
+    if ((N + 15ull) / 16 * ((K + 127ull) / 128) * 64 >= (1ull << 32) - 256) return VNPU_ERR_INVALID_ARGUMENT;
+    return guard([&]() -> vnpu_status_t {
+        *out_weights = pack_weights_i4(device, B, scales, zeros, K, N, group_size, ldb, trans_b);
+        return *out_weights ? VNPU_OK : VNPU_ERR_INVALID_ARGUMENT;
+    });
+}
+
+VNPU_API void VNPU_CALL vnpu_packed_weights_i4_destroy(vnpu_packed_weights_i4_t *weights)
+{
+    destroy_packed_i4(weights);
+}
+
+VNPU_API vnpu_status_t VNPU_CALL vnpu_packed_weights_i4_info(const vnpu_packed_weights_i4_t *weights, uint32_t *K,
+                                                             uint32_t *N, uint32_t *group_size, uint64_t *bytes)
+{
+    if (!weights) return VNPU_ERR_INVALID_ARGUMENT;
+    if (K) *K = weights->K;
+    if (N) *N = weights->N;
+    if (group_size) *group_size = weights->group;
+    if (bytes) *bytes = weights->bytes;
+    return VNPU_OK;
+}
+
 // ---------------------------------------------------------------------------
 // Synchronous wrappers (reference scheduler.cpp:864-902)
 // ---------------------------------------------------------------------------
@@ -1262,6 +1318,10 @@ VNPU_SYNC_WRAPPER(vnpu_mtp_head_f32, VNPU_OP_MTP_HEAD_F32, mtp_head, vnpu_mtp_he
 VNPU_SYNC_WRAPPER(vnpu_kv_append_i8, VNPU_OP_KV_APPEND_I8, kv_append, vnpu_kv_append_i8_args_t)
 VNPU_SYNC_WRAPPER(vnpu_kv_attention_i8, VNPU_OP_KV_ATTENTION_I8, kv_attention, vnpu_kv_attention_i8_args_t)
 VNPU_SYNC_WRAPPER(vnpu_kv_read_f32, VNPU_OP_KV_READ_F32, kv_read, vnpu_kv_read_f32_args_t)
+VNPU_SYNC_WRAPPER(vnpu_matmul_i4, VNPU_OP_MATMUL_I4, matmul_i4, vnpu_matmul_i4_args_t)
+VNPU_SYNC_WRAPPER(vnpu_rope_axes_f32, VNPU_OP_ROPE_AXES_F32, rope_axes, vnpu_rope_axes_f32_args_t)
+VNPU_SYNC_WRAPPER(vnpu_kv_prefix_attention_i8, VNPU_OP_KV_PREFIX_ATTENTION_I8, kv_prefix_attention,
+                  vnpu_kv_prefix_attention_i8_args_t)
 
 #undef VNPU_SYNC_WRAPPER
 
@@ -1290,7 +1350,7 @@ VNPU_API vnpu_status_t VNPU_CALL vnpu_trace_get_summary(const vnpu_device_t *dev
     tr.resolve();
     std::memset(summary, 0, sizeof(*summary));
     std::lock_guard<std::mutex> lock(tr.mutex);
-    constexpr uint32_t kOps = VNPU_OP_KV_READ_F32 + 1;
+    constexpr uint32_t kOps = VNPU_OP_KV_PREFIX_ATTENTION_I8 + 1;
     uint64_t per_op[kOps] = {};
     for (const auto &r : tr.records) {
         summary->events++;

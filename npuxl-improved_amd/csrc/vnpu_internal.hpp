@@ -123,6 +123,18 @@ struct vnpu_packed_weights {
     std::vector<int32_t> column_sums;
 };
 
+struct vnpu_packed_weights_i4 {
+    vnpu_device_t *device = nullptr;
+    uint32_t K = 0, N = 0, group = 0;
+    uint32_t KB = 0, Np = 0;       // blocks of 128 of K, N rounded up to 16
+    uint32_t slots = 0;            // groups of a strip as stored
+    uint32_t groups_of_block = 1, blocks_of_group = 1;   // one of them is 1
+    uint8_t *codes = nullptr;      // HBM, [Np/16][KB][64][16]
+    float *scales = nullptr;       // HBM, [Np/16][slots][16]
+    uint8_t *zeros = nullptr;      // HBM, the same; null: all 8
+    uint64_t bytes = 0;
+};
+
 struct vnpu_stream {
     vnpu_device_t *device = nullptr;
     int priority = 0;
@@ -253,7 +265,15 @@ void enqueue_attention_noalloc(vnpu_stream_t *s, const vnpu_attention_f32_args_t
 void enqueue_kv_noalloc(vnpu_stream_t *s, const vnpu_command_t *commands, uint64_t count, ExecStats &st);
 // Bytes of workspace of a KV_ATTENTION_I8 call; throws ArgError where it is refused.
 uint64_t kv_attention_workspace(const vnpu_device_t *dev, const vnpu_kv_attention_i8_args_t &a);
+uint64_t kv_prefix_attention_workspace(const vnpu_device_t *dev, const vnpu_kv_prefix_attention_i8_args_t &a);
+uint64_t matmul_i4_workspace(const vnpu_device_t *dev, const vnpu_matmul_i4_args_t &a);
 inline bool is_kv_opcode(uint32_t op) { return op >= VNPU_OP_KV_APPEND_I8 && op <= VNPU_OP_KV_READ_F32; }
+// MATMUL_I4, ROPE_AXES_F32, KV_PREFIX_ATTENTION_I8.
+inline bool is_serving_opcode(uint32_t op) { return op >= VNPU_OP_MATMUL_I4 && op <= VNPU_OP_KV_PREFIX_ATTENTION_I8; }
+// Pack 4-bit weights (synchronous); host or device pointers.
+vnpu_packed_weights_i4_t *pack_weights_i4(vnpu_device_t *dev, const uint8_t *B, const float *scales, const uint8_t *zeros,
+                                          uint32_t K, uint32_t N, uint32_t group, uint32_t ldb, uint32_t trans_b);
+void destroy_packed_i4(vnpu_packed_weights_i4_t *w);
 // Pack int8 weights (synchronous); B and tile_mask may be host or device
 // pointers.  A non-null tile_mask ([ceil(K/64)][mask_ld] bytes; mask_ld 0 =
 // ceil(N/64)) packs the 64 x 64 tiles whose byte is zero as zeros.

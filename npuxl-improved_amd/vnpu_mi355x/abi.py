@@ -40,10 +40,13 @@ OP_ROPE_F32, OP_SWIGLU_F32, OP_GELU_F32, OP_ADD_F32, OP_MUL_F32 = 5, 6, 7, 8, 9
 OP_ATTENTION_F32, OP_QUANTIZE_I8, OP_PACK_WEIGHTS_I8, OP_MTP_HEAD_F32 = 10, 11, 12, 13
 OP_COPY, OP_MEMSET, OP_BARRIER, OP_COUNT = 14, 15, 16, 17
 OP_KV_APPEND_I8, OP_KV_ATTENTION_I8, OP_KV_READ_F32 = 64, 65, 66   # MI355X additive extension
+OP_MATMUL_I4, OP_ROPE_AXES_F32, OP_KV_PREFIX_ATTENTION_I8 = 80, 81, 82   # MI355X additive extension
 
 UNIT_AUTO, UNIT_VOODOO, UNIT_WILDCAT, UNIT_CELL, UNIT_GPU = 0, 1, 2, 3, 16
 EPI_NONE, EPI_RELU, EPI_SILU, EPI_GELU_TANH, EPI_GELU_ERF = 0, 1, 2, 3, 4
 ROTATE_NONE, ROTATE_HALF, ROTATE_INTERLEAVED = 0, 1, 2
+AXES_BLOCKS, AXES_TURNS = 0, 1
+AXES_ONE_LADDER, AXES_OWN_LADDERS = 0, 1
 QUANT_PER_ROW, QUANT_PER_COLUMN, QUANT_PER_TENSOR = 0, 1, 2
 COPY_H2H, COPY_H2D, COPY_D2H, COPY_D2D = 0, 1, 2, 3
 
@@ -270,6 +273,27 @@ class KvReadArgs(C.Structure):
                 ("seq_start", C.c_void_p), ("batch", C.c_uint32), ("tokens", C.c_uint32), *_strides("k", "v")]
 
 
+class MatmulI4Args(C.Structure):
+    _fields_ = [("A", C.c_void_p), ("B", C.c_void_p), ("bias", C.c_void_p), ("C", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64), ("M", C.c_uint32),
+                ("K", C.c_uint32), ("N", C.c_uint32), ("lda", C.c_uint32), ("ldc", C.c_uint32),
+                ("epilogue", C.c_uint32), ("unit", C.c_uint32), ("reserved0", C.c_uint32)]
+
+
+class RopeAxesArgs(C.Structure):
+    _fields_ = [("Q", C.c_void_p), ("Q_out", C.c_void_p), ("K", C.c_void_p), ("K_out", C.c_void_p),
+                ("positions", C.c_void_p), ("batch", C.c_uint32), ("tokens", C.c_uint32),
+                ("heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("position_ld", C.c_uint32), *_strides("q", "o", "k", "ko"), ("axes", C.c_uint32),
+                ("sections", C.c_uint32 * 4), ("order", C.c_uint32), ("ladders", C.c_uint32),
+                ("rotation", C.c_uint32), ("theta_base", C.c_float), ("scaling", C.c_float)]
+
+
+class KvPrefixAttentionArgs(C.Structure):
+    _fields_ = [("attention", KvAttentionArgs), ("prefix_table", C.c_void_p), ("prefix_len", C.c_uint32),
+                ("reserved0", C.c_uint32)]
+
+
 class _CmdArgs(C.Union):
     _fields_ = [("matmul_f32", MatmulF32Args), ("matmul_i8", MatmulI8Args),
                 ("rmsnorm", RmsnormArgs), ("softmax", SoftmaxArgs), ("rope", RopeArgs),
@@ -277,7 +301,9 @@ class _CmdArgs(C.Union):
                 ("attention", AttentionArgs), ("quantize_i8", QuantizeArgs),
                 ("pack_weights_i8", PackArgs), ("mtp_head", MtpHeadArgs),
                 ("copy", CopyArgs), ("memset", MemsetArgs), ("kv_append", KvAppendArgs),
-                ("kv_attention", KvAttentionArgs), ("kv_read", KvReadArgs), ("raw", C.c_uint8 * 192)]
+                ("kv_attention", KvAttentionArgs), ("kv_read", KvReadArgs), ("matmul_i4", MatmulI4Args),
+                ("rope_axes", RopeAxesArgs), ("kv_prefix_attention", KvPrefixAttentionArgs),
+                ("raw", C.c_uint8 * 192)]
 
 
 class Command(C.Structure):
@@ -296,6 +322,8 @@ OP_FIELD = {
     OP_MTP_HEAD_F32: ("mtp_head", MtpHeadArgs), OP_COPY: ("copy", CopyArgs),
     OP_MEMSET: ("memset", MemsetArgs), OP_KV_APPEND_I8: ("kv_append", KvAppendArgs),
     OP_KV_ATTENTION_I8: ("kv_attention", KvAttentionArgs), OP_KV_READ_F32: ("kv_read", KvReadArgs),
+    OP_MATMUL_I4: ("matmul_i4", MatmulI4Args), OP_ROPE_AXES_F32: ("rope_axes", RopeAxesArgs),
+    OP_KV_PREFIX_ATTENTION_I8: ("kv_prefix_attention", KvPrefixAttentionArgs),
 }
 
 # Every function the C ABI exports (vnpu.h:474-751, vnpu_backend.h:150):
@@ -380,6 +408,14 @@ SIGNATURES = {
     "vnpu_kv_read_f32": (st, [vp, vp]),
     "vnpu_kv_attention_workspace": (u64, [vp, vp]),
     "vnpu_kv_enqueue_noalloc": (st, [vp, vp, u64]),
+    "vnpu_pack_weights_i4": (st, [vp, vp, vp, vp, u32, u32, u32, u32, u32, vp]),   # 4-bit weights, positions with
+    "vnpu_packed_weights_i4_destroy": (None, [vp]),   # several axes, a shared prompt: MI355X additive extension
+    "vnpu_packed_weights_i4_info": (st, [vp, vp, vp, vp, vp]),
+    "vnpu_matmul_i4": (st, [vp, vp]),
+    "vnpu_rope_axes_f32": (st, [vp, vp]),
+    "vnpu_kv_prefix_attention_i8": (st, [vp, vp]),
+    "vnpu_matmul_i4_workspace": (u64, [vp, vp]),
+    "vnpu_kv_prefix_attention_workspace": (u64, [vp, vp]),
 }
 
 LAYOUT = {  # LP64 sizes measured on the reference header
@@ -388,6 +424,7 @@ LAYOUT = {  # LP64 sizes measured on the reference header
     TuneResult: 72, SpeculativeConfig: 32, SpeculativeResult: 312, ClusterConfig: 32,
     RemoteNodeConfig: 32, ClusterStats: 80, NodeConfig: 40,
     KvCache: 64, KvAppendArgs: 192, KvAttentionArgs: 168, KvReadArgs: 128,
+    MatmulI4Args: 80, RopeAxesArgs: 152, KvPrefixAttentionArgs: 184,
 }
 
 

@@ -71,6 +71,7 @@ class Session:
             raise VnpuError("vnpu_stream_create", rc)
         self._buffers: list[Buffer] = []
         self._packed: list[C.c_void_p] = []
+        self._packed_i4: list[C.c_void_p] = []
 
     # -- lifecycle -----------------------------------------------------
     def close(self) -> None:
@@ -79,9 +80,12 @@ class Session:
         self.lib.vnpu_stream_sync(self.stream)
         for w in self._packed:
             self.lib.vnpu_packed_weights_destroy(w)
+        for w in self._packed_i4:
+            self.lib.vnpu_packed_weights_i4_destroy(w)
         for b in self._buffers:
             self.lib.vnpu_buffer_free(b.handle)
         self._packed.clear()
+        self._packed_i4.clear()
         self._buffers.clear()
         self.lib.vnpu_stream_destroy(self.stream)
         self.lib.vnpu_device_destroy(self.dev)
@@ -216,3 +220,27 @@ class Session:
     def release_packed(self, w: C.c_void_p) -> None:
         self.lib.vnpu_packed_weights_destroy(w)
         self._packed = [x for x in self._packed if x is not w]
+
+    def pack_i4(self, codes: Buffer | np.ndarray, scales: Buffer | np.ndarray, K: int, N: int, group_size: int,
+                zeros: Buffer | np.ndarray | None = None, ldb: int = 0, trans_b: int = 0) -> C.c_void_p:
+        """vnpu_pack_weights_i4: codes uint8, two a byte; scales f32 and zeros uint8 [ceil(K / group_size), N]."""
+        kept = []
+
+        def pointer(x, dtype):
+            if x is None:
+                return None
+            if isinstance(x, Buffer):
+                return C.c_void_p(x.ptr)
+            kept.append(np.ascontiguousarray(x, dtype=dtype))
+            return kept[-1].ctypes.data_as(C.c_void_p)
+
+        w = C.c_void_p()
+        self.check("vnpu_pack_weights_i4", self.lib.vnpu_pack_weights_i4(
+            self.dev, pointer(codes, np.uint8), pointer(scales, np.float32), pointer(zeros, np.uint8), K, N, group_size,
+            ldb, trans_b, C.byref(w)))
+        self._packed_i4.append(w)
+        return w
+
+    def release_packed_i4(self, w: C.c_void_p) -> None:
+        self.lib.vnpu_packed_weights_i4_destroy(w)
+        self._packed_i4 = [x for x in self._packed_i4 if x is not w]
