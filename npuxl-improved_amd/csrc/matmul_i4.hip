@@ -18,6 +18,7 @@
 //   scales [Np/16][groups][16] f32, zeros the same in bytes; padding 0.
 #include "device_math.hpp"
 #include "kernels.hpp"
+#include "lds_dma.hpp"
 
 #include <algorithm>
 #include <cstdio>
@@ -28,6 +29,8 @@ namespace {
 
 using v4i = int __attribute__((ext_vector_type(4)));
 using v4f = float __attribute__((ext_vector_type(4)));
+using v2h = _Float16 __attribute__((ext_vector_type(2)));
+using v8h = _Float16 __attribute__((ext_vector_type(8)));
 
 // ---------------------------------------------------------------------------
 // Packing
@@ -324,6 +327,309 @@ void launch_few(hipStream_t s, const I4Gemm &p, uint32_t waves)
     else launch_few<RQ, T, 1>(s, p, waves);
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: bound by the matrix cores.  A row of A times a power of two, so that its
+// largest is below 2^15, is hi + lo, two f16 (22 bits, and 2^-25 where those end);
+// code - zero is exact in f16, a product with each part sums in f32, and a group's sum
+// is scaled into the result's.  A kernel splits A into fragments, operands of
+// v_mfma_f32_16x16x32_f16 as they are read: [row tile of 16][32 of K][hi, lo][64
+// lanes][8], lane (kg, row), element e the K of place order(e) among its 8.
+// ---------------------------------------------------------------------------
+
+// Place in 8 of K of a fragment's element e: the order in which codes come out of a word.
+__device__ __forceinline__ constexpr uint32_t order(uint32_t e) { return (e & 4) | (e & 1) << 1 | (e >> 1 & 1); }
+
+// A workgroup has 16 rows and a part of their blocks; it looks for the rows' largest
+// itself, in all of K.
+constexpr uint32_t kSplitThreads = 512;
+template <bool ALIGNED>
+__global__ __launch_bounds__(kSplitThreads) void matmul_i4_split(I4Gemm p, uint32_t row0, int8_t *frags, float *down)
+{
+    __shared__ uint32_t largest[16];
+    const uint32_t tid = threadIdx.x, tile = blockIdx.x;
+    if (tid < 16) largest[tid] = 0;
+    __syncthreads();
+    {
+        const uint32_t r = tid / (kSplitThreads / 16), at = tid % (kSplitThreads / 16);
+        const float *row = p.A + static_cast<uint64_t>(min(row0 + tile * 16 + r, p.M - 1)) * p.lda;
+        uint32_t most = 0;
+        if constexpr (ALIGNED) {
+#pragma unroll 4
+            for (uint32_t k = 4 * at; k < p.K; k += kSplitThreads / 4) {
+                const v4f x = *reinterpret_cast<const v4f *>(row + k);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+            }
+        } else {
+#pragma unroll 4
+            for (uint32_t k = at; k < p.K; k += kSplitThreads / 16) most = max(most, __float_as_uint(row[k]) & 0x7fffffffu);
+        }
+        for (int o = 16; o; o >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o)));
+        if (at == 0) largest[r] = most;
+    }
+    __syncthreads();
+    const uint32_t lane = tid & 63, r = lane & 15, kg = lane >> 4, most = largest[r], e = max(most >> 23, 1u);
+    // 2^(141 - e) in two factors; a row's results take it back.
+    const uint32_t up = 141 - min(e, 141u), first = min(up, 100u);
+    const float by = e <= 141 ? __uint_as_float((127 + first) << 23) : __uint_as_float((268 - min(e, 254u)) << 23);
+    const float more = __uint_as_float((127 + up - first) << 23);
+    if (blockIdx.y == 0 && tid < 16)
+        down[tile * 16 + r] = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : ldexpf(1.0f, static_cast<int>(e) - 141);
+    const float *row = p.A + static_cast<uint64_t>(min(row0 + tile * 16 + r, p.M - 1)) * p.lda;
+    const uint32_t blocks = 4 * p.KB, begin = static_cast<uint32_t>(static_cast<uint64_t>(blocks) * blockIdx.y / gridDim.y);
+    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(blocks) * (blockIdx.y + 1) / gridDim.y);
+    for (uint32_t b = begin + tid / 64; b < end; b += kSplitThreads / 64) {
+        const uint32_t k = 32 * b + 8 * kg;
+        float x[8];
+        if constexpr (ALIGNED) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const v4f v = *reinterpret_cast<const v4f *>(row + (k + 4 * i < p.K ? k + 4 * i : 0));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = row[k + i < p.K ? k + i : 0];
+        }
+        v8h hi, lo;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t at = order(i);
+            const float y = k + at < p.K ? x[at] * by * more : 0.0f;
+            const _Float16 h = static_cast<_Float16>(y);
+            hi[i] = h;
+            lo[i] = static_cast<_Float16>(y - static_cast<float>(h));
+        }
+        v8h *to = reinterpret_cast<v8h *>(frags + (static_cast<uint64_t>(tile) * blocks + b) * 2048) + lane;
+        to[0] = hi;
+        to[64] = lo;
+    }
+}
+
+// The work of a call of many rows.
+struct I4Tiles {
+    uint32_t row_tiles, col_tiles;   // workgroups' tiles
+    uint32_t splits;                 // ranges of K
+    uint32_t row0, rows;             // of this pass
+};
+
+// Codes of 32 of K: words w of a strip's block, their lower or upper halves, less zero.
+template <bool HIGH>
+__device__ __forceinline__ v8h differences(uint32_t w0, uint32_t w1, v2h zero)
+{
+    auto two = [&](uint32_t w) {
+        if constexpr (HIGH) {   // 1024 + 16 code
+            const v2h x = __builtin_bit_cast(v2h, (w & 0x00f000f0u) | 0x64006400u), sixteenth = {0.0625f16, 0.0625f16};
+            return __builtin_elementwise_fma(x, sixteenth, v2h{960.0f16, 960.0f16} - zero);
+        } else {
+            return __builtin_bit_cast(v2h, (w & 0x000f000fu) | 0x64006400u) - zero;
+        }
+    };
+    const v2h a = two(w0), b = two(w0 >> 8), c = two(w1), d = two(w1 >> 8);
+    return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+template <int RT, int CT, int GB, bool ZEROS>
+__global__ __launch_bounds__(256, RT * CT <= 16 ? 2 : 1) void matmul_i4_tile(I4Gemm p, I4Tiles tl, const int8_t *frags, const float *down, float *part)
+{
+    extern __shared__ __align__(1024) int8_t lds[];
+    constexpr uint32_t kStage = RT * 8192;
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Neighbouring tiles on one XCD, the row tiles of a column tile next to each other.
+    const uint32_t tiles = tl.row_tiles * tl.col_tiles, each = (tiles + 7) / 8, id = blockIdx.x % 8 * each + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= each || id >= tiles) return;
+    const uint32_t row_tile = id % tl.row_tiles, col_tile = id / tl.row_tiles, strips = p.Np / 16;
+    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(p.KB) * blockIdx.y / tl.splits);
+    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(p.KB) * (blockIdx.y + 1) / tl.splits);
+
+    const uint8_t *codes[CT];
+    const float *scales[CT];
+    const uint8_t *zeros[CT];
+    const uint32_t strip0 = (col_tile * 4 + wave) * CT;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+        const uint64_t strip = min(strip0 + t, strips - 1);
+        codes[t] = p.codes + strip * p.KB * 1024;
+        scales[t] = p.scales + strip * p.slots * 16;
+        zeros[t] = ZEROS ? p.zeros + strip * p.slots * 16 : nullptr;
+    }
+    const int8_t *from = frags + static_cast<uint64_t>(row_tile) * RT * p.KB * 8192;
+    auto copy = [&](uint32_t kb, int8_t *buf) {
+#pragma unroll
+        for (int i = 0; i < 2 * RT; ++i) {
+            const uint32_t piece = wave * 2 * RT + i;
+            lds::dma16_s(from + (static_cast<uint64_t>(piece / 8) * p.KB + kb) * 8192 + piece % 8 * 1024, lane * 16, buf + piece * 1024);
+        }
+    };
+    struct Block {
+        v4i codes[CT];
+        float scale[CT][GB];
+        uint32_t zero[CT][GB];
+    };
+    auto load = [&](Block &b, uint32_t kb) {
+        const uint32_t slot = GB > 1 ? GB * kb : kb / p.blocks_of_group;
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            b.codes[t] = *reinterpret_cast<const v4i *>(codes[t] + static_cast<uint64_t>(kb) * 1024 + lane * 16);
+#pragma unroll
+            for (int i = 0; i < GB; ++i) {
+                b.scale[t][i] = scales[t][(slot + i) * 16 + c];
+                b.zero[t][i] = ZEROS ? zeros[t][(slot + i) * 16 + c] : 8;
+            }
+        }
+    };
+
+    v4f total[RT][CT], acc[RT][CT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < CT; ++t) total[r][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    Block now, next;
+    copy(begin, lds);
+    load(now, begin);
+    lds::wait_vmcnt<0>();
+    __syncthreads();
+    for (uint32_t kb = begin; kb < end; ++kb) {
+        const int8_t *buf = lds + ((kb - begin) & 1) * kStage;
+        if (kb + 1 < end) {
+            copy(kb + 1, lds + ((kb + 1 - begin) & 1) * kStage);
+            load(next, kb + 1);
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            constexpr int per = 4 / GB;   // of 32 of K in a group
+            v8h b[CT];
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                const _Float16 z = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x6400 + now.zero[t][h / per]));   // 1024 + zero
+                const v2h zero = {z, z};
+                const uint32_t w0 = static_cast<uint32_t>(now.codes[t][2 * (h & 1)]), w1 = static_cast<uint32_t>(now.codes[t][2 * (h & 1) + 1]);
+                b[t] = h < 2 ? differences<false>(w0, w1, zero) : differences<true>(w0, w1, zero);
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const v8h hi = *reinterpret_cast<const v8h *>(buf + (r * 8 + 2 * h) * 1024 + lane * 16);
+                const v8h lo = *reinterpret_cast<const v8h *>(buf + (r * 8 + 2 * h + 1) * 1024 + lane * 16);
+#pragma unroll
+                for (int t = 0; t < CT; ++t)
+                    acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, b[t], h % per ? acc[r][t] : v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < CT; ++t) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, b[t], acc[r][t], 0, 0, 0);
+            }
+            if (h % per == per - 1) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int t = 0; t < CT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) total[r][t][i] = fmaf(acc[r][t][i], now.scale[t][h / per], total[r][t][i]);
+            }
+        }
+        lds::wait_vmcnt<0>();
+        __syncthreads();
+        now = next;
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const uint32_t tile_row = (row_tile * RT + r) * 16 + 4 * g;
+        const v4f by = *reinterpret_cast<const v4f *>(down + tile_row);
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            const uint32_t n = (strip0 + t) * 16 + c;
+            if (n >= p.N) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (tile_row + i >= tl.rows) continue;
+                float x = total[r][t][i] * by[i];
+                if (tl.splits > 1) {
+                    part[(static_cast<uint64_t>(blockIdx.y) * tl.rows + tile_row + i) * p.N + n] = x;
+                } else {
+                    if (p.bias) x += p.bias[n];
+                    p.C[static_cast<uint64_t>(tl.row0 + tile_row + i) * p.ldc + n] = finished(x, p.epilogue);
+                }
+            }
+        }
+    }
+}
+
+// The ranges of K together, in their order.
+__global__ __launch_bounds__(256) void matmul_i4_join(I4Gemm p, I4Tiles tl, const float *part)
+{
+    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x, all = static_cast<uint64_t>(tl.rows) * p.N;
+    if (at >= all) return;
+    float x = 0.0f;
+    for (uint32_t z = 0; z < tl.splits; ++z) x += part[z * all + at];
+    const uint32_t row = static_cast<uint32_t>(at / p.N), n = static_cast<uint32_t>(at % p.N);
+    if (p.bias) x += p.bias[n];
+    p.C[static_cast<uint64_t>(tl.row0 + row) * p.ldc + n] = finished(x, p.epilogue);
+}
+
+struct I4Plan {
+    bool tiled = false;
+    uint32_t rt = 0, ct = 0, splits = 1;
+    uint32_t pass_rows = 0;   // rows of a pass; fragments take 4 bytes an element
+    size_t frag_bytes = 0, down_bytes = 0, part_bytes = 0;
+};
+constexpr uint64_t kMostFragments = 256ull << 20;
+I4Plan plan_of(const I4Gemm &p)
+{
+    I4Plan r;
+    r.tiled = p.M > 16;
+    if (!r.tiled) return r;
+    r.rt = 4;
+    r.ct = 4;
+    const uint32_t wg_rows = 16 * r.rt;
+    const uint64_t row_bytes = 512ull * p.KB;
+    r.pass_rows = static_cast<uint32_t>(std::max<uint64_t>(1, kMostFragments / (row_bytes * wg_rows))) * wg_rows;
+    r.pass_rows = std::min(r.pass_rows, (p.M + wg_rows - 1) / wg_rows * wg_rows);
+    r.frag_bytes = static_cast<size_t>(r.pass_rows) * row_bytes;
+    r.down_bytes = static_cast<size_t>(r.pass_rows) * 4;
+    const uint64_t grid = static_cast<uint64_t>(r.pass_rows / wg_rows) * ((p.Np + 64 * r.ct - 1) / (64 * r.ct));
+    r.splits = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(1, 2 * p.cus / grid), std::max(1u, p.KB / 4)));
+    if (r.splits > 1) r.part_bytes = static_cast<size_t>(r.splits) * std::min(r.pass_rows, p.M) * p.N * 4;
+    return r;
+}
+
+template <int RT, int CT, int GB>
+void launch_tile(hipStream_t s, const I4Gemm &p, const I4Tiles &tl, const int8_t *frags, const float *down, float *part)
+{
+    constexpr uint32_t bytes = 2 * RT * 8192;
+    const auto kernel = p.zeros ? matmul_i4_tile<RT, CT, GB, true> : matmul_i4_tile<RT, CT, GB, false>;
+    if (bytes > 60 * 1024)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    kernel<<<dim3((tl.row_tiles * tl.col_tiles + 7) / 8 * 8, tl.splits), 256, bytes, s>>>(p, tl, frags, down, part);
+}
+template <int RT, int CT>
+void launch_tile(hipStream_t s, const I4Gemm &p, const I4Tiles &tl, const int8_t *frags, const float *down, float *part)
+{
+    if (p.groups_of_block == 4) launch_tile<RT, CT, 4>(s, p, tl, frags, down, part);
+    else if (p.groups_of_block == 2) launch_tile<RT, CT, 2>(s, p, tl, frags, down, part);
+    else launch_tile<RT, CT, 1>(s, p, tl, frags, down, part);
+}
+void launch_tiles(hipStream_t s, const I4Gemm &p, const I4Plan &pl, int8_t *ws)
+{
+    int8_t *frags = ws;
+    float *down = reinterpret_cast<float *>(ws + pl.frag_bytes), *part = reinterpret_cast<float *>(ws + pl.frag_bytes + (pl.down_bytes + 255) / 256 * 256);
+    const bool aligned = !((reinterpret_cast<uintptr_t>(p.A) & 15) | (p.lda & 3) | (p.K & 3));
+    for (uint32_t row0 = 0; row0 < p.M; row0 += pl.pass_rows) {
+        I4Tiles tl;
+        tl.row0 = row0;
+        tl.rows = std::min(pl.pass_rows, p.M - row0);
+        tl.row_tiles = (tl.rows + 16 * pl.rt - 1) / (16 * pl.rt);
+        tl.col_tiles = (p.Np + 64 * pl.ct - 1) / (64 * pl.ct);
+        tl.splits = pl.splits;
+        const uint32_t tiles = tl.row_tiles * pl.rt, parts = std::max(1u, std::min(2 * p.cus / tiles, p.KB / 2));
+        (aligned ? matmul_i4_split<true> : matmul_i4_split<false>)<<<dim3(tiles, parts), kSplitThreads, 0, s>>>(p, row0, frags, down);
+        launch_tile<4, 4>(s, p, tl, frags, down, part);
+        if (tl.splits > 1) {
+            const uint64_t all = static_cast<uint64_t>(tl.rows) * p.N;
+            matmul_i4_join<<<static_cast<uint32_t>((all + 255) / 256), 256, 0, s>>>(p, tl, part);
+        }
+    }
+}
+
 }  // namespace
 
 void pack_i4(hipStream_t s, const uint8_t *B, const float *scales, const uint8_t *zeros, uint32_t K, uint32_t N, uint32_t groups,
@@ -334,19 +640,35 @@ void pack_i4(hipStream_t s, const uint8_t *B, const float *scales, const uint8_t
     pack_scales<<<static_cast<uint32_t>((count + 255) / 256), 256, 0, s>>>(scales, zeros, groups, w.slots, N, w.scales, w.zeros, count, bad);
 }
 
-// A grid's work-items count in 32 bits in x, workgroups in 16 in y.
-bool matmul_i4_fits(const I4Gemm &p) { return p.Np / 16 < (1u << 22) && p.M <= 16u * 65535; }
-
-size_t matmul_i4_ws_bytes(const I4Gemm &) { return 0; }
-
-void matmul_i4(hipStream_t s, const I4Gemm &p, void *)
+// A grid's work-items count in 32 bits, workgroups in 16 in y.
+bool matmul_i4_fits(const I4Gemm &p)
 {
-    if (p.M <= 4) launch_few<1, 1>(s, p, 16);
+    const I4Plan pl = plan_of(p);
+    return p.Np / 16 < (1u << 22) && (!pl.tiled || static_cast<uint64_t>(std::min(pl.pass_rows, p.M)) * p.N < (1ull << 32) - 256);
+}
+
+size_t matmul_i4_ws_bytes(const I4Gemm &p)
+{
+    const I4Plan pl = plan_of(p);
+    return pl.tiled ? pl.frag_bytes + (pl.down_bytes + 255) / 256 * 256 + pl.part_bytes : 0;
+}
+
+void matmul_i4(hipStream_t s, const I4Gemm &p, void *ws)
+{
+    const I4Plan pl = plan_of(p);
+    if (pl.tiled) launch_tiles(s, p, pl, static_cast<int8_t *>(ws));
+    else if (p.M <= 4) launch_few<1, 1>(s, p, 16);
     else if (p.M <= 8) launch_few<2, 1>(s, p, 16);
     else launch_few<4, 1>(s, p, 16);
 }
 
-std::string matmul_i4_route(const I4Gemm &) { return "few"; }
+std::string matmul_i4_route(const I4Gemm &p)
+{
+    const I4Plan pl = plan_of(p);
+    char text[96];
+    std::snprintf(text, sizeof(text), "few=%u tile=%ux%u splits=%u", pl.tiled ? 0 : 1, 16 * pl.rt, 64 * pl.ct, pl.splits);
+    return text;
+}
 
 }  // namespace k
 }  // namespace vnpu
