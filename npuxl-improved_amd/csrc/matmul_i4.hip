@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 namespace vnpu {
 namespace k {
@@ -93,15 +94,22 @@ __device__ __forceinline__ float finished(float x, uint32_t epilogue)
 // Few rows: bound by the codes.
 // ---------------------------------------------------------------------------
 
-// Largest bits over the lanes of a row of A: 4 lanes side by side, 4 groups of 16.
-__device__ __forceinline__ uint32_t row_largest(uint32_t x)
+// Largest over the 4 groups of 16 lanes; NaN is above all.
+__device__ __forceinline__ float groups_largest(float x)
 {
-    x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0xB1, 0xf, 0xf, true)));
-    x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x4E, 0xf, 0xf, true)));
-    const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    x = max(a[0], a[1]);
-    const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    return max(b[0], b[1]);
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __builtin_elementwise_maximum(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __builtin_elementwise_maximum(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// And over 4 lanes side by side: the lanes of a row of A.
+__device__ __forceinline__ float row_largest(float x)
+{
+    auto dpp = [](float y, auto ctrl) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(y), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    x = __builtin_elementwise_maximum(x, dpp(x, std::integral_constant<int, 0xB1>()));
+    return groups_largest(__builtin_elementwise_maximum(x, dpp(x, std::integral_constant<int, 0x4E>())));
 }
 // Biased exponent e: x * 2^(157 - e) of an x no larger than these bits fits four balanced digits,
 // 127 * (2^24 + 2^16 + 2^8 + 1) = 2139062143 = 2^30 (2 - 65793 / 2^23), 0x10400 is 66560.
@@ -124,172 +132,202 @@ __device__ __forceinline__ float digits_sum(const v4i &a)
     return fmaf(static_cast<float>(a[3] * 256 + a[2]), 65536.0f, static_cast<float>(a[1] * 256 + a[0]));
 }
 
-// A workgroup has T strips and 4 RQ rows, its waves every W-th block of 128 of K.
-// GB: groups of a block (4, 2, or 1 where a group is a block or more).
-template <int RQ, int T, int GB, bool ZEROS, bool ALIGNED>
-__global__ __launch_bounds__(1024) void matmul_i4_few(I4Gemm p)
+constexpr int kBufferWord3 = 0x00020000;   // raw buffer, 32-bit data format
+constexpr uint32_t kOut = 0x80000000u;      // an offset past any buffer
+
+// Buffers over a workgroup's T strips and blocks begin .. end: what is behind them is zero.
+template <int T, int GB>
+struct Weights {
+    v4i codes[T];
+    float scale[T][GB];
+    uint32_t zero[T][GB];
+};
+template <int T, int GB, bool ZEROS>
+struct Strips {
+    __amdgpu_buffer_rsrc_t codes[T], scales[T], zeros[T];
+    uint32_t slot0, begin, of_group;
+    __device__ __forceinline__ Strips(const I4Gemm &p, uint32_t strip0, uint32_t first, uint32_t end)
+    {
+        begin = first;
+        of_group = p.blocks_of_group;
+        slot0 = slot(begin);
+        const uint32_t strips = p.Np / 16, slots = GB > 1 ? GB * (end - begin) : slot(end - 1) + 1 - slot0;
+        uint8_t *c = const_cast<uint8_t *>(p.codes) + (static_cast<uint64_t>(strip0) * p.KB + begin) * 1024;
+        const uint64_t at = (static_cast<uint64_t>(strip0) * p.slots + slot0) * 16;
+        float *s = const_cast<float *>(p.scales) + at;
+        uint8_t *z = const_cast<uint8_t *>(p.zeros) + at;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            const bool in = strip0 + t < strips;
+            codes[t] = __builtin_amdgcn_make_buffer_rsrc(c + static_cast<uint64_t>(t) * p.KB * 1024, 0, in ? (end - begin) * 1024 : 0, kBufferWord3);
+            scales[t] = __builtin_amdgcn_make_buffer_rsrc(s + static_cast<uint64_t>(t) * p.slots * 16, 0, in ? slots * 64 : 0, kBufferWord3);
+            if (ZEROS) zeros[t] = __builtin_amdgcn_make_buffer_rsrc(z + static_cast<uint64_t>(t) * p.slots * 16, 0, in ? slots * 16 : 0, kBufferWord3);
+        }
+    }
+    __device__ __forceinline__ uint32_t slot(uint32_t kb) const { return GB > 1 ? GB * kb : of_group == 1 ? kb : kb / of_group; }
+    // Block begin + at.
+    __device__ __forceinline__ void load(Weights<T, GB> &w, uint32_t at) const
+    {
+        const uint32_t lane = threadIdx.x & 63, c = lane & 15, from = slot(begin + at) - slot0;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            w.codes[t] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(codes[t], lane * 16, at * 1024, 2));   // nontemporal
+#pragma unroll
+            for (int g = 0; g < GB; ++g) {
+                w.scale[t][g] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(scales[t], c * 4, (from + g) * 64, 0));
+                w.zero[t][g] = ZEROS ? __builtin_amdgcn_raw_buffer_load_b8(zeros[t], c, (from + g) * 16, 0) : 8;
+            }
+        }
+    }
+};
+
+// A workgroup has T strips, 4 RQ rows and a range of the blocks of 128 of K, its waves every
+// W-th block of that, U of them under way.  GB: groups of a block (4, 2, or 1 where a group is
+// a block or more).  Every load is a buffer's, whose range check gives zeros behind
+// the range, the last row and K without a branch.
+template <int RQ, int T, int W, int U, int GB, bool ZEROS>
+__global__ __launch_bounds__(64 * W) void matmul_i4_few(I4Gemm p, uint32_t per, float *part)
 {
     extern __shared__ __align__(16) int8_t lds[];
     const uint32_t lane = threadIdx.x & 63, m = (lane & 15) >> 2, d = lane & 3, kg = lane >> 4, c = lane & 15;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t strip0 = blockIdx.x * T, row0 = blockIdx.y * 4 * RQ, strips = p.Np / 16;
+    const uint32_t begin = blockIdx.z * per, end = min(begin + per, p.KB);
     int8_t *mine = lds + wave * 2048;
-
-    const v4i *codes[T];
-    const float *scales[T];
-    const uint8_t *zeros[T];
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-        const uint64_t strip = min(strip0 + t, strips - 1);
-        codes[t] = reinterpret_cast<const v4i *>(p.codes + strip * p.KB * 1024) + lane;
-        scales[t] = p.scales + strip * p.slots * 16 + c;
-        zeros[t] = ZEROS ? p.zeros + strip * p.slots * 16 + c : nullptr;
-    }
-    const float *rows[RQ];
-#pragma unroll
-    for (int q = 0; q < RQ; ++q) rows[q] = p.A + static_cast<uint64_t>(min(row0 + 4 * q + m, p.M - 1)) * p.lda;
-
+    const Strips<T, GB, ZEROS> strip(p, strip0, begin, end);
+    const uint32_t rows = min(p.M - row0, 4u * RQ), last = min(p.K, 128 * end);
+    const auto a = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p.A) + static_cast<uint64_t>(row0) * p.lda, 0,
+                                                     ((rows - 1) * p.lda + p.K) * 4, kBufferWord3);
     struct Block {
-        v4i codes[T];
-        float scale[T][GB];
-        uint8_t zero[T][GB];
-        float x[RQ][8];
+        Weights<T, GB> w;
+        v4f x[RQ][2];
     };
-    // What is behind the last block is the last again; behind K, zeros times whatever was read.
-    auto load = [&](Block &b, uint32_t kb) {
-        kb = min(kb, p.KB - 1);
-        const uint32_t k = 128 * kb + 32 * d + 8 * kg;
+    auto load = [&](Block &b, uint32_t i) {   // the wave's i-th
+        const uint32_t at = wave + W * i, k = 128 * (begin + at) + 32 * d + 8 * kg;
 #pragma unroll
-        for (int q = 0; q < RQ; ++q) {
-            if constexpr (ALIGNED) {
+        for (int q = 0; q < RQ; ++q)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const v4f v = *reinterpret_cast<const v4f *>(rows[q] + (k + 4 * i < p.K ? k + 4 * i : 0));
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) b.x[q][4 * i + j] = v[j];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) b.x[q][i] = rows[q][k + i < p.K ? k + i : 0];
+            for (int j = 0; j < 2; ++j) {
+                const bool in = 4 * q + m < rows && k + 4 * j < last;
+                b.x[q][j] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(a, in ? ((4 * q + m) * p.lda + k + 4 * j) * 4 : kOut, 0, 0));
             }
-        }
-        const uint32_t slot = GB > 1 ? GB * kb : kb / p.blocks_of_group;
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            b.codes[t] = __builtin_nontemporal_load(codes[t] + static_cast<uint64_t>(kb) * 64);
-#pragma unroll
-            for (int i = 0; i < GB; ++i) {
-                b.scale[t][i] = scales[t][(slot + i) * 16];
-                b.zero[t][i] = ZEROS ? zeros[t][(slot + i) * 16] : 8;
-            }
-        }
+        strip.load(b.w, at);
     };
 
     float acc[RQ][T] = {};   // row 4 q + kg, column c
     auto of_row_kg = [&](float x) {   // as lane 4 kg has it
         return __int_as_float(__builtin_amdgcn_ds_bpermute(static_cast<int>(16 * kg), __float_as_int(x)));
     };
-    auto work = [&](const Block &b, uint32_t kb) {
+    auto work = [&](const Block &b, uint32_t i) {
         v4i low[T], high[T];
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                low[t][i] = b.codes[t][i] & 0x0f0f0f0f;
-                high[t][i] = (b.codes[t][i] >> 4) & 0x0f0f0f0f;
+            for (int j = 0; j < 4; ++j) {
+                low[t][j] = b.w.codes[t][j] & 0x0f0f0f0f;
+                high[t][j] = (b.w.codes[t][j] >> 4) & 0x0f0f0f0f;
             }
-        const uint32_t k = 128 * kb + 32 * d + 8 * kg;
+        const uint32_t kb = begin + wave + W * i;
 #pragma unroll
         for (int q = 0; q < RQ; ++q) {
             float x[8];
-            uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = k + i < p.K ? b.x[q][i] : 0.0f;
-                most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+            for (int j = 0; j < 8; ++j) x[j] = b.x[q][j / 4][j % 4];
+            if (128 * kb + 128 > p.K) {   // four that begin before K may end behind it
+                const uint32_t k = 128 * kb + 32 * d + 8 * kg;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = k + j < p.K ? x[j] : 0.0f;
             }
+            float most = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = __builtin_elementwise_maximum(most, fabsf(x[j]));
             most = row_largest(most);
             // Below 2^-96 the unit would not be a normal number: 2^96 times as large, and back at the end.
-            const bool tiny = most - 1u < 0x0f800000u - 1u, rare = __any(tiny);
+            const bool tiny = __float_as_uint(most) - 1u < 0x0f800000u - 1u, rare = __any(tiny);
             float down = 1.0f;
             if (rare) {
                 const float by = tiny ? 7.922816251426434e28f : 1.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] *= by;
-                most = tiny ? __float_as_uint(__uint_as_float(most) * by) : most;
+                for (int j = 0; j < 8; ++j) x[j] *= by;
+                most *= by;
                 down = of_row_kg(tiny ? 1.262177448353619e-29f : 1.0f);
             }
-            const uint32_t e = digits_exponent(most);
+            const uint32_t e = digits_exponent(__float_as_uint(most));
             const float up = __uint_as_float((284u - e) << 23);
             uint32_t u[8], plane[2][4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                u[i] = (static_cast<uint32_t>(static_cast<int>(rintf(x[i] * up))) + 0x80808080u) ^ 0x80808080u;   // bytes: balanced digits
+            for (int j = 0; j < 8; ++j)
+                u[j] = (static_cast<uint32_t>(static_cast<int>(rintf(x[j] * up))) + 0x80808080u) ^ 0x80808080u;   // bytes: balanced digits
             planes_of(u, plane[0]);
             planes_of(u + 4, plane[1]);
             // Lane (m, d, kg) has 8 of K and all digits; as an operand it wants digit d of 32 of K.
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<uint2 *>(mine + ((m * 4 + i) * 4 + kg) * 32 + d * 8) = make_uint2(plane[0][i], plane[1][i]);
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint2 *>(mine + ((m * 4 + j) * 4 + kg) * 32 + d * 8) = make_uint2(plane[0][j], plane[1][j]);
             __builtin_amdgcn_wave_barrier();
             const v4i a0 = *reinterpret_cast<const v4i *>(mine + (c * 4 + kg) * 32), a1 = *reinterpret_cast<const v4i *>(mine + (c * 4 + kg) * 32 + 16);
             __builtin_amdgcn_wave_barrier();
-            const float own = most >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((e - 30u) << 23);
-            const float unit = of_row_kg(own);
-            const v4i ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101}, none = {0, 0, 0, 0};
+            const float unit = of_row_kg(__float_as_uint(most) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((e - 30u) << 23));
+            // Less the digits' sum, times the zero: 8 where there are none.
+            const int less = ZEROS ? -1 : static_cast<int>(0xf8f8f8f8u);
+            const v4i minus = {less, less, less, less}, none = {0, 0, 0, 0};
             auto product = [&](const v4i &x, const v4i &y, const v4i &s) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(x, y, s, 0, 0, 0); };
-            auto half = [&](const v4i &x, const v4i &y, int i, const v4i &s) {
-                const long xs = static_cast<long>(static_cast<uint32_t>(x[2 * i])) | static_cast<long>(x[2 * i + 1]) << 32;
-                const long ys = static_cast<long>(static_cast<uint32_t>(y[2 * i])) | static_cast<long>(y[2 * i + 1]) << 32;
+            auto half = [&](const v4i &x, const v4i &y, int j, const v4i &s) {
+                const long xs = static_cast<long>(static_cast<uint32_t>(x[2 * j])) | static_cast<long>(x[2 * j + 1]) << 32;
+                const long ys = static_cast<long>(static_cast<uint32_t>(y[2 * j])) | static_cast<long>(y[2 * j + 1]) << 32;
                 return __builtin_amdgcn_mfma_i32_16x16x32_i8(xs, ys, s, 0, 0, 0);
             };
-            auto less = [&](const v4i &sums, int zero) {
-                v4i r;
+            auto first = [&](const v4i &sums, uint32_t zero) {
+                v4i r = sums;
+                if (ZEROS)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = __mul24(sums[i], -zero);
+                    for (int j = 0; j < 4; ++j) r[j] = __mul24(sums[j], static_cast<int>(zero));
                 return r;
             };
             v4i sums[GB];
             if constexpr (GB == 1) {
-                sums[0] = product(a1, ones, product(a0, ones, none));
+                sums[0] = product(a1, minus, product(a0, minus, none));
             } else if constexpr (GB == 2) {
-                sums[0] = product(a0, ones, none);
-                sums[1] = product(a1, ones, none);
+                sums[0] = product(a0, minus, none);
+                sums[1] = product(a1, minus, none);
             } else {
-                sums[0] = half(a0, ones, 0, none);
-                sums[1] = half(a0, ones, 1, none);
-                sums[2] = half(a1, ones, 0, none);
-                sums[3] = half(a1, ones, 1, none);
+                sums[0] = half(a0, minus, 0, none);
+                sums[1] = half(a0, minus, 1, none);
+                sums[2] = half(a1, minus, 0, none);
+                sums[3] = half(a1, minus, 1, none);
             }
 #pragma unroll
             for (int t = 0; t < T; ++t) {
                 v4i r[GB];
                 if constexpr (GB == 1) {
-                    r[0] = product(a1, high[t], product(a0, low[t], less(sums[0], b.zero[t][0])));
+                    r[0] = product(a1, high[t], product(a0, low[t], first(sums[0], b.w.zero[t][0])));
                 } else if constexpr (GB == 2) {
-                    r[0] = product(a0, low[t], less(sums[0], b.zero[t][0]));
-                    r[1] = product(a1, high[t], less(sums[1], b.zero[t][1]));
+                    r[0] = product(a0, low[t], first(sums[0], b.w.zero[t][0]));
+                    r[1] = product(a1, high[t], first(sums[1], b.w.zero[t][1]));
                 } else {
-                    r[0] = half(a0, low[t], 0, less(sums[0], b.zero[t][0]));
-                    r[1] = half(a0, low[t], 1, less(sums[1], b.zero[t][1]));
-                    r[2] = half(a1, high[t], 0, less(sums[2], b.zero[t][2]));
-                    r[3] = half(a1, high[t], 1, less(sums[3], b.zero[t][3]));
+                    r[0] = half(a0, low[t], 0, first(sums[0], b.w.zero[t][0]));
+                    r[1] = half(a0, low[t], 1, first(sums[1], b.w.zero[t][1]));
+                    r[2] = half(a1, high[t], 0, first(sums[2], b.w.zero[t][2]));
+                    r[3] = half(a1, high[t], 1, first(sums[3], b.w.zero[t][3]));
                 }
 #pragma unroll
-                for (int i = 0; i < GB; ++i) {
-                    float x = digits_sum(r[i]);
+                for (int g = 0; g < GB; ++g) {
+                    float x = digits_sum(r[g]);
                     if (rare) x *= down;
-                    acc[q][t] = fmaf(x, unit * b.scale[t][i], acc[q][t]);
+                    acc[q][t] = fmaf(x, unit * b.w.scale[t][g], acc[q][t]);
                 }
             }
         }
     };
-    Block now, next;
-    if (wave < p.KB) load(now, wave);
-    for (uint32_t kb = wave; kb < p.KB; kb += W) {
-        load(next, kb + W);
-        work(now, kb);
-        now = next;
+    Block ring[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) load(ring[j], j);
+    for (uint32_t i = 0; wave + W * i < end - begin; i += U) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (j == 0 || wave + W * (i + j) < end - begin) work(ring[j], i + j);
+            load(ring[j], i + j + U);
+        }
     }
     // The waves' sums together, in the waves' order.
     __syncthreads();
@@ -299,32 +337,228 @@ __global__ __launch_bounds__(1024) void matmul_i4_few(I4Gemm p)
 #pragma unroll
         for (int t = 0; t < T; ++t) sums[(wave * RQ * T + q * T + t) * 64 + lane] = acc[q][t];
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < RQ * T * 64; e += blockDim.x) {
+    for (uint32_t e = threadIdx.x; e < RQ * T * 64; e += 64 * W) {
         const uint32_t q = e / (T * 64), row = row0 + 4 * q + (e >> 4 & 3), n = (strip0 + e / 64 % T) * 16 + (e & 15);
         if (row >= p.M || n >= p.N) continue;
         float x = 0.0f;
+#pragma unroll
         for (uint32_t w = 0; w < W; ++w) x += sums[w * RQ * T * 64 + e];
-        if (p.bias) x += p.bias[n];
-        p.C[static_cast<uint64_t>(row) * p.ldc + n] = finished(x, p.epilogue);
+        if (part) {
+            part[(static_cast<uint64_t>(blockIdx.z) * p.M + row) * p.N + n] = x;
+        } else {
+            if (p.bias) x += p.bias[n];
+            p.C[static_cast<uint64_t>(row) * p.ldc + n] = finished(x, p.epilogue);
+        }
     }
 }
 
-template <int RQ, int T, int GB>
-void launch_few(hipStream_t s, const I4Gemm &p, uint32_t waves)
+// per: blocks of a range of K; part: where their sums go if there is more than one.
+template <int RQ, int T, int W, int U, int GB>
+void launch_few(hipStream_t s, const I4Gemm &p, uint32_t per, float *part)
 {
-    const dim3 grid((p.Np / 16 + T - 1) / T, (p.M + 4 * RQ - 1) / (4 * RQ));
-    const uint32_t bytes = std::max<uint32_t>(waves * 2048, waves * RQ * T * 256);
-    const bool aligned = !((reinterpret_cast<uintptr_t>(p.A) & 15) | (p.lda & 3) | (p.K & 3));
-    const auto kernel = p.zeros ? (aligned ? matmul_i4_few<RQ, T, GB, true, true> : matmul_i4_few<RQ, T, GB, true, false>)
-                                : (aligned ? matmul_i4_few<RQ, T, GB, false, true> : matmul_i4_few<RQ, T, GB, false, false>);
-    kernel<<<grid, 64 * waves, bytes, s>>>(p);
+    const dim3 grid((p.Np / 16 + T - 1) / T, (p.M + 4 * RQ - 1) / (4 * RQ), (p.KB + per - 1) / per);
+    constexpr uint32_t bytes = W * (RQ * T > 8 ? RQ * T * 256 : 2048);
+    const auto kernel = p.zeros ? matmul_i4_few<RQ, T, W, U, GB, true> : matmul_i4_few<RQ, T, W, U, GB, false>;
+    kernel<<<grid, 64 * W, bytes, s>>>(p, per, part);
 }
-template <int RQ, int T>
-void launch_few(hipStream_t s, const I4Gemm &p, uint32_t waves)
+template <int RQ, int T, int W, int U>
+void launch_few(hipStream_t s, const I4Gemm &p, uint32_t per, float *part)
 {
-    if (p.groups_of_block == 4) launch_few<RQ, T, 4>(s, p, waves);
-    else if (p.groups_of_block == 2) launch_few<RQ, T, 2>(s, p, waves);
-    else launch_few<RQ, T, 1>(s, p, waves);
+    if (p.groups_of_block == 4) launch_few<RQ, T, W, U, 4>(s, p, per, part);
+    else if (p.groups_of_block == 2) launch_few<RQ, T, W, U, 2>(s, p, per, part);
+    else launch_few<RQ, T, W, U, 1>(s, p, per, part);
+}
+
+// ---------------------------------------------------------------------------
+// Tens of rows: a row's 128 of K times a power of two, so that their largest is below
+// 2^15, are hi + lo, two f16 (22 bits, and 2^-25 where those end); code - zero is exact in
+// f16, and v_mfma_f32_16x16x32_f16 sums the products with each part in f32.  A lane has
+// the f32 values that it needs as operands, so nothing goes through LDS, and 16 rows take
+// one product where whole numbers of 4 digits take four.
+// ---------------------------------------------------------------------------
+
+// Place in 8 of K of a fragment's element e: the order in which codes come out of a word.
+__device__ __forceinline__ constexpr uint32_t order(uint32_t e) { return (e & 4) | (e & 1) << 1 | (e >> 1 & 1); }
+
+// Codes of 32 of K: words w of a strip's block, their lower or upper halves, less zero.
+template <bool HIGH>
+__device__ __forceinline__ v8h differences(uint32_t w0, uint32_t w1, v2h zero)
+{
+    auto two = [&](uint32_t w) {
+        if constexpr (HIGH) {   // 1024 + 16 code
+            const v2h x = __builtin_bit_cast(v2h, (w & 0x00f000f0u) | 0x64006400u), sixteenth = {0.0625f16, 0.0625f16};
+            return __builtin_elementwise_fma(x, sixteenth, v2h{960.0f16, 960.0f16} - zero);
+        } else {
+            return __builtin_bit_cast(v2h, (w & 0x000f000fu) | 0x64006400u) - zero;
+        }
+    };
+    const v2h a = two(w0), b = two(w0 >> 8), c = two(w1), d = two(w1 >> 8);
+    return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+using v2f = float __attribute__((ext_vector_type(2)));
+
+// A workgroup has T strips, 16 RT rows and a range of the blocks of K, its waves every W-th.
+template <int RT, int T, int W, int GB, bool ZEROS>
+__global__ __launch_bounds__(64 * W) void matmul_i4_mid(I4Gemm p, uint32_t per, float *part)
+{
+    extern __shared__ __align__(16) int8_t lds[];
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t strip0 = blockIdx.x * T, row0 = blockIdx.y * 16 * RT;
+    const uint32_t begin = blockIdx.z * per, end = min(begin + per, p.KB);
+    const Strips<T, GB, ZEROS> strip(p, strip0, begin, end);
+    const uint32_t rows = min(p.M - row0, 16u * RT), last = min(p.K, 128 * end);
+    const auto a = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p.A) + static_cast<uint64_t>(row0) * p.lda, 0,
+                                                     ((rows - 1) * p.lda + p.K) * 4, kBufferWord3);
+    struct Block {
+        Weights<T, GB> w;
+        v4f x[RT][4][2];
+    };
+    auto load = [&](Block &b, uint32_t i) {
+        const uint32_t at = wave + W * i, k = 128 * (begin + at) + 8 * g;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const bool in = 16 * r + c < rows && k + 32 * h + 4 * j < last;
+                    b.x[r][h][j] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(a, in ? ((16 * r + c) * p.lda + k + 32 * h + 4 * j) * 4 : kOut, 0, 0));
+                }
+        strip.load(b.w, at);
+    };
+    v4f total[RT][T];   // rows 16 r + 4 g + i, column c
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < T; ++t) total[r][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    auto work = [&](const Block &b, uint32_t i) {
+        const uint32_t kb = begin + wave + W * i;
+        v8h hi[RT][4], lo[RT][4];
+        float unit[RT][4], down[RT][4];
+        bool rare = false;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            float x[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = b.x[r][j / 8][j / 4 % 2][j % 4];
+            if (128 * kb + 128 > p.K) {   // four that begin before K may end behind it
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = 128 * kb + 32 * (j / 8) + 8 * g + j % 8 < p.K ? x[j] : 0.0f;
+            }
+            float most = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) most = __builtin_elementwise_maximum(most, fabsf(x[j]));
+            most = groups_largest(most);
+            // As for few rows.
+            const bool tiny = __float_as_uint(most) - 1u < 0x0f800000u - 1u;
+            if (__any(tiny)) {
+                const float by = tiny ? 7.922816251426434e28f : 1.0f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] *= by;
+                most *= by;
+                rare = true;
+            }
+            const uint32_t e = max(__float_as_uint(most) >> 23, 31u);
+            const float up = __uint_as_float((268u - min(e, 254u)) << 23);   // 2^(141 - e)
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const v2f y = {x[8 * h + order(j)] * up, x[8 * h + order(j + 1)] * up};
+                    const v2h top = __builtin_convertvector(y, v2h), rest = __builtin_convertvector(y - __builtin_convertvector(top, v2f), v2h);
+                    hi[r][h][j] = top[0];
+                    hi[r][h][j + 1] = top[1];
+                    lo[r][h][j] = rest[0];
+                    lo[r][h][j + 1] = rest[1];
+                }
+            // Of rows 4 g + i: lane 4 g + i has row 4 g + i.
+            const float own = __float_as_uint(most) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((e - 14u) << 23);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int from = static_cast<int>(4 * (4 * g + j));
+                unit[r][j] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(own)));
+                down[r][j] = rare ? __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(tiny ? 1.262177448353619e-29f : 1.0f))) : 1.0f;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            v4f acc[RT], sum[RT];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                constexpr int of = 4 / GB;   // of 32 of K in a group
+                const _Float16 z = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x6400 + b.w.zero[t][h / of]));   // 1024 + zero
+                const uint32_t w0 = static_cast<uint32_t>(b.w.codes[t][2 * (h & 1)]), w1 = static_cast<uint32_t>(b.w.codes[t][2 * (h & 1) + 1]);
+                const v8h w = h < 2 ? differences<false>(w0, w1, v2h{z, z}) : differences<true>(w0, w1, v2h{z, z});
+#pragma unroll
+                for (int r = 0; r < RT; ++r) acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[r][h], w, h % of ? acc[r] : v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[r][h], w, acc[r], 0, 0, 0);
+                if (h % of == of - 1)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sum[r][j] = h == of - 1 ? acc[r][j] * b.w.scale[t][0] : fmaf(acc[r][j], b.w.scale[t][h / of], sum[r][j]);
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (rare) sum[r][j] *= down[r][j];
+                    total[r][t][j] = fmaf(sum[r][j], unit[r][j], total[r][t][j]);
+                }
+        }
+    };
+    Block block;
+    load(block, 0);
+    for (uint32_t i = 0; wave + W * i < end - begin; ++i) {
+        work(block, i);
+        load(block, i + 1);
+    }
+    // The waves' sums together, in the waves' order.
+    v4f *sums = reinterpret_cast<v4f *>(lds);
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < T; ++t) sums[((wave * RT + r) * T + t) * 64 + lane] = total[r][t];
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < RT * T * 64; e += 64 * W) {
+        const uint32_t n = (strip0 + e / 64 % T) * 16 + (e & 15), row = row0 + 16 * (e / (64 * T)) + 4 * (e >> 4 & 3);
+        if (n >= p.N) continue;
+        v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t w = 0; w < W; ++w) x += sums[w * RT * T * 64 + e];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (row + j >= p.M) continue;
+            if (part) {
+                part[(static_cast<uint64_t>(blockIdx.z) * p.M + row + j) * p.N + n] = x[j];
+            } else {
+                float y = x[j];
+                if (p.bias) y += p.bias[n];
+                p.C[static_cast<uint64_t>(row + j) * p.ldc + n] = finished(y, p.epilogue);
+            }
+        }
+    }
+}
+
+template <int RT, int T, int W, int GB>
+void launch_mid(hipStream_t s, const I4Gemm &p, uint32_t per, float *part)
+{
+    const dim3 grid((p.Np / 16 + T - 1) / T, (p.M + 16 * RT - 1) / (16 * RT), (p.KB + per - 1) / per);
+    constexpr uint32_t bytes = W * RT * T * 1024;
+    const auto kernel = p.zeros ? matmul_i4_mid<RT, T, W, GB, true> : matmul_i4_mid<RT, T, W, GB, false>;
+    if (bytes > 60 * 1024)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    kernel<<<grid, 64 * W, bytes, s>>>(p, per, part);
+}
+template <int RT, int T, int W>
+void launch_mid(hipStream_t s, const I4Gemm &p, uint32_t per, float *part)
+{
+    if (p.groups_of_block == 4) launch_mid<RT, T, W, 4>(s, p, per, part);
+    else if (p.groups_of_block == 2) launch_mid<RT, T, W, 2>(s, p, per, part);
+    else launch_mid<RT, T, W, 1>(s, p, per, part);
 }
 
 // ---------------------------------------------------------------------------
@@ -335,9 +569,6 @@ void launch_few(hipStream_t s, const I4Gemm &p, uint32_t waves)
 // v_mfma_f32_16x16x32_f16 as they are read: [row tile of 16][32 of K][hi, lo][64
 // lanes][8], lane (kg, row), element e the K of place order(e) among its 8.
 // ---------------------------------------------------------------------------
-
-// Place in 8 of K of a fragment's element e: the order in which codes come out of a word.
-__device__ __forceinline__ constexpr uint32_t order(uint32_t e) { return (e & 4) | (e & 1) << 1 | (e >> 1 & 1); }
 
 // A workgroup has 16 rows and a part of their blocks; it looks for the rows' largest
 // itself, in all of K.
@@ -413,22 +644,6 @@ struct I4Tiles {
     uint32_t splits;                 // ranges of K
     uint32_t row0, rows;             // of this pass
 };
-
-// Codes of 32 of K: words w of a strip's block, their lower or upper halves, less zero.
-template <bool HIGH>
-__device__ __forceinline__ v8h differences(uint32_t w0, uint32_t w1, v2h zero)
-{
-    auto two = [&](uint32_t w) {
-        if constexpr (HIGH) {   // 1024 + 16 code
-            const v2h x = __builtin_bit_cast(v2h, (w & 0x00f000f0u) | 0x64006400u), sixteenth = {0.0625f16, 0.0625f16};
-            return __builtin_elementwise_fma(x, sixteenth, v2h{960.0f16, 960.0f16} - zero);
-        } else {
-            return __builtin_bit_cast(v2h, (w & 0x000f000fu) | 0x64006400u) - zero;
-        }
-    };
-    const v2h a = two(w0), b = two(w0 >> 8), c = two(w1), d = two(w1 >> 8);
-    return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 
 template <int RT, int CT, int GB, bool ZEROS>
 __global__ __launch_bounds__(256, RT * CT <= 16 ? 2 : 1) void matmul_i4_tile(I4Gemm p, I4Tiles tl, const int8_t *frags, const float *down, float *part)
@@ -576,7 +791,7 @@ constexpr uint64_t kMostFragments = 256ull << 20;
 I4Plan plan_of(const I4Gemm &p)
 {
     I4Plan r;
-    r.tiled = p.M > 16;
+    r.tiled = p.M > 64;
     if (!r.tiled) return r;
     r.rt = 4;
     r.ct = 4;
@@ -657,9 +872,10 @@ void matmul_i4(hipStream_t s, const I4Gemm &p, void *ws)
 {
     const I4Plan pl = plan_of(p);
     if (pl.tiled) launch_tiles(s, p, pl, static_cast<int8_t *>(ws));
-    else if (p.M <= 4) launch_few<1, 1>(s, p, 16);
-    else if (p.M <= 8) launch_few<2, 1>(s, p, 16);
-    else launch_few<4, 1>(s, p, 16);
+    else if (p.M <= 4) launch_few<1, 1, 16, 1>(s, p, p.KB, nullptr);
+    else if (p.M <= 8) launch_few<2, 1, 16, 1>(s, p, p.KB, nullptr);
+    else if (p.M <= 16) launch_mid<1, 2, 8>(s, p, p.KB, nullptr);
+    else launch_mid<2, 2, 8>(s, p, p.KB, nullptr);
 }
 
 std::string matmul_i4_route(const I4Gemm &p)
