@@ -1295,7 +1295,8 @@ void exec_kv(vnpu_stream_t *s, const vnpu_command_t &cmd, ExecStats &st)
 // checked and staged as the KV commands are.
 // ---------------------------------------------------------------------------
 
-k::I4Gemm matmul_i4_params(vnpu_stream_t *s, const vnpu_matmul_i4_args_t &a, const KvSource &src)
+// look: at the weights; without it they are any of these sizes, with groups of 128.
+k::I4Gemm matmul_i4_params(vnpu_stream_t *s, const vnpu_matmul_i4_args_t &a, const KvSource &src, bool look = true)
 {
     const vnpu_packed_weights_i4_t *w = a.B;
     require(a.A && w && a.C && a.M && a.K && a.N, "invalid matmul_i4 arguments");
@@ -1309,19 +1310,18 @@ k::I4Gemm matmul_i4_params(vnpu_stream_t *s, const vnpu_matmul_i4_args_t &a, con
     p.Np = cdiv(a.N, 16u) * 16;
     p.epilogue = a.epilogue;
     p.cus = s->device ? std::max(1u, s->device->cu_count) : 256;
-    require(a.K <= (1u << 30) && a.N <= (1u << 30) && k::matmul_i4_fits(p), "matmul_i4 too large");
-    if (src.sizes_only) {
-        p.A = a.A;
-        return p;
+    if (look) {
+        require(w->K == a.K && w->N == a.N, "packed weight shape mismatch");
+        require(w->device->hip_device == s->device->hip_device, "packed weights live on another device");
+        p.codes = w->codes;
+        p.scales = w->scales;
+        p.zeros = w->zeros;
+        p.slots = w->slots;
+        p.groups_of_block = w->groups_of_block;
+        p.blocks_of_group = w->blocks_of_group;
     }
-    require(w->K == a.K && w->N == a.N, "packed weight shape mismatch");
-    require(w->device->hip_device == s->device->hip_device, "packed weights live on another device");
-    p.codes = w->codes;
-    p.scales = w->scales;
-    p.zeros = w->zeros;
-    p.slots = w->slots;
-    p.groups_of_block = w->groups_of_block;
-    p.blocks_of_group = w->blocks_of_group;
+    require(a.M <= (1u << 28) && a.K <= (1u << 30) && a.N <= (1u << 30) && k::matmul_i4_lay_out(p), "matmul_i4 too large");
+    if (src.sizes_only) return p;
     p.A = src.in(a.A, static_cast<uint64_t>(a.M - 1) * p.lda + a.K);
     p.bias = src.in(a.bias, a.N);
     p.C = src.out(a.C, static_cast<uint64_t>(a.M - 1) * p.ldc + a.N);
@@ -1912,7 +1912,7 @@ extern "C" VNPU_API int32_t VNPU_CALL vnpu_debug_route(const vnpu_command_t *cmd
         }
         if (cmd->opcode == VNPU_OP_MATMUL_I4) {   // the weights are not looked at
             vnpu_stream_t on;
-            const vnpu::k::I4Gemm p = vnpu::matmul_i4_params(&on, cmd->args.matmul_i4, {nullptr, true});
+            const vnpu::k::I4Gemm p = vnpu::matmul_i4_params(&on, cmd->args.matmul_i4, {nullptr, true}, false);
             std::snprintf(out, size, "%s ws=%zu", vnpu::k::matmul_i4_route(p).c_str(), vnpu::k::matmul_i4_ws_bytes(p));
             return VNPU_OK;
         }

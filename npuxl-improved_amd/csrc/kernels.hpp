@@ -336,9 +336,15 @@ struct I4Gemm {
     uint32_t groups_of_block = 1, blocks_of_group = 1;   // one of them is 1
     uint32_t M = 0, K = 0, N = 0, lda = 0, ldc = 0, epilogue = 0;
     uint32_t cus = 256;
+    // The kernel and how the work is cut (matmul_i4_lay_out).
+    enum : uint32_t { kFew, kMid, kTile } kernel = kFew;
+    uint32_t rows = 0, strips = 0, waves = 0;   // of a workgroup: quads or tiles of 16 rows, strips of a wave or workgroup
+    uint32_t per = 0, splits = 1;               // blocks of a range of K, ranges
+    uint32_t pass_rows = 0;                     // of A in fragments at a time
 };
-// ws holds matmul_i4_ws_bytes(p) bytes (0: none is used).
-bool matmul_i4_fits(const I4Gemm &p);
+// Chooses the kernel; false: too large.
+bool matmul_i4_lay_out(I4Gemm &p);
+// Of a call that is laid out: ws holds matmul_i4_ws_bytes(p) bytes (0: none is used).
 size_t matmul_i4_ws_bytes(const I4Gemm &p);
 void matmul_i4(hipStream_t s, const I4Gemm &p, void *ws);
 std::string matmul_i4_route(const I4Gemm &p);

@@ -21,6 +21,7 @@
 #include "lds_dma.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <type_traits>
 
@@ -182,10 +183,10 @@ struct Strips {
 };
 
 // A workgroup has T strips, 4 RQ rows and a range of the blocks of 128 of K, its waves every
-// W-th block of that, U of them under way.  GB: groups of a block (4, 2, or 1 where a group is
+// W-th block of that.  GB: groups of a block (4, 2, or 1 where a group is
 // a block or more).  Every load is a buffer's, whose range check gives zeros behind
 // the range, the last row and K without a branch.
-template <int RQ, int T, int W, int U, int GB, bool ZEROS>
+template <int RQ, int T, int W, int GB, bool ZEROS>
 __global__ __launch_bounds__(64 * W) void matmul_i4_few(I4Gemm p, uint32_t per, float *part)
 {
     extern __shared__ __align__(16) int8_t lds[];
@@ -319,15 +320,11 @@ __global__ __launch_bounds__(64 * W) void matmul_i4_few(I4Gemm p, uint32_t per, 
             }
         }
     };
-    Block ring[U];
-#pragma unroll
-    for (int j = 0; j < U; ++j) load(ring[j], j);
-    for (uint32_t i = 0; wave + W * i < end - begin; i += U) {
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            if (j == 0 || wave + W * (i + j) < end - begin) work(ring[j], i + j);
-            load(ring[j], i + j + U);
-        }
+    Block block;
+    load(block, 0);
+    for (uint32_t i = 0; wave + W * i < end - begin; ++i) {
+        work(block, i);
+        load(block, i + 1);
     }
     // The waves' sums together, in the waves' order.
     __syncthreads();
@@ -352,21 +349,21 @@ __global__ __launch_bounds__(64 * W) void matmul_i4_few(I4Gemm p, uint32_t per, 
     }
 }
 
-// per: blocks of a range of K; part: where their sums go if there is more than one.
-template <int RQ, int T, int W, int U, int GB>
-void launch_few(hipStream_t s, const I4Gemm &p, uint32_t per, float *part)
+// part: where the sums of ranges of K go, null if there is one range.
+template <int RQ, int T, int W, int GB>
+void launch_few(hipStream_t s, const I4Gemm &p, float *part)
 {
-    const dim3 grid((p.Np / 16 + T - 1) / T, (p.M + 4 * RQ - 1) / (4 * RQ), (p.KB + per - 1) / per);
+    const dim3 grid((p.Np / 16 + T - 1) / T, (p.M + 4 * RQ - 1) / (4 * RQ), p.splits);
     constexpr uint32_t bytes = W * (RQ * T > 8 ? RQ * T * 256 : 2048);
-    const auto kernel = p.zeros ? matmul_i4_few<RQ, T, W, U, GB, true> : matmul_i4_few<RQ, T, W, U, GB, false>;
-    kernel<<<grid, 64 * W, bytes, s>>>(p, per, part);
+    const auto kernel = p.zeros ? matmul_i4_few<RQ, T, W, GB, true> : matmul_i4_few<RQ, T, W, GB, false>;
+    kernel<<<grid, 64 * W, bytes, s>>>(p, p.per, part);
 }
-template <int RQ, int T, int W, int U>
-void launch_few(hipStream_t s, const I4Gemm &p, uint32_t per, float *part)
+template <int RQ, int T, int W>
+void launch_few(hipStream_t s, const I4Gemm &p, float *part)
 {
-    if (p.groups_of_block == 4) launch_few<RQ, T, W, U, 4>(s, p, per, part);
-    else if (p.groups_of_block == 2) launch_few<RQ, T, W, U, 2>(s, p, per, part);
-    else launch_few<RQ, T, W, U, 1>(s, p, per, part);
+    if (p.groups_of_block == 4) launch_few<RQ, T, W, 4>(s, p, part);
+    else if (p.groups_of_block == 2) launch_few<RQ, T, W, 2>(s, p, part);
+    else launch_few<RQ, T, W, 1>(s, p, part);
 }
 
 // ---------------------------------------------------------------------------
@@ -544,21 +541,21 @@ __global__ __launch_bounds__(64 * W) void matmul_i4_mid(I4Gemm p, uint32_t per, 
 }
 
 template <int RT, int T, int W, int GB>
-void launch_mid(hipStream_t s, const I4Gemm &p, uint32_t per, float *part)
+void launch_mid(hipStream_t s, const I4Gemm &p, float *part)
 {
-    const dim3 grid((p.Np / 16 + T - 1) / T, (p.M + 16 * RT - 1) / (16 * RT), (p.KB + per - 1) / per);
+    const dim3 grid((p.Np / 16 + T - 1) / T, (p.M + 16 * RT - 1) / (16 * RT), p.splits);
     constexpr uint32_t bytes = W * RT * T * 1024;
     const auto kernel = p.zeros ? matmul_i4_mid<RT, T, W, GB, true> : matmul_i4_mid<RT, T, W, GB, false>;
     if (bytes > 60 * 1024)
         (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    kernel<<<grid, 64 * W, bytes, s>>>(p, per, part);
+    kernel<<<grid, 64 * W, bytes, s>>>(p, p.per, part);
 }
 template <int RT, int T, int W>
-void launch_mid(hipStream_t s, const I4Gemm &p, uint32_t per, float *part)
+void launch_mid(hipStream_t s, const I4Gemm &p, float *part)
 {
-    if (p.groups_of_block == 4) launch_mid<RT, T, W, 4>(s, p, per, part);
-    else if (p.groups_of_block == 2) launch_mid<RT, T, W, 2>(s, p, per, part);
-    else launch_mid<RT, T, W, 1>(s, p, per, part);
+    if (p.groups_of_block == 4) launch_mid<RT, T, W, 4>(s, p, part);
+    else if (p.groups_of_block == 2) launch_mid<RT, T, W, 2>(s, p, part);
+    else launch_mid<RT, T, W, 1>(s, p, part);
 }
 
 // ---------------------------------------------------------------------------
@@ -641,7 +638,7 @@ __global__ __launch_bounds__(kSplitThreads) void matmul_i4_split(I4Gemm p, uint3
 // The work of a call of many rows.
 struct I4Tiles {
     uint32_t row_tiles, col_tiles;   // workgroups' tiles
-    uint32_t splits;                 // ranges of K
+    uint32_t splits, per;            // ranges of K, blocks of a range
     uint32_t row0, rows;             // of this pass
 };
 
@@ -656,8 +653,7 @@ __global__ __launch_bounds__(256, RT * CT <= 16 ? 2 : 1) void matmul_i4_tile(I4G
     const uint32_t tiles = tl.row_tiles * tl.col_tiles, each = (tiles + 7) / 8, id = blockIdx.x % 8 * each + blockIdx.x / 8;
     if (blockIdx.x / 8 >= each || id >= tiles) return;
     const uint32_t row_tile = id % tl.row_tiles, col_tile = id / tl.row_tiles, strips = p.Np / 16;
-    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(p.KB) * blockIdx.y / tl.splits);
-    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(p.KB) * (blockIdx.y + 1) / tl.splits);
+    const uint32_t begin = blockIdx.y * tl.per, end = min(begin + tl.per, p.KB);
 
     const uint8_t *codes[CT];
     const float *scales[CT];
@@ -781,32 +777,6 @@ __global__ __launch_bounds__(256) void matmul_i4_join(I4Gemm p, I4Tiles tl, cons
     p.C[static_cast<uint64_t>(tl.row0 + row) * p.ldc + n] = finished(x, p.epilogue);
 }
 
-struct I4Plan {
-    bool tiled = false;
-    uint32_t rt = 0, ct = 0, splits = 1;
-    uint32_t pass_rows = 0;   // rows of a pass; fragments take 4 bytes an element
-    size_t frag_bytes = 0, down_bytes = 0, part_bytes = 0;
-};
-constexpr uint64_t kMostFragments = 256ull << 20;
-I4Plan plan_of(const I4Gemm &p)
-{
-    I4Plan r;
-    r.tiled = p.M > 64;
-    if (!r.tiled) return r;
-    r.rt = 4;
-    r.ct = 4;
-    const uint32_t wg_rows = 16 * r.rt;
-    const uint64_t row_bytes = 512ull * p.KB;
-    r.pass_rows = static_cast<uint32_t>(std::max<uint64_t>(1, kMostFragments / (row_bytes * wg_rows))) * wg_rows;
-    r.pass_rows = std::min(r.pass_rows, (p.M + wg_rows - 1) / wg_rows * wg_rows);
-    r.frag_bytes = static_cast<size_t>(r.pass_rows) * row_bytes;
-    r.down_bytes = static_cast<size_t>(r.pass_rows) * 4;
-    const uint64_t grid = static_cast<uint64_t>(r.pass_rows / wg_rows) * ((p.Np + 64 * r.ct - 1) / (64 * r.ct));
-    r.splits = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(1, 2 * p.cus / grid), std::max(1u, p.KB / 4)));
-    if (r.splits > 1) r.part_bytes = static_cast<size_t>(r.splits) * std::min(r.pass_rows, p.M) * p.N * 4;
-    return r;
-}
-
 template <int RT, int CT, int GB>
 void launch_tile(hipStream_t s, const I4Gemm &p, const I4Tiles &tl, const int8_t *frags, const float *down, float *part)
 {
@@ -823,26 +793,81 @@ void launch_tile(hipStream_t s, const I4Gemm &p, const I4Tiles &tl, const int8_t
     else if (p.groups_of_block == 2) launch_tile<RT, CT, 2>(s, p, tl, frags, down, part);
     else launch_tile<RT, CT, 1>(s, p, tl, frags, down, part);
 }
-void launch_tiles(hipStream_t s, const I4Gemm &p, const I4Plan &pl, int8_t *ws)
+constexpr uint64_t kMostFragments = 256ull << 20, kMostParts = 256ull << 20;   // bytes
+size_t frag_bytes(const I4Gemm &p) { return static_cast<size_t>(p.pass_rows) * p.KB * 512; }
+size_t down_bytes(const I4Gemm &p) { return (static_cast<size_t>(p.pass_rows) * 4 + 255) / 256 * 256; }
+size_t part_bytes(const I4Gemm &p)
+{
+    const uint64_t rows = p.kernel == I4Gemm::kTile ? std::min(p.pass_rows, p.M) : p.M;
+    return p.splits > 1 ? static_cast<size_t>(p.splits) * rows * p.N * 4 : 0;
+}
+
+void launch_join(hipStream_t s, const I4Gemm &p, const I4Tiles &tl, const float *part)
+{
+    const uint64_t all = static_cast<uint64_t>(tl.rows) * p.N;
+    matmul_i4_join<<<static_cast<uint32_t>((all + 255) / 256), 256, 0, s>>>(p, tl, part);
+}
+void launch_tiles(hipStream_t s, const I4Gemm &p, int8_t *ws)
 {
     int8_t *frags = ws;
-    float *down = reinterpret_cast<float *>(ws + pl.frag_bytes), *part = reinterpret_cast<float *>(ws + pl.frag_bytes + (pl.down_bytes + 255) / 256 * 256);
+    float *down = reinterpret_cast<float *>(ws + frag_bytes(p)), *part = reinterpret_cast<float *>(ws + frag_bytes(p) + down_bytes(p));
     const bool aligned = !((reinterpret_cast<uintptr_t>(p.A) & 15) | (p.lda & 3) | (p.K & 3));
-    for (uint32_t row0 = 0; row0 < p.M; row0 += pl.pass_rows) {
+    for (uint32_t row0 = 0; row0 < p.M; row0 += p.pass_rows) {
         I4Tiles tl;
         tl.row0 = row0;
-        tl.rows = std::min(pl.pass_rows, p.M - row0);
-        tl.row_tiles = (tl.rows + 16 * pl.rt - 1) / (16 * pl.rt);
-        tl.col_tiles = (p.Np + 64 * pl.ct - 1) / (64 * pl.ct);
-        tl.splits = pl.splits;
-        const uint32_t tiles = tl.row_tiles * pl.rt, parts = std::max(1u, std::min(2 * p.cus / tiles, p.KB / 2));
+        tl.rows = std::min(p.pass_rows, p.M - row0);
+        tl.row_tiles = (tl.rows + 16 * p.rows - 1) / (16 * p.rows);
+        tl.col_tiles = (p.Np + 64 * p.strips - 1) / (64 * p.strips);
+        tl.splits = p.splits;
+        tl.per = p.per;
+        const uint32_t tiles = tl.row_tiles * p.rows, parts = std::max(1u, std::min(2 * p.cus / tiles, p.KB / 2));
         (aligned ? matmul_i4_split<true> : matmul_i4_split<false>)<<<dim3(tiles, parts), kSplitThreads, 0, s>>>(p, row0, frags, down);
-        launch_tile<4, 4>(s, p, tl, frags, down, part);
-        if (tl.splits > 1) {
-            const uint64_t all = static_cast<uint64_t>(tl.rows) * p.N;
-            matmul_i4_join<<<static_cast<uint32_t>((all + 255) / 256), 256, 0, s>>>(p, tl, part);
-        }
+        if (p.rows == 2 && p.strips == 1) launch_tile<2, 1>(s, p, tl, frags, down, part);
+        else if (p.rows == 2) launch_tile<2, 2>(s, p, tl, frags, down, part);
+        else if (p.strips == 2) launch_tile<4, 2>(s, p, tl, frags, down, part);
+        else launch_tile<4, 4>(s, p, tl, frags, down, part);
+        if (tl.splits > 1) launch_join(s, p, tl, part);
     }
+}
+template <int RQ>
+void launch_few_of(hipStream_t s, const I4Gemm &p, float *part)
+{
+    if (p.waves == 16) p.strips == 1 ? launch_few<RQ, 1, 16>(s, p, part) : launch_few<RQ, 2, 16>(s, p, part);
+    else if (p.strips == 2) launch_few<RQ, 2, 8>(s, p, part);
+    else if (p.strips == 3) launch_few<RQ, 3, 8>(s, p, part);
+    else launch_few<RQ, 4, 8>(s, p, part);
+}
+template <int RT>
+void launch_mid_of(hipStream_t s, const I4Gemm &p, float *part)
+{
+    if (p.strips == 1) launch_mid<RT, 1, 8>(s, p, part);
+    else if (p.strips == 2) launch_mid<RT, 2, 8>(s, p, part);
+    else if (p.strips == 3) launch_mid<RT, 3, 8>(s, p, part);
+    else launch_mid<RT, 4, 8>(s, p, part);
+}
+
+uint32_t parts_of(uint64_t x, uint32_t y) { return static_cast<uint32_t>((x + y - 1) / y); }
+
+// The time of a call as p says, us: a fit to 7000 measured ones (1 to 256 rows, K 512 to 16384,
+// N 512 to 28672, groups of 32 and 128; within 15 to 18 %; what it chooses is 3 % slower in the
+// mean than the fastest).  ops: vector instructions of a wave and block.
+double estimate(const I4Gemm &p, uint32_t kernel, uint32_t rows, uint32_t strips, uint32_t waves, uint32_t per, uint32_t splits)
+{
+    const double GB = p.groups_of_block, joined = splits > 1 ? 4.0 * splits * p.M * p.N / 3e6 : 0.0;
+    if (kernel == I4Gemm::kTile) {
+        const double groups = static_cast<double>(parts_of(p.M, 16 * rows)) * parts_of(p.Np / 16, 4 * strips) * splits;
+        const double load = std::ceil(groups / p.cus), tiles = rows * strips, at_once = tiles <= 2 ? 4 : tiles <= 4 ? 3 : 2;
+        const double matrix = load * per * tiles * 128 / 2400, vector = load * per * (40 * strips + 4 * tiles * GB) * 4 / 2400;
+        return 6.4 + 2.2 * std::max(matrix, vector) + 0.35 * std::ceil(groups / (p.cus * at_once)) * per +
+               3.6e-6 * p.M * p.K + 1.9 * std::ceil(p.K / 2048.0) +
+               (splits > 1 ? 2.25 : 0.0) + 1.5 * joined;
+    }
+    const uint32_t wg_rows = kernel == I4Gemm::kFew ? 4 * rows : 16 * rows;
+    const double again = parts_of(p.M, wg_rows), groups = parts_of(p.Np / 16, strips) * again * splits, load = std::ceil(groups / p.cus);
+    const double ops = kernel == I4Gemm::kFew ? 95.0 * rows + strips * (12 + rows * GB * 11) : 130.0 * rows + strips * (38 + rows * (4 * GB + 4));
+    const double vector = load * per * ops / 2400, rounds = std::ceil(groups / (p.cus * (waves == 16 ? 1 : 2)));
+    if (kernel == I4Gemm::kFew) return 3.0 + 1.7 * vector + 0.094 * rounds * parts_of(per, waves) + (splits > 1 ? 2.7 : 0.0) + 8.8 * joined;
+    return 3.7 + 2.7 * vector + (splits > 1 ? 2.2 : 0.0) + 4.5 * joined;
 }
 
 }  // namespace
@@ -855,34 +880,84 @@ void pack_i4(hipStream_t s, const uint8_t *B, const float *scales, const uint8_t
     pack_scales<<<static_cast<uint32_t>((count + 255) / 256), 256, 0, s>>>(scales, zeros, groups, w.slots, N, w.scales, w.zeros, count, bad);
 }
 
-// A grid's work-items count in 32 bits, workgroups in 16 in y.
-bool matmul_i4_fits(const I4Gemm &p)
+bool matmul_i4_lay_out(I4Gemm &p)
 {
-    const I4Plan pl = plan_of(p);
-    return p.Np / 16 < (1u << 22) && (!pl.tiled || static_cast<uint64_t>(std::min(pl.pass_rows, p.M)) * p.N < (1ull << 32) - 256);
+    // Offsets into A and a strip's codes are 31 bits in the kernels of few and tens of rows.
+    const uint64_t most_rows = std::min(p.M, 32u);
+    const bool short_offsets = ((most_rows - 1) * p.lda + p.K) * 4 < (1ull << 31) && p.KB < (1u << 21);
+    double best = 1e30;
+    auto consider = [&](uint32_t kernel, uint32_t rows, uint32_t strips, uint32_t waves) {
+        for (uint32_t splits = 1; splits <= 8; splits *= 2) {
+            const uint32_t per = parts_of(p.KB, splits);
+            if (splits > 1 && (per < 4 || 4ull * splits * std::min<uint64_t>(p.M, 1u << 20) * p.N > kMostParts)) break;
+            if (parts_of(p.KB, per) != splits || (waves == 16 && per < 16)) continue;
+            const double us = estimate(p, kernel, rows, strips, waves, per, splits);
+            if (us >= best) continue;
+            best = us;
+            p.kernel = static_cast<decltype(p.kernel)>(kernel);
+            p.rows = rows;
+            p.strips = strips;
+            p.waves = waves;
+            p.per = per;
+            p.splits = splits;
+        }
+    };
+    if (p.M <= 8 && short_offsets) {
+        const uint32_t quads = p.M <= 4 ? 1 : 2;
+        consider(I4Gemm::kFew, quads, 1, 16);
+        consider(I4Gemm::kFew, quads, 2, 16);
+        for (uint32_t t = 2; t <= 4; ++t) consider(I4Gemm::kFew, quads, t, 8);
+    }
+    if (p.M > 4 && p.M <= 512 && short_offsets)
+        for (uint32_t t = 1; t <= 4; ++t) {
+            consider(I4Gemm::kMid, 1, t, 8);
+            if (p.M > 16) consider(I4Gemm::kMid, 2, t, 8);
+        }
+    if (p.M > 16 || !short_offsets) {
+        consider(I4Gemm::kTile, 2, 1, 4);
+        consider(I4Gemm::kTile, 2, 2, 4);
+        consider(I4Gemm::kTile, 4, 2, 4);
+        consider(I4Gemm::kTile, 4, 4, 4);
+    }
+    uint64_t groups = static_cast<uint64_t>(parts_of(p.Np / 16, p.strips)), pass = p.M;
+    if (p.kernel == I4Gemm::kTile) {
+        const uint32_t wg_rows = 16 * p.rows;
+        p.pass_rows = static_cast<uint32_t>(std::max<uint64_t>(1, kMostFragments / (512ull * p.KB * wg_rows))) * wg_rows;
+        p.pass_rows = std::min(p.pass_rows, parts_of(p.M, wg_rows) * wg_rows);
+        pass = std::min(p.pass_rows, p.M);
+        groups = static_cast<uint64_t>(p.pass_rows / wg_rows) * parts_of(p.Np / 16, 4 * p.strips) + 7;
+    }
+    // A grid's work-items count in 32 bits.
+    return groups * 64 * p.waves < (1ull << 32) && (p.splits == 1 || pass * p.N < (1ull << 32) - 256);
 }
 
 size_t matmul_i4_ws_bytes(const I4Gemm &p)
 {
-    const I4Plan pl = plan_of(p);
-    return pl.tiled ? pl.frag_bytes + (pl.down_bytes + 255) / 256 * 256 + pl.part_bytes : 0;
+    return p.kernel == I4Gemm::kTile ? frag_bytes(p) + down_bytes(p) + part_bytes(p) : part_bytes(p);
 }
 
 void matmul_i4(hipStream_t s, const I4Gemm &p, void *ws)
 {
-    const I4Plan pl = plan_of(p);
-    if (pl.tiled) launch_tiles(s, p, pl, static_cast<int8_t *>(ws));
-    else if (p.M <= 4) launch_few<1, 1, 16, 1>(s, p, p.KB, nullptr);
-    else if (p.M <= 8) launch_few<2, 1, 16, 1>(s, p, p.KB, nullptr);
-    else if (p.M <= 16) launch_mid<1, 2, 8>(s, p, p.KB, nullptr);
-    else launch_mid<2, 2, 8>(s, p, p.KB, nullptr);
+    if (p.kernel == I4Gemm::kTile) {
+        launch_tiles(s, p, static_cast<int8_t *>(ws));
+        return;
+    }
+    float *part = p.splits > 1 ? static_cast<float *>(ws) : nullptr;
+    if (p.kernel == I4Gemm::kFew) p.rows == 1 ? launch_few_of<1>(s, p, part) : launch_few_of<2>(s, p, part);
+    else p.rows == 1 ? launch_mid_of<1>(s, p, part) : launch_mid_of<2>(s, p, part);
+    if (part) {
+        I4Tiles tl{};
+        tl.splits = p.splits;
+        tl.rows = p.M;
+        launch_join(s, p, tl, part);
+    }
 }
 
 std::string matmul_i4_route(const I4Gemm &p)
 {
-    const I4Plan pl = plan_of(p);
+    static const char *names[] = {"few", "mid", "tile"};
     char text[96];
-    std::snprintf(text, sizeof(text), "few=%u tile=%ux%u splits=%u", pl.tiled ? 0 : 1, 16 * pl.rt, 64 * pl.ct, pl.splits);
+    std::snprintf(text, sizeof(text), "%s rows=%u strips=%u waves=%u splits=%u", names[p.kernel], p.rows, p.strips, p.waves, p.splits);
     return text;
 }
 
