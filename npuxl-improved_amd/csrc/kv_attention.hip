@@ -916,7 +916,7 @@ template <uint32_t M>
 __device__ __forceinline__ bool find_tile(const KvAttn &p, const Tiles &tl, uint32_t group, uint32_t unit, uint32_t &b, uint32_t &tile)
 {
     const KvCall &c = p.call;
-    if (!c.seq_start) {
+    if (!c.seq_start || !c.lengths) {   // without lengths: one sequence
         b = unit / tl.per_seq;
         tile = unit % tl.per_seq;
         return b < c.batch;
@@ -1289,6 +1289,28 @@ uint32_t few_rows(const KvAttn &p)
     return keys <= 32768 ? 2 * one : one;
 }
 
+// Key ranges of a shared prefix, whose tiles all have its keys: the fullest CU's chunks at 1.3 us
+// (128 dimensions; a quarter less where two or more workgroups take turns) and each range's results written and
+// read (64 x 4 rows of 8 heads, 32768 keys: 16 ranges 77 us, 32 of 5 tiles, one of them empty, 82; 32 x 4 rows, 4096
+// keys: 12 ranges 16.5 us, 16 14.3, 24 15.9).
+uint64_t shared_parts(const KvAttn &p, uint32_t tile_rows, uint32_t chunks)
+{
+    const uint32_t G = p.call.c.kv_heads, D = p.call.c.head_dim, DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    const uint64_t rows = static_cast<uint64_t>(p.call.tokens) * (p.heads / G), tiles = (rows + tile_rows - 1) / tile_rows * G;
+    uint64_t best = 1;
+    double least = 1e30;
+    for (uint64_t parts = 1; parts <= std::min(chunks, 64u); ++parts) {
+        const uint64_t load = (tiles * parts + p.cus - 1) / p.cus, per = (chunks + parts - 1) / parts;
+        const double chunk = (0.35 + 0.0075 * DP) * tile_rows / 64 * (load > 1 && D <= 128 ? 0.75 : 1.0);
+        const double us = static_cast<double>(load * per) * chunk + 1.6e-6 * static_cast<double>(rows * G * parts) * (D + 4);
+        if (us < least) {
+            least = us;
+            best = parts;
+        }
+    }
+    return best;
+}
+
 struct Plan {
     bool few = false, tiled = false;   // kernels of the call: sequences of few rows, of many
     Split split{};
@@ -1342,7 +1364,7 @@ Plan plan_of(const KvAttn &p)
         auto tiles_of = [&](uint32_t rows) {   // of all kv heads
             r.tile_rows = rows;
             r.tiles.per_seq = static_cast<uint32_t>((most + rows - 1) / rows);
-            r.tiles.count = c.seq_start ? static_cast<uint32_t>(static_cast<uint64_t>(c.tokens) * group / rows) + c.batch
+            r.tiles.count = c.seq_start && c.lengths ? static_cast<uint32_t>(static_cast<uint64_t>(c.tokens) * group / rows) + c.batch
                                         : r.tiles.per_seq * c.batch;
             return static_cast<uint64_t>(r.tiles.count) * G;
         };
@@ -1353,13 +1375,15 @@ Plan plan_of(const KvAttn &p)
         // even ones with keys for 16 chunks a range (512 tokens of 4096, 8 kv heads: 76 us
         // against 79; a ragged batch of 1 to 331 tokens, 4 kv heads of 80, 43 against 35).
         uint64_t grid = D <= 128 ? tiles_of(128) : 0;
-        if (grid <= 2 * p.cus && (c.seq_start || grid >= p.cus || grid * (chunks / 16) < 2 * p.cus)) grid = tiles_of(64);
+        const bool shared = !c.lengths;
+        if (grid <= 2 * p.cus && (c.seq_start || shared || grid >= p.cus || grid * (chunks / 16) < 2 * p.cus)) grid = tiles_of(64);
         // Key ranges of 4 chunks at least for a workgroup a CU, of 8 for as many as
         // run at a time (32 tiles, 47 chunks: 8 ranges 20.5 us, 5 24.2, 10 22.1; 64 chunks: 8
         // ranges 23.7 us, 5 28.8, 10 26.2).  Where sequences differ the shorter have fewer.
         const uint64_t at_once = (D > 128 ? 1 : r.tile_rows == 128 ? 2 : 3) * p.cus;
-        const uint64_t parts = std::max(std::min<uint64_t>(p.cus / grid, chunks / 4),
-                                        std::min<uint64_t>(at_once * (c.seq_start ? 5 : 3) / (3 * grid), chunks / (c.seq_start ? 5 : 8)));
+        uint64_t parts = std::max(std::min<uint64_t>(p.cus / grid, chunks / 4),
+                                  std::min<uint64_t>(at_once * (c.seq_start ? 5 : 3) / (3 * grid), chunks / (c.seq_start ? 5 : 8)));
+        if (shared) parts = shared_parts(p, r.tile_rows, chunks);
         r.tiles.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(parts, 1), 64));
         r.tiles.per = (chunks + r.tiles.parts - 1) / r.tiles.parts;
         if (r.tiles.parts > 1 || p.partial) r.ws += static_cast<size_t>(grid) * r.tiles.parts * r.tile_rows * (D + 4) * sizeof(float);
@@ -1427,84 +1451,129 @@ struct Side {
     uint32_t rows, tile_rows;   // rows of a slot; of a tile (0: the call has none)
     const float *few, *tile;
 };
-__device__ __forceinline__ Found find_results(const Side &s, uint32_t b, const kv::Seq &seq, uint32_t row, uint32_t h)
+__device__ __forceinline__ Found find_results(const Side &s, uint32_t b, const kv::Seq &seq, int32_t len, uint32_t row, uint32_t h)
 {
     const KvCall &c = s.p.call;
     const uint32_t G = c.c.kv_heads, D = c.c.head_dim, group = s.p.heads / G;
     const uint64_t rows = static_cast<uint64_t>(seq.n) * group;
     if (s.tile_rows && rows > s.tiles.low_rows) {
-        const uint32_t len = static_cast<uint32_t>(kv::length(c, b)), M = s.tile_rows, tile = row / M;
-        const uint32_t unit = c.seq_start ? static_cast<uint32_t>(static_cast<uint64_t>(seq.row) * group / M) + b + tile
-                                          : b * s.tiles.per_seq + tile;
+        const uint32_t M = s.tile_rows, tile = row / M;
+        const uint32_t unit = c.seq_start && c.lengths ? static_cast<uint32_t>(static_cast<uint64_t>(seq.row) * group / M) + b + tile
+                                                       : b * s.tiles.per_seq + tile;
         const uint32_t last = min(seq.n * group, tile * M + M) - 1;
-        const uint32_t chunks = (static_cast<uint32_t>(keys_of(s.p, len, seq.n, last, group)) + kChunk - 1) / kChunk;
+        const uint32_t chunks = (static_cast<uint32_t>(keys_of(s.p, static_cast<uint32_t>(len), seq.n, last, group)) + kChunk - 1) / kChunk;
         return {s.tile + ((static_cast<uint64_t>(unit) * G + h) * s.tiles.parts * M + (row - tile * M)) * (D + 4),
                 static_cast<uint64_t>(M) * (D + 4), ranges_of(s.tiles, chunks)};
     }
     Slot sl;
     sl.b = b;
-    uint32_t slot = s.split.whole ? b : 0;
-    if (!find_slot(s.p, s.split, true, slot, sl)) return {s.few, 0, 0};
-    if (s.split.whole) slot = b;
+    sl.parts = 1;
+    uint32_t slot = b;
+    if (!s.split.whole && !find_slot(s.p, s.split, true, slot, sl)) return {s.few, 0, 0};
     return {s.few + ((static_cast<uint64_t>(slot) * G + h) * s.rows + row) * (D + 2), static_cast<uint64_t>(G) * s.rows * (D + 2), sl.parts};
 }
 
-// A wave a token and kv head.
+// One row's results of both calls.
+template <int DS>
+struct Joined {
+    float top = kNegInf, sum = 0.0f, o[DS] = {};
+    uint32_t d[DS];
+    __device__ __forceinline__ explicit Joined(uint32_t D)
+    {
+#pragma unroll
+        for (int y = 0; y < DS; ++y) d[y] = min((threadIdx.x & 63) + 64 * y, D - 1);
+    }
+    // Up to N parts at a time are asked for before their weights; lanes behind head_dim and parts
+    // behind the last load what is there (loads under a condition are waited for one by one).
+    template <uint32_t N>
+    __device__ __forceinline__ void add(const Found &f, uint32_t D)
+    {
+        const uint32_t lane = threadIdx.x & 63;
+        for (uint32_t j0 = 0; j0 < f.parts; j0 += 64) {
+            const uint32_t n = min(64u, f.parts - j0);
+            const float *at = f.at + j0 * f.step, *mine = at + min(lane, n - 1) * f.step + D;
+            float m = mine[0], l = mine[1], x[N][DS];
+            auto ask = [&](uint32_t from) {
+#pragma unroll
+                for (uint32_t j = 0; j < N; ++j)
+#pragma unroll
+                    for (int y = 0; y < DS; ++y) x[j][y] = at[min(from + j, n - 1) * f.step + d[y]];
+            };
+            ask(0);
+            if (lane >= n) {
+                m = kNegInf;
+                l = 0.0f;
+            }
+            const float now = fmaxf(top, groups_max(row_max(m))), base = now == kNegInf ? 0.0f : now;
+            const float before = __builtin_amdgcn_exp2f(top - base), w = l * __builtin_amdgcn_exp2f(m - base);
+            top = now;
+            sum = fmaf(sum, before, groups_sum(row_sum(w)));
+#pragma unroll
+            for (int y = 0; y < DS; ++y) o[y] *= before;
+            for (uint32_t from = 0;;) {
+#pragma unroll
+                for (uint32_t j = 0; j < N; ++j) {
+                    const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), (from + j) & 63));
+                    if (from + j < n)
+#pragma unroll
+                        for (int y = 0; y < DS; ++y) o[y] = fmaf(wj, x[j][y], o[y]);
+                }
+                from += N;
+                if (from >= n) break;
+                ask(from);
+            }
+        }
+    }
+};
+
+// A wave a token and query head.  Where the token's sequence is comes from one load of the starts
+// and lengths, a sequence a lane: what follows waits for every load once.
+template <int DS>
 __global__ __launch_bounds__(256) void kv_attention_prefix_join(Side shared, Side own)
 {
     const KvAttn &p = own.p;
     const KvCall &c = p.call;
     const uint32_t lane = threadIdx.x & 63, G = c.c.kv_heads, D = c.c.head_dim, group = p.heads / G;
-    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t t = static_cast<uint32_t>(item / G), h = static_cast<uint32_t>(item % G);
+    const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t t = item / p.heads, head = item % p.heads, h = head / group, r = head % group;
     if (t >= c.tokens) return;
+    const kv::Seq all = kv::sequence(shared.p.call, 0);
     uint32_t b = 0;
+    kv::Seq seq;
+    int32_t len;
     if (!c.seq_start) {
         b = t / (c.tokens / c.batch);
-    } else {   // how many sequences end at this token or before it
-        for (uint32_t i = 0; i < c.batch; i += 64) {
-            const uint32_t at = i + lane;
-            b += __popcll(__ballot(at < c.batch && static_cast<int64_t>(c.seq_start[at + 1]) <= static_cast<int64_t>(t)));
+        seq = kv::sequence(c, b);
+        len = kv::length(c, b);
+    } else {
+        for (;; b += 64) {
+            if (b >= c.batch) return;   // behind the last
+            const uint32_t at = min(b + lane, c.batch - 1);
+            const int32_t from = c.seq_start[at], to = c.seq_start[at + 1], n = kv::length(c, at);
+            const uint64_t ends = __ballot(b + lane < c.batch && static_cast<int64_t>(to) > static_cast<int64_t>(t));   // behind this token
+            if (!ends) continue;
+            const int first = __ffsll(static_cast<unsigned long long>(ends)) - 1;
+            const int32_t row = __builtin_amdgcn_readlane(from, first), end = __builtin_amdgcn_readlane(to, first);
+            len = __builtin_amdgcn_readlane(n, first);
+            seq = {static_cast<uint32_t>(row), static_cast<uint32_t>(end - row), row >= 0 && end >= row && static_cast<uint32_t>(end) <= c.tokens};
+            b += first;
+            break;
         }
-        if (b >= c.batch) return;   // behind the last
     }
-    const kv::Seq seq = kv::sequence(c, b), all = kv::sequence(shared.p.call, 0);
-    const int32_t len = kv::length(c, b);
-    if (!seq.ok || !all.ok || t < seq.row || t - seq.row >= seq.n || seq.n > p.max_tokens || len < 0 || static_cast<uint32_t>(len) > p.max_kv ||
-        !kv::behind_prefix(c, seq, len, p.causal))
+    if (!seq.ok || !all.ok || t < seq.row || t - seq.row >= seq.n || t < all.row || seq.n > p.max_tokens || len < 0 ||
+        static_cast<uint32_t>(len) > p.max_kv || !kv::behind_prefix(c, seq, len, p.causal))
         return;   // check_all told
-    const uint32_t i = t - seq.row, i_all = t - all.row;
-    Found f[2] = {find_results(shared, 0, all, i_all * group, h), find_results(own, b, seq, i * group, h)};
-    float *out = p.O + kv::rows_base(c, p.o, b, seq) + i * p.o.token + static_cast<uint64_t>(h) * group * p.o.head;
-    for (uint32_t r = 0; r < group; ++r, out += p.o.head) {
-        if (r) {   // a token's rows may lie in two tiles
-            f[0] = find_results(shared, 0, all, i_all * group + r, h);
-            f[1] = find_results(own, b, seq, i * group + r, h);
-        }
-        float top = kNegInf;
-        for (int k = 0; k < 2; ++k)
-            for (uint32_t j = lane; j < f[k].parts; j += 64) top = fmaxf(top, f[k].at[j * f[k].step + D]);
-        for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-        const float base = top == kNegInf ? 0.0f : top;
-        float sum = 0.0f, o[4] = {};
-        for (int k = 0; k < 2; ++k)
-            for (uint32_t j0 = 0; j0 < f[k].parts; j0 += 64) {
-                const uint32_t n = min(64u, f[k].parts - j0);
-                const float *at = f[k].at + j0 * f[k].step, *mine = at + min(lane, n - 1) * f[k].step + D;
-                const float w = lane < n ? mine[1] * __builtin_amdgcn_exp2f(mine[0] - base) : 0.0f;
-                sum += w;
-                for (uint32_t j = 0; j < n; ++j) {
-                    const float wj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), j));
+    const Found first = find_results(shared, 0, all, static_cast<int32_t>(shared.p.call.length), (t - all.row) * group + r, h);
+    const Found second = find_results(own, b, seq, len, (t - seq.row) * group + r, h);
+    Joined<DS> joined(D);
+    if (first.parts > 4) joined.template add<16>(first, D);
+    else joined.template add<4>(first, D);
+    if (second.parts > 4) joined.template add<16>(second, D);
+    else joined.template add<4>(second, D);
+    float *out = p.O + kv::rows_base(c, p.o, b, seq) + (t - seq.row) * p.o.token + static_cast<uint64_t>(head) * p.o.head;
 #pragma unroll
-                    for (uint32_t x = 0; x < 4; ++x)
-                        if (lane + 64 * x < D) o[x] = fmaf(wj, at[j * f[k].step + lane + 64 * x], o[x]);
-                }
-            }
-        for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-#pragma unroll
-        for (uint32_t x = 0; x < 4; ++x)
-            if (lane + 64 * x < D) out[lane + 64 * x] = sum != 0.0f ? o[x] / sum : 0.0f;
-    }
+    for (int y = 0; y < DS; ++y)
+        if (lane + 64 * y < D) out[lane + 64 * y] = joined.sum != 0.0f ? joined.o[y] / joined.sum : 0.0f;
 }
 
 // The call over the prefix's keys of what own attends to behind it.
@@ -1573,7 +1642,7 @@ size_t kv_prefix_attention_ws_bytes(const KvAttn &own, const int32_t *prefix_tab
 bool kv_prefix_attention_fits(const KvAttn &own, const int32_t *prefix_table)
 {
     return kv_attention_fits(own) && kv_attention_fits(shared_call(own, prefix_table)) &&
-           static_cast<uint64_t>(own.call.tokens) * own.call.c.kv_heads * 64 < (1ull << 32) - 256;
+           static_cast<uint64_t>(own.call.tokens) * own.heads * 64 < (1ull << 32) - 256;
 }
 
 std::string kv_prefix_attention_route(const KvAttn &own, const int32_t *prefix_table)
@@ -1588,9 +1657,10 @@ void kv_prefix_attention(hipStream_t s, const KvAttn &own, const int32_t *prefix
     float *own_ws = static_cast<float *>(ws), *shared_ws = own_ws + padded(own_plan.ws) / sizeof(float);
     launch_any(s, shared, shared_plan, shared_ws);
     launch_any(s, own, own_plan, own_ws);
-    const uint64_t items = static_cast<uint64_t>(own.call.tokens) * own.call.c.kv_heads;
-    kv_attention_prefix_join<<<static_cast<uint32_t>((items + 3) / 4), 256, 0, s>>>(side_of(shared, shared_plan, shared_ws),
-                                                                                  side_of(own, own_plan, own_ws));
+    const uint64_t items = static_cast<uint64_t>(own.call.tokens) * own.heads;
+    const uint32_t D = own.call.c.head_dim;
+    (D <= 64 ? kv_attention_prefix_join<1> : D <= 128 ? kv_attention_prefix_join<2> : kv_attention_prefix_join<4>)
+        <<<static_cast<uint32_t>((items + 3) / 4), 256, 0, s>>>(side_of(shared, shared_plan, shared_ws), side_of(own, own_plan, own_ws));
 }
 
 }  // namespace k
