@@ -417,8 +417,9 @@ constexpr uint32_t few_lds()
     return WAVES * (128 * DP + 1024 + RT * DP * 16) + RT * (DP / 64) * 1024;
 }
 
+// A workgroup's slot, kv head and rows from 4 RT row_tile on.
 template <int DP, int RT, bool FULL, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) void kv_attention_few(KvAttn p, Split sp, float *ws, uint32_t ws_rows)
+__device__ __forceinline__ void few_rows_of(const KvAttn &p, const Split &sp, float *ws, uint32_t ws_rows, uint32_t slot, const uint32_t h, uint32_t row_tile)
 {
     constexpr int DS = DP / 64, DT = DP / 16, R = 4 * RT;
     extern __shared__ __align__(1024) int8_t lds[];
@@ -426,17 +427,16 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) vo
     const KvCall &c = p.call;
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t h = blockIdx.y, G = c.c.kv_heads, D = FULL ? DP : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
+    const uint32_t G = c.c.kv_heads, D = FULL ? DP : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
     int8_t *k_lds = lds + wave * 128 * DP, *v_lds = k_lds + 64 * DP;
     uint32_t *sh_p = reinterpret_cast<uint32_t *>(lds + WAVES * 128 * DP) + wave * 256;
     float *sh_o_all = reinterpret_cast<float *>(lds + WAVES * (128 * DP + 1024)), *sh_o = sh_o_all + wave * RT * DT * 64;
-    if (blockIdx.x == 0 && h == 0) kv::check_all(c, false, p.max_kv, p.max_tokens, p.causal);
-    uint32_t slot = blockIdx.x;
+    if (slot == 0 && h == 0) kv::check_all(c, false, p.max_kv, p.max_tokens, p.causal);
     Slot sl;
     if (!find_slot(p, sp, false, slot, sl)) return;
     const uint32_t b = __builtin_amdgcn_readfirstlane(sl.b), parts = __builtin_amdgcn_readfirstlane(sl.parts);
     const kv::Seq seq = kv::sequence(c, b);
-    const uint32_t n = __builtin_amdgcn_readfirstlane(seq.n), rows = n * group, row0 = blockIdx.z * R;
+    const uint32_t n = __builtin_amdgcn_readfirstlane(seq.n), rows = n * group, row0 = row_tile * R;
     if (row0 >= rows) return;
     const int len = __builtin_amdgcn_readfirstlane(kv::length(c, b));
     // Even parts of the keys.
@@ -803,6 +803,12 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) vo
     }
 }
 
+template <int DP, int RT, bool FULL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) void kv_attention_few(KvAttn p, Split sp, float *ws, uint32_t ws_rows)
+{
+    few_rows_of<DP, RT, FULL, WAVES>(p, sp, ws, ws_rows, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
 // Parts of a row, `step` floats apart, each o / l with its m and l behind it:
 // weighed by l 2^(m - max m).  A workgroup a row: the weights first, a part a
 // thread, then the sums, threads over the dimensions and every few parts.  The
@@ -958,8 +964,9 @@ __device__ __forceinline__ uint32_t ranges_of(const Tiles &tl, uint32_t chunks)
     return tl.parts == 1 ? 1 : max(1u, (chunks + tl.per - 1) / tl.per);
 }
 
+// A workgroup's place among the tiles of all kv heads and its key range.
 template <int DP, int RT, bool FULL, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
+__device__ __forceinline__ void tile_of(const KvAttn &p, const Tiles &tl, float *ws, const uint32_t place, const uint32_t range)
 {
     constexpr int DS = DP / 64, DT = DP / 16;
     constexpr uint32_t M = 16 * RT * WAVES;
@@ -968,12 +975,12 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attenti
     const KvCall &c = p.call;
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t G = c.c.kv_heads, h = blockIdx.x % G, D = FULL ? DP : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
-    if (blockIdx.x == 0 && blockIdx.y == 0) kv::check_all(c, false, p.max_kv, p.max_tokens, p.causal);
+    const uint32_t G = c.c.kv_heads, h = place % G, D = FULL ? DP : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
+    if (place == 0 && range == 0) kv::check_all(c, false, p.max_kv, p.max_tokens, p.causal);
     // The last tiles of a causal sequence have the most keys: they come first.
     uint32_t b, tile, len;
     kv::Seq seq;
-    const uint32_t unit = tl.count - 1 - blockIdx.x / G;
+    const uint32_t unit = tl.count - 1 - place / G;
     if (!find_tile<M>(p, tl, group, unit, b, tile) || !tile_sequence(p, tl, group, b, seq, len)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     tile = __builtin_amdgcn_readfirstlane(tile);
@@ -982,12 +989,12 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attenti
     if (static_cast<uint64_t>(tile) * M >= rows) return;
     const uint32_t row0 = tile * M + wave * 16 * RT;   // the wave's first
     const uint32_t chunks = tile_chunks<M>(p, len, n, tile, group), ranges = ranges_of(tl, chunks);
-    if (blockIdx.y >= ranges) return;
+    if (range >= ranges) return;
     auto sees = [&](uint32_t row) { return keys_of(p, len, n, row, group); };
     // Keys of the wave; below `least` every row of the wave sees all.
     const int wave_keys = row0 < rows ? sees(min(rows, row0 + 16 * RT) - 1) : 0, least = row0 < rows ? sees(row0) : 0;
-    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * blockIdx.y / ranges);
-    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * (blockIdx.y + 1) / ranges);
+    const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * range / ranges);
+    const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * (range + 1) / ranges);
 
     Query<DS> q[RT];
     State<DT> st[RT];
@@ -1212,7 +1219,7 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attenti
                     for (int i = 0; i < 4; ++i) at[16 * t + i] = x[i];
             }
         } else {
-            float *at = ws + (((static_cast<uint64_t>(unit) * G + h) * tl.parts + blockIdx.y) * M + (row - tile * M)) * (D + 4);
+            float *at = ws + (((static_cast<uint64_t>(unit) * G + h) * tl.parts + range) * M + (row - tile * M)) * (D + 4);
 #pragma unroll
             for (int t = 0; t < DT; ++t)
                 if (16 * t < static_cast<int>(D)) *reinterpret_cast<v4f *>(at + 4 * g + 16 * t) = result(t);
@@ -1222,6 +1229,12 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attenti
             }
         }
     }
+}
+
+template <int DP, int RT, bool FULL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
+{
+    tile_of<DP, RT, FULL, WAVES>(p, tl, ws, blockIdx.x, blockIdx.y);
 }
 
 // A tile's key ranges, at most 64, together: kJoinRows rows a wave, a range's
@@ -1391,6 +1404,12 @@ Plan plan_of(const KvAttn &p)
     return r;
 }
 
+template <typename K>
+void allow_lds(K kernel, uint32_t bytes)
+{
+    if (bytes > 60 * 1024)
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
 template <int DP, int RT>
 void launch_few(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 {
@@ -1398,18 +1417,22 @@ void launch_few(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
     constexpr uint32_t bytes = few_lds<DP, RT, W>();
     const bool full = p.call.c.head_dim == DP;
     const auto kernel = full ? kv_attention_few<DP, RT, true, W> : kv_attention_few<DP, RT, false, W>;
-    if (bytes > 60 * 1024)
-        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    allow_lds(kernel, bytes);
     const uint32_t tiles = (pl.rows + 4 * RT - 1) / (4 * RT);
     kernel<<<dim3(pl.slots, p.call.c.kv_heads, tiles), 64 * W, bytes, s>>>(p, pl.split, ws, pl.rows);
+}
+// Bytes of dynamic LDS: two chunks' operands.
+template <int DP>
+constexpr uint32_t tile_lds()
+{
+    return 2 * (4 * (DP / 64) * 1024 + (DP / 16) * 2048);
 }
 template <int DP, int RT, int WAVES>
 void launch_tile(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 {
-    constexpr uint32_t bytes = 2 * (4 * (DP / 64) * 1024 + (DP / 16) * 2048);
+    constexpr uint32_t bytes = tile_lds<DP>();
     const auto kernel = p.call.c.head_dim == DP ? kv_attention_tile<DP, RT, true, WAVES> : kv_attention_tile<DP, RT, false, WAVES>;
-    if (bytes > 60 * 1024)
-        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    allow_lds(kernel, bytes);
     const uint32_t grid = pl.tiles.count * p.call.c.kv_heads;
     kernel<<<dim3(grid, pl.tiles.parts), 64 * WAVES, bytes, s>>>(p, pl.tiles, ws);
     if (pl.tiles.parts > 1 && !p.partial) kv_attention_join<16 * RT * WAVES, DP / 64><<<dim3(grid, 4 * RT * WAVES / kJoinRows), 256, 0, s>>>(p, pl.tiles, ws);
@@ -1576,6 +1599,65 @@ __global__ __launch_bounds__(256) void kv_attention_prefix_join(Side shared, Sid
         if (lane + 64 * y < D) out[lane + 64 * y] = joined.sum != 0.0f ? joined.o[y] / joined.sum : 0.0f;
 }
 
+// Both calls in one launch: neither waits for the other, and where one is bound by the codes and
+// the other by vector instructions they share the CUs.  A call's workgroups come in chunks of some
+// eights, an eight one for each XCD, so that a head's stay on their XCD, and a chunk one for each CU at
+// most: chunks of the call with fewer are spread among the other's, the first first.  (Eight by eight in
+// turn, each call's workgroups went to every other CU: 64 sequences behind 32768 tokens 136 us.)
+struct Mix {
+    uint32_t less;        // the call with fewer workgroups: 0 the prefix's, 1 the sequences' own
+    uint32_t chunk;       // eights
+    uint32_t chunks[2];   // of the call with fewer, of the other
+    uint32_t wide[2];     // workgroups in x of the prefix's and of the own grid
+    uint32_t first;       // workgroups of tiles before those of few rows
+};
+// Whose workgroup this is and which of those.
+__device__ __forceinline__ bool of_own(const Mix &mix, uint32_t &index)
+{
+    const uint32_t eight = blockIdx.x / 8, chunk = eight / mix.chunk, period = (mix.chunks[0] + mix.chunks[1]) / mix.chunks[0];
+    const uint32_t round = chunk / period;
+    const bool fewer = chunk == round * period && round < mix.chunks[0];
+    const uint32_t before = fewer ? round : chunk - min(round + 1, mix.chunks[0]);
+    index = __builtin_amdgcn_readfirstlane((before * mix.chunk + eight - chunk * mix.chunk) * 8 + blockIdx.x % 8);
+    return __builtin_amdgcn_readfirstlane(fewer == (mix.less == 1));
+}
+// (Each call's arguments by name: through a reference to either they would be read again and again.)
+template <int DP, int RT, bool FULL, int WAVES>
+__device__ __forceinline__ void few_rows_at(const Side &s, uint32_t wide, uint32_t at)
+{
+    const uint32_t G = s.p.call.c.kv_heads, rest = __builtin_amdgcn_readfirstlane(at / wide), z = __builtin_amdgcn_readfirstlane(rest / G);
+    if (z * 4 * RT < s.rows)
+        few_rows_of<DP, RT, FULL, WAVES>(s.p, s.split, const_cast<float *>(s.few), s.rows, at - rest * wide, rest - z * G, z);
+}
+template <int DP, int RT, bool FULL>
+__device__ __forceinline__ void tile_at(const Side &s, uint32_t wide, uint32_t at)
+{
+    const uint32_t range = __builtin_amdgcn_readfirstlane(at / wide);
+    if (range < s.tiles.parts) tile_of<DP, RT, FULL, 4>(s.p, s.tiles, const_cast<float *>(s.tile), at - range * wide, range);
+}
+template <int DP, int RT, bool FULL, int WAVES>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_attention_tile_and_few(Side shared, Side own, Mix mix)
+{
+    // Tiles first: with their turns behind few rows' they were alone on the CUs at the end (112 us
+    // instead of 83).
+    if (blockIdx.x < mix.first) tile_at<DP, 1, FULL>(shared, mix.wide[0], blockIdx.x);
+    else if (WAVES == 4 || threadIdx.x < 64 * WAVES) few_rows_at<DP, RT, FULL, WAVES>(own, mix.wide[1], blockIdx.x - mix.first);
+}
+template <int DP, int RT, bool FULL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) void kv_attention_few_twice(Side shared, Side own, Mix mix)
+{
+    uint32_t at;
+    if (of_own(mix, at)) few_rows_at<DP, RT, FULL, WAVES>(own, mix.wide[1], at);
+    else few_rows_at<DP, RT, FULL, WAVES>(shared, mix.wide[0], at);
+}
+template <int DP, int RT, bool FULL>
+__global__ __launch_bounds__(256, DP * RT <= 128 ? 3 : 2) void kv_attention_tile_twice(Side shared, Side own, Mix mix)
+{
+    uint32_t at;
+    if (of_own(mix, at)) tile_at<DP, RT, FULL>(own, mix.wide[1], at);
+    else tile_at<DP, RT, FULL>(shared, mix.wide[0], at);
+}
+
 // The call over the prefix's keys of what own attends to behind it.
 KvAttn shared_call(const KvAttn &own, const int32_t *prefix_table)
 {
@@ -1598,6 +1680,82 @@ Side side_of(const KvAttn &p, const Plan &pl, const float *ws)
 {
     return {p, pl.split, pl.tiles, pl.rows, pl.tiled ? pl.tile_rows : 0, ws, ws + pl.few_ws / sizeof(float)};
 }
+// groups: workgroups of each call; the launch's.
+uint32_t mixed(Mix &mix, uint32_t cus, const uint64_t groups[2])
+{
+    const uint32_t eights[2] = {static_cast<uint32_t>((groups[0] + 7) / 8), static_cast<uint32_t>((groups[1] + 7) / 8)};
+    mix.less = eights[1] <= eights[0] ? 1 : 0;
+    mix.chunk = std::min(std::max(cus / 8, 1u), eights[mix.less]);
+    mix.chunks[0] = (eights[mix.less] + mix.chunk - 1) / mix.chunk;
+    mix.chunks[1] = (eights[1 - mix.less] + mix.chunk - 1) / mix.chunk;
+    return 8 * mix.chunk * (mix.chunks[0] + mix.chunks[1]);
+}
+// The two calls of a shared prefix in one launch: tiles of 64 rows and few rows, few rows twice, or the
+// same tiles twice; false: they are of other kinds.
+template <int DP, int RT>
+void launch_with_few(hipStream_t s, const Side &shared, const Side &own, const uint32_t slots[2], bool tiled)
+{
+    // Beside tiles, as many waves of few rows as leave three workgroups their LDS.
+    constexpr int W = DP > 128 ? 2 : 4, beside = DP > 64 ? 2 : 4;
+    const uint32_t G = own.p.call.c.kv_heads;
+    const bool full = own.p.call.c.head_dim == DP;
+    const Side *sides[2] = {&shared, &own};
+    Mix mix{};
+    uint64_t groups[2];
+    for (int k = 0; k < 2; ++k) {
+        mix.wide[k] = slots[k];
+        groups[k] = static_cast<uint64_t>(slots[k]) * G * ((sides[k]->rows + 4 * RT - 1) / (4 * RT));
+    }
+    if (tiled) {
+        mix.wide[0] = shared.tiles.count * G;
+        groups[0] = static_cast<uint64_t>(mix.wide[0]) * shared.tiles.parts;
+    }
+    const uint32_t grid = tiled ? static_cast<uint32_t>(groups[0] + groups[1]) : mixed(mix, own.p.cus, groups);
+    mix.first = static_cast<uint32_t>(groups[0]);
+    if (tiled) {
+        constexpr uint32_t bytes = std::max(tile_lds<DP>(), few_lds<DP, RT, beside>());
+        const auto kernel = full ? kv_attention_tile_and_few<DP, RT, true, beside> : kv_attention_tile_and_few<DP, RT, false, beside>;
+        allow_lds(kernel, bytes);
+        kernel<<<grid, 256, bytes, s>>>(shared, own, mix);
+    } else {
+        constexpr uint32_t bytes = few_lds<DP, RT, W>();
+        const auto kernel = full ? kv_attention_few_twice<DP, RT, true, W> : kv_attention_few_twice<DP, RT, false, W>;
+        allow_lds(kernel, bytes);
+        kernel<<<grid, 64 * W, bytes, s>>>(shared, own, mix);
+    }
+}
+template <int DP, int RT>
+void launch_tiles_twice(hipStream_t s, const Side &shared, const Side &own)
+{
+    const Side *sides[2] = {&shared, &own};
+    Mix mix{};
+    uint64_t groups[2];
+    for (int k = 0; k < 2; ++k) {
+        mix.wide[k] = sides[k]->tiles.count * own.p.call.c.kv_heads;
+        groups[k] = static_cast<uint64_t>(mix.wide[k]) * sides[k]->tiles.parts;
+    }
+    const uint32_t grid = mixed(mix, own.p.cus, groups);
+    const auto kernel = own.p.call.c.head_dim == DP ? kv_attention_tile_twice<DP, RT, true> : kv_attention_tile_twice<DP, RT, false>;
+    allow_lds(kernel, tile_lds<DP>());
+    kernel<<<grid, 256, tile_lds<DP>(), s>>>(shared, own, mix);
+}
+template <int DP>
+bool launch_both(hipStream_t s, const Side &shared, const Plan &shared_plan, const Side &own, const Plan &own_plan)
+{
+    if (shared_plan.tiled && !shared_plan.few && own_plan.tiled && !own_plan.few && shared.tile_rows == own.tile_rows) {
+        if (DP > 128 || own.tile_rows == 64) launch_tiles_twice<DP, 1>(s, shared, own);
+        else if constexpr (DP <= 128) launch_tiles_twice<DP, 2>(s, shared, own);
+        return true;
+    }
+    if (own_plan.tiled || (shared_plan.tiled && (shared_plan.few || shared.tile_rows != 64))) return false;
+    uint32_t slots[2] = {shared_plan.slots, own_plan.slots};
+    const uint32_t rows = shared_plan.tiled ? own.rows : std::max(shared.rows, own.rows);
+    if (rows <= 4) launch_with_few<DP, 1>(s, shared, own, slots, shared_plan.tiled);
+    else if (DP > 128 || rows <= 8) launch_with_few<DP, 2>(s, shared, own, slots, shared_plan.tiled);
+    else if constexpr (DP <= 128) launch_with_few<DP, 4>(s, shared, own, slots, shared_plan.tiled);
+    return true;
+}
+
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 void launch_any(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
@@ -1634,6 +1792,14 @@ void kv_attention(hipStream_t s, const KvAttn &p, void *ws)
     launch_any(s, p, plan_of(p), static_cast<float *>(ws));
 }
 
+// Workgroups of a call, all kernels'.
+static uint64_t groups_of(const KvAttn &p)
+{
+    const Plan pl = plan_of(p);
+    const uint64_t G = p.call.c.kv_heads;
+    return pl.slots * G * ((pl.rows + 3) / 4) + static_cast<uint64_t>(pl.tiles.count) * G * pl.tiles.parts;
+}
+
 size_t kv_prefix_attention_ws_bytes(const KvAttn &own, const int32_t *prefix_table)
 {
     return padded(plan_of(own).ws) + padded(plan_of(shared_call(own, prefix_table)).ws);
@@ -1642,7 +1808,8 @@ size_t kv_prefix_attention_ws_bytes(const KvAttn &own, const int32_t *prefix_tab
 bool kv_prefix_attention_fits(const KvAttn &own, const int32_t *prefix_table)
 {
     return kv_attention_fits(own) && kv_attention_fits(shared_call(own, prefix_table)) &&
-           static_cast<uint64_t>(own.call.tokens) * own.heads * 64 < (1ull << 32) - 256;
+           static_cast<uint64_t>(own.call.tokens) * own.heads * 64 < (1ull << 32) - 256 &&
+           groups_of(own) + groups_of(shared_call(own, prefix_table)) < (1ull << 23);
 }
 
 std::string kv_prefix_attention_route(const KvAttn &own, const int32_t *prefix_table)
@@ -1655,12 +1822,18 @@ void kv_prefix_attention(hipStream_t s, const KvAttn &own, const int32_t *prefix
     const KvAttn shared = shared_call(own, prefix_table);
     const Plan own_plan = plan_of(own), shared_plan = plan_of(shared);
     float *own_ws = static_cast<float *>(ws), *shared_ws = own_ws + padded(own_plan.ws) / sizeof(float);
-    launch_any(s, shared, shared_plan, shared_ws);
-    launch_any(s, own, own_plan, own_ws);
+    const Side first = side_of(shared, shared_plan, shared_ws), second = side_of(own, own_plan, own_ws);
     const uint64_t items = static_cast<uint64_t>(own.call.tokens) * own.heads;
     const uint32_t D = own.call.c.head_dim;
+    const bool both = D <= 64    ? launch_both<64>(s, first, shared_plan, second, own_plan)
+                      : D <= 128 ? launch_both<128>(s, first, shared_plan, second, own_plan)
+                                 : launch_both<256>(s, first, shared_plan, second, own_plan);
+    if (!both) {
+        launch_any(s, shared, shared_plan, shared_ws);
+        launch_any(s, own, own_plan, own_ws);
+    }
     (D <= 64 ? kv_attention_prefix_join<1> : D <= 128 ? kv_attention_prefix_join<2> : kv_attention_prefix_join<4>)
-        <<<static_cast<uint32_t>((items + 3) / 4), 256, 0, s>>>(side_of(shared, shared_plan, shared_ws), side_of(own, own_plan, own_ws));
+        <<<static_cast<uint32_t>((items + 3) / 4), 256, 0, s>>>(first, second);
 }
 
 }  // namespace k
