@@ -1348,17 +1348,8 @@ k::RopeAxes rope_axes_params(const vnpu_rope_axes_f32_args_t &a, const KvSource 
     }
     require(2 * p.pairs <= a.head_dim, "rope_axes sections are more than a head");
     p.half = a.rotation == VNPU_ROTATE_HALF;
-    const double theta = a.theta_base > 0.0f ? a.theta_base : 10000.0, scaling = a.scaling > 0.0f ? a.scaling : 1.0;
-    uint32_t used[4] = {}, axis = 0;
-    for (uint32_t j = 0; j < p.pairs; ++j) {
-        while (used[axis] == a.sections[axis]) axis = (axis + 1) % a.axes;
-        const double power = a.ladders == VNPU_AXES_OWN_LADDERS ? static_cast<double>(used[axis]) / a.sections[axis]
-                                                                : static_cast<double>(j) / p.pairs;
-        p.axis[j] = static_cast<uint8_t>(axis);
-        p.turns[j] = scaling * std::pow(theta, -power) / 6.283185307179586476925;
-        ++used[axis];
-        if (a.order == VNPU_AXES_TURNS) axis = (axis + 1) % a.axes;
-    }
+    k::rope_axes_rates(p, a.order == VNPU_AXES_TURNS, a.ladders == VNPU_AXES_OWN_LADDERS, a.axes, a.sections,
+                       a.theta_base > 0.0f ? a.theta_base : 10000.0f, a.scaling > 0.0f ? a.scaling : 1.0f);
     auto side = [&](const float *in, float *out, uint32_t heads, const uint32_t from[3], const uint32_t to[3], k::KvRows &in_rows,
                     k::KvRows &out_rows) -> std::pair<uint64_t, uint64_t> {
         if (!in) return {0, 0};

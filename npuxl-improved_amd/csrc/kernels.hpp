@@ -357,9 +357,13 @@ struct RopeAxes {
     uint32_t batch = 1, tokens = 0, heads = 0, kv_heads = 0, head_dim = 0, position_ld = 0, pairs = 0;
     uint32_t half = 0;       // pairs (j, j + pairs), else (2 j, 2 j + 1)
     KvRows q, qo, k, ko;
-    double turns[128];       // angle / 2 pi of position 1, of each pair
-    uint8_t axis[128];
+    struct Pairs {
+        double turns[128];   // angle / 2 pi of position 1
+        uint8_t axis[128];
+    } of;
 };
+// Each pair's axis and rate; sections: pairs of each axis, p.pairs together.
+void rope_axes_rates(RopeAxes &p, bool in_turn, bool own_ladders, uint32_t axes, const uint32_t *sections, float theta, float scaling);
 bool rope_axes_fits(const RopeAxes &p);
 void rope_axes(hipStream_t s, const RopeAxes &p);
 

@@ -11,6 +11,11 @@
 #include "kernels.hpp"
 
 #include <algorithm>
+#include <cmath>
+#include <map>
+#include <mutex>
+#include <tuple>
+#include <vector>
 
 namespace vnpu {
 namespace k {
@@ -40,7 +45,7 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxes p, uint32_t uni
     }
     if (turn) {
         double c, s;
-        dev::cos_sin_turns(static_cast<double>(p.positions[static_cast<uint64_t>(p.axis[i]) * p.position_ld + token]) * p.turns[i], c, s);
+        dev::cos_sin_turns(static_cast<double>(p.positions[static_cast<uint64_t>(p.of.axis[i]) * p.position_ld + token]) * p.of.turns[i], c, s);
 #pragma unroll
         for (int h = 0; h < PER; ++h) {
             const double u = x[h], v = y[h];
@@ -68,6 +73,33 @@ void launch(hipStream_t s, const RopeAxes &p)
 
 }  // namespace
 
+// Kept by value for a call's parameters: the powers of 64 pairs are microseconds on the host.
+void rope_axes_rates(RopeAxes &p, bool in_turn, bool own_ladders, uint32_t axes, const uint32_t *sections, float theta, float scaling)
+{
+    using Key = std::tuple<bool, bool, std::vector<uint32_t>, float, float>;
+    static std::mutex mutex;
+    static auto *known = new std::map<Key, RopeAxes::Pairs>();
+    std::lock_guard<std::mutex> lock(mutex);
+    const Key key(in_turn, own_ladders, std::vector<uint32_t>(sections, sections + axes), theta, scaling);
+    const auto it = known->find(key);
+    if (it != known->end()) {
+        p.of = it->second;
+        return;
+    }
+    p.of = {};
+    uint32_t used[4] = {}, axis = 0;
+    for (uint32_t j = 0; j < p.pairs; ++j) {
+        while (used[axis] == sections[axis]) axis = (axis + 1) % axes;
+        const double power = own_ladders ? static_cast<double>(used[axis]) / sections[axis] : static_cast<double>(j) / p.pairs;
+        p.of.axis[j] = static_cast<uint8_t>(axis);
+        p.of.turns[j] = static_cast<double>(scaling) * std::pow(static_cast<double>(theta), -power) / (2.0 * M_PI);
+        ++used[axis];
+        if (in_turn) axis = (axis + 1) % axes;
+    }
+    if (known->size() >= 64) known->clear();
+    known->emplace(key, p.of);
+}
+
 // A grid's work-items count in 32 bits.
 bool rope_axes_fits(const RopeAxes &p) { return static_cast<uint64_t>(p.tokens) * (p.head_dim / 2) < (1ull << 32) - 256; }
 
@@ -77,7 +109,8 @@ void rope_axes(hipStream_t s, const RopeAxes &p)
 {
     const uint64_t work = static_cast<uint64_t>(p.tokens) * (p.head_dim / 2) * (p.heads + p.kv_heads);
     const uint32_t heads = std::max(p.heads, p.kv_heads);
-    if (work < 400000 || heads <= 2) launch<2>(s, p);
+    if (work < 30000) launch<1>(s, p);
+    else if (work < 400000 || heads <= 2) launch<2>(s, p);
     else if (work < 1600000 || heads <= 4) launch<4>(s, p);
     else launch<8>(s, p);
 }
