@@ -837,13 +837,13 @@ void launch_few_of(hipStream_t s, const I4Gemm &p, float *part)
     else if (p.strips == 3) launch_few<RQ, 3, 8>(s, p, part);
     else launch_few<RQ, 4, 8>(s, p, part);
 }
-template <int RT>
 void launch_mid_of(hipStream_t s, const I4Gemm &p, float *part)
 {
-    if (p.strips == 1) launch_mid<RT, 1, 8>(s, p, part);
-    else if (p.strips == 2) launch_mid<RT, 2, 8>(s, p, part);
-    else if (p.strips == 3) launch_mid<RT, 3, 8>(s, p, part);
-    else launch_mid<RT, 4, 8>(s, p, part);
+    if (p.rows == 2) p.strips == 3 ? launch_mid<2, 3, 8>(s, p, part) : launch_mid<2, 4, 8>(s, p, part);
+    else if (p.strips == 1) launch_mid<1, 1, 8>(s, p, part);
+    else if (p.strips == 2) launch_mid<1, 2, 8>(s, p, part);
+    else if (p.strips == 3) launch_mid<1, 3, 8>(s, p, part);
+    else launch_mid<1, 4, 8>(s, p, part);
 }
 
 uint32_t parts_of(uint64_t x, uint32_t y) { return static_cast<uint32_t>((x + y - 1) / y); }
@@ -911,7 +911,7 @@ bool matmul_i4_lay_out(I4Gemm &p)
     if (p.M > 4 && p.M <= 512 && short_offsets)
         for (uint32_t t = 1; t <= 4; ++t) {
             consider(I4Gemm::kMid, 1, t, 8);
-            if (p.M > 16) consider(I4Gemm::kMid, 2, t, 8);
+            if (p.M > 16 && t >= 3) consider(I4Gemm::kMid, 2, t, 8);
         }
     if (p.M > 16 || !short_offsets) {
         consider(I4Gemm::kTile, 2, 1, 4);
@@ -944,7 +944,7 @@ void matmul_i4(hipStream_t s, const I4Gemm &p, void *ws)
     }
     float *part = p.splits > 1 ? static_cast<float *>(ws) : nullptr;
     if (p.kernel == I4Gemm::kFew) p.rows == 1 ? launch_few_of<1>(s, p, part) : launch_few_of<2>(s, p, part);
-    else p.rows == 1 ? launch_mid_of<1>(s, p, part) : launch_mid_of<2>(s, p, part);
+    else launch_mid_of(s, p, part);
     if (part) {
         I4Tiles tl{};
         tl.splits = p.splits;

@@ -86,6 +86,18 @@ def test_sizes_of_models(gpu, M, K, N, group):
     case(gpu, M, K, N, group)
 
 
+@pytest.mark.parametrize("M,K,N", [
+    (1, 2048, 48), (1, 16384, 16), (1, 2048, 6000), (1, 16384, 1001), (3, 64, 16), (3, 8192, 16), (2, 64, 11008), (2, 11008, 6000),
+    (1, 300, 16001), (4, 8192, 2048), (5, 2048, 16), (7, 16384, 16), (8, 2048, 6000), (6, 16384, 1001), (5, 64, 17), (8, 4096, 16),
+    (5, 100, 11008), (5, 64, 16000), (6, 4096, 2048), (9, 64, 16), (13, 2048, 16), (9, 64, 6000), (17, 4096, 500), (9, 64, 11008),
+    (48, 4096, 1001), (17, 64, 8192), (17, 4096, 1001), (17, 64, 11008), (33, 2000, 11008), (17, 64, 16000), (19, 8192, 2048),
+    (600, 64, 16), (601, 1000, 16), (600, 64, 4096), (601, 100, 6000), (600, 64, 11008), (600, 700, 300)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_every_kernel(gpu, M, K, N, group):
+    """Sizes that between them take every kernel and cut, as test_serving_host has them."""
+    case(gpu, M, K, N, group, zeros=group != 128, bias=N % 2 == 1)
+
+
 @pytest.mark.parametrize("M", [1, 5, 20, 70, 130])
 @pytest.mark.parametrize("epilogue", [0, 1, 2, 3, 4])
 @pytest.mark.parametrize("bias", [False, True])

@@ -105,3 +105,42 @@ def test_names_and_null_arguments():
     assert lib.vnpu_pack_weights_i4(None, None, None, None, 1, 1, 0, 0, 0, C.byref(out)) == abi.ERR_INVALID_ARGUMENT
     assert lib.vnpu_packed_weights_i4_info(None, None, None, None, None) == abi.ERR_INVALID_ARGUMENT
     lib.vnpu_packed_weights_i4_destroy(None)
+
+
+def test_every_kernel_of_the_products_is_some_call_s():
+    """Strips and waves of few rows, rows and strips of tens of rows, tiles of four shapes; with and without ranges of K."""
+    seen = set()
+    for M in (1, 2, 4, 5, 8, 9, 16, 17, 48, 96, 128, 256, 600, 2048):
+        for K in (64, 300, 1000, 2048, 4096, 8192, 16384):
+            for N in (16, 500, 1001, 2048, 4096, 6000, 11008, 16000, 32000):
+                name, rows, strips, waves, splits, _ = route(*matmul(M=M, K=K, N=N)).split()
+                seen.add((name, int(rows[5:]), int(strips[7:]), int(waves[6:])))
+                assert 1 <= int(splits[7:]) <= 8
+                assert name == "few" or M > 4
+                assert name != "few" or M <= 8
+    few = {("few", r, t, w) for r in (1, 2) for t, w in ((1, 16), (2, 16), (2, 8), (3, 8), (4, 8))}
+    mid = {("mid", 1, t, 8) for t in (1, 2, 3, 4)} | {("mid", 2, t, 8) for t in (3, 4)}
+    assert seen == few | mid | {("tile", r, t, 4) for r, t in ((2, 1), (2, 2), (4, 2), (4, 4))}
+
+
+def test_rows_too_far_apart_for_32_bits_go_in_tiles():
+    assert route(*matmul(M=1, K=64, N=64, lda=1 << 31)).startswith("few")   # one row
+    assert route(*matmul(M=2, K=64, N=64, lda=1 << 30)).startswith("tile")
+    assert route(*matmul(M=2, K=64, N=64, lda=1 << 20)).startswith("few")
+
+
+def test_routes_of_a_shared_prefix():
+    """Few rows against the prefix and own keys, tiles against the prefix, tiles on both sides."""
+    def text(batch, n, prefix_len, mine):
+        c = dict(page_size=16, kv_heads=8, head_dim=128, table_ld=1 << 14)
+        words = route(*prefix(c=c, prefix_len=prefix_len, batch=batch, tokens=batch * n, heads=32,
+                              max_kv=prefix_len + mine)).split()
+        at = words.index("own:")
+        return [dict(x.split("=") for x in words[a:b]) for a, b in ((1, at), (at + 1, at + 5))]
+
+    shared, own = text(2, 1, 320, 40)
+    assert shared["few"] != "0" and own["few"] != "0" and shared["tile"] == own["tile"] == "0"
+    shared, own = text(32, 1, 4096, 500)
+    assert shared["tile"] == "64" and int(shared["parts"]) > 4 and own["few"] == "32" and own["tile"] == "0"
+    shared, own = text(4, 300, 2048, 700)
+    assert shared["tile"] != "0" and own["tile"] != "0" and own["few"] == "0"
