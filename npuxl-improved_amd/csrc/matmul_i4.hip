@@ -377,16 +377,26 @@ void launch_few(hipStream_t s, const I4Gemm &p, float *part)
 // Place in 8 of K of a fragment's element e: the order in which codes come out of a word.
 __device__ __forceinline__ constexpr uint32_t order(uint32_t e) { return (e & 4) | (e & 1) << 1 | (e >> 1 & 1); }
 
-// Codes of 32 of K: words w of a strip's block, their lower or upper halves, less zero.
+// Codes of 32 of K: words w of a strip's block, their lower or upper halves, less zero.  The mask
+// and the exponent bits are in registers: as literals they would take an instruction each.
+struct Masks {
+    uint32_t low, high, bits;
+    __device__ __forceinline__ Masks()
+    {
+        asm("s_mov_b32 %0, 0x000f000f" : "=s"(low));
+        asm("s_mov_b32 %0, 0x00f000f0" : "=s"(high));
+        asm("v_mov_b32 %0, 0x64006400" : "=v"(bits));
+    }
+};
 template <bool HIGH>
-__device__ __forceinline__ v8h differences(uint32_t w0, uint32_t w1, v2h zero)
+__device__ __forceinline__ v8h differences(const Masks &m, uint32_t w0, uint32_t w1, v2h zero)
 {
     auto two = [&](uint32_t w) {
         if constexpr (HIGH) {   // 1024 + 16 code
-            const v2h x = __builtin_bit_cast(v2h, (w & 0x00f000f0u) | 0x64006400u), sixteenth = {0.0625f16, 0.0625f16};
+            const v2h x = __builtin_bit_cast(v2h, (w & m.high) | m.bits), sixteenth = {0.0625f16, 0.0625f16};
             return __builtin_elementwise_fma(x, sixteenth, v2h{960.0f16, 960.0f16} - zero);
         } else {
-            return __builtin_bit_cast(v2h, (w & 0x000f000fu) | 0x64006400u) - zero;
+            return __builtin_bit_cast(v2h, (w & m.low) | m.bits) - zero;
         }
     };
     const v2h a = two(w0), b = two(w0 >> 8), c = two(w1), d = two(w1 >> 8);
@@ -408,6 +418,7 @@ __global__ __launch_bounds__(64 * W) void matmul_i4_mid(I4Gemm p, uint32_t per, 
     const uint32_t rows = min(p.M - row0, 16u * RT), last = min(p.K, 128 * end);
     const auto a = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(p.A) + static_cast<uint64_t>(row0) * p.lda, 0,
                                                      ((rows - 1) * p.lda + p.K) * 4, kBufferWord3);
+    const Masks masks;
     struct Block {
         Weights<T, GB> w;
         v4f x[RT][4][2];
@@ -487,7 +498,7 @@ __global__ __launch_bounds__(64 * W) void matmul_i4_mid(I4Gemm p, uint32_t per, 
                 constexpr int of = 4 / GB;   // of 32 of K in a group
                 const _Float16 z = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x6400 + b.w.zero[t][h / of]));   // 1024 + zero
                 const uint32_t w0 = static_cast<uint32_t>(b.w.codes[t][2 * (h & 1)]), w1 = static_cast<uint32_t>(b.w.codes[t][2 * (h & 1) + 1]);
-                const v8h w = h < 2 ? differences<false>(w0, w1, v2h{z, z}) : differences<true>(w0, w1, v2h{z, z});
+                const v8h w = h < 2 ? differences<false>(masks, w0, w1, v2h{z, z}) : differences<true>(masks, w0, w1, v2h{z, z});
 #pragma unroll
                 for (int r = 0; r < RT; ++r) acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[r][h], w, h % of ? acc[r] : v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
@@ -569,7 +580,7 @@ void launch_mid(hipStream_t s, const I4Gemm &p, float *part)
 
 // A workgroup has 16 rows and a part of their blocks; it looks for the rows' largest
 // itself, in all of K.
-constexpr uint32_t kSplitThreads = 512;
+constexpr uint32_t kSplitThreads = 1024;
 template <bool ALIGNED>
 __global__ __launch_bounds__(kSplitThreads) void matmul_i4_split(I4Gemm p, uint32_t row0, int8_t *frags, float *down)
 {
@@ -582,17 +593,17 @@ __global__ __launch_bounds__(kSplitThreads) void matmul_i4_split(I4Gemm p, uint3
         const float *row = p.A + static_cast<uint64_t>(min(row0 + tile * 16 + r, p.M - 1)) * p.lda;
         uint32_t most = 0;
         if constexpr (ALIGNED) {
-#pragma unroll 4
+#pragma unroll 8
             for (uint32_t k = 4 * at; k < p.K; k += kSplitThreads / 4) {
                 const v4f x = *reinterpret_cast<const v4f *>(row + k);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
             }
         } else {
-#pragma unroll 4
+#pragma unroll 8
             for (uint32_t k = at; k < p.K; k += kSplitThreads / 16) most = max(most, __float_as_uint(row[k]) & 0x7fffffffu);
         }
-        for (int o = 16; o; o >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o)));
+        for (int o = kSplitThreads / 32; o; o >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o)));
         if (at == 0) largest[r] = most;
     }
     __syncthreads();
@@ -702,40 +713,54 @@ __global__ __launch_bounds__(256, RT * CT <= 16 ? 2 : 1) void matmul_i4_tile(I4G
     load(now, begin);
     lds::wait_vmcnt<0>();
     __syncthreads();
+    const Masks masks;
+    constexpr int per = 4 / GB;   // of 32 of K in a group
+    auto weights = [&](int h, int t) {
+        const _Float16 z = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x6400 + now.zero[t][h / per]));   // 1024 + zero
+        const uint32_t w0 = static_cast<uint32_t>(now.codes[t][2 * (h & 1)]), w1 = static_cast<uint32_t>(now.codes[t][2 * (h & 1) + 1]);
+        return h < 2 ? differences<false>(masks, w0, w1, v2h{z, z}) : differences<true>(masks, w0, w1, v2h{z, z});
+    };
     for (uint32_t kb = begin; kb < end; ++kb) {
         const int8_t *buf = lds + ((kb - begin) & 1) * kStage;
         if (kb + 1 < end) {
             copy(kb + 1, lds + ((kb + 1 - begin) & 1) * kStage);
             load(next, kb + 1);
         }
+        // Steps of 32 of K and a row tile.  A step's fragments are read a step ahead, the next 32 of K's weights are
+        // made beside its products.
+        auto fragment = [&](int step, int part) { return *reinterpret_cast<const v8h *>(buf + (step % RT * 8 + 2 * (step / RT) + part) * 1024 + lane * 16); };
+        v8h hi = fragment(0, 0), lo = fragment(0, 1), b[CT], soon[CT];
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            constexpr int per = 4 / GB;   // of 32 of K in a group
-            v8h b[CT];
+        for (int t = 0; t < CT; ++t) b[t] = weights(0, t);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // the first step's
 #pragma unroll
-            for (int t = 0; t < CT; ++t) {
-                const _Float16 z = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x6400 + now.zero[t][h / per]));   // 1024 + zero
-                const v2h zero = {z, z};
-                const uint32_t w0 = static_cast<uint32_t>(now.codes[t][2 * (h & 1)]), w1 = static_cast<uint32_t>(now.codes[t][2 * (h & 1) + 1]);
-                b[t] = h < 2 ? differences<false>(w0, w1, zero) : differences<true>(w0, w1, zero);
-            }
+        for (int step = 0; step < 4 * RT; ++step) {
+            const int h = step / RT, r = step % RT;
+            const v8h next_hi = step + 1 < 4 * RT ? fragment(step + 1, 0) : hi, next_lo = step + 1 < 4 * RT ? fragment(step + 1, 1) : lo;
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const v8h hi = *reinterpret_cast<const v8h *>(buf + (r * 8 + 2 * h) * 1024 + lane * 16);
-                const v8h lo = *reinterpret_cast<const v8h *>(buf + (r * 8 + 2 * h + 1) * 1024 + lane * 16);
+            for (int t = 0; t < CT; ++t)
+                acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, b[t], h % per ? acc[r][t] : v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-                for (int t = 0; t < CT; ++t)
-                    acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, b[t], h % per ? acc[r][t] : v4f{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+            for (int t = 0; t < CT; ++t) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, b[t], acc[r][t], 0, 0, 0);
+            if (h < 3)
 #pragma unroll
-                for (int t = 0; t < CT; ++t) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, b[t], acc[r][t], 0, 0, 0);
-            }
+                for (int t = r * CT / RT; t < (r + 1) * CT / RT; ++t) soon[t] = weights(h + 1, t);
             if (h % per == per - 1) {
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
+                for (int t = 0; t < CT; ++t)
 #pragma unroll
-                    for (int t = 0; t < CT; ++t)
+                    for (int i = 0; i < 4; ++i) total[r][t][i] = fmaf(acc[r][t][i], now.scale[t][h / per], total[r][t][i]);
+            }
+            hi = next_hi;
+            lo = next_lo;
+            if (r == RT - 1)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) total[r][t][i] = fmaf(acc[r][t][i], now.scale[t][h / per], total[r][t][i]);
+                for (int t = 0; t < CT; ++t) b[t] = soon[t];
+            if (step + 1 < 4 * RT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // the next step's, then each product with what else there is
+#pragma unroll
+            for (int t = 0; t < 2 * CT; ++t) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
             }
         }
         lds::wait_vmcnt<0>();
@@ -820,7 +845,7 @@ void launch_tiles(hipStream_t s, const I4Gemm &p, int8_t *ws)
         tl.col_tiles = (p.Np + 64 * p.strips - 1) / (64 * p.strips);
         tl.splits = p.splits;
         tl.per = p.per;
-        const uint32_t tiles = tl.row_tiles * p.rows, parts = std::max(1u, std::min(2 * p.cus / tiles, p.KB / 2));
+        const uint32_t tiles = tl.row_tiles * p.rows, parts = std::max(1u, std::min(p.cus / tiles, p.KB / 4));
         (aligned ? matmul_i4_split<true> : matmul_i4_split<false>)<<<dim3(tiles, parts), kSplitThreads, 0, s>>>(p, row0, frags, down);
         if (p.rows == 2 && p.strips == 1) launch_tile<2, 1>(s, p, tl, frags, down, part);
         else if (p.rows == 2) launch_tile<2, 2>(s, p, tl, frags, down, part);
