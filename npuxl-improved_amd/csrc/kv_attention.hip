@@ -965,17 +965,21 @@ __device__ __forceinline__ uint32_t ranges_of(const Tiles &tl, uint32_t chunks)
 }
 
 // A workgroup's place among the tiles of all kv heads and its key range.
-template <int DP, int RT, bool FULL, int WAVES>
-__device__ __forceinline__ void tile_of(const KvAttn &p, const Tiles &tl, float *ws, const uint32_t place, const uint32_t range)
+// DIM: a head's dimensions, where they are not the call's alone; with the keys of the call's shared prefix
+// too, whose pages are in `prefix`.
+template <int DP, int RT, bool FULL, int WAVES, int DIM = 0>
+__device__ __forceinline__ void tile_of(const KvAttn &p, const Tiles &tl, float *ws, const uint32_t place, const uint32_t range,
+                                        const int32_t *prefix = nullptr)
 {
-    constexpr int DS = DP / 64, DT = DP / 16;
+    constexpr int DS = DP / 64, DT = DIM ? DIM / 16 : DP / 16;
+    constexpr bool PREFIX = DIM > 0;
     constexpr uint32_t M = 16 * RT * WAVES;
     constexpr uint32_t kK = 4 * DS * 1024, kV = DT * 2048, kBuf = kK + kV;   // bytes of a chunk's operands
     extern __shared__ __align__(1024) int8_t lds[];
     const KvCall &c = p.call;
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t G = c.c.kv_heads, h = place % G, D = FULL ? DP : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
+    const uint32_t G = c.c.kv_heads, h = place % G, D = FULL ? DP : DIM ? DIM : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
     if (place == 0 && range == 0) kv::check_all(c, false, p.max_kv, p.max_tokens, p.causal);
     // The last tiles of a causal sequence have the most keys: they come first.
     uint32_t b, tile, len;
@@ -984,7 +988,7 @@ __device__ __forceinline__ void tile_of(const KvAttn &p, const Tiles &tl, float 
     if (!find_tile<M>(p, tl, group, unit, b, tile) || !tile_sequence(p, tl, group, b, seq, len)) return;
     b = __builtin_amdgcn_readfirstlane(b);
     tile = __builtin_amdgcn_readfirstlane(tile);
-    len = __builtin_amdgcn_readfirstlane(len);
+    len = __builtin_amdgcn_readfirstlane(len) + (PREFIX ? c.skip : 0);
     const uint32_t rows = __builtin_amdgcn_readfirstlane(seq.n) * group, n = __builtin_amdgcn_readfirstlane(seq.n);
     if (static_cast<uint64_t>(tile) * M >= rows) return;
     const uint32_t row0 = tile * M + wave * 16 * RT;   // the wave's first
@@ -1011,16 +1015,18 @@ __device__ __forceinline__ void tile_of(const KvAttn &p, const Tiles &tl, float 
     }
 
     const uint32_t kb = col >> 2, last16 = len ? (len - 1) / 16 : 0, log16 = c.c.log_page - 4;
-    const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld + (c.skip >> c.c.log_page);
+    const uint32_t shared = c.skip >> c.c.log_page;
+    const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld + (PREFIX ? 0 : shared);
     auto checked = [&](int32_t id) -> uint32_t {
         if (static_cast<uint32_t>(id) < c.c.pages) return static_cast<uint32_t>(id);
         kv::fail(c.err);
         return 0;
     };
     int32_t k_id = 0, v_id = 0;
+    auto id_of = [&](uint32_t page) { return PREFIX ? (page < shared ? prefix : table)[page] : table[page]; };
     auto ids = [&](uint32_t chunk) {
-        k_id = table[min(4 * chunk + kb, last16) >> log16];
-        v_id = table[min(4 * chunk + g, last16) >> log16];
+        k_id = id_of(min(4 * chunk + kb, last16) >> log16);
+        v_id = id_of(min(4 * chunk + g, last16) >> log16);
     };
     constexpr int VW = (DT + WAVES - 1) / WAVES, KW = (4 * DS + WAVES - 1) / WAVES;   // tiles of V, pieces of K that a wave brings in
     v4i vf[VW];
@@ -1236,13 +1242,21 @@ __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attenti
 {
     tile_of<DP, RT, FULL, WAVES>(p, tl, ws, blockIdx.x, blockIdx.y);
 }
+constexpr int padded_dims(int dims) { return dims <= 64 ? 64 : dims <= 128 ? 128 : 256; }
+// For each head_dim: with one kernel for up to 128, dimensions that a head does not have cost branches among the
+// products (865 rows of 16 heads of 80, 2000 keys and up to 777: 62.8 us, 58.3 so).
+template <int D, int RT>
+__global__ __launch_bounds__(256, padded_dims(D) * RT <= 128 ? 3 : 2) void kv_attention_tile_through(KvAttn p, Tiles tl, float *ws, const int32_t *prefix)
+{
+    tile_of<padded_dims(D), RT, D == padded_dims(D), 4, D>(p, tl, ws, blockIdx.x, blockIdx.y, prefix);
+}
 
 // A tile's key ranges, at most 64, together: kJoinRows rows a wave, a range's
 // weight a lane.  Lanes behind head_dim load its last element: loads under a
 // condition are waited for one by one (10.8 us instead of 7.9 for 220 tiles of 64 rows
 // and up to 5 ranges).
 constexpr int kJoinRows = 2;
-template <uint32_t M, int DS>
+template <uint32_t M, int DS, bool PREFIX = false>
 __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, const float *ws)
 {
     const KvCall &c = p.call;
@@ -1252,6 +1266,7 @@ __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, con
     if (!find_tile<M>(p, tl, group, unit, b, tile) || !tile_sequence(p, tl, group, b, seq, len)) return;
     const uint32_t lane = threadIdx.x & 63, in = (blockIdx.y * 4 + (threadIdx.x >> 6)) * kJoinRows, row = tile * M + in;
     if (static_cast<uint64_t>(tile) * M + in >= static_cast<uint64_t>(seq.n) * group) return;
+    if constexpr (PREFIX) len += c.skip;
     const uint32_t ranges = __builtin_amdgcn_readfirstlane(ranges_of(tl, tile_chunks<M>(p, len, seq.n, tile, group)));
     if (ranges == 1) return;   // written by the tile itself
     const uint64_t step = static_cast<uint64_t>(M) * (D + 4);
@@ -1756,6 +1771,74 @@ bool launch_both(hipStream_t s, const Side &shared, const Plan &shared_plan, con
     return true;
 }
 
+// One pass over the prefix and what lies behind it, by tiles of a sequence's rows: no results to write, read
+// and join, but a sequence's last tile has the prefix's keys too, however few its rows.  Ragged sequences leave
+// half a tile each.  (110 calls of 1 to 128 sequences: one pass 1.28 times as fast at the mean; 128 sequences of up
+// to 60 tokens behind 320, 32 heads on 8 of 128: 113 us, in two parts 244; 6 sequences of up to 24 tokens behind 16384,
+// 16 heads on 8: 82 and 46.  Of the faster of both this choice loses 0.8% at the mean, 16% at most.)
+bool through(const KvAttn &own)
+{
+    const KvCall &c = own.call;
+    const uint32_t G = c.c.kv_heads, group = own.heads / G;
+    const uint64_t rows = static_cast<uint64_t>(own.max_tokens) * group, chunks = (c.skip + kChunk - 1) / kChunk;
+    if (rows <= few_rows(own)) return false;
+    const double empty = c.seq_start ? 0.5 : static_cast<double>((rows + 63) / 64) - static_cast<double>(rows) / 64;
+    return 2.0 * empty * c.batch * G * static_cast<double>(chunks) <= static_cast<double>(c.tokens) * own.heads;
+}
+// Its tiles and key ranges, by a fit of 110 calls in 1900 ways (the choice is 3% from the fastest at the mean):
+// the start, the fullest CU's chunks (64 keys of 128 dimensions take a workgroup of 64 rows 1.45 us alone, 0.87 of its CU's
+// beside others, of 128 rows 2.1 and 1.6), each range's results written and read by the join.
+Plan plan_through(const KvAttn &own)
+{
+    const KvCall &c = own.call;
+    const uint32_t G = c.c.kv_heads, group = own.heads / G, D = c.c.head_dim, DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    const uint64_t rows = static_cast<uint64_t>(own.max_tokens) * group, all = static_cast<uint64_t>(c.tokens) * group;
+    const uint32_t chunks = (own.max_kv + c.skip + kChunk - 1) / kChunk;
+    Plan r;
+    r.tiled = true;
+    double least = 1e30;
+    for (uint32_t M = 64; M <= (D <= 128 ? 128u : 64u); M += 64) {
+        const uint64_t per_seq = (rows + M - 1) / M, count = c.seq_start ? all / M + c.batch : per_seq * c.batch;
+        const uint64_t tiles = (c.seq_start ? all / M + (c.batch + 1) / 2 : count) * G;
+        for (uint32_t parts = 1; parts <= std::min(chunks, 64u); ++parts) {
+            const uint64_t load = (tiles * parts + own.cus - 1) / own.cus;
+            const uint32_t per = (chunks + parts - 1) / parts;
+            const double alone = M == 64 ? 0.41 + 0.0081 * DP : 1.1 + 0.008 * DP;
+            const double beside = M == 128 ? 0.75 + 0.0066 * DP : D > 128 ? alone : 0.41 + 0.0036 * DP;
+            const double us = (M == 64 ? 5.0 : 8.0) + per * std::max(alone, load * beside) +
+                              (parts > 1 ? 5.7 + 1.3e-6 * static_cast<double>(all * G * parts) * (D + 4) : 0.0);
+            if (us >= least) continue;
+            least = us;
+            r.tile_rows = M;
+            r.tiles.per_seq = static_cast<uint32_t>(per_seq);
+            r.tiles.count = static_cast<uint32_t>(count);
+            r.tiles.parts = parts;
+            r.tiles.per = per;
+            r.ws = parts > 1 ? static_cast<size_t>(count) * G * parts * M * (D + 4) * sizeof(float) : 0;
+        }
+    }
+    return r;
+}
+template <int D, int RT>
+void launch_through(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws, const int32_t *prefix)
+{
+    constexpr int DP = padded_dims(D);
+    const auto kernel = kv_attention_tile_through<D, RT>;
+    allow_lds(kernel, tile_lds<DP>());
+    const uint32_t grid = pl.tiles.count * p.call.c.kv_heads;
+    kernel<<<dim3(grid, pl.tiles.parts), 256, tile_lds<DP>(), s>>>(p, pl.tiles, ws, prefix);
+    if (pl.tiles.parts > 1) kv_attention_join<64 * RT, DP / 64, true><<<dim3(grid, 16 * RT / kJoinRows), 256, 0, s>>>(p, pl.tiles, ws);
+}
+template <int D = 16>
+void launch_through(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws, const int32_t *prefix)
+{
+    if constexpr (D <= 256) {
+        if (p.call.c.head_dim != D) launch_through<D + 16>(s, p, pl, ws, prefix);
+        else if (D > 128 || pl.tile_rows == 64) launch_through<D, 1>(s, p, pl, ws, prefix);
+        else if constexpr (D <= 128) launch_through<D, 2>(s, p, pl, ws, prefix);
+    }
+}
+
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 void launch_any(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
@@ -1802,11 +1885,16 @@ static uint64_t groups_of(const KvAttn &p)
 
 size_t kv_prefix_attention_ws_bytes(const KvAttn &own, const int32_t *prefix_table)
 {
+    if (through(own)) return plan_through(own).ws;
     return padded(plan_of(own).ws) + padded(plan_of(shared_call(own, prefix_table)).ws);
 }
 
 bool kv_prefix_attention_fits(const KvAttn &own, const int32_t *prefix_table)
 {
+    if (through(own)) {
+        const Tiles tl = plan_through(own).tiles;
+        return static_cast<uint64_t>(tl.count) * own.call.c.kv_heads * 256 < (1ull << 32);
+    }
     return kv_attention_fits(own) && kv_attention_fits(shared_call(own, prefix_table)) &&
            static_cast<uint64_t>(own.call.tokens) * own.heads * 64 < (1ull << 32) - 256 &&
            groups_of(own) + groups_of(shared_call(own, prefix_table)) < (1ull << 23);
@@ -1814,11 +1902,24 @@ bool kv_prefix_attention_fits(const KvAttn &own, const int32_t *prefix_table)
 
 std::string kv_prefix_attention_route(const KvAttn &own, const int32_t *prefix_table)
 {
+    if (through(own)) {
+        const Plan pl = plan_through(own);
+        char text[96];
+        std::snprintf(text, sizeof(text), "through: tile=%u parts=%u", pl.tile_rows, pl.tiles.parts);
+        return text;
+    }
     return "shared: " + kv_attention_route(shared_call(own, prefix_table)) + " own: " + kv_attention_route(own);
 }
 
 void kv_prefix_attention(hipStream_t s, const KvAttn &own, const int32_t *prefix_table, void *ws)
 {
+    if (through(own)) {
+        KvAttn p = own;
+        p.partial = 0;
+        const Plan pl = plan_through(own);
+        launch_through(s, p, pl, static_cast<float *>(ws), prefix_table);
+        return;
+    }
     const KvAttn shared = shared_call(own, prefix_table);
     const Plan own_plan = plan_of(own), shared_plan = plan_of(shared);
     float *own_ws = static_cast<float *>(ws), *shared_ws = own_ws + padded(own_plan.ws) / sizeof(float);

@@ -6,6 +6,7 @@ import pytest
 
 import kv_ops as kv
 import serving_ops as ops
+from gpu_ops import route
 from vnpu_mi355x import Session, abi
 
 pytestmark = pytest.mark.gpu
@@ -123,6 +124,29 @@ def test_ragged(gpu, causal, d, heads, kv_heads, page):
 @pytest.mark.parametrize("batch", [1, 2, 7])
 def test_row_counts(gpu, batch, n):
     case(gpu, 8, 2, 64, 16, 208, [n + 20] * batch, [n] * batch, ragged=batch == 2)
+
+
+# One pass over the prefix and what lies behind it, by tiles of 64 and 128 rows, each in one and in several ranges of
+# keys; the ranges are joined where they are several.
+@pytest.mark.parametrize("d", range(16, 257, 16))
+@pytest.mark.parametrize("batch,n,prefix,parts", [(40, 33, 64, False), (2, 150, 1024, True)])
+def test_through_the_prefix(gpu, d, batch, n, prefix, parts):
+    x = Call(gpu, 8, 4, d, 16, prefix, [n + 45 + b % 7 for b in range(batch)], [n - b % 3 for b in range(batch)])
+    way = route(abi.OP_KV_PREFIX_ATTENTION_I8, attention=abi.KvAttentionArgs(**x.args), prefix_table=x.held[2].ptr, prefix_len=prefix)
+    assert way.startswith("through: tile=64") and (way.split()[2] != "parts=1") == parts, way
+    x.check(x.run())
+    x.check(x.run(causal=1, max_tokens=n, max_kv=prefix + n + 60))
+    x.free()
+
+
+@pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("heads,kv_heads,batch,n,prefix,parts", [(16, 16, 6, 500, 320, False), (8, 2, 6, 257, 4000, True)])
+def test_through_the_prefix_by_large_tiles(gpu, d, heads, kv_heads, batch, n, prefix, parts):
+    x = Call(gpu, heads, kv_heads, d, 32, prefix, [n + 50 - b % 3 for b in range(batch)], [n - 2 * b for b in range(batch)])
+    way = route(abi.OP_KV_PREFIX_ATTENTION_I8, attention=abi.KvAttentionArgs(**x.args), prefix_table=x.held[2].ptr, prefix_len=prefix)
+    assert way.startswith("through: tile=128") and (way.split()[2] != "parts=1") == parts, way
+    x.check(x.run())
+    x.free()
 
 
 @pytest.mark.parametrize("layout", ["rows", "wide", "heads"])
