@@ -626,12 +626,13 @@ typedef struct vnpu_kv_read_f32_args_t {
 /* MI355X extension (additive): products with 4-bit weights.
  * C[m][n] = epi(sum over k of A[m][k] * w[k][n] + bias[n]), w[k][n] = (code -
  * zero[k / group_size][n]) * scale[k / group_size][n] as packed.  Differences code
- * - zero are whole numbers and enter exactly; an element of A enters to 2^-29 of
- * the largest of its row among the same 128 of K (up to 16 rows) or to 2^-22 of
- * itself (2^-38 of the largest of its row where that is more); sums
- * are f32 or wider, each group's scaled once.  A row of A with an infinity or NaN
- * gives NaN in all of its results.  SILU, GELU_TANH and GELU_ERF are the
- * functions themselves to some 2^-21 of the result (not the polynomials of the int8
+ * - zero are whole numbers and enter exactly; an element of A enters to 2^-30 of
+ * the largest of its row among the same 128 of K (kernel of up to 8 rows), or to
+ * 2^-23 of itself (2^-39 of the largest of its row, or of its row's same 128, where
+ * that is more); sums are f32 or wider, each group's scaled once.  M, K and N choose the
+ * kernel.  A row of A with an infinity or NaN gives NaN in all of its results.
+ * M is up to 2^28, K and N up to 2^30.  SILU, GELU_TANH and GELU_ERF are the functions
+ * themselves in f32, to some 2^-21 of the result (not the polynomials of the int8
  * and f32 products). `workspace`: as in vnpu_kv_attention_i8_args_t, its bytes
  * from vnpu_matmul_i4_workspace. */
 typedef struct vnpu_matmul_i4_args_t {
@@ -689,7 +690,8 @@ typedef struct vnpu_rope_axes_f32_args_t {
 } vnpu_rope_axes_f32_args_t;
 
 /* MI355X extension (additive): KV_ATTENTION_I8 of a batch whose sequences all begin
- * with the same prefix_len cached tokens, which are read once for all of them.
+ * with the same prefix_len cached tokens, which are read once for all of them (or
+ * once for 64 or 128 rows of a sequence where it has as many).
  * Token j < prefix_len of every sequence is in the pages of prefix_table, the
  * others are in the sequence's row of attention.cache.table as always; entries of
  * that row below prefix_len / page_size are not read.  prefix_len is a whole
