@@ -1569,7 +1569,7 @@ void enqueue_kv_noalloc(vnpu_stream_t *s, const vnpu_command_t *commands, uint64
                 const k::KvAttn p = kv_prefix_params(s, a, {}, table);
                 const size_t need = k::kv_prefix_attention_ws_bytes(p, table);
                 void *ws = given_workspace(a.attention.workspace, a.attention.workspace_bytes, need);
-                require(ws, "this kv_prefix_attention needs a workspace");
+                require(ws || !need, "this kv_prefix_attention needs a workspace");
                 if (!pass) continue;
                 k::kv_prefix_attention(s->hip, p, table, ws);
                 VNPU_HIP(hipGetLastError());

@@ -314,6 +314,25 @@ def test_workspace_of_the_size_asked_for(own, batch, n):
         s.close()
 
 
+# 64-row tiles in one range write their results themselves and need no workspace; several ranges need one.
+@pytest.mark.parametrize("batch,n,prefix,parts", [(40, 33, 64, False), (2, 150, 1024, True)])
+def test_through_the_prefix_without_allocation(own, batch, n, prefix, parts):
+    x = Call(own, 8, 4, 64, 16, prefix, [n + 45] * batch, [n] * batch)
+    want = x.run()
+    cmds = (abi.Command * 1)(x.command())
+    need = own.lib.vnpu_kv_prefix_attention_workspace(own.dev, C.byref(cmds[0].args.kv_prefix_attention))
+    assert (need > 0) == parts
+    own.write(x.ro.buffer, np.full_like(want, 7.0))
+    assert own.lib.vnpu_kv_enqueue_noalloc(own.stream, cmds, 1) == (abi.ERR_INVALID_ARGUMENT if parts else abi.OK)
+    if parts:
+        ws = own.alloc(need)
+        cmds[0] = x.command(workspace=ws.ptr, workspace_bytes=need)
+        assert own.lib.vnpu_kv_enqueue_noalloc(own.stream, cmds, 1) == abi.OK
+    assert own.sync() == abi.OK
+    assert np.array_equal(x.ro.download(own), want)
+    x.check(want)
+
+
 def test_the_same_call_gives_the_same_bits(gpu):
     for n in (1, 33):
         x = Call(gpu, 8, 2, 128, 16, 2048, [n + 300] * 9, [n] * 9)
