@@ -130,17 +130,21 @@ def test_rows_too_far_apart_for_32_bits_go_in_tiles():
 
 
 def test_routes_of_a_shared_prefix():
-    """Few rows against the prefix and own keys, tiles against the prefix, tiles on both sides."""
-    def text(batch, n, prefix_len, mine):
+    """Few rows against the prefix and own keys, tiles against the prefix, tiles on both sides; one pass over both."""
+    def words(batch, n, prefix_len, mine):
         c = dict(page_size=16, kv_heads=8, head_dim=128, table_ld=1 << 14)
-        words = route(*prefix(c=c, prefix_len=prefix_len, batch=batch, tokens=batch * n, heads=32,
-                              max_kv=prefix_len + mine)).split()
-        at = words.index("own:")
-        return [dict(x.split("=") for x in words[a:b]) for a, b in ((1, at), (at + 1, at + 5))]
+        return route(*prefix(c=c, prefix_len=prefix_len, batch=batch, tokens=batch * n, heads=32, max_kv=prefix_len + mine)).split()
+
+    def text(*call):
+        w = words(*call)
+        at = w.index("own:")
+        return [dict(x.split("=") for x in w[a:b]) for a, b in ((1, at), (at + 1, at + 5))]
 
     shared, own = text(2, 1, 320, 40)
     assert shared["few"] != "0" and own["few"] != "0" and shared["tile"] == own["tile"] == "0"
     shared, own = text(32, 1, 4096, 500)
     assert shared["tile"] == "64" and int(shared["parts"]) > 4 and own["few"] == "32" and own["tile"] == "0"
-    shared, own = text(4, 300, 2048, 700)
+    shared, own = text(3, 20, 16384, 440)
     assert shared["tile"] != "0" and own["tile"] != "0" and own["few"] == "0"
+    assert words(4, 300, 2048, 700)[0] == "through:"
+    assert words(4, 17, 64, 64)[0] == "through:" and words(4, 17, 32768, 64)[0] == "shared:"
