@@ -314,6 +314,36 @@ def test_workspace_of_the_size_asked_for(own, batch, n):
         s.close()
 
 
+def tiles_of(x):
+    """Rows of a tile of the prefix's and the own part; slots of few rows of the own part."""
+    way = route(abi.OP_KV_PREFIX_ATTENTION_I8, attention=abi.KvAttentionArgs(**x.args), prefix_table=x.held[2].ptr, prefix_len=x.prefix)
+    assert way.startswith("shared: "), way
+    shared, own = (dict(w.split("=") for w in part.split()[:4]) for part in way[8:].split("own: "))
+    return int(shared["tile"]), int(own["tile"]), int(own["few"])
+
+
+# In two parts by tiles: a long prefix and too few rows for one pass; beside them sequences of few rows.
+@pytest.mark.parametrize("d", [16, 64, 80, 128, 256])
+def test_tiles_of_both_parts(gpu, d):
+    x = Call(gpu, 8, 2, d, 16, 8192, [60, 20, 41], [20] * 3, ragged=False)
+    assert tiles_of(x) == (64, 64, 0)
+    x.check(x.run())
+    x.free()
+    n = [40 if b % 8 == 3 else 1 + b % 5 for b in range(40)]
+    x = Call(gpu, 8, 4, d, 16, 8192, [m + 7 * b % 60 for b, m in enumerate(n)], n)
+    assert tiles_of(x)[:2] == (64, 64) and tiles_of(x)[2] > 0
+    x.check(x.run())
+    x.free()
+
+
+@pytest.mark.parametrize("d", [16, 128])
+def test_large_tiles_of_both_parts(gpu, d):
+    x = Call(gpu, 4, 4, d, 16, 2304, [65 + b % 16 for b in range(256)], [65] * 256, ragged=False)
+    assert tiles_of(x) == (128, 128, 0)
+    x.check(x.run())
+    x.free()
+
+
 # 64-row tiles in one range write their results themselves and need no workspace; several ranges need one.
 @pytest.mark.parametrize("batch,n,prefix,parts", [(40, 33, 64, False), (2, 150, 1024, True)])
 def test_through_the_prefix_without_allocation(own, batch, n, prefix, parts):
