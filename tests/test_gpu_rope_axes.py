@@ -70,6 +70,11 @@ def test_axes(gpu, d, sections, order, ladders, rotation):
     case(gpu, 13, 5, 2, d, sections, order, ladders, rotation)
 
 
+@pytest.mark.parametrize("tokens,heads,kv_heads", [(1, 65535, 65535), (1, 14000, 14000), (7, 65535, 1)])
+def test_as_many_heads_as_there_may_be(gpu, tokens, heads, kv_heads):
+    case(gpu, tokens, heads, kv_heads, 2, (1,))
+
+
 @pytest.mark.parametrize("tokens", [1, 2, 3, 63, 64, 65, 300, 1601])
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (32, 8), (7, 0), (0, 3), (17, 9)])
 def test_tokens_and_heads(gpu, tokens, heads, kv_heads):
