@@ -690,8 +690,8 @@ typedef struct vnpu_rope_axes_f32_args_t {
 } vnpu_rope_axes_f32_args_t;
 
 /* MI355X extension (additive): KV_ATTENTION_I8 of a batch whose sequences all begin
- * with the same prefix_len cached tokens, which are read once for all of them (or
- * once for 64 or 128 rows of a sequence where it has as many).
+ * with the same prefix_len cached tokens, which are read once for all of them (where
+ * a sequence has rows enough, or the prefix is short, once for some of its rows).
  * Token j < prefix_len of every sequence is in the pages of prefix_table, the
  * others are in the sequence's row of attention.cache.table as always; entries of
  * that row below prefix_len / page_size are not read.  prefix_len is a whole

@@ -417,9 +417,11 @@ constexpr uint32_t few_lds()
     return WAVES * (128 * DP + 1024 + RT * DP * 16) + RT * (DP / 64) * 1024;
 }
 
-// A workgroup's slot, kv head and rows from 4 RT row_tile on.
-template <int DP, int RT, bool FULL, int WAVES>
-__device__ __forceinline__ void few_rows_of(const KvAttn &p, const Split &sp, float *ws, uint32_t ws_rows, uint32_t slot, const uint32_t h, uint32_t row_tile)
+// A workgroup's slot, kv head and rows from 4 RT row_tile on.  PREFIX: a slot is a sequence, with the keys
+// of the call's shared prefix too, whose pages are in `prefix`.
+template <int DP, int RT, bool FULL, int WAVES, bool PREFIX = false>
+__device__ __forceinline__ void few_rows_of(const KvAttn &p, const Split &sp, float *ws, uint32_t ws_rows, uint32_t slot, const uint32_t h, uint32_t row_tile,
+                                            const int32_t *prefix = nullptr)
 {
     constexpr int DS = DP / 64, DT = DP / 16, R = 4 * RT;
     extern __shared__ __align__(1024) int8_t lds[];
@@ -438,16 +440,17 @@ __device__ __forceinline__ void few_rows_of(const KvAttn &p, const Split &sp, fl
     const kv::Seq seq = kv::sequence(c, b);
     const uint32_t n = __builtin_amdgcn_readfirstlane(seq.n), rows = n * group, row0 = row_tile * R;
     if (row0 >= rows) return;
-    const int len = __builtin_amdgcn_readfirstlane(kv::length(c, b));
+    const int len = __builtin_amdgcn_readfirstlane(kv::length(c, b)) + (PREFIX ? static_cast<int>(c.skip) : 0);
     // Even parts of the keys.
-    const uint32_t chunks = __builtin_amdgcn_readfirstlane(sl.chunks), part = __builtin_amdgcn_readfirstlane(sl.part);
+    const uint32_t chunks = PREFIX ? (static_cast<uint32_t>(len) + kChunk - 1) / kChunk : __builtin_amdgcn_readfirstlane(sl.chunks), part = __builtin_amdgcn_readfirstlane(sl.part);
     const uint32_t begin = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * part / parts);
     const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * (part + 1) / parts);
 
     // Pages of a chunk's four blocks of 16 keys (blocks behind the last are
     // the last) and, of the chunk in LDS, their scales.
     const uint32_t last16 = len ? (len - 1) / 16 : 0, log16 = c.c.log_page - 4, tiles = D / 16;
-    const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld + (c.skip >> c.c.log_page);
+    const uint32_t shared = c.skip >> c.c.log_page;
+    const int32_t *table = c.c.table + static_cast<uint64_t>(b) * c.c.table_ld + (PREFIX ? 0 : shared);
     bool strange = false;   // a page outside the pool: page 0 is read in its place
     int32_t id[4] = {};
     uint64_t unit[4] = {};
@@ -455,7 +458,10 @@ __device__ __forceinline__ void few_rows_of(const KvAttn &p, const Split &sp, fl
     // Asked for a chunk ahead: `pages` waits for nothing, `units` for them.
     auto pages = [&](uint32_t chunk) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) id[j] = scalar_load(table + (min(4 * chunk + j, last16) >> log16));
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t page = min(4 * chunk + j, last16) >> log16;
+            id[j] = scalar_load((PREFIX && page < shared ? prefix : table) + page);
+        }
     };
     auto units = [&]() {
 #pragma unroll
@@ -807,6 +813,12 @@ template <int DP, int RT, bool FULL, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) void kv_attention_few(KvAttn p, Split sp, float *ws, uint32_t ws_rows)
 {
     few_rows_of<DP, RT, FULL, WAVES>(p, sp, ws, ws_rows, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+template <int DP, int RT, bool FULL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) void kv_attention_few_through(KvAttn p, Split sp, const int32_t *prefix)
+{
+    few_rows_of<DP, RT, FULL, WAVES, true>(p, sp, nullptr, 0, blockIdx.x, blockIdx.y, blockIdx.z, prefix);
 }
 
 // Parts of a row, `step` floats apart, each o / l with its m and l behind it:
@@ -1842,6 +1854,47 @@ void launch_through(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws, c
     }
 }
 
+// Few rows: a sequence and kv head by one workgroup, the prefix's keys read again by each, or in two parts, which take
+// launch and join. us of the one: 5.4, and for each turn of the workgroups on the CUs and 256 keys 1 for 64 dimensions and
+// 1.6 for 128, half as much again for each 4 rows more; the two take some 12 more than half of the own keys alone.  (120 calls:
+// 1.24 times as fast at the mean as two parts always, 1.4% behind the faster of both; 16 sequences of 11 tokens behind 16, 4
+// heads on 1 of 128, 6.8 us and 12.0; 16 of 201 behind 4096, 8 heads, 32 and 20.)
+double whole_us(const KvAttn &own, uint32_t keys)
+{
+    const uint32_t G = own.call.c.kv_heads, D = own.call.c.head_dim, DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    const uint32_t rows = own.max_tokens * (own.heads / G), tile = rows <= 4 ? 4 : rows <= 8 || DP > 128 ? 8 : 16;
+    const double groups = static_cast<double>(own.call.batch) * G * ((rows + tile - 1) / tile), at_once = tile == 16 || DP > 128 ? 1 : 2;
+    const uint32_t steps = (keys + (DP > 128 ? 127u : 255u)) / (DP > 128 ? 128 : 256);
+    return 5.4 + std::max(1.0, 1.45 * groups / (own.cus * at_once)) * steps * (0.5 + 1.1 / 128 * DP) * (1.0 + 0.125 * (tile - 4));
+}
+bool few_through(const KvAttn &own)
+{
+    const uint64_t rows = static_cast<uint64_t>(own.max_tokens) * (own.heads / own.call.c.kv_heads);
+    if (rows > (own.call.c.head_dim > 128 ? 8 : 16)) return false;
+    const double alone = whole_us(own, own.max_kv);
+    return whole_us(own, own.max_kv + own.call.skip) < std::max(12.0 + 0.5 * alone, alone + 5.0);
+}
+template <int DP, int RT>
+void launch_few_through(hipStream_t s, const KvAttn &p, uint32_t rows, const int32_t *prefix)
+{
+    constexpr int W = DP > 128 ? 2 : 4;
+    constexpr uint32_t bytes = few_lds<DP, RT, W>();
+    const auto kernel = p.call.c.head_dim == DP ? kv_attention_few_through<DP, RT, true, W> : kv_attention_few_through<DP, RT, false, W>;
+    allow_lds(kernel, bytes);
+    Split sp{};
+    sp.whole = 1;
+    sp.high_rows = rows;
+    kernel<<<dim3(p.call.batch, p.call.c.kv_heads, (rows + 4 * RT - 1) / (4 * RT)), 64 * W, bytes, s>>>(p, sp, prefix);
+}
+template <int DP>
+void launch_few_through(hipStream_t s, const KvAttn &p, const int32_t *prefix)
+{
+    const uint32_t rows = p.max_tokens * (p.heads / p.call.c.kv_heads);
+    if (rows <= 4) launch_few_through<DP, 1>(s, p, rows, prefix);
+    else if (DP > 128 || rows <= 8) launch_few_through<DP, 2>(s, p, rows, prefix);
+    else if constexpr (DP <= 128) launch_few_through<DP, 4>(s, p, rows, prefix);
+}
+
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 void launch_any(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
@@ -1889,6 +1942,7 @@ static uint64_t groups_of(const KvAttn &p)
 size_t kv_prefix_attention_ws_bytes(const KvAttn &own, const int32_t *prefix_table)
 {
     if (through(own)) return plan_through(own).ws;
+    if (few_through(own)) return 0;
     return padded(plan_of(own).ws) + padded(plan_of(shared_call(own, prefix_table)).ws);
 }
 
@@ -1898,6 +1952,7 @@ bool kv_prefix_attention_fits(const KvAttn &own, const int32_t *prefix_table)
         const Tiles tl = plan_through(own).tiles;
         return static_cast<uint64_t>(tl.count) * own.call.c.kv_heads * 256 < (1ull << 32);
     }
+    if (few_through(own)) return static_cast<uint64_t>(own.call.batch) * 256 < (1ull << 32);
     return kv_attention_fits(own) && kv_attention_fits(shared_call(own, prefix_table)) &&
            static_cast<uint64_t>(own.call.tokens) * own.heads * 64 < (1ull << 32) - 256 &&
            groups_of(own) + groups_of(shared_call(own, prefix_table)) < (1ull << 23);
@@ -1911,6 +1966,7 @@ std::string kv_prefix_attention_route(const KvAttn &own, const int32_t *prefix_t
         std::snprintf(text, sizeof(text), "through: tile=%u parts=%u", pl.tile_rows, pl.tiles.parts);
         return text;
     }
+    if (few_through(own)) return "through: few";
     return "shared: " + kv_attention_route(shared_call(own, prefix_table)) + " own: " + kv_attention_route(own);
 }
 
@@ -1921,6 +1977,13 @@ void kv_prefix_attention(hipStream_t s, const KvAttn &own, const int32_t *prefix
         p.partial = 0;
         const Plan pl = plan_through(own);
         launch_through(s, p, pl, static_cast<float *>(ws), prefix_table);
+        return;
+    }
+    if (few_through(own)) {
+        KvAttn p = own;
+        p.partial = 0;
+        const uint32_t D = own.call.c.head_dim;
+        (D <= 64 ? launch_few_through<64> : D <= 128 ? launch_few_through<128> : launch_few_through<256>)(s, p, prefix_table);
         return;
     }
     const KvAttn shared = shared_call(own, prefix_table);

@@ -139,6 +139,22 @@ def test_through_the_prefix(gpu, d, batch, n, prefix, parts):
     x.free()
 
 
+# And by a workgroup for each sequence and kv head where rows are few and the prefix is short.
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("d", [16, 48, 64, 80, 128, 144, 256])
+@pytest.mark.parametrize("heads,n", [(2, 1), (2, 2), (6, 2), (2, 5), (8, 2)])
+def test_through_the_prefix_by_few_rows(gpu, page, d, heads, n):
+    mine = [n, n + 1, n + 15, n + 63, n + 70, n + 130, n]
+    for prefix, causal, ragged in ((page, 1, True), (256, 0, False), (512, 1, True)):
+        tokens = [n - b % 2 for b in range(7)] if ragged else [n] * 7
+        x = Call(gpu, heads, 2 if heads == 6 else 1, d, page, prefix, mine, tokens, causal, ragged=ragged)
+        way = route(abi.OP_KV_PREFIX_ATTENTION_I8, attention=abi.KvAttentionArgs(**x.args), prefix_table=x.held[2].ptr, prefix_len=prefix)
+        if prefix == 16:
+            assert (way == "through: few ws=0") == (n * heads // (2 if heads == 6 else 1) <= (8 if d > 128 else 16)), way
+        x.check(x.run())
+        x.free()
+
+
 @pytest.mark.parametrize("d", [16, 32, 48, 64, 80, 96, 112, 128])
 @pytest.mark.parametrize("heads,kv_heads,batch,n,prefix,parts", [(16, 16, 6, 500, 320, False), (8, 2, 6, 257, 4000, True)])
 def test_through_the_prefix_by_large_tiles(gpu, d, heads, kv_heads, batch, n, prefix, parts):
@@ -289,9 +305,9 @@ def test_a_sequence_without_tokens_may_have_any_length(gpu):
     x.free()
 
 
-@pytest.mark.parametrize("batch,n", [(4, 1), (3, 30), (40, 1)])
-def test_workspace_of_the_size_asked_for(own, batch, n):
-    x = Call(own, 8, 2, 64, 16, 1024, [n + 100] * batch, [n] * batch, ragged=False)
+@pytest.mark.parametrize("batch,n,prefix", [(4, 1, 4096), (3, 30, 1024), (40, 1, 4096)])
+def test_workspace_of_the_size_asked_for(own, batch, n, prefix):
+    x = Call(own, 8, 2, 64, 16, prefix, [n + 100] * batch, [n] * batch, ragged=False)
     want = x.run()
     cmd = x.command()
     need = own.lib.vnpu_kv_prefix_attention_workspace(own.dev, C.byref(cmd.args.kv_prefix_attention))
@@ -307,7 +323,7 @@ def test_workspace_of_the_size_asked_for(own, batch, n):
     s = Session()
     try:
         small = s.alloc(need)
-        y = Call(s, 8, 2, 64, 16, 1024, [n + 100] * batch, [n] * batch, ragged=False)
+        y = Call(s, 8, 2, 64, 16, prefix, [n + 100] * batch, [n] * batch, ragged=False)
         assert s.submit([y.command(workspace=small.ptr, workspace_bytes=need - 1)]) == abi.OK
         assert s.sync() == abi.ERR_DEVICE_ERROR
     finally:
@@ -320,6 +336,18 @@ def tiles_of(x):
     assert way.startswith("shared: "), way
     shared, own = (dict(w.split("=") for w in part.split()[:4]) for part in way[8:].split("own: "))
     return int(shared["tile"]), int(own["tile"]), int(own["few"])
+
+
+# In two parts behind a long prefix: few rows of both, and tiles of the prefix beside few rows.
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("d", [16, 48, 64, 80, 128, 192, 256])
+@pytest.mark.parametrize("batch,n", [(2, 1), (3, 2), (24, 1), (24, 3)])
+def test_few_rows_of_both_parts(gpu, page, d, batch, n):
+    x = Call(gpu, 2, 1, d, page, 4096, [n + 50 * b % 170 for b in range(batch)], [n] * batch, ragged=n == 3)
+    shared, own, few = tiles_of(x)
+    assert own == 0 and few > 0 and (shared > 0) == (batch == 24)
+    x.check(x.run())
+    x.free()
 
 
 # In two parts by tiles: a long prefix and too few rows for one pass; beside them sequences of few rows.

@@ -37,20 +37,20 @@ def within(got, want_bound):
 class Layer:
     """x -> QKV (4 bits) -> turned by three axes -> cache -> attention behind the prefix -> projection (4 bits)."""
 
-    def __init__(self, s, batch, room, seed=1, workspace=0, projections=None):
-        self.s, self.batch, self.room, self.rng = s, batch, room, np.random.default_rng(seed)
+    def __init__(self, s, batch, room, seed=1, workspace=0, projections=None, prefix=PREFIX):
+        self.s, self.batch, self.room, self.prefix, self.rng = s, batch, room, prefix, np.random.default_rng(seed)
         rng = np.random.default_rng(99)   # the model
         self.w_qkv, self.w_o = ops.Weights(rng, WIDTH, ROW, 64), ops.Weights(rng, HEADS * D, WIDTH, 128, zeros=False, trans=True)
         self.bias = normal(rng, ROW)
         self.qkv_packed, self.o_packed = projections or (self.w_qkv.pack(s), self.w_o.pack(s))
-        self.c, table = ops.shared_cache(self.rng, batch, KV_HEADS, D, PAGE, PREFIX, 400)
+        self.c, table = ops.shared_cache(self.rng, batch, KV_HEADS, D, PAGE, prefix, 400)
         self.cache, self.bufs = kv.upload(s, self.c)
         size = dict(x=room * WIDTH, qkv=room * ROW, q=room * HEADS * D, o=room * HEADS * D, y=room * WIDTH, positions=3 * room,
                     past=batch, len=batch, start=batch + 1, bias=ROW)
         self.b = {n: s.alloc(4 * v) for n, v in size.items()}
         self.b["table"] = s.upload(table)
         s.write(self.b["bias"], self.bias)
-        self.lengths = np.full(batch, PREFIX, np.int32)
+        self.lengths = np.full(batch, prefix, np.int32)
         self.ws = []
         if workspace:
             for i, cmd in enumerate(self.commands(workspace, 1, False)):
@@ -81,7 +81,7 @@ class Layer:
             s.command(abi.OP_KV_APPEND_I8, cache=self.cache, K=qkv + 4 * HEADS * D, V=qkv + 4 * (HEADS + KV_HEADS) * D,
                       past=b["past"], seq_start=start, batch=self.batch, tokens=tokens, rotation=abi.ROTATE_NONE,
                       k_token_stride=ROW, v_token_stride=ROW),
-            s.command(abi.OP_KV_PREFIX_ATTENTION_I8, attention=attention, prefix_table=b["table"], prefix_len=PREFIX),
+            s.command(abi.OP_KV_PREFIX_ATTENTION_I8, attention=attention, prefix_table=b["table"], prefix_len=self.prefix),
             s.command(abi.OP_MATMUL_I4, A=b["o"], B=self.o_packed, C=b["y"], M=tokens, K=HEADS * D, N=WIDTH),
         ]
         for held in self.ws:
@@ -146,12 +146,13 @@ def test_chunks_of_prompts_then_tokens(gpu):
     x.free()
 
 
+@pytest.mark.parametrize("prefix", [PREFIX, 4096])   # without and with workspaces
 @pytest.mark.parametrize("batch", [1, 5, 24])
-def test_captured_steps(own, batch):
+def test_captured_steps(own, batch, prefix):
     """A captured step of a token each, replayed over growing sequences with eager steps of another layer between: each
     replay is the eager step's bits, and within the oracle's bounds."""
-    x, y = Layer(own, batch, 8 * batch, workspace=batch), Layer(own, batch, 8 * batch)
-    assert any(x.ws) or batch == 1
+    x, y = Layer(own, batch, 8 * batch, workspace=batch, prefix=prefix), Layer(own, batch, 8 * batch, prefix=prefix)
+    assert any(x.ws) == (prefix > PREFIX)
     g = None
     for step in range(6):
         n = [7] * batch if step == 0 else [1] * batch
@@ -175,12 +176,13 @@ def test_captured_steps(own, batch):
     y.free()
 
 
-def test_two_graphs_at_once(own):
+@pytest.mark.parametrize("prefix", [PREFIX, 4096])
+def test_two_graphs_at_once(own, prefix):
     """Two streams of one device share the weights; each graph has its own workspaces; replayed without a wait between."""
     other = Session()
     try:
-        a = Layer(own, 6, 12, seed=3, workspace=6)
-        b = Layer(other, 6, 12, seed=4, workspace=6, projections=(a.qkv_packed, a.o_packed))
+        a = Layer(own, 6, 12, seed=3, workspace=6, prefix=prefix)
+        b = Layer(other, 6, 12, seed=4, workspace=6, projections=(a.qkv_packed, a.o_packed), prefix=prefix)
         graphs = []
         for z in (a, b):
             z.draw([1] * 6)
@@ -221,7 +223,7 @@ def test_two_streams_at_once(own):
 
 def test_noalloc_refusals_enqueue_nothing(own):
     """Host memory, a missing, small or unaligned workspace, another opcode, a bad command behind a good one."""
-    x = Layer(own, 24, 24, workspace=24)
+    x = Layer(own, 24, 24, workspace=24, prefix=4096)
     x.draw([1] * 24)
 
     def rc(cmds):

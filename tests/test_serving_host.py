@@ -140,11 +140,12 @@ def test_routes_of_a_shared_prefix():
         at = w.index("own:")
         return [dict(x.split("=") for x in w[a:b]) for a, b in ((1, at), (at + 1, at + 5))]
 
-    shared, own = text(2, 1, 320, 40)
+    shared, own = text(2, 1, 4096, 40)
     assert shared["few"] != "0" and own["few"] != "0" and shared["tile"] == own["tile"] == "0"
     shared, own = text(32, 1, 4096, 500)
     assert shared["tile"] == "64" and int(shared["parts"]) > 4 and own["few"] == "32" and own["tile"] == "0"
     shared, own = text(3, 20, 16384, 440)
     assert shared["tile"] != "0" and own["tile"] != "0" and own["few"] == "0"
     assert words(4, 300, 2048, 700)[0] == "through:"
+    assert words(4, 1, 320, 20)[:2] == ["through:", "few"]
     assert words(4, 17, 64, 64)[0] == "through:" and words(4, 17, 32768, 64)[0] == "shared:"
