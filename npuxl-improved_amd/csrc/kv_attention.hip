@@ -26,8 +26,8 @@
 #include "lds_dma.hpp"
 
 #include <algorithm>
-#include <type_traits>
 #include <cstdio>
+#include <type_traits>
 
 namespace vnpu {
 namespace k {
@@ -1725,7 +1725,7 @@ uint32_t mixed(Mix &mix, uint32_t cus, const uint64_t groups[2])
 template <int DP, int RT>
 void launch_with_few(hipStream_t s, const Side &shared, const Side &own, const uint32_t slots[2], bool tiled)
 {
-    // Beside tiles, as many waves of few rows as leave three workgroups their LDS.
+    // Beside tiles, as many waves of few rows as leave a CU's three workgroups their LDS.
     constexpr int W = DP > 128 ? 2 : 4, beside = DP > 64 ? 2 : 4;
     const uint32_t G = own.p.call.c.kv_heads;
     const bool full = own.p.call.c.head_dim == DP;
@@ -1742,11 +1742,20 @@ void launch_with_few(hipStream_t s, const Side &shared, const Side &own, const u
     }
     const uint32_t grid = tiled ? static_cast<uint32_t>(groups[0] + groups[1]) : mixed(mix, own.p.cus, groups);
     mix.first = static_cast<uint32_t>(groups[0]);
-    if (tiled) {
-        constexpr uint32_t bytes = std::max(tile_lds<DP>(), few_lds<DP, RT, beside>());
-        const auto kernel = full ? kv_attention_tile_and_few<DP, RT, true, beside> : kv_attention_tile_and_few<DP, RT, false, beside>;
+    auto launch_beside = [&](auto waves) {
+        constexpr int N = decltype(waves)::value;
+        constexpr uint32_t bytes = std::max(tile_lds<DP>(), few_lds<DP, RT, N>());
+        const auto kernel = full ? kv_attention_tile_and_few<DP, RT, true, N> : kv_attention_tile_and_few<DP, RT, false, N>;
         allow_lds(kernel, bytes);
         kernel<<<grid, 256, bytes, s>>>(shared, own, mix);
+    };
+    if (tiled) {
+        // Four waves where no CU has more than two workgroups (32 sequences behind 4096 tokens 21.7 us, with two waves
+        // 23.4; 64 behind 32768 100 and 84).
+        if constexpr (DP == 128 && RT == 1) {
+            if (grid <= 2 * own.p.cus) return launch_beside(std::integral_constant<int, 4>());
+        }
+        launch_beside(std::integral_constant<int, beside>());
     } else {
         constexpr uint32_t bytes = few_lds<DP, RT, W>();
         const auto kernel = full ? kv_attention_few_twice<DP, RT, true, W> : kv_attention_few_twice<DP, RT, false, W>;
