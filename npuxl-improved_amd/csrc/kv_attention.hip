@@ -433,7 +433,7 @@ __device__ __forceinline__ void few_rows_of(const KvAttn &p, const Split &sp, fl
     int8_t *k_lds = lds + wave * 128 * DP, *v_lds = k_lds + 64 * DP;
     uint32_t *sh_p = reinterpret_cast<uint32_t *>(lds + WAVES * 128 * DP) + wave * 256;
     float *sh_o_all = reinterpret_cast<float *>(lds + WAVES * (128 * DP + 1024)), *sh_o = sh_o_all + wave * RT * DT * 64;
-    if (slot == 0 && h == 0) kv::check_all(c, false, p.max_kv, p.max_tokens, p.causal);
+    if (slot == 0 && h == 0) kv::check_all(c, 64 * WAVES, false, p.max_kv, p.max_tokens, p.causal);
     Slot sl;
     if (!find_slot(p, sp, false, slot, sl)) return;
     const uint32_t b = __builtin_amdgcn_readfirstlane(sl.b), parts = __builtin_amdgcn_readfirstlane(sl.parts);
@@ -992,7 +992,7 @@ __device__ __forceinline__ void tile_of(const KvAttn &p, const Tiles &tl, float 
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t G = c.c.kv_heads, h = place % G, D = FULL ? DP : DIM ? DIM : c.c.head_dim, ps = c.c.page_size, group = p.heads / G;
-    if (place == 0 && range == 0) kv::check_all(c, false, p.max_kv, p.max_tokens, p.causal);
+    if (place == 0 && range == 0) kv::check_all(c, 64 * WAVES, false, p.max_kv, p.max_tokens, p.causal);
     // The last tiles of a causal sequence have the most keys: they come first.
     uint32_t b, tile, len;
     kv::Seq seq;

@@ -290,7 +290,7 @@ __global__ __launch_bounds__(T) void kv_append_kernel(KvAppend p, Rates rates, A
     extern __shared__ __align__(16) int8_t tile[];
     __shared__ uint32_t red[T / 64];
     const KvCall &c = p.call;
-    if (blockIdx.x == 0) kv::check_all(c, true, kv::capacity(c), c.tokens);
+    if (blockIdx.x == 0) kv::check_all(c, blockDim.x, true, kv::capacity(c), c.tokens);
     const uint32_t appends = 2 * grid.units * c.c.kv_heads;
     if (blockIdx.x >= appends) {
         turn_queries<T>(p, rates, grid.half_magic, blockIdx.x - appends, grid.q_splits);
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(kReadThreads) void kv_read_kernel(KvRead p, uint32_
     const KvCall &c = p.call;
     const bool values = blockIdx.z || !p.K;
     const uint32_t h = blockIdx.y, tid = threadIdx.x;
-    if (blockIdx.x == 0 && h == 0 && blockIdx.z == 0) kv::check_all(c, true, kv::capacity(c), c.tokens);
+    if (blockIdx.x == 0 && h == 0 && blockIdx.z == 0) kv::check_all(c, blockDim.x, true, kv::capacity(c), c.tokens);
     uint32_t b;
     kv::Piece pc;
     if (!kv::find_piece(c, blockIdx.x, b, pc)) return;

@@ -87,10 +87,12 @@ inline uint32_t unit_count(const KvCall &c)
 
 // Every sequence's rows and lengths, looked over by one workgroup of a call so
 // that what no workgroup meets is an error too.  extra: the call's tokens count
-// towards the length (append, read).  most: tokens of a sequence.
-__device__ __forceinline__ void check_all(const KvCall &c, bool extra, uint32_t limit, uint32_t most, uint32_t causal = 0)
+// towards the length (append, read).  most: tokens of a sequence.  threads: of the
+// workgroup, those that come here, the first ones (where calls share a launch they are
+// fewer than the launch's).
+__device__ __forceinline__ void check_all(const KvCall &c, uint32_t threads, bool extra, uint32_t limit, uint32_t most, uint32_t causal = 0)
 {
-    for (uint32_t b = threadIdx.x; b < c.batch; b += blockDim.x) {
+    for (uint32_t b = threadIdx.x; b < c.batch; b += threads) {
         const Seq s = sequence(c, b);
         if (c.skip) {
             const int32_t own = length(c, b);
