@@ -1209,7 +1209,7 @@ k::KvAttn kv_prefix_params(vnpu_stream_t *s, const vnpu_kv_prefix_attention_i8_a
     k::KvAttn p = kv_attention_params(s, a.attention, src);
     require(a.prefix_len <= p.max_kv, "a kv prefix is longer than max_kv or the table");
     p.call.skip = a.prefix_len;
-    p.max_kv = std::max(1u, p.max_kv - a.prefix_len);
+    p.max_kv -= a.prefix_len;   // 0: no sequence may have keys of its own
     p.partial = 1;
     prefix_table = src.in(a.prefix_table, a.prefix_len / ps);
     require(k::kv_prefix_attention_fits(p, prefix_table), "kv_prefix_attention too large");

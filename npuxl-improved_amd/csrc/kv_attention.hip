@@ -1318,6 +1318,9 @@ __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, con
     }
 }
 
+// Keys of a sequence that the work is laid out for: max_kv, which is 0 where a prefix is all that a sequence may have.
+uint32_t planned_keys(const KvAttn &p) { return std::max(1u, p.max_kv); }
+
 // Rows that the kernel of few rows takes: one workgroup's, or two's where all
 // sequences' keys together are few.  (20 rows of 8 heads of 128, 3001 keys:
 // 1 sequence 17.4 us and 16.7 in tiles, heads of 64 14.3 and 14.7, 12 rows of 256 22.9 and
@@ -1325,7 +1328,7 @@ __global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, con
 uint32_t few_rows(const KvAttn &p)
 {
     const uint32_t one = p.call.c.head_dim > 128 ? 8 : 16;
-    const double keys = (p.call.seq_start ? 0.6 : 1.0) * p.call.batch * p.call.c.kv_heads * p.max_kv;
+    const double keys = (p.call.seq_start ? 0.6 : 1.0) * p.call.batch * p.call.c.kv_heads * planned_keys(p);
     return keys <= 32768 ? 2 * one : one;
 }
 
@@ -1365,7 +1368,7 @@ Plan plan_of(const KvAttn &p)
     const KvCall &c = p.call;
     const uint32_t G = c.c.kv_heads, group = p.heads / G, D = c.c.head_dim;
     const uint64_t most = static_cast<uint64_t>(p.max_tokens) * group;
-    const uint32_t at_most = few_rows(p);
+    const uint32_t at_most = few_rows(p), keys = planned_keys(p);
     r.tiled = most > at_most;
     // Without seq_start all sequences have max_tokens.  Beside sequences of many
     // rows the few-row ones have a launch of their own where they may be many;
@@ -1387,15 +1390,15 @@ Plan plan_of(const KvAttn &p)
         // Sequences are taken to be 0.8 of max_kv long, with seq_start 0.6.  It does not know
         // that more rows and larger heads take longer for a chunk (16 sequences of 4096 keys,
         // 16 rows on 8 heads of 128: 67 whole as it says, 56 split).
-        const double mb = (c.seq_start ? 1.2e-6 : 1.6e-6) * c.batch * G * D * p.max_kv;
-        r.split.whole = std::max(9.0 + 1.05 * ((p.max_kv + 255) / 256), mb / 6.4) <= 12.0 + mb / 6.4;
+        const double mb = (c.seq_start ? 1.2e-6 : 1.6e-6) * c.batch * G * D * keys;
+        r.split.whole = std::max(9.0 + 1.05 * ((keys + 255) / 256), mb / 6.4) <= 12.0 + mb / 6.4;
         r.split.low_rows = 0;
         r.split.high_rows = at_most;
         // No more slots than parts of the longest: a workgroup without work takes its turn too.
         r.slots = r.split.whole ? c.batch
                                 : static_cast<uint32_t>(std::min<uint64_t>(
                                       r.split.target + c.batch,
-                                      static_cast<uint64_t>(c.batch) * ((p.max_kv + r.split.min_per * kChunk - 1) / (r.split.min_per * kChunk))));
+                                      static_cast<uint64_t>(c.batch) * ((keys + r.split.min_per * kChunk - 1) / (r.split.min_per * kChunk))));
         if (!r.split.whole || p.partial) r.few_ws = (static_cast<size_t>(r.slots) * G * r.rows * (D + 2) * sizeof(float) + 15) / 16 * 16;
     }
     r.ws = r.few_ws;
@@ -1408,7 +1411,7 @@ Plan plan_of(const KvAttn &p)
                                         : r.tiles.per_seq * c.batch;
             return static_cast<uint64_t>(r.tiles.count) * G;
         };
-        const uint32_t chunks = (p.max_kv + kChunk - 1) / kChunk;
+        const uint32_t chunks = (keys + kChunk - 1) / kChunk;
         // 128 rows share K and V of a chunk where the card has more of such tiles
         // than run at a time (32 heads of 128, causal: 4096 tokens of 8 kv heads
         // 248 us against 254 with 64 rows, 2048 of 32 kv heads 84 and 81), or a few
@@ -1817,7 +1820,7 @@ Plan plan_through(const KvAttn &own)
     const KvCall &c = own.call;
     const uint32_t G = c.c.kv_heads, group = own.heads / G, D = c.c.head_dim, DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
     const uint64_t rows = static_cast<uint64_t>(own.max_tokens) * group, all = static_cast<uint64_t>(c.tokens) * group;
-    const uint32_t chunks = (own.max_kv + c.skip + kChunk - 1) / kChunk;
+    const uint32_t chunks = (planned_keys(own) + c.skip + kChunk - 1) / kChunk;
     Plan r;
     r.tiled = true;
     double least = 1e30;
@@ -1880,8 +1883,8 @@ bool few_through(const KvAttn &own)
 {
     const uint64_t rows = static_cast<uint64_t>(own.max_tokens) * (own.heads / own.call.c.kv_heads);
     if (rows > (own.call.c.head_dim > 128 ? 8 : 16)) return false;
-    const double alone = whole_us(own, own.max_kv);
-    return whole_us(own, own.max_kv + own.call.skip) < std::max(12.0 + 0.5 * alone, alone + 5.0);
+    const double alone = whole_us(own, planned_keys(own));
+    return whole_us(own, planned_keys(own) + own.call.skip) < std::max(12.0 + 0.5 * alone, alone + 5.0);
 }
 template <int DP, int RT>
 void launch_few_through(hipStream_t s, const KvAttn &p, uint32_t rows, const int32_t *prefix)

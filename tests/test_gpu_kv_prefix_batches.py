@@ -97,3 +97,30 @@ def test_bad_arrays_of_a_large_batch_fail_the_stream(gpu, d):
     assert not accepted
     x.check()
     x.free()
+
+
+# A prefix that is all that a sequence may have, because the table ends with it or because max_kv says so.  Few rows and
+# tiles in one pass; few rows twice, tiles and few rows, tiles twice.
+@pytest.mark.parametrize("room", [0, 2])
+@pytest.mark.parametrize("way,batch,n,page,prefix", [
+    ("through: few", 4, 1, 16, 64), ("through: tile=64", 5, 40, 16, 64), ("through: tile=64", 2, 150, 16, 1024),
+    ("shared: few=", 2, 1, 64, 4096), ("shared: few=0", 24, 1, 64, 4096), ("shared: few=0", 3, 20, 256, 16384)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_a_prefix_without_room_behind_it(gpu, way, batch, n, page, prefix, room, ragged):
+    x = Batch(gpu, 8, 2, 64, page, prefix, [0] * batch, [n] * batch, causal=0, ragged=ragged, table_ld=prefix // page + room)
+    assert x.route().startswith(way), x.route()
+    x.check()
+    accepted = []
+    for at in (0, batch - 1):
+        lengths = np.array(x.kv_len, np.int32)
+        lengths[at] = prefix + 1
+        gpu.write(x.held[0], lengths)
+        if not x.fails():
+            accepted.append(at)
+        if not room and not x.fails(max_kv=0):   # the table's room
+            accepted.append(("table", at))
+    assert not accepted
+    gpu.write(x.held[0], np.array(x.kv_len, np.int32))
+    assert x.fails(causal=1)   # new tokens would be keys of their own
+    x.check()
+    x.free()
