@@ -145,7 +145,8 @@ __device__ __forceinline__ float digits_sum(const v4i &a)
 constexpr int kBufferWord3 = 0x00020000;   // raw buffer, 32-bit data format
 constexpr uint32_t kOut = 0x80000000u;      // an offset past any buffer
 
-// Buffers over a workgroup's T strips and blocks begin .. end: what is behind them is zero.
+// Buffers over a workgroup's T strips and blocks begin .. end: what is behind them is zero.  A load's whole offset is in the
+// lanes' operand, which the range check covers; a scalar operand's part it would not.
 template <int T, int GB>
 struct Weights {
     v4i codes[T];
@@ -178,14 +179,14 @@ struct Strips {
     // Block begin + at.
     __device__ __forceinline__ void load(Weights<T, GB> &w, uint32_t at) const
     {
-        const uint32_t lane = threadIdx.x & 63, c = lane & 15, from = slot(begin + at) - slot0;
+        const uint32_t lane = threadIdx.x & 63, from = (slot(begin + at) - slot0) * 16 + (lane & 15);
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            w.codes[t] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(codes[t], lane * 16, at * 1024, 2));   // nontemporal
+            w.codes[t] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(codes[t], at * 1024 + lane * 16, 0, 2));   // nontemporal
 #pragma unroll
             for (int g = 0; g < GB; ++g) {
-                w.scale[t][g] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(scales[t], c * 4, (from + g) * 64, 0));
-                w.zero[t][g] = ZEROS ? __builtin_amdgcn_raw_buffer_load_b8(zeros[t], c, (from + g) * 16, 0) : 8;
+                w.scale[t][g] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(scales[t], (from + 16 * g) * 4, 0, 0));
+                w.zero[t][g] = ZEROS ? __builtin_amdgcn_raw_buffer_load_b8(zeros[t], from + 16 * g, 0, 0) : 8;
             }
         }
     }

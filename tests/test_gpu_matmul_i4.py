@@ -146,6 +146,21 @@ def test_not_finite(gpu, M):
     assert np.array_equal(np.isnan(got), want)
 
 
+@pytest.mark.parametrize("M", [1, 3, 8, 9, 20, 40])
+@pytest.mark.parametrize("K", [1, 100, 129, 700, 1100, 2100])
+@pytest.mark.parametrize("N", [16, 33, 49, 80, 1000])
+def test_waves_without_blocks_and_strips_behind_the_last(gpu, M, K, N):
+    """What lies behind a range of blocks or the last strip, and a last scale that is none, changes nothing else."""
+    for group in (32, 64, 256):
+        def change(a, w):
+            w.scales[-1, N - 1] = np.nan
+        got, a, w = case(gpu, M, K, N, group, zeros=group != 64, change=change, check=False)
+        assert np.all(np.isnan(got[:, N - 1]))
+        w.scales[-1, N - 1] = 0
+        want, bound = ops.matmul(a, w)
+        assert np.all(np.abs(got - want)[:, :N - 1] <= bound[:, :N - 1])
+
+
 @pytest.mark.parametrize("M", [1, 3, 9, 40, 140])
 def test_extreme_codes_and_signs(gpu, M):
     """Every product at its largest: 15 less zero of either sign, rows of one value."""
