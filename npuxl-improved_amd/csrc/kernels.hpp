@@ -336,7 +336,8 @@ struct I4Gemm {
     uint32_t groups_of_block = 1, blocks_of_group = 1;   // one of them is 1
     uint32_t M = 0, K = 0, N = 0, lda = 0, ldc = 0, epilogue = 0;
     uint32_t cus = 256;
-    // The kernel and how the work is cut (matmul_i4_lay_out).
+    // Division by blocks_of_group, the kernel and how the work is cut (matmul_i4_lay_out).
+    uint32_t group_factor = 0, group_shift = 0;
     enum : uint32_t { kFew, kMid, kTile } kernel = kFew;
     uint32_t rows = 0, strips = 0, waves = 0;   // of a workgroup: quads or tiles of 16 rows, strips of a wave or workgroup
     uint32_t per = 0, splits = 1;               // blocks of a range of K, ranges

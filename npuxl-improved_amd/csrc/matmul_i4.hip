@@ -156,11 +156,12 @@ struct Weights {
 template <int T, int GB, bool ZEROS>
 struct Strips {
     __amdgpu_buffer_rsrc_t codes[T], scales[T], zeros[T];
-    uint32_t slot0, begin, of_group;
+    uint32_t slot0, begin, factor, shift;
     __device__ __forceinline__ Strips(const I4Gemm &p, uint32_t strip0, uint32_t first, uint32_t end)
     {
         begin = first;
-        of_group = p.blocks_of_group;
+        factor = p.group_factor;
+        shift = p.group_shift;
         slot0 = slot(begin);
         const uint32_t strips = p.Np / 16, slots = GB > 1 ? GB * (end - begin) : slot(end - 1) + 1 - slot0;
         uint8_t *c = const_cast<uint8_t *>(p.codes) + (static_cast<uint64_t>(strip0) * p.KB + begin) * 1024;
@@ -175,7 +176,10 @@ struct Strips {
             if (ZEROS) zeros[t] = __builtin_amdgcn_make_buffer_rsrc(z + static_cast<uint64_t>(t) * p.slots * 16, 0, in ? slots * 16 : 0, kBufferWord3);
         }
     }
-    __device__ __forceinline__ uint32_t slot(uint32_t kb) const { return GB > 1 ? GB * kb : of_group == 1 ? kb : kb / of_group; }
+    // kb / blocks_of_group without the division's 15 scalar instructions, and without a condition for groups of one block: that
+    // becomes a branch, and where one lies between a product and its first use the compiler has counted the longer of
+    // the two ways alone for the wait that the result needs.
+    __device__ __forceinline__ uint32_t slot(uint32_t kb) const { return GB > 1 ? GB * kb : __umulhi(kb << 9, factor) >> shift; }
     // Block begin + at.
     __device__ __forceinline__ void load(Weights<T, GB> &w, uint32_t at) const
     {
@@ -213,23 +217,20 @@ __global__ __launch_bounds__(64 * W) void matmul_i4_few(I4Gemm p, uint32_t per, 
         Weights<T, GB> w;
         v4f x[RQ][2];
     };
-    auto load = [&](Block &b, uint32_t i) {   // the wave's i-th
-        const uint32_t at = wave + W * i, k = 128 * (begin + at) + 32 * d + 8 * kg;
+    auto load_rows = [&](Block &b, uint32_t i, int q) {   // of the wave's i-th block
+        const uint32_t k = 128 * (begin + wave + W * i) + 32 * d + 8 * kg;
 #pragma unroll
-        for (int q = 0; q < RQ; ++q)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const bool in = 4 * q + m < rows && k + 4 * j < last;
-                b.x[q][j] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(a, in ? ((4 * q + m) * p.lda + k + 4 * j) * 4 : kOut, 0, 0));
-            }
-        strip.load(b.w, at);
+        for (int j = 0; j < 2; ++j) {
+            const bool in = 4 * q + m < rows && k + 4 * j < last;
+            b.x[q][j] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(a, in ? ((4 * q + m) * p.lda + k + 4 * j) * 4 : kOut, 0, 0));
+        }
     };
 
     float acc[RQ][T] = {};   // row 4 q + kg, column c
     auto of_row_kg = [&](float x) {   // as lane 4 kg has it
         return __int_as_float(__builtin_amdgcn_ds_bpermute(static_cast<int>(16 * kg), __float_as_int(x)));
     };
-    auto work = [&](const Block &b, uint32_t i) {
+    auto work = [&](Block &b, uint32_t i) {
         v4i low[T], high[T];
 #pragma unroll
         for (int t = 0; t < T; ++t)
@@ -276,6 +277,8 @@ __global__ __launch_bounds__(64 * W) void matmul_i4_few(I4Gemm p, uint32_t per, 
             for (int j = 0; j < 4; ++j)
                 *reinterpret_cast<uint2 *>(mine + ((m * 4 + j) * 4 + kg) * 32 + d * 8) = make_uint2(plane[0][j], plane[1][j]);
             __builtin_amdgcn_wave_barrier();
+            load_rows(b, i + 1, q);   // before the products and the next weights: its digits are made while those come
+            __builtin_amdgcn_sched_barrier(0x86);   // no product or load passes
             const v4i a0 = *reinterpret_cast<const v4i *>(mine + (c * 4 + kg) * 32), a1 = *reinterpret_cast<const v4i *>(mine + (c * 4 + kg) * 32 + 16);
             __builtin_amdgcn_wave_barrier();
             const float unit = of_row_kg(__float_as_uint(most) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float((e - 30u) << 23));
@@ -331,10 +334,13 @@ __global__ __launch_bounds__(64 * W) void matmul_i4_few(I4Gemm p, uint32_t per, 
         }
     };
     Block block;
-    load(block, 0);
+#pragma unroll
+    for (int q = 0; q < RQ; ++q) load_rows(block, 0, q);
+    __builtin_amdgcn_sched_barrier(0);
+    strip.load(block.w, wave);
     for (uint32_t i = 0; wave + W * i < end - begin; ++i) {
         work(block, i);
-        load(block, i + 1);
+        strip.load(block.w, wave + W * (i + 1));
     }
     // The waves' sums together, in the waves' order.
     __syncthreads();
@@ -446,6 +452,7 @@ __global__ __launch_bounds__(64 * W) void matmul_i4_mid(I4Gemm p, uint32_t per, 
                     const bool in = 16 * r + c < rows && k + 32 * h + 4 * j < last;
                     b.x[r][h][j] = __builtin_bit_cast(v4f, __builtin_amdgcn_raw_buffer_load_b128(a, in ? ((16 * r + c) * p.lda + k + 32 * h + 4 * j) * 4 : kOut, 0, 0));
                 }
+        if (GB == 1) __builtin_amdgcn_sched_barrier(0);   // A's first: its halves are made while the weights come
         strip.load(b.w, at);
     };
     v4f total[RT][T];   // rows 16 r + 4 g + i, column c
@@ -927,6 +934,10 @@ void pack_i4(hipStream_t s, const uint8_t *B, const float *scales, const uint8_t
 
 bool matmul_i4_lay_out(I4Gemm &p)
 {
+    // kb / g = (kb 2^9 f / 2^32) / 2^s for kb below 2^23, s = log2 g rounded up, f = 2^(23 + s) / g rounded up: f g is less than g
+    // above 2^(23 + s), so the quotient is less than 2^-s, at most 1 / g, too high.
+    while ((1u << p.group_shift) < p.blocks_of_group) ++p.group_shift;
+    p.group_factor = static_cast<uint32_t>(((1ull << (23 + p.group_shift)) + p.blocks_of_group - 1) / p.blocks_of_group);
     // Offsets into A and a strip's codes are 31 bits in the kernels of few and tens of rows.
     const uint64_t most_rows = std::min(p.M, 32u);
     const bool short_offsets = ((most_rows - 1) * p.lda + p.K) * 4 < (1ull << 31) && p.KB < (1u << 21);
