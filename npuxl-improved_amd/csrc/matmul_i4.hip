@@ -326,9 +326,9 @@ __global__ __launch_bounds__(64 * W) void matmul_i4_few(I4Gemm p, uint32_t per, 
                 }
 #pragma unroll
                 for (int g = 0; g < GB; ++g) {
-                    float x = digits_sum(r[g]);
+                    float x = digits_sum(r[g]) * b.w.scale[t][g];   // the unit last: its product with a scale may be denormal
                     if (rare) x *= down;
-                    acc[q][t] = fmaf(x, unit * b.w.scale[t][g], acc[q][t]);
+                    acc[q][t] = fmaf(x, unit, acc[q][t]);
                 }
             }
         }

@@ -123,6 +123,18 @@ def test_sizes_of_values(gpu, M, factor):
         case(gpu, M, 200, 40, 64, change=change)
 
 
+@pytest.mark.parametrize("M", [1, 4, 8, 12, 40, 140])
+@pytest.mark.parametrize("power", [-97, -96, -95, -88, -80, -64])
+@pytest.mark.parametrize("scale", [1e-3, 1e-5, 1e-7])
+def test_small_values_with_small_scales(gpu, M, power, scale):
+    """A row's power of two and a scale whose product is no normal number; the results are."""
+    def change(a, w):
+        a *= np.float32(2.0**power / 8)
+        w.scales *= np.float32(scale / 0.02)
+    for group in (32, 64, 128):
+        case(gpu, M, 260, 40, group, zeros=group != 128, change=change)
+
+
 @pytest.mark.parametrize("M", [3, 14, 40, 140])
 def test_values_far_apart(gpu, M):
     """A row whose largest element is 2^60 times the others, in a block of its own and among them."""
