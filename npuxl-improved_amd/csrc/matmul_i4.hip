@@ -79,15 +79,30 @@ __global__ __launch_bounds__(256) void pack_scales(const float *scales, const ui
 // Epilogue
 // ---------------------------------------------------------------------------
 
+// A function's relative error is its argument's absolute one: GELU's arguments, 88 and 10 in size where results are still
+// normal numbers, are worked out in 64 bits and go in as f32 and what that leaves.  The tiles' kernels have this once
+// for each of 64 elements, so it is kept short (with an exponential and a division more, 2048 x 4096 x 11008 took 358 us
+// instead of 341 without any epilogue).
 __device__ __forceinline__ float finished(float x, uint32_t epilogue)
 {
-    switch (epilogue) {
-    case 1: return x > 0.0f ? x : x != x ? x : 0.0f;
-    case 2: return x / (1.0f + expf(-x));
-    case 3: return x / (1.0f + expf(-1.5957691216057308f * fmaf(0.044715f * x * x, x, x)));   // 1 + tanh(u) = 2 / (1 + exp(-2 u))
-    case 4: return 0.5f * x * erfcf(-0.70710678118654752f * x);
-    default: return x;
+    if (epilogue == 0) return x;
+    if (epilogue == 1) return x > 0.0f ? x : x != x ? x : 0.0f;
+    if (__builtin_expect(epilogue != 4, 1)) {
+        // x / (1 + exp(-u)); u = x, or sqrt(8 / pi) (x + 0.044715 x^3): 1 + tanh(u / 2) = 2 / (1 + exp(-u)).  exp(-|u|) ends in
+        // 0 and not in infinity.
+        float top = -fabsf(x), rest = 0.0f;
+        if (__builtin_expect(epilogue == 3, 0)) {
+            const double y = x, u = fmax(-fabs(y) * fma(0.07135481627260025 * y, y, 1.5957691216057308), -200.0);
+            top = static_cast<float>(u);
+            rest = static_cast<float>(u - top);
+        }
+        const float e = expf(top), down = fmaf(e, rest, e);
+        return (x < 0.0f ? x * down : x) / (1.0f + down);
     }
+    // erfc' = -2 / sqrt(pi) exp(-y^2)
+    const double u = -0.70710678118654752440 * x;
+    const float y = static_cast<float>(u), rest = fabsf(y) < 16.0f ? static_cast<float>(u - y) : 0.0f;
+    return 0.5f * x * fmaf(-1.12837917f * rest, __builtin_amdgcn_exp2f(-1.44269504f * y * y), erfcf(y));
 }
 
 // ---------------------------------------------------------------------------

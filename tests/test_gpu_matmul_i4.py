@@ -105,6 +105,31 @@ def test_bias_and_epilogues(gpu, M, epilogue, bias):
     case(gpu, M, 200, 70, 32, bias=bias, epilogue=epilogue)
 
 
+@pytest.mark.parametrize("M,K", [(1, 40), (3, 8192), (12, 40), (20, 8192), (600, 40)])
+@pytest.mark.parametrize("epilogue", [abi.EPI_SILU, abi.EPI_GELU_TANH, abi.EPI_GELU_ERF])
+def test_epilogues_to_a_part_of_the_result(gpu, M, K, epilogue):
+    """Of the bias alone, A being zero.  To a part of the result, down its left tail too: an exponential is off by 2^-23 at most (1
+    ulp), and there are four roundings of 2^-24 beside it, one more for GELU_TANH: together below 2^-21.  erfc may be off by
+    2^-19 (16 ulp, what OpenCL allows a device library).  An exponential or erfc in steps of 2^-149, times x up to 104, is
+    2^-142."""
+    x = np.concatenate([-np.geomspace(104, 1e-30, 3000), np.linspace(-16, 16, 3001), np.geomspace(1e-30, 1e30, 1000), [0.0, -1e4, -1e30]])
+    x = x.astype(np.float32)
+    N = x.size
+    w = ops.Weights(np.random.default_rng(2), K, N, 0)
+    packed = w.pack(gpu)
+    ba, bb, bc = gpu.upload(np.zeros((M, K), np.float32)), gpu.upload(x), gpu.alloc(4 * M * N)
+    gpu.run(abi.OP_MATMUL_I4, A=ba, B=packed, C=bc, bias=bb, M=M, K=K, N=N, epilogue=epilogue)
+    got = gpu.download(bc, np.float32, (M, N))
+    for b in (ba, bb, bc):
+        gpu.free(b)
+    gpu.release_packed_i4(packed)
+    with np.errstate(over="ignore"):
+        want = ops.finished(x.astype(np.float64), epilogue)
+    part = 2.0**-21 + (2.0**-19 if epilogue == abi.EPI_GELU_ERF else 0)
+    off = np.abs(got - want) / (part * np.abs(want) + 2.0**-142)
+    assert np.all(off <= 1), [(float(x[i]), float(got[r, i]), float(want[i])) for r, i in np.argwhere(~(off <= 1))[:5]]
+
+
 @pytest.mark.parametrize("M", [1, 4, 19, 66, 131])
 @pytest.mark.parametrize("a_gap,c_gap,shift,pad", [(4, 0, 0, 0), (1, 3, 0, 0), (0, 5, 1, 3), (3, 1, 2, 0), (8, 4, 4, 1), (0, 0, 3, 16)])
 def test_strides_and_alignment(gpu, M, a_gap, c_gap, shift, pad):
