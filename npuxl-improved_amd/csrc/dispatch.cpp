@@ -1790,7 +1790,7 @@ vnpu_packed_weights_i4_t *pack_weights_i4(vnpu_device_t *dev, const uint8_t *B, 
     w->group = group ? group : K;
     w->KB = cdiv(K, 128u);
     w->Np = cdiv(N, 16u) * 16;
-    const uint32_t groups = group ? cdiv(K, group) : 1;
+    const uint32_t groups = group ? (K - 1) / group + 1 : 1;   // a group may be near 2^32
     if (group == 32 || group == 64) w->groups_of_block = 128 / group;
     else w->blocks_of_group = group ? group / 128 : w->KB;
     w->slots = w->groups_of_block > 1 ? w->KB * w->groups_of_block : groups;

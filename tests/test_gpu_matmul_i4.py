@@ -240,6 +240,22 @@ def test_packing_from_the_device_and_info(gpu):
             gpu.free(x)
 
 
+@pytest.mark.parametrize("group", [384, 4096, 1 << 31, 0xffffff80])
+def test_groups_of_more_than_a_column(gpu, group):
+    """They are one group, however large."""
+    for M in (1, 10, 40):
+        got, a, w = case(gpu, M, 300, 40, 0)
+        w.group = group
+        packed, size = w.pack(gpu), C.c_uint32()
+        assert gpu.lib.vnpu_packed_weights_i4_info(packed, None, None, C.byref(size), None) == abi.OK and size.value == group
+        ba, bc = gpu.upload(a), gpu.alloc(4 * M * 40)
+        gpu.run(abi.OP_MATMUL_I4, A=ba, B=packed, C=bc, M=M, K=300, N=40)
+        assert np.array_equal(gpu.download(bc, np.float32, (M, 40)), got)
+        gpu.release_packed_i4(packed)
+        gpu.free(ba)
+        gpu.free(bc)
+
+
 def test_bad_weights_are_refused(gpu):
     codes, scales, out = np.zeros((64, 8), np.uint8), np.ones((2, 16), np.float32), C.c_void_p()
     zeros = np.full((2, 16), 15, np.uint8)
