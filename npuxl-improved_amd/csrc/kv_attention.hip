@@ -183,6 +183,17 @@ __device__ __forceinline__ bool find_slot(const KvAttn &p, const Split &sp, bool
     return false;
 }
 
+// A call of its own, not a side of a shared prefix's: what those alone have is constant, so that nothing is read or
+// worked out for it (one token of 8 heads of 64 over 128 keys 5.24 us, 5.57 with it; prompts and tokens mixed 35.0 and 35.6).
+__device__ __forceinline__ KvAttn alone(KvAttn p)
+{
+    p.call.skip = 0;
+    p.call.every = 1;
+    p.partial = p.per = 0;
+    __builtin_assume(p.call.lengths != nullptr);
+    return p;
+}
+
 // Token i of the sequence's queries, from its first.
 __device__ __forceinline__ uint64_t query_at(const KvAttn &p, uint32_t i)
 {
@@ -809,10 +820,10 @@ __device__ __forceinline__ void few_rows_of(const KvAttn &p, const Split &sp, fl
     }
 }
 
-template <int DP, int RT, bool FULL, int WAVES>
+template <int DP, int RT, bool FULL, int WAVES, bool SIDE>
 __global__ __launch_bounds__(64 * WAVES, DP * RT <= 256 && DP <= 128 ? 2 : 1) void kv_attention_few(KvAttn p, Split sp, float *ws, uint32_t ws_rows)
 {
-    few_rows_of<DP, RT, FULL, WAVES>(p, sp, ws, ws_rows, blockIdx.x, blockIdx.y, blockIdx.z);
+    few_rows_of<DP, RT, FULL, WAVES>(SIDE ? p : alone(p), sp, ws, ws_rows, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 template <int DP, int RT, bool FULL, int WAVES>
@@ -886,8 +897,9 @@ __device__ __forceinline__ void join_parts(const float *at, uint64_t step, uint3
 }
 
 // A sequence's parts together.
-__global__ __launch_bounds__(kJoinThreads) void kv_attention_merge(KvAttn p, Split sp, const float *ws, uint32_t ws_rows)
+__global__ __launch_bounds__(kJoinThreads) void kv_attention_merge(KvAttn call, Split sp, const float *ws, uint32_t ws_rows)
 {
+    const KvAttn p = alone(call);
     const KvCall &c = p.call;
     const uint32_t h = blockIdx.y, row = blockIdx.z, D = c.c.head_dim, group = p.heads / c.c.kv_heads;
     Slot sl;
@@ -1249,10 +1261,10 @@ __device__ __forceinline__ void tile_of(const KvAttn &p, const Tiles &tl, float 
     }
 }
 
-template <int DP, int RT, bool FULL, int WAVES>
+template <int DP, int RT, bool FULL, int WAVES, bool SIDE>
 __global__ __launch_bounds__(64 * WAVES, DP * RT <= 128 ? 3 : 2) void kv_attention_tile(KvAttn p, Tiles tl, float *ws)
 {
-    tile_of<DP, RT, FULL, WAVES>(p, tl, ws, blockIdx.x, blockIdx.y);
+    tile_of<DP, RT, FULL, WAVES>(SIDE ? p : alone(p), tl, ws, blockIdx.x, blockIdx.y);
 }
 constexpr int padded_dims(int dims) { return dims <= 64 ? 64 : dims <= 128 ? 128 : 256; }
 // For each head_dim: with one kernel for up to 128, dimensions that a head does not have cost branches among the
@@ -1269,8 +1281,9 @@ __global__ __launch_bounds__(256, padded_dims(D) * RT <= 128 ? 3 : 2) void kv_at
 // and up to 5 ranges).
 constexpr int kJoinRows = 2;
 template <uint32_t M, int DS, bool PREFIX = false>
-__global__ __launch_bounds__(256) void kv_attention_join(KvAttn p, Tiles tl, const float *ws)
+__global__ __launch_bounds__(256) void kv_attention_join(KvAttn call, Tiles tl, const float *ws)
 {
+    const KvAttn p = PREFIX ? call : alone(call);
     const KvCall &c = p.call;
     const uint32_t G = c.c.kv_heads, h = blockIdx.x % G, unit = blockIdx.x / G, D = c.c.head_dim, group = p.heads / G;
     uint32_t b, tile, len;
@@ -1446,7 +1459,8 @@ void launch_few(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
     constexpr int W = DP > 128 ? 2 : 4;
     constexpr uint32_t bytes = few_lds<DP, RT, W>();
     const bool full = p.call.c.head_dim == DP;
-    const auto kernel = full ? kv_attention_few<DP, RT, true, W> : kv_attention_few<DP, RT, false, W>;
+    const auto kernel = p.partial ? (full ? kv_attention_few<DP, RT, true, W, true> : kv_attention_few<DP, RT, false, W, true>)
+                                  : (full ? kv_attention_few<DP, RT, true, W, false> : kv_attention_few<DP, RT, false, W, false>);
     allow_lds(kernel, bytes);
     const uint32_t tiles = (pl.rows + 4 * RT - 1) / (4 * RT);
     kernel<<<dim3(pl.slots, p.call.c.kv_heads, tiles), 64 * W, bytes, s>>>(p, pl.split, ws, pl.rows);
@@ -1461,7 +1475,9 @@ template <int DP, int RT, int WAVES>
 void launch_tile(hipStream_t s, const KvAttn &p, const Plan &pl, float *ws)
 {
     constexpr uint32_t bytes = tile_lds<DP>();
-    const auto kernel = p.call.c.head_dim == DP ? kv_attention_tile<DP, RT, true, WAVES> : kv_attention_tile<DP, RT, false, WAVES>;
+    const bool full = p.call.c.head_dim == DP;
+    const auto kernel = p.partial ? (full ? kv_attention_tile<DP, RT, true, WAVES, true> : kv_attention_tile<DP, RT, false, WAVES, true>)
+                                  : (full ? kv_attention_tile<DP, RT, true, WAVES, false> : kv_attention_tile<DP, RT, false, WAVES, false>);
     allow_lds(kernel, bytes);
     const uint32_t grid = pl.tiles.count * p.call.c.kv_heads;
     kernel<<<dim3(grid, pl.tiles.parts), 64 * WAVES, bytes, s>>>(p, pl.tiles, ws);
