@@ -1739,13 +1739,29 @@ uint32_t mixed(Mix &mix, uint32_t cus, const uint64_t groups[2])
     mix.chunks[1] = (eights[1 - mix.less] + mix.chunk - 1) / mix.chunk;
     return 8 * mix.chunk * (mix.chunks[0] + mix.chunks[1]);
 }
+// Rows of few of a workgroup of DP padded dimensions, in fours.
+uint32_t few_quads(uint32_t rows, uint32_t DP) { return rows <= 4 ? 1 : DP > 128 || rows <= 8 ? 2 : 4; }
+// Workgroups of a prefix's tiles and of few rows in their launch.
+uint64_t groups_beside(const Plan &shared, const Plan &own, uint32_t G, uint32_t DP)
+{
+    const uint32_t quads = few_quads(own.rows, DP);
+    return static_cast<uint64_t>(shared.tiles.count) * G * shared.tiles.parts + static_cast<uint64_t>(own.slots) * G * ((own.rows + 4 * quads - 1) / (4 * quads));
+}
+// Waves of few rows beside tiles: as many as leave a CU's three workgroups their LDS, two for more than 64 dimensions.  Four
+// where no CU has more than two workgroups, for up to 4 rows of 128 dimensions (32 sequences behind 4096 tokens 21.7 us, with
+// two waves 23.4; 64 behind 32768 100 and 84); more rows and dimensions, whose four waves take more LDS, were not timed.
+uint32_t waves_beside(const Plan &shared, const Plan &own, uint32_t G, uint32_t DP, uint32_t cus)
+{
+    return DP == 64 || (DP == 128 && own.rows <= 4 && groups_beside(shared, own, G, DP) <= 2 * cus) ? 4 : 2;
+}
+bool tiles_beside_few(const Plan &shared, const Plan &own) { return shared.tiled && !shared.few && shared.tile_rows == 64 && !own.tiled; }
+
 // The two calls of a shared prefix in one launch: tiles of 64 rows and few rows, few rows twice, or the
 // same tiles twice; false: they are of other kinds.
 template <int DP, int RT>
-void launch_with_few(hipStream_t s, const Side &shared, const Side &own, const uint32_t slots[2], bool tiled)
+void launch_with_few(hipStream_t s, const Side &shared, const Side &own, const uint32_t slots[2], bool tiled, uint32_t waves)
 {
-    // Beside tiles, as many waves of few rows as leave a CU's three workgroups their LDS.
-    constexpr int W = DP > 128 ? 2 : 4, beside = DP > 64 ? 2 : 4;
+    constexpr int W = DP > 128 ? 2 : 4;
     const uint32_t G = own.p.call.c.kv_heads;
     const bool full = own.p.call.c.head_dim == DP;
     const Side *sides[2] = {&shared, &own};
@@ -1769,12 +1785,10 @@ void launch_with_few(hipStream_t s, const Side &shared, const Side &own, const u
         kernel<<<grid, 256, bytes, s>>>(shared, own, mix);
     };
     if (tiled) {
-        // Four waves where no CU has more than two workgroups (32 sequences behind 4096 tokens 21.7 us, with two waves
-        // 23.4; 64 behind 32768 100 and 84).
-        if constexpr (DP == 128 && RT == 1) {
-            if (grid <= 2 * own.p.cus) return launch_beside(std::integral_constant<int, 4>());
+        if constexpr (DP == 64 || (DP == 128 && RT == 1)) {
+            if (waves == 4) return launch_beside(std::integral_constant<int, 4>());
         }
-        launch_beside(std::integral_constant<int, beside>());
+        if constexpr (DP > 64) launch_beside(std::integral_constant<int, 2>());
     } else {
         constexpr uint32_t bytes = few_lds<DP, RT, W>();
         const auto kernel = full ? kv_attention_few_twice<DP, RT, true, W> : kv_attention_few_twice<DP, RT, false, W>;
@@ -1805,12 +1819,14 @@ bool launch_both(hipStream_t s, const Side &shared, const Plan &shared_plan, con
         else if constexpr (DP <= 128) launch_tiles_twice<DP, 2>(s, shared, own);
         return true;
     }
-    if (own_plan.tiled || (shared_plan.tiled && (shared_plan.few || shared.tile_rows != 64))) return false;
+    const bool tiled = tiles_beside_few(shared_plan, own_plan);
+    if (!tiled && (own_plan.tiled || shared_plan.tiled)) return false;
     uint32_t slots[2] = {shared_plan.slots, own_plan.slots};
-    const uint32_t rows = shared_plan.tiled ? own.rows : std::max(shared.rows, own.rows);
-    if (rows <= 4) launch_with_few<DP, 1>(s, shared, own, slots, shared_plan.tiled);
-    else if (DP > 128 || rows <= 8) launch_with_few<DP, 2>(s, shared, own, slots, shared_plan.tiled);
-    else if constexpr (DP <= 128) launch_with_few<DP, 4>(s, shared, own, slots, shared_plan.tiled);
+    const uint32_t quads = few_quads(tiled ? own.rows : std::max(shared.rows, own.rows), DP);
+    const uint32_t waves = waves_beside(shared_plan, own_plan, own.p.call.c.kv_heads, DP, own.p.cus);
+    if (quads == 1) launch_with_few<DP, 1>(s, shared, own, slots, tiled, waves);
+    else if (quads == 2) launch_with_few<DP, 2>(s, shared, own, slots, tiled, waves);
+    else if constexpr (DP <= 128) launch_with_few<DP, 4>(s, shared, own, slots, tiled, waves);
     return true;
 }
 
@@ -1995,7 +2011,12 @@ std::string kv_prefix_attention_route(const KvAttn &own, const int32_t *prefix_t
         return text;
     }
     if (few_through(own)) return "through: few";
-    return "shared: " + kv_attention_route(shared_call(own, prefix_table)) + " own: " + kv_attention_route(own);
+    const KvAttn shared = shared_call(own, prefix_table);
+    std::string text = "shared: " + kv_attention_route(shared) + " own: " + kv_attention_route(own);
+    const Plan shared_plan = plan_of(shared), own_plan = plan_of(own);
+    if (tiles_beside_few(shared_plan, own_plan))
+        text += " waves=" + std::to_string(waves_beside(shared_plan, own_plan, own.call.c.kv_heads, padded_dims(own.call.c.head_dim), own.cus));
+    return text;
 }
 
 void kv_prefix_attention(hipStream_t s, const KvAttn &own, const int32_t *prefix_table, void *ws)

@@ -124,3 +124,21 @@ def test_a_prefix_without_room_behind_it(gpu, way, batch, n, page, prefix, room,
     assert x.fails(causal=1)   # new tokens would be keys of their own
     x.check()
     x.free()
+
+
+# Prefix tiles beside few rows of four waves and of two, with 4, 8 and 16 rows a workgroup; of up to 128 dimensions and 4 rows
+# four waves where the launch has no more than two workgroups a CU (512 here) and two where it has more.
+@pytest.mark.parametrize("waves,d,heads,kv_heads,batch,n,prefix", [
+    (4, 80, 8, 2, 120, 1, 2048), (4, 128, 8, 2, 120, 1, 2048), (4, 128, 8, 8, 30, 2, 2048),
+    (2, 80, 8, 2, 250, 1, 2048), (2, 128, 8, 2, 250, 1, 2048), (2, 128, 16, 8, 64, 1, 2048), (2, 112, 8, 8, 60, 3, 2048),
+    (2, 128, 8, 2, 120, 2, 2048), (2, 128, 8, 2, 48, 3, 2048), (2, 80, 8, 2, 48, 4, 2048),
+    (2, 144, 8, 2, 120, 1, 1024), (2, 256, 8, 2, 64, 2, 1024), (2, 256, 4, 4, 64, 1, 1024),
+    (4, 64, 8, 2, 64, 2, 2048), (4, 48, 8, 2, 64, 4, 2048)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_tiles_beside_few_rows(gpu, waves, d, heads, kv_heads, batch, n, prefix, ragged):
+    tokens = [n - (b % n if ragged else 0) for b in range(batch)]
+    x = Batch(gpu, heads, kv_heads, d, 64, prefix, [m + 11 * b % 150 for b, m in enumerate(tokens)], tokens, ragged=ragged)
+    way = x.route()
+    assert way.startswith("shared: few=0 rows=0 tile=64 ") and f" tile=0 parts=0 waves={waves} " in way, way
+    x.check()
+    x.free()

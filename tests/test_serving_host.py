@@ -149,3 +149,16 @@ def test_routes_of_a_shared_prefix():
     assert words(4, 300, 2048, 700)[0] == "through:"
     assert words(4, 1, 320, 20)[:2] == ["through:", "few"]
     assert words(4, 17, 64, 64)[0] == "through:" and words(4, 17, 32768, 64)[0] == "shared:"
+
+
+def test_waves_of_few_rows_beside_tiles():
+    """Four where the launch has no more than two workgroups a CU, for up to 4 rows of 65 to 128 dimensions; always for less."""
+    def waves(d, heads, kv_heads, batch, n=1, prefix_len=4096):
+        c = dict(page_size=16, kv_heads=kv_heads, head_dim=d, table_ld=1 << 14)
+        way = route(*prefix(c=c, prefix_len=prefix_len, batch=batch, tokens=batch * n, heads=heads, max_kv=prefix_len + 64))
+        return next((int(w[6:]) for w in way.split() if w.startswith("waves=")), None)
+
+    assert waves(128, 32, 8, 32) == 4 and waves(128, 32, 8, 64, prefix_len=32768) == 2
+    assert waves(80, 8, 2, 120) == 4 and waves(80, 8, 2, 250) == 2
+    assert waves(64, 8, 2, 250) == 4 and waves(128, 8, 2, 30, n=2) == 2 and waves(256, 8, 2, 30) == 2
+    assert waves(128, 32, 8, 2) is None   # few rows twice
