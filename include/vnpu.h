@@ -631,7 +631,8 @@ typedef struct vnpu_kv_read_f32_args_t {
  * 2^-23 of itself (2^-39 of the largest of its row, or of its row's same 128, where
  * that is more); sums are f32 or wider, each group's scaled once.  M, K and N choose the
  * kernel.  A row of A with an infinity or NaN gives NaN in all of its results.
- * M is up to 2^28, K and N up to 2^30.  SILU, GELU_TANH and GELU_ERF are the functions
+ * M is up to 2^28, K and N up to 2^30, a scale is up to 2^64 in size (larger ones may
+ * overflow where the result would not).  SILU, GELU_TANH and GELU_ERF are the functions
  * themselves, to some 2^-21 of the result or 2^-142, whichever is more (not the
  * polynomials of the int8 and f32 products). `workspace`: as in vnpu_kv_attention_i8_args_t, its bytes
  * from vnpu_matmul_i4_workspace. */

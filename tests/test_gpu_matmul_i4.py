@@ -160,6 +160,17 @@ def test_small_values_with_small_scales(gpu, M, power, scale):
         case(gpu, M, 260, 40, group, zeros=group != 128, change=change)
 
 
+@pytest.mark.parametrize("M", [1, 4, 8, 12, 40, 140])
+@pytest.mark.parametrize("power,scale", [(-96, 1e17), (-70, 1e17), (-96, 1e25), (-20, 1e-25), (0, 1e-30), (60, 1e-34), (100, 1e-30)])
+def test_values_and_scales_at_opposite_ends(gpu, M, power, scale):
+    """A sum in a row's own unit, or that unit, times a scale is beyond the normal numbers; the results are not."""
+    def change(a, w):
+        a *= np.float32(2.0**power / 8)
+        w.scales *= np.float32(scale / 0.02)
+    for group in (32, 64, 128):
+        case(gpu, M, 260, 40, group, zeros=group != 128, change=change)
+
+
 @pytest.mark.parametrize("M", [3, 14, 40, 140])
 def test_values_far_apart(gpu, M):
     """A row whose largest element is 2^60 times the others, in a block of its own and among them."""
