@@ -114,9 +114,10 @@ __device__ __forceinline__ float finished(float x, uint32_t epilogue)
 // first summand, -zero * (sum of the digits), which a product with ones gives.
 //
 // 1 x 4096 x 4096 4.5 us (a launch; the codes are 1.7 us of a copy), 1 x 4096 x 32000, groups of
-// 128, zeros 12.9 us, 5.5 TB/s; 8 x 11008 x 4096, groups of 64, 13.5 us with the join, vector
-// instructions in 53% of the SIMD cycles (A's digits, made again in each of 64 workgroups) and 3 us of start.
-// Blocks asked for two ahead instead of one: no gain.
+// 128, zeros 13.2 us with three sets of weights in turn, which the last cache holds, and 13.9 with twelve, which it does not:
+// 5.1 TB/s; 8 x 11008 x 4096, groups of 64, 12.5 us with the join, vector instructions in 57% of the SIMD cycles
+// (A's digits, made again in each of 64 workgroups) and 3 us of start.  Blocks asked for two ahead instead of one: no
+// gain.
 // ---------------------------------------------------------------------------
 
 // Largest over the 4 groups of 16 lanes; NaN is above all.
@@ -410,7 +411,8 @@ void launch_few(hipStream_t s, const I4Gemm &p, float *part)
 // Place in 8 of K of a fragment's element e: the order in which codes come out of a word.
 __device__ __forceinline__ constexpr uint32_t order(uint32_t e) { return (e & 4) | (e & 1) << 1 | (e >> 1 & 1); }
 
-// Codes of 32 of K: words w of a strip's block, their lower or upper halves, less zero.  The mask
+// Codes of 32 of K: words w of a strip's block, their lower or upper halves, less zero.  A code set under the exponent of
+// 1024 is 1024 + code, a published way that f16's format gives.  The mask
 // and the exponent bits are in registers: as literals they would take an instruction each.
 struct Masks {
     uint32_t low, high, bits;
@@ -611,10 +613,10 @@ void launch_mid(hipStream_t s, const I4Gemm &p, float *part)
 // v_mfma_f32_16x16x32_f16 as they are read: [row tile of 16][32 of K][hi, lo][64
 // lanes][8], lane (kg, row), element e the K of place order(e) among its 8.
 //
-// 2048 x 4096 x 11008, groups of 128: 355 us, 520 TFLOP/s of the result's, 1.04 PFLOP/s of products
-// (a large f16 product of the library 1.16), the split 19 of them; in groups of 32, which take four times as many
+// 2048 x 4096 x 11008, groups of 128: 337 to 358 us as the card's clock goes, 530 TFLOP/s of the result's, 1.06 PFLOP/s of
+// products (a large f16 product of the library 1.16), the split 19 of them; in groups of 32, which take four times as many
 // scalings, 422.  A tile's wave has its strips' codes alone and shares the rows' fragments through LDS.  Its matrix cores are
-// busy in 54% of the cycles, its vector issue in 42%; 2.7 tiles for each that runs at a time are 3 rounds.
+// busy in 56% of the cycles, its vector issue in 43%; 2.7 tiles for each that runs at a time are 3 rounds.
 // ---------------------------------------------------------------------------
 
 // A workgroup has 16 rows and a part of their blocks; it looks for the rows' largest
@@ -701,7 +703,7 @@ __global__ __launch_bounds__(256, RT * CT <= 16 ? 2 : 1) void matmul_i4_tile(I4G
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Neighbouring tiles on one XCD, in bands of 8 row tiles: the 64 that run there at a time share 8 tiles of rows and
-    // 8 of columns (2048 x 4096 x 11008: 387 us; a column tile's row tiles one after the other 407).
+    // 8 of columns (2048 x 4096 x 11008: 347 us; a column tile's row tiles one after the other 356, timed in turn).
     const uint32_t tiles = tl.row_tiles * tl.col_tiles, each = (tiles + 7) / 8, id = blockIdx.x % 8 * each + blockIdx.x / 8;
     if (blockIdx.x / 8 >= each || id >= tiles) return;
     const uint32_t band = id / (kBand * tl.col_tiles), in = id - band * kBand * tl.col_tiles;
