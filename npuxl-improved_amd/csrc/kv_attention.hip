@@ -504,7 +504,8 @@ __device__ __forceinline__ void few_rows_of(const KvAttn &p, const Split &sp, fl
                 constexpr int kPer = DP / 64;   // copies of a block
                 const uint32_t j = i / kPer, in = (16 * min(4 * chunk + j, last16)) & (ps - 1);
                 const uint32_t piece = 64 * (i % kPer) + lane, key = piece / (DP / 16), at = piece % (DP / 16);
-                lds::dma16_nt(c.c.k + (unit[j] * ps + in + key) * DP + 16 * (at ^ ((4 * j + key / 4) & kSwap)), k_lds + 1024 * i);
+                const int8_t *from = c.c.k + (unit[j] * ps + in) * DP;   // the block's: scalar
+                lds::dma16_nt(from + key * DP + 16 * (at ^ ((4 * j + key / 4) & kSwap)), k_lds + 1024 * i);
             } else {
                 const uint32_t piece = 64 * i + lane, j = piece / D, in = (16 * min(4 * chunk + j, last16)) & (ps - 1);
                 lds::dma16_nt(c.c.k + (of_block(j, unit) * ps + in) * D + 16 * (piece - j * D), k_lds + 1024 * i);
